@@ -2,10 +2,11 @@
 
     python -m cpde_b200.build
 
-nvcc cross-compiles without a GPU. The library is four translation units
+nvcc cross-compiles without a GPU. The library is five translation units
 compiled in parallel (csrc/library.cu: engine core, C ABI, allocation-free
 entry; fast_forward.cu, fast_backward.cu, fast_head.cu: the fast-tier
-dispatch and the kernels it instantiates); the server is a host program
+dispatch and the kernels it instantiates; operators.cu: the device-tensor
+operators); the server is a host program
 linked against it with an $ORIGIN-relative rpath so the pair can be moved
 together.
 """
@@ -20,7 +21,7 @@ LIBRARY = PACKAGE / 'libcpde_b200.so'
 SERVER = PACKAGE / 'bin' / 'cpde_server'
 BUILD = PACKAGE / '_build'
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
-UNITS = ['library', 'fast_forward', 'fast_backward', 'fast_head']
+UNITS = ['library', 'fast_forward', 'fast_backward', 'fast_head', 'operators']
 
 
 def _run(cmd):

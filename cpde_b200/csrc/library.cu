@@ -2,3 +2,4 @@
 #include "engine.cu"
 #include "capi.cu"
 #include "noalloc.cu"
+#include "operators_capi.cu"

@@ -1,0 +1,379 @@
+// Launches of the device-tensor operators (operators.hpp).
+#include "operators.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "common.hpp"
+#include "kernels_dropout.cuh"
+#include "kernels_embedding.cuh"
+#include "kernels_norm.cuh"
+
+namespace cpde::ops {
+namespace {
+
+constexpr int SMS = 148;
+
+enum Type : int32_t { F32 = 0, BF16 = 1, F16 = 2 };
+size_t bytes_of(int32_t type) { return type == F32 ? 4 : 2; }
+
+template <class T> struct Tag { using type = T; };
+
+// Calls f with the C++ type of a type code.
+template <class F>
+void with_type(int32_t type, F&& f) {
+    if (type == F32) f(Tag<float>{});
+    else if (type == BF16) f(Tag<__nv_bfloat16>{});
+    else f(Tag<__half>{});
+}
+
+// Equal types, or the one on the WIDE_IN side FP32 and the other of 16 bits.
+template <bool WIDE_IN, class F>
+void with_types(int32_t in, int32_t out, F&& f) {
+    with_type(WIDE_IN ? out : in, [&](auto narrow) {
+        using N = typename decltype(narrow)::type;
+        if (in == out) f(Tag<N>{}, Tag<N>{});
+        else if constexpr (WIDE_IN) f(Tag<float>{}, Tag<N>{});
+        else f(Tag<N>{}, Tag<float>{});
+    });
+}
+
+uint32_t power_of_two_from(int64_t n) {
+    uint32_t p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+// The most elements, a power of two up to `most`, that divide a row of
+// `channels` and whose accesses are aligned at every given address and stride.
+struct Alignment {
+    uint64_t odd = 0;  // bits that an access's alignment must not have
+    Alignment& at(const void* p, size_t element) { odd |= reinterpret_cast<uintptr_t>(p) / element; return *this; }
+    Alignment& stride(int64_t elements) { odd |= uint64_t(elements); return *this; }
+    int vector(int most) const {
+        int v = most;
+        while (v > 1 && odd % v) v /= 2;
+        return v;
+    }
+};
+
+template <int... VS, class F>
+void with_vector(int v, F&& f) {
+    ((v == VS ? f(std::integral_constant<int, VS>{}) : void()), ...);
+}
+
+template <class K>
+void dynamic_shared(K kernel, size_t bytes) {
+    CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+}
+
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// --- embedding -------------------------------------------------------------
+
+struct SortPlan {
+    int passes, digit_bits;
+    uint32_t cluster;
+};
+SortPlan sort_plan(int64_t tokens, int64_t rows) {
+    int bits = 1;
+    while ((int64_t(1) << bits) < rows + 1) ++bits;
+    SortPlan p;
+    p.passes = (bits + 9) / 10;
+    p.digit_bits = (bits + p.passes - 1) / p.passes;
+    p.cluster = std::min<uint32_t>(16, power_of_two_from((tokens + 2047) / 2048));
+    return p;
+}
+
+SumShape sum_shape(int64_t tokens, int64_t rows, int64_t channels, int v) {
+    SumShape s;
+    s.tokens = uint32_t(tokens);
+    s.rows = uint32_t(rows);
+    s.channels = channels;
+    s.vectors = uint32_t(channels / v);
+    s.lanes = power_of_two_from(std::min<int64_t>(s.vectors, 32));
+    s.tiles = (s.vectors + s.lanes - 1) / s.lanes;
+    s.chunk = 64;
+    while (s.chunk > 8 && (tokens / s.chunk) * s.tiles * s.lanes / 32 < SMS * 32) s.chunk /= 2;
+    s.chunks = uint32_t((tokens + s.chunk - 1) / s.chunk);
+    s.grad_stride = 0;
+    return s;
+}
+
+}  // namespace
+
+void embedding(const EmbeddingCall& c, cudaStream_t stream) {
+    if (!c.tokens) return;
+    with_types<true>(c.in_type, c.out_type, [&](auto in, auto out) {
+        using TI = typename decltype(in)::type;
+        using TO = typename decltype(out)::type;
+        const int v = Alignment().at(c.in, sizeof(TI)).at(c.out, sizeof(TO)).stride(c.in_stride).stride(c.channels)
+                          .vector(16 / sizeof(TO));
+        with_vector<8, 4, 2, 1>(v, [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            if constexpr (V * sizeof(TO) <= 16) {
+                const int64_t vectors = c.channels / V;
+                // Slabs of tokens whose vectors a 31-bit index counts.
+                const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / vectors);
+                for (int64_t t = 0; t < c.tokens; t += slab) {
+                    const uint32_t count = uint32_t(std::min(slab, c.tokens - t) * vectors);
+                    const uint32_t blocks = (count + 256 * LOOKUPS - 1) / (256 * LOOKUPS);
+                    TO* to = static_cast<TO*>(c.out) + t * c.channels;
+                    if (c.id_type)
+                        k_embedding<TI, TO, int64_t, V><<<blocks, 256, 0, stream>>>(
+                            static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int64_t*>(c.ids) + t,
+                            to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
+                    else
+                        k_embedding<TI, TO, int32_t, V><<<blocks, 256, 0, stream>>>(
+                            static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int32_t*>(c.ids) + t,
+                            to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
+                    CPDE_LAUNCHED();
+                }
+            }
+        });
+    });
+}
+
+size_t embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channels) {
+    size_t partials = 0;
+    for (int v : {8, 4, 2, 1})
+        if (channels % v == 0)
+            partials = std::max(partials, size_t(sum_shape(tokens, rows, channels, v).chunks) * 2 * channels);
+    return 4 * padded(size_t(tokens) * 4) + padded(partials * 4);
+}
+
+void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream) {
+    const size_t out_bytes = size_t(c.rows) * c.channels * bytes_of(c.out_type);
+    const bool words = (reinterpret_cast<uintptr_t>(c.out) | out_bytes) % 16 == 0;
+    if (!c.tokens || !words) CPDE_CUDA(cudaMemsetAsync(c.out, 0, out_bytes, stream));
+    if (!c.tokens) return;
+
+    char* at = static_cast<char*>(c.workspace);
+    auto take = [&](size_t bytes) { char* p = at; at += padded(bytes); return p; };
+    SortBuffers buffers;
+    for (int i = 0; i < 2; ++i) {
+        buffers.row[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
+        buffers.token[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
+    }
+    float* partial = reinterpret_cast<float*>(at);
+
+    const SortPlan plan = sort_plan(c.tokens, c.rows);
+    const int64_t fill_words = words ? int64_t(out_bytes / 16) : 0;
+    const int64_t fillers = std::min<int64_t>(112, (fill_words + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
+    const size_t shared = (size_t(SORT_WARPS) + 1) * (size_t(4) << plan.digit_bits);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(plan.cluster + (fillers + plan.cluster - 1) / plan.cluster * plan.cluster));
+    config.blockDim = dim3(SORT_THREADS);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = plan.cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    auto sort = [&](auto kernel, auto* ids) {
+        static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limits are raised
+        if (!(ready.load() >> (device & 63) & 1)) {
+            dynamic_shared(kernel, (size_t(SORT_WARPS) + 1) * 4096);
+            CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            ready.fetch_or(uint64_t(1) << (device & 63));
+        }
+        CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, ids, uint32_t(c.tokens), c.rows, plan.passes, plan.digit_bits,
+                                     buffers, static_cast<uint4*>(c.out), fill_words));
+    };
+    if (c.id_type) sort(k_sort_tokens<int64_t>, static_cast<const int64_t*>(c.ids));
+    else sort(k_sort_tokens<int32_t>, static_cast<const int32_t*>(c.ids));
+
+    const uint32_t* row = buffers.row[sorted_buffer(plan.passes)];
+    const uint32_t* token = buffers.token[sorted_buffer(plan.passes)];
+    with_types<false>(c.in_type, c.out_type, [&](auto in, auto out) {
+        using TI = typename decltype(in)::type;
+        using TO = typename decltype(out)::type;
+        const int v = Alignment().at(c.in, sizeof(TI)).at(c.out, sizeof(TO)).stride(c.in_stride).stride(c.channels)
+                          .vector(16 / sizeof(TI));
+        with_vector<8, 4, 2, 1>(v, [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            if constexpr (V * sizeof(TI) <= 16) {
+                SumShape s = sum_shape(c.tokens, c.rows, c.channels, V);
+                s.grad_stride = c.in_stride;
+                const uint64_t threads = uint64_t(s.chunks) * s.tiles * s.lanes;
+                k_sum_tokens<TI, TO, V><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(
+                    row, token, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), partial, s, c.scale);
+                CPDE_LAUNCHED();
+                if (s.chunks > 1) {
+                    const uint32_t x = power_of_two_from(std::min<int64_t>(c.channels, 256));
+                    k_join_chunks<TO><<<s.chunks - 1, dim3(x, 256 / x), 0, stream>>>(
+                        row, static_cast<TO*>(c.out), partial, s, c.scale);
+                    CPDE_LAUNCHED();
+                }
+            }
+        });
+    });
+}
+
+// --- dropout ---------------------------------------------------------------
+
+namespace {
+
+DropoutRule dropout_rule(double rate, uint64_t seed, uint64_t offset) {
+    const uint32_t threshold = uint32_t(std::lround(rate * 65536));
+    return {seed, offset, threshold, threshold < 65536 ? float(65536.0 / (65536.0 - threshold)) : 0.0f};
+}
+
+}  // namespace
+
+void dropout(const DropoutCall& c, cudaStream_t stream) {
+    if (!c.rows || !c.columns) return;
+    DropoutShape s = {c.rows, c.columns, c.x_stride, c.residual ? c.residual_stride : c.columns};
+    const int64_t count = c.rows * c.columns;
+    const bool contiguous = c.rows == 1 || (s.x_stride == c.columns && s.residual_stride == c.columns);
+    with_type(c.type, [&](auto tag) {
+        using T = typename decltype(tag)::type;
+        Alignment a;
+        a.at(c.x, sizeof(T)).at(c.residual, sizeof(T)).at(c.y, sizeof(T));
+        if (!contiguous) a.stride(s.x_stride).stride(s.residual_stride).stride(c.columns);
+        const int mode = a.vector(8) == 8 ? (contiguous ? 2 : 1) : 0;
+        const unsigned blocks = unsigned((count + 2047) / 2048);
+        const DropoutRule rule = dropout_rule(c.rate, c.seed, c.offset);
+        with_vector<0, 1, 2>(mode, [&](auto m) {
+            constexpr int MODE = decltype(m)::value;
+            const T *x = static_cast<const T*>(c.x), *r = static_cast<const T*>(c.residual);
+            if (r) k_dropout<T, true, MODE><<<blocks, 256, 0, stream>>>(x, r, static_cast<T*>(c.y), s, count, rule);
+            else k_dropout<T, false, MODE><<<blocks, 256, 0, stream>>>(x, r, static_cast<T*>(c.y), s, count, rule);
+            CPDE_LAUNCHED();
+        });
+    });
+}
+
+// --- group norm --------------------------------------------------------------
+
+namespace {
+
+NormShape norm_shape(int64_t instances, int64_t points, int64_t channels, int64_t groups, int v) {
+    NormShape s = {};
+    s.instances = int32_t(instances);
+    s.points = int32_t(points);
+    s.channels = int32_t(channels);
+    s.groups = int32_t(groups);
+    s.width = int32_t(channels / groups);
+    s.vectors = s.channels / v;
+    s.tiles = (s.vectors + 63) / 64;
+    s.tile = (s.vectors + s.tiles - 1) / s.tiles;
+    s.tiles = (s.vectors + s.tile - 1) / s.tile;
+    s.pieces = std::min(s.groups, (s.tile * v - 1) / s.width + 2);
+    const int64_t ys = NORM_THREADS / s.tile, blocks = instances * s.tiles;
+    s.splits = int32_t(std::max<int64_t>(1, std::min((SMS * 8 + blocks - 1) / blocks, (points + ys * 4 - 1) / (ys * 4))));
+    s.splits = int32_t(std::max<int64_t>(s.splits, (points + ys * 512 - 1) / (ys * 512)));
+    s.apply_splits = s.splits;
+    return s;
+}
+
+size_t norm_workspace(const NormShape& s) {
+    const size_t blocks = size_t(s.instances) * s.splits;
+    return padded(blocks * s.tiles * s.pieces * sizeof(Moments)) + padded(blocks * s.channels * sizeof(float2));
+}
+
+// V and the strides, lengths and dropout of a call.
+template <class T>
+NormShape norm_call_shape(const NormCall& c, int v) {
+    NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, v);
+    s.x_point = c.x_point;
+    s.x_instance = c.x_instance;
+    s.grad_point = c.grad_point;
+    s.grad_instance = c.grad_instance;
+    s.activation = c.activation;
+    s.eps = float(c.eps);
+    s.lengths = c.lengths;
+    s.rule = dropout_rule(c.rate, c.seed, c.offset);
+    return s;
+}
+
+template <class F>
+void with_norm_types(const NormCall& c, F&& f) {
+    with_type(c.type, [&](auto tag) {
+        using T = typename decltype(tag)::type;
+        Alignment a;
+        a.at(c.x, sizeof(T)).at(c.out, sizeof(T)).stride(c.x_point).stride(c.channels);
+        if (c.instances > 1) a.stride(c.x_instance);
+        if (c.grad) {
+            a.at(c.grad, sizeof(T)).stride(c.grad_point);
+            if (c.instances > 1) a.stride(c.grad_instance);
+        }
+        const int fit = a.vector(8);
+        with_vector<8, 4, 1>(fit == 2 ? 1 : fit, [&](auto width) {
+            if (c.parameter_type == F32) f(tag, Tag<float>{}, width);
+            else f(tag, tag, width);
+        });
+    });
+}
+
+}  // namespace
+
+size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups) {
+    size_t bytes = 0;
+    for (int v : {8, 4, 1})
+        if (channels % v == 0)
+            bytes = std::max(bytes, norm_workspace(norm_shape(instances, points, channels, groups, v)));
+    return bytes;
+}
+
+void group_norm(const NormCall& c, cudaStream_t stream) {
+    if (!c.instances) return;
+    if (!c.points) {
+        CPDE_CUDA(cudaMemsetAsync(c.mean, 0, size_t(c.instances * c.groups) * 4, stream));
+        CPDE_CUDA(cudaMemsetAsync(c.rstd, 0, size_t(c.instances * c.groups) * 4, stream));
+        return;
+    }
+    with_norm_types(c, [&](auto type, auto parameter_type, auto width) {
+        using T = typename decltype(type)::type;
+        using P = typename decltype(parameter_type)::type;
+        constexpr int V = decltype(width)::value;
+        const NormShape s = norm_call_shape<T>(c, V);
+        auto* pieces = static_cast<Moments*>(c.workspace);
+        const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
+        k_norm_moments<T, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
+            static_cast<const T*>(c.x), s, pieces);
+        CPDE_LAUNCHED();
+        k_norm_apply<T, P, V><<<dim3(unsigned(s.instances) * s.apply_splits, s.tiles), NORM_THREADS,
+                                size_t(s.pieces) * 8, stream>>>(
+            static_cast<const T*>(c.x), static_cast<const P*>(c.weight), static_cast<const P*>(c.bias),
+            static_cast<T*>(c.out), c.mean, c.rstd, pieces, s);
+        CPDE_LAUNCHED();
+    });
+}
+
+void group_norm_gradient(const NormCall& c, cudaStream_t stream) {
+    if (!c.instances || !c.points) {
+        const size_t bytes = size_t(c.channels) * bytes_of(c.parameter_type);
+        if (c.dweight) CPDE_CUDA(cudaMemsetAsync(c.dweight, 0, bytes, stream));
+        if (c.dbias) CPDE_CUDA(cudaMemsetAsync(c.dbias, 0, bytes, stream));
+        return;
+    }
+    with_norm_types(c, [&](auto type, auto parameter_type, auto width) {
+        using T = typename decltype(type)::type;
+        using P = typename decltype(parameter_type)::type;
+        constexpr int V = decltype(width)::value;
+        const NormShape s = norm_call_shape<T>(c, V);
+        auto* pieces = static_cast<float2*>(c.workspace);
+        auto* channel_sums = reinterpret_cast<float2*>(
+            static_cast<char*>(c.workspace) +
+            padded(size_t(s.instances) * s.splits * s.tiles * s.pieces * sizeof(Moments)));
+        const T *grad = static_cast<const T*>(c.grad), *x = static_cast<const T*>(c.x);
+        const P *weight = static_cast<const P*>(c.weight), *bias = static_cast<const P*>(c.bias);
+        const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
+        k_norm_sums<T, P, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
+            grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);
+        CPDE_LAUNCHED();
+        const unsigned parameter_blocks = c.dweight || c.dbias ? unsigned(s.channels + 31) / 32 : 0;
+        k_norm_input_gradient<T, P, V>
+            <<<dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
+               std::max<size_t>(size_t(s.pieces) * 8, NORM_WARPS * 32 * 8), stream>>>(
+                grad, x, c.mean, c.rstd, weight, bias, static_cast<T*>(c.out), static_cast<P*>(c.dweight),
+                static_cast<P*>(c.dbias), channel_sums, pieces, s);
+        CPDE_LAUNCHED();
+    });
+}
+
+}  // namespace cpde::ops

@@ -23,6 +23,7 @@ _lib = None
 
 # name -> (restype, argtypes); mirrors include/cpde_b200.h
 P, U64, I32, SZ = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int32, ctypes.c_size_t
+I64, F32, F64 = ctypes.c_int64, ctypes.c_float, ctypes.c_double
 PI32, PF32, PF64, PU64 = (ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_float),
                           ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_uint64))
 SIGNATURES = {
@@ -58,6 +59,15 @@ SIGNATURES = {
     'cpde_set_tier': (I32, [P, I32]),
     'cpde_jet_plan': (I32, [PI32, I32, I32, PI32, SZ, ctypes.POINTER(SZ)]),
     'cpde_layer_gradient_static': (I32, [P, P, P, I32, I32, ctypes.c_int64, I32, P, P]),
+    'cpde_embedding': (I32, [P, I32, P, I64, I64, I64, I32, P, I64, F32, I32, P, P]),
+    'cpde_embedding_gradient_workspace': (I32, [I64, I64, I64, ctypes.POINTER(SZ)]),
+    'cpde_embedding_gradient': (I32, [P, I32, P, I64, I32, P, I64, I64, I64, F32, I32, P, P, SZ, P]),
+    'cpde_dropout': (I32, [P, I32, P, I64, P, I64, I64, I64, F64, U64, U64, P, P]),
+    'cpde_group_norm_workspace': (I32, [I64, I64, I64, I64, ctypes.POINTER(SZ)]),
+    'cpde_group_norm': (I32, [P, I32, P, I64, I64, I64, I64, I64, I64, I32, P, P, F64, I32, P, F64, U64, U64, P, P, P,
+                              P, SZ, P]),
+    'cpde_group_norm_gradient': (I32, [P, I32, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I32, P, P, I32, P,
+                                       F64, U64, U64, P, P, P, P, SZ, P]),
 }
 
 
@@ -149,6 +159,7 @@ class Engine:
 
     def __init__(self, device=0, rank=0, world=1, unique_id=None):
         self.lib = load()
+        self.device = device
         handle = ctypes.c_void_p()
         if world > 1:
             uid = ctypes.create_string_buffer(bytes(unique_id), 128)

@@ -178,6 +178,82 @@ int cpde_set_tier(cpde_engine* engine, int32_t tier);
 int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float* activations, int32_t outputs,
                                int32_t inputs, int64_t points, int32_t rows, float* gradient, void* stream);
 
+/* --- Operators on caller-owned device arrays (no reference counterpart) ---
+ *
+ * Embedding lookup, dropout and group norm with their gradients, for networks
+ * that condition the point networks above (a latent code per instance, features
+ * per cell, normalised and regularised trunk layers).
+ *  - All arrays are device memory of the engine's device, aligned to their
+ *    element type; 16-byte aligned addresses and strides take the fast kernels.
+ *    Strides are in elements. Outputs are contiguous and do not overlap inputs.
+ *  - Nothing is allocated and nothing is kept between calls. Where a workspace
+ *    is asked for, it is 256-byte aligned device memory of at least the queried
+ *    size, contents undefined, that no other call in flight uses.
+ *  - Calls are asynchronous on `stream` (NULL: the engine's stream) and may be
+ *    captured into a CUDA graph. Results do not depend on the order in which
+ *    blocks run: equal inputs give equal bits.
+ *  - Computation and sums are in FP32, rounded once to the output's type. */
+#define CPDE_F32 0
+#define CPDE_BF16 1
+#define CPDE_F16 2
+#define CPDE_I32 0
+#define CPDE_I64 1
+
+/* out[t,:] = scale * table[ids[t],:] for `tokens` ids of type `id_type`. An id
+ * outside [0, rows) is absent: its row of `out` is zero. `out_type` equals
+ * `table_type`, or is a 16-bit type for an FP32 table. rows and tokens below
+ * 2^31 - 1, channels up to 2^24. */
+int cpde_embedding(cpde_engine* engine, int32_t table_type, const void* table, int64_t table_stride, int64_t rows,
+                   int64_t channels, int32_t id_type, const void* ids, int64_t tokens, float scale, int32_t out_type,
+                   void* out, void* stream);
+/* out[r,:] = scale * (sum of grad[t,:] over the tokens t with ids[t] == r), for
+ * every row of the table (rows that no token names are zeros); absent ids add
+ * nothing. The tokens are sorted by row and each row's are added in an order
+ * that depends on the ids alone. `out_type` equals `grad_type` or is CPDE_F32. */
+int cpde_embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channels, size_t* bytes);
+int cpde_embedding_gradient(cpde_engine* engine, int32_t grad_type, const void* grad, int64_t grad_stride,
+                            int32_t id_type, const void* ids, int64_t tokens, int64_t rows, int64_t channels,
+                            float scale, int32_t out_type, void* out, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* y = residual + drop(x) over a rows x columns array (`residual` may be NULL).
+ * The mask is a function of (seed, offset, element index row * columns +
+ * column) alone and is never stored: element i takes 16 bits of Philox4x32-10
+ * with key `seed` and counter (i / 8, offset), halfword i % 8 counted from the
+ * low end, and is kept when they are >= T = round(65536 * rate). Kept elements are
+ * scaled by 65536 / (65536 - T); the others are zeros, whatever x holds there.
+ * The gradient is the same map of the gradient, without residual. A captured
+ * call replays the same mask. */
+int cpde_dropout(cpde_engine* engine, int32_t type, const void* x, int64_t x_stride, const void* residual,
+                 int64_t residual_stride, int64_t rows, int64_t columns, double rate, uint64_t seed, uint64_t offset,
+                 void* y, void* stream);
+
+/* Group norm over (instance, point, channel) arrays, channels last: mean and
+ * biased variance over the points of an instance and the channels of a group,
+ * y = drop(act(w (x - mean) rstd + b)), rstd = 1 / sqrt(var + eps). `activation`
+ * counts as the layers' flags do: 0 sigmoid, 1 linear, 2 tanh, and 3 SiLU.
+ * `weight` and `bias` (channels, either may be NULL) are FP32 or of x's type.
+ * `lengths` (int32, NULL: all points) limits instance n to its first
+ * clamp(lengths[n], 0, points) points: the others are not read and y is zero
+ * there; an instance without points has mean = rstd = 0. `rate`, `seed` and
+ * `offset` are those of cpde_dropout over y's elements. mean and rstd are FP32
+ * (instances x groups). The group count divides channels. */
+int cpde_group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, size_t* bytes);
+int cpde_group_norm(cpde_engine* engine, int32_t type, const void* x, int64_t x_point_stride,
+                    int64_t x_instance_stride, int64_t instances, int64_t points, int64_t channels, int64_t groups,
+                    int32_t parameter_type, const void* weight, const void* bias, double eps, int32_t activation,
+                    const int32_t* lengths, double rate, uint64_t seed, uint64_t offset, void* y, float* mean,
+                    float* rstd, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradient: dx (contiguous), and dweight and dbias (either may be NULL) of
+ * the parameter type, from the forward's inputs, mean and rstd. */
+int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad, int64_t grad_point_stride,
+                             int64_t grad_instance_stride, const void* x, int64_t x_point_stride,
+                             int64_t x_instance_stride, const float* mean, const float* rstd, int64_t instances,
+                             int64_t points, int64_t channels, int64_t groups, int32_t parameter_type,
+                             const void* weight, const void* bias, int32_t activation, const int32_t* lengths,
+                             double rate, uint64_t seed, uint64_t offset, void* dx, void* dweight, void* dbias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* Host-only schema compiler (no device needed): Leibniz jet tables for the
  * given rows x variables count matrix, packed as documented in schema.hpp. */
 int cpde_jet_plan(const int32_t* counts, int32_t rows, int32_t variables, int32_t* packed, size_t capacity,
