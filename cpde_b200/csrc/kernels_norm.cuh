@@ -43,7 +43,15 @@ __device__ __forceinline__ int32_t length_of(const NormShape& s, int32_t n) {
     return l < 0 ? 0 : l < s.points ? l : s.points;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __frcp_rn(1.0f + __expf(-z)); }
+// 1 / (1 + e^-z) from the special function unit's exponential and reciprocal
+// (a few 2^-23 off): an IEEE reciprocal alone would take as many instructions
+// as the rest of an element.
+__device__ __forceinline__ float sigmoid(float z) {
+    float e, f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.0f + e));
+    return f;
+}
 
 template <int V>
 __device__ __forceinline__ void activate(float (&z)[V], int32_t activation) {
@@ -187,16 +195,29 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(const T* __restri
     }
 }
 
-// Per-channel terms of a thread's vector.
-template <int V>
+// Terms of a thread's vector by channel; ONE: its channels are of one group, so
+// that the statistics are two registers and not 2 V.
+template <int V, bool ONE>
 struct Terms {
-    float mean[V], rstd[V], weight[V], bias[V];
+    static constexpr int M = ONE ? 1 : V;
+    float mean[M], rstd[M], weight[V], bias[V];
+    __device__ __forceinline__ float mean_of(int j) const { return mean[ONE ? 0 : j]; }
+    __device__ __forceinline__ float rstd_of(int j) const { return rstd[ONE ? 0 : j]; }
 };
+
+// drop(act((f - mean) weight + bias)), with rstd in the weight.
+template <int V, bool ONE>
+__device__ __forceinline__ void norm_value(float (&f)[V], const Terms<V, ONE>& k, uint64_t at, const NormShape& s) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = fmaf(f[j] - k.mean_of(j), k.weight[j], k.bias[j]);
+    activate<V>(f, s.activation);
+    if (s.rule.threshold) drop_at<V>(f, at, s.rule);
+}
 
 // y = drop(act(norm(x))). The block first joins the moments of its groups'
 // pieces; the first split of the tile that holds a group's first channel also
 // writes mean and rstd.
-template <class T, class P, int V>
+template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict__ x, const P* __restrict__ weight,
                                                               const P* __restrict__ bias, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd,
@@ -232,11 +253,11 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
     const int32_t ty = threadIdx.x / s.tile, tx = threadIdx.x % s.tile;
     if (ty >= ys || tx * V >= t.count) return;
     const int32_t channel = t.first + tx * V;
-    Terms<V> k;
+    Terms<V, ONE> k;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int32_t g = (channel + j) / s.width - t.group;
-        k.mean[j] = norm_shared[2 * g];
+        if (!ONE || j == 0) k.mean[j] = norm_shared[2 * g];
         k.weight[j] = parameter(weight, channel + j, 1.0f) * norm_shared[2 * g + 1];
         k.bias[j] = parameter(bias, channel + j, 0.0f);
     }
@@ -244,8 +265,9 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
     split_range(s.points, split, s.apply_splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
     const int64_t row = int64_t(n) * s.points;
-#pragma unroll 2
-    for (int32_t p = lo + ty; p < hi; p += ys) {
+    // From the back: the moments' pass has left the ends of the ranges in L2.
+#pragma unroll 4
+    for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
         const int64_t at = (row + p) * s.channels + channel;
         if (p >= length) {
             store<T, V>(y + at, zeros<T, V>());
@@ -253,38 +275,37 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
         }
         float f[V];
         unpack<T, V>(load<T, V>(from + p * s.x_point), f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = fmaf(f[j] - k.mean[j], k.weight[j], k.bias[j]);
-        activate<V>(f, s.activation);
-        if (s.rule.threshold) drop_at<V>(f, uint64_t(at), s.rule);
+        norm_value<V, ONE>(f, k, uint64_t(at), s);
         store<T, V>(y + at, pack<T, V>(f));
     }
 }
 
 // xhat and h of a thread's vector at one point.
-template <class T, int V>
-__device__ __forceinline__ void norm_adjoint(const Vector<T, V>& vx, const Vector<T, V>& vg, const Terms<V>& k,
+template <class T, int V, bool ONE>
+__device__ __forceinline__ void norm_adjoint(const Vector<T, V>& vx, const Vector<T, V>& vg, const Terms<V, ONE>& k,
                                              uint64_t at, const NormShape& s, float (&xhat)[V], float (&h)[V]) {
     float z[V];
     unpack<T, V>(vx, xhat);
     unpack<T, V>(vg, h);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        xhat[j] = (xhat[j] - k.mean[j]) * k.rstd[j];
+        xhat[j] = (xhat[j] - k.mean_of(j)) * k.rstd_of(j);
         z[j] = fmaf(xhat[j], k.weight[j], k.bias[j]);
     }
     if (s.rule.threshold) drop_at<V>(h, at, s.rule);
     activate_gradient<V>(h, z, s.activation);
 }
 
-template <class P, int V>
-__device__ __forceinline__ void load_terms(Terms<V>& k, const NormShape& s, int32_t n, int32_t channel,
+template <class P, int V, bool ONE>
+__device__ __forceinline__ void load_terms(Terms<V, ONE>& k, const NormShape& s, int32_t n, int32_t channel,
                                            const float* mean, const float* rstd, const P* weight, const P* bias) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t g = int64_t(n) * s.groups + (channel + j) / s.width;
-        k.mean[j] = mean[g];
-        k.rstd[j] = rstd[g];
+        if (!ONE || j == 0) {
+            k.mean[j] = mean[g];
+            k.rstd[j] = rstd[g];
+        }
         k.weight[j] = parameter(weight, channel + j, 1.0f);
         k.bias[j] = parameter(bias, channel + j, 0.0f);
     }
@@ -293,7 +314,7 @@ __device__ __forceinline__ void load_terms(Terms<V>& k, const NormShape& s, int3
 // Sums of h and h xhat over a block's points: per channel for dw and db
 // (channel_sums[instance][split][channel]), and times w per piece of a group
 // for dx (pieces[instance][split][tile][piece]).
-template <class T, class P, int V>
+template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict__ grad, const T* __restrict__ x,
                                                              const float* __restrict__ mean,
                                                              const float* __restrict__ rstd,
@@ -311,8 +332,8 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
     split_range(length_of(s, n), split, s.splits, lo, hi);
     if (ty < ys && tx * V < t.count) {
         const int32_t channel = t.first + tx * V;
-        Terms<V> k;
-        load_terms<P, V>(k, s, n, channel, mean, rstd, weight, bias);
+        Terms<V, ONE> k;
+        load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
         float sh[V], sx[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) sh[j] = sx[j] = 0.0f;
@@ -321,7 +342,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
 #pragma unroll 2
         for (int32_t p = lo + ty; p < hi; p += ys) {
             float xhat[V], h[V];
-            norm_adjoint<T, V>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k,
+            norm_adjoint<T, V, ONE>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k,
                                uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s, xhat, h);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -363,9 +384,37 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
     }
 }
 
+// dw and db of 32 channels: sums over the rows of channel_sums in a fixed order.
+template <class P>
+__device__ __forceinline__ void sum_parameters(P* __restrict__ dweight, P* __restrict__ dbias,
+                                               const float2* __restrict__ channel_sums, int32_t rows,
+                                               int32_t channels, int32_t block) {
+    __shared__ float2 shared[NORM_WARPS][32];
+    const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, channel = block * 32 + lane;
+    float2 sum = make_float2(0.0f, 0.0f);
+    if (channel < channels) {
+#pragma unroll 4
+        for (int32_t i = warp; i < rows; i += NORM_WARPS) {
+            const float2 v = channel_sums[int64_t(i) * channels + channel];
+            sum.x += v.x;
+            sum.y += v.y;
+        }
+    }
+    shared[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && channel < channels) {
+        for (int w = 1; w < NORM_WARPS; ++w) {
+            sum.x += shared[w][lane].x;
+            sum.y += shared[w][lane].y;
+        }
+        if (dbias) dbias[channel] = from_float<P>(sum.x);
+        if (dweight) dweight[channel] = from_float<P>(sum.y);
+    }
+}
+
 // dx, and in the blocks behind those of the last instance dw and db: 32
 // channels each, summed over instances and splits in a fixed order.
-template <class T, class P, int V>
+template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const P* __restrict__ weight, const P* __restrict__ bias, T* __restrict__ dx,
@@ -376,26 +425,9 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int32_t n = blockIdx.x / s.apply_splits;
     if (n >= s.instances) {
-        const int32_t block = blockIdx.x - s.instances * s.apply_splits;
-        const int32_t channel = block * 32 + lane;
-        if (blockIdx.y) return;
-        float2 sum = make_float2(0.0f, 0.0f);
-        if (channel < s.channels)
-            for (int32_t i = warp; i < s.instances * s.splits; i += NORM_WARPS) {
-                const float2 v = channel_sums[int64_t(i) * s.channels + channel];
-                sum.x += v.x;
-                sum.y += v.y;
-            }
-        shared[warp * 32 + lane] = sum;
-        __syncthreads();
-        if (warp == 0 && channel < s.channels) {
-            for (int w = 1; w < NORM_WARPS; ++w) {
-                sum.x += shared[w * 32 + lane].x;
-                sum.y += shared[w * 32 + lane].y;
-            }
-            if (dbias) dbias[channel] = from_float<P>(sum.x);
-            if (dweight) dweight[channel] = from_float<P>(sum.y);
-        }
+        if (blockIdx.y == 0)
+            sum_parameters<P>(dweight, dbias, channel_sums, s.instances * s.splits, s.channels,
+                              blockIdx.x - s.instances * s.apply_splits);
         return;
     }
     const int32_t split = blockIdx.x % s.apply_splits;
@@ -426,11 +458,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const int32_t ty = threadIdx.x / s.tile, tx = threadIdx.x % s.tile;
     if (ty >= ys || tx * V >= t.count) return;
     const int32_t channel = t.first + tx * V;
-    Terms<V> k;
-    load_terms<P, V>(k, s, n, channel, mean, rstd, weight, bias);
-    float m1[V], m2[V];
+    Terms<V, ONE> k;
+    load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
+    constexpr int M = Terms<V, ONE>::M;
+    float m1[M], m2[M];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int j = 0; j < M; ++j) {
         const float2 m = shared[(channel + j) / s.width - t.group];
         m1[j] = m.x;
         m2[j] = m.y;
@@ -439,18 +472,20 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     split_range(s.points, split, s.apply_splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
     const T* gfrom = grad + n * s.grad_instance + channel;
+    // From the back, as the forward.
 #pragma unroll 2
-    for (int32_t p = lo + ty; p < hi; p += ys) {
+    for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
         const int64_t at = (int64_t(n) * s.points + p) * s.channels + channel;
         if (p >= length) {
             store<T, V>(dx + at, zeros<T, V>());
             continue;
         }
         float xhat[V], h[V];
-        norm_adjoint<T, V>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k, uint64_t(at), s,
+        norm_adjoint<T, V, ONE>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k, uint64_t(at), s,
                            xhat, h);
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = (h[j] * k.weight[j] - fmaf(xhat[j], m2[j], m1[j])) * k.rstd[j];
+        for (int j = 0; j < V; ++j)
+            h[j] = (h[j] * k.weight[j] - fmaf(xhat[j], m2[ONE ? 0 : j], m1[ONE ? 0 : j])) * k.rstd_of(j);
         store<T, V>(dx + at, pack<T, V>(h));
     }
 }

@@ -9,6 +9,7 @@
 #include "kernels_dropout.cuh"
 #include "kernels_embedding.cuh"
 #include "kernels_norm.cuh"
+#include "kernels_norm_slab.cuh"
 
 namespace cpde::ops {
 namespace {
@@ -72,9 +73,15 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // --- embedding -------------------------------------------------------------
 
+// Above this many tokens a sort takes the whole GPU, two launches a pass, and
+// below it one cluster in one launch.
+constexpr int64_t CLUSTER_TOKENS = 65536;
+
 struct SortPlan {
     int passes, digit_bits;
-    uint32_t cluster;
+    uint32_t cluster;   // CTAs of the one-launch sort
+    uint32_t tiles;     // CTAs of a launch of the other (0: it is not taken)
+    uint32_t per_warp;  // its pairs of a warp
 };
 SortPlan sort_plan(int64_t tokens, int64_t rows) {
     int bits = 1;
@@ -83,6 +90,8 @@ SortPlan sort_plan(int64_t tokens, int64_t rows) {
     p.passes = (bits + 9) / 10;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
     p.cluster = std::min<uint32_t>(16, power_of_two_from((tokens + 2047) / 2048));
+    p.tiles = tokens > CLUSTER_TOKENS ? SMS : 0;
+    p.per_warp = p.tiles ? uint32_t((tokens + p.tiles * SORT_WARPS - 1) / (p.tiles * SORT_WARPS)) : 0;
     return p;
 }
 
@@ -95,10 +104,56 @@ SumShape sum_shape(int64_t tokens, int64_t rows, int64_t channels, int v) {
     s.lanes = power_of_two_from(std::min<int64_t>(s.vectors, 32));
     s.tiles = (s.vectors + s.lanes - 1) / s.lanes;
     s.chunk = 64;
-    while (s.chunk > 8 && (tokens / s.chunk) * s.tiles * s.lanes / 32 < SMS * 32) s.chunk /= 2;
+    while (s.chunk > 8 && (tokens / s.chunk) * s.tiles * s.lanes / 32 < SMS * 12) s.chunk /= 2;
     s.chunks = uint32_t((tokens + s.chunk - 1) / s.chunk);
     s.grad_stride = 0;
     return s;
+}
+
+// Sorts the tokens into buffer sorted_buffer(passes) and clears the output's words.
+template <class Id>
+void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, const SortBuffers& buffers,
+                 uint32_t* counts, int64_t fill_words, int device, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernels' limits are raised
+    if (!(ready.load() >> (device & 63) & 1)) {
+        dynamic_shared(k_sort_tokens<Id>, (size_t(SORT_WARPS) + 1) * 4096);
+        dynamic_shared(k_place_tokens<Id>, size_t(SORT_WARPS) * 4096);
+        CPDE_CUDA(cudaFuncSetAttribute(k_sort_tokens<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready.fetch_or(uint64_t(1) << (device & 63));
+    }
+    uint4* fill = static_cast<uint4*>(c.out);
+    if (plan.tiles) {
+        SortPass s = {uint32_t(c.tokens), plan.per_warp, 1u << plan.digit_bits, 0, 0, 0};
+        const int launches = 2 * plan.passes;
+        for (int launch = 0; launch < launches; ++launch) {
+            const int pass = launch / 2, from = (pass + 1) & 1, to = pass & 1;
+            const SortInput<Id> in = {ids, c.rows, pass ? buffers.row[from] : nullptr, buffers.token[from]};
+            s.shift = pass * plan.digit_bits;
+            s.fill_from = fill_words * launch / launches;
+            s.fill_to = fill_words * (launch + 1) / launches;
+            if (launch % 2 == 0)
+                k_count_digits<Id><<<plan.tiles, SORT_THREADS, s.bins * 4, stream>>>(in, s, counts, fill);
+            else
+                k_place_tokens<Id><<<plan.tiles, SORT_THREADS, size_t(SORT_WARPS) * s.bins * 4, stream>>>(
+                    in, s, counts, buffers.row[to], buffers.token[to], fill);
+            CPDE_LAUNCHED();
+        }
+        return;
+    }
+    const int64_t fillers = std::min<int64_t>(112, (fill_words + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(plan.cluster + (fillers + plan.cluster - 1) / plan.cluster * plan.cluster));
+    config.blockDim = dim3(SORT_THREADS);
+    config.dynamicSmemBytes = (size_t(SORT_WARPS) + 1) * (size_t(4) << plan.digit_bits);
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = plan.cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    CPDE_CUDA(cudaLaunchKernelEx(&config, k_sort_tokens<Id>, ids, uint32_t(c.tokens), c.rows, plan.passes,
+                                 plan.digit_bits, buffers, fill, fill_words));
 }
 
 }  // namespace
@@ -140,7 +195,8 @@ size_t embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channe
     for (int v : {8, 4, 2, 1})
         if (channels % v == 0)
             partials = std::max(partials, size_t(sum_shape(tokens, rows, channels, v).chunks) * 2 * channels);
-    return 4 * padded(size_t(tokens) * 4) + padded(partials * 4);
+    const SortPlan plan = sort_plan(tokens, rows);
+    return 4 * padded(size_t(tokens) * 4) + padded(partials * 4) + padded((size_t(plan.tiles) << plan.digit_bits) * 4);
 }
 
 void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream) {
@@ -156,35 +212,12 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
         buffers.row[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
         buffers.token[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
     }
-    float* partial = reinterpret_cast<float*>(at);
-
     const SortPlan plan = sort_plan(c.tokens, c.rows);
+    uint32_t* counts = reinterpret_cast<uint32_t*>(take((size_t(plan.tiles) << plan.digit_bits) * 4));
+    float* partial = reinterpret_cast<float*>(at);
     const int64_t fill_words = words ? int64_t(out_bytes / 16) : 0;
-    const int64_t fillers = std::min<int64_t>(112, (fill_words + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
-    const size_t shared = (size_t(SORT_WARPS) + 1) * (size_t(4) << plan.digit_bits);
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(plan.cluster + (fillers + plan.cluster - 1) / plan.cluster * plan.cluster));
-    config.blockDim = dim3(SORT_THREADS);
-    config.dynamicSmemBytes = shared;
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = plan.cluster;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    auto sort = [&](auto kernel, auto* ids) {
-        static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limits are raised
-        if (!(ready.load() >> (device & 63) & 1)) {
-            dynamic_shared(kernel, (size_t(SORT_WARPS) + 1) * 4096);
-            CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            ready.fetch_or(uint64_t(1) << (device & 63));
-        }
-        CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, ids, uint32_t(c.tokens), c.rows, plan.passes, plan.digit_bits,
-                                     buffers, static_cast<uint4*>(c.out), fill_words));
-    };
-    if (c.id_type) sort(k_sort_tokens<int64_t>, static_cast<const int64_t*>(c.ids));
-    else sort(k_sort_tokens<int32_t>, static_cast<const int32_t*>(c.ids));
+    if (c.id_type) sort_tokens(c, static_cast<const int64_t*>(c.ids), plan, buffers, counts, fill_words, device, stream);
+    else sort_tokens(c, static_cast<const int32_t*>(c.ids), plan, buffers, counts, fill_words, device, stream);
 
     const uint32_t* row = buffers.row[sorted_buffer(plan.passes)];
     const uint32_t* token = buffers.token[sorted_buffer(plan.passes)];
@@ -203,9 +236,8 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
                     row, token, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), partial, s, c.scale);
                 CPDE_LAUNCHED();
                 if (s.chunks > 1) {
-                    const uint32_t x = power_of_two_from(std::min<int64_t>(c.channels, 256));
-                    k_join_chunks<TO><<<s.chunks - 1, dim3(x, 256 / x), 0, stream>>>(
-                        row, static_cast<TO*>(c.out), partial, s, c.scale);
+                    k_join_chunks<TO, V><<<dim3((s.chunks + JOIN_WARPS - 2) / JOIN_WARPS, s.tiles), JOIN_WARPS * 32, 0,
+                                           stream>>>(row, static_cast<TO*>(c.out), partial, s, c.scale);
                     CPDE_LAUNCHED();
                 }
             }
@@ -275,10 +307,8 @@ size_t norm_workspace(const NormShape& s) {
     return padded(blocks * s.tiles * s.pieces * sizeof(Moments)) + padded(blocks * s.channels * sizeof(float2));
 }
 
-// V and the strides, lengths and dropout of a call.
-template <class T>
-NormShape norm_call_shape(const NormCall& c, int v) {
-    NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, v);
+// Strides, lengths and dropout of a call.
+void add_call(NormShape& s, const NormCall& c) {
     s.x_point = c.x_point;
     s.x_instance = c.x_instance;
     s.grad_point = c.grad_point;
@@ -287,25 +317,110 @@ NormShape norm_call_shape(const NormCall& c, int v) {
     s.eps = float(c.eps);
     s.lengths = c.lengths;
     s.rule = dropout_rule(c.rate, c.seed, c.offset);
-    return s;
 }
 
+// How a cluster holds one instance's points in a tile of whole groups.
+struct SlabPlan {
+    int32_t cluster = 0;  // CTAs; 0: it does not hold them
+    int32_t tile, tiles;  // vectors of a tile, tiles
+    int32_t slots;        // vectors of a thread, and array
+    size_t shared;
+};
+constexpr size_t SLAB_TILE_BYTES = 128;                    // of a point, at least: whole lines of memory
+constexpr size_t SLAB_THREE = 72 << 10, SLAB_TWO = 108 << 10, SLAB_ONE = 220 << 10;  // shared memory of a CTA
+
+// Vectors of at most 16 bytes (a copy's most) whose channels are of one group.
+int slab_vector(int fit, size_t element, int64_t width) {
+    int v = std::min<int>(fit, int(16 / element));
+    while (v > 1 && width % v) v /= 2;
+    return v;
+}
+
+SlabPlan slab_plan(const NormShape& s, int v, size_t element, int arrays) {
+    SlabPlan p;
+    const size_t vector_bytes = v * element;
+    const int64_t group = s.width / v, groups = s.groups;
+    int64_t tile_groups = std::max<int64_t>(1, int64_t(SLAB_TILE_BYTES / vector_bytes) / group);
+    tile_groups = std::min(tile_groups, groups);
+    p.tile = int32_t(tile_groups * group);
+    if (p.tile > NORM_THREADS) return p;
+    p.tiles = int32_t((groups + tile_groups - 1) / tile_groups);
+    const int64_t ys = NORM_THREADS / p.tile;
+    auto plan = [&](int32_t cluster) {
+        const int64_t points = (int64_t(s.points) + cluster - 1) / cluster;
+        const int64_t slots = (points + ys - 1) / ys;
+        p.slots = int32_t(std::min<int64_t>(slots, 1 << 16));
+        const int64_t width = int64_t(p.tile) * v, rows = slab_rows_are_warps(p.tile) ? NORM_WARPS : ys;
+        p.shared = size_t(p.slots) * NORM_THREADS * vector_bytes * arrays +
+                   (arrays == 1 ? sizeof(SlabMoments) : size_t((rows + 2) * width + tile_groups) * sizeof(float2));
+        return p.shared;
+    };
+    int32_t cluster = 0;
+    for (size_t limit : {SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
+        for (int32_t c = 1; c <= 16 && !cluster; c *= 2)
+            if (plan(c) <= limit) cluster = c;
+        if (cluster) break;
+    }
+    if (!cluster) return p;
+    // Few instances: smaller shares, for more of the GPU.
+    while (cluster < 16 && int64_t(s.instances) * p.tiles * cluster < 2 * SMS && (plan(cluster), p.slots >= 4))
+        cluster *= 2;
+    plan(cluster);
+    p.cluster = cluster;
+    return p;
+}
+
+template <auto kernel, class... A>
+void launch_slab(const SlabPlan& plan, int64_t instances, int device, cudaStream_t stream, A... arguments) {
+    static std::atomic<uint64_t> ready{0};  // devices on which this kernel's limits are raised
+    if (!(ready.load() >> (device & 63) & 1)) {
+        dynamic_shared(kernel, SLAB_ONE);
+        CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready.fetch_or(uint64_t(1) << (device & 63));
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(instances * plan.tiles * plan.cluster));
+    config.blockDim = dim3(NORM_THREADS);
+    config.dynamicSmemBytes = plan.shared;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = plan.cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, arguments...));
+}
+
+// The widest vectors that the call's addresses and strides allow.
+template <class T>
+int norm_vector(const NormCall& c) {
+    Alignment a;
+    a.at(c.x, sizeof(T)).at(c.out, sizeof(T)).stride(c.x_point).stride(c.channels);
+    if (c.instances > 1) a.stride(c.x_instance);
+    if (c.grad) {
+        a.at(c.grad, sizeof(T)).stride(c.grad_point);
+        if (c.instances > 1) a.stride(c.grad_instance);
+    }
+    return a.vector(8);
+}
+
+// Calls f with the types of the array and of the parameters.
 template <class F>
 void with_norm_types(const NormCall& c, F&& f) {
     with_type(c.type, [&](auto tag) {
-        using T = typename decltype(tag)::type;
-        Alignment a;
-        a.at(c.x, sizeof(T)).at(c.out, sizeof(T)).stride(c.x_point).stride(c.channels);
-        if (c.instances > 1) a.stride(c.x_instance);
-        if (c.grad) {
-            a.at(c.grad, sizeof(T)).stride(c.grad_point);
-            if (c.instances > 1) a.stride(c.grad_instance);
-        }
-        const int fit = a.vector(8);
-        with_vector<8, 4, 1>(fit == 2 ? 1 : fit, [&](auto width) {
-            if (c.parameter_type == F32) f(tag, Tag<float>{}, width);
-            else f(tag, tag, width);
-        });
+        if (c.parameter_type == F32) f(tag, Tag<float>{});
+        else f(tag, tag);
+    });
+}
+
+// Calls f with the vector width, one of 8, 4 and 1, and whether a vector's
+// channels are of one group.
+template <class F>
+void with_norm_vector(int v, int64_t width, F&& f) {
+    with_vector<8, 4, 1>(v == 2 ? 1 : v, [&](auto w) {
+        if (width % decltype(w)::value == 0) f(w, std::true_type{});
+        else if constexpr (decltype(w)::value > 1) f(w, std::false_type{});
     });
 }
 
@@ -319,60 +434,110 @@ size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels,
     return bytes;
 }
 
-void group_norm(const NormCall& c, cudaStream_t stream) {
+void group_norm(const NormCall& c, int device, cudaStream_t stream) {
     if (!c.instances) return;
     if (!c.points) {
         CPDE_CUDA(cudaMemsetAsync(c.mean, 0, size_t(c.instances * c.groups) * 4, stream));
         CPDE_CUDA(cudaMemsetAsync(c.rstd, 0, size_t(c.instances * c.groups) * 4, stream));
         return;
     }
-    with_norm_types(c, [&](auto type, auto parameter_type, auto width) {
+    with_norm_types(c, [&](auto type, auto parameter_type) {
         using T = typename decltype(type)::type;
         using P = typename decltype(parameter_type)::type;
-        constexpr int V = decltype(width)::value;
-        const NormShape s = norm_call_shape<T>(c, V);
-        auto* pieces = static_cast<Moments*>(c.workspace);
-        const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
-        k_norm_moments<T, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
-            static_cast<const T*>(c.x), s, pieces);
-        CPDE_LAUNCHED();
-        k_norm_apply<T, P, V><<<dim3(unsigned(s.instances) * s.apply_splits, s.tiles), NORM_THREADS,
-                                size_t(s.pieces) * 8, stream>>>(
-            static_cast<const T*>(c.x), static_cast<const P*>(c.weight), static_cast<const P*>(c.bias),
-            static_cast<T*>(c.out), c.mean, c.rstd, pieces, s);
-        CPDE_LAUNCHED();
+        const T* x = static_cast<const T*>(c.x);
+        const P *weight = static_cast<const P*>(c.weight), *bias = static_cast<const P*>(c.bias);
+        T* y = static_cast<T*>(c.out);
+        const int fit = norm_vector<T>(c);
+        bool done = false;
+        with_vector<8, 4>(slab_vector(fit, sizeof(T), c.channels / c.groups), [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            if constexpr (V * sizeof(T) <= 16) {
+                NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+                const SlabPlan plan = slab_plan(s, V, sizeof(T), 1);
+                if (!plan.cluster) return;
+                add_call(s, c);
+                s.tile = plan.tile;
+                s.tiles = plan.tiles;
+                launch_slab<k_norm_slab<T, P, V>>(plan, s.instances, device, stream, x, weight, bias, y, c.mean, c.rstd,
+                            s, plan.slots);
+                done = true;
+            }
+        });
+        if (done) return;
+        with_norm_vector(fit, c.channels / c.groups, [&](auto width, auto one) {
+            constexpr int V = decltype(width)::value;
+            NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+            add_call(s, c);
+            auto* pieces = static_cast<Moments*>(c.workspace);
+            const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
+            k_norm_moments<T, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
+                x, s, pieces);
+            CPDE_LAUNCHED();
+            k_norm_apply<T, P, V, decltype(one)::value>
+                <<<dim3(unsigned(s.instances) * s.apply_splits, s.tiles), NORM_THREADS, size_t(s.pieces) * 8, stream>>>(
+                    x, weight, bias, y, c.mean, c.rstd, pieces, s);
+            CPDE_LAUNCHED();
+        });
     });
 }
 
-void group_norm_gradient(const NormCall& c, cudaStream_t stream) {
+void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
     if (!c.instances || !c.points) {
         const size_t bytes = size_t(c.channels) * bytes_of(c.parameter_type);
         if (c.dweight) CPDE_CUDA(cudaMemsetAsync(c.dweight, 0, bytes, stream));
         if (c.dbias) CPDE_CUDA(cudaMemsetAsync(c.dbias, 0, bytes, stream));
         return;
     }
-    with_norm_types(c, [&](auto type, auto parameter_type, auto width) {
+    with_norm_types(c, [&](auto type, auto parameter_type) {
         using T = typename decltype(type)::type;
         using P = typename decltype(parameter_type)::type;
-        constexpr int V = decltype(width)::value;
-        const NormShape s = norm_call_shape<T>(c, V);
-        auto* pieces = static_cast<float2*>(c.workspace);
-        auto* channel_sums = reinterpret_cast<float2*>(
-            static_cast<char*>(c.workspace) +
-            padded(size_t(s.instances) * s.splits * s.tiles * s.pieces * sizeof(Moments)));
         const T *grad = static_cast<const T*>(c.grad), *x = static_cast<const T*>(c.x);
         const P *weight = static_cast<const P*>(c.weight), *bias = static_cast<const P*>(c.bias);
-        const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
-        k_norm_sums<T, P, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
-            grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);
-        CPDE_LAUNCHED();
-        const unsigned parameter_blocks = c.dweight || c.dbias ? unsigned(s.channels + 31) / 32 : 0;
-        k_norm_input_gradient<T, P, V>
-            <<<dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
-               std::max<size_t>(size_t(s.pieces) * 8, NORM_WARPS * 32 * 8), stream>>>(
-                grad, x, c.mean, c.rstd, weight, bias, static_cast<T*>(c.out), static_cast<P*>(c.dweight),
-                static_cast<P*>(c.dbias), channel_sums, pieces, s);
-        CPDE_LAUNCHED();
+        T* dx = static_cast<T*>(c.out);
+        P *dweight = static_cast<P*>(c.dweight), *dbias = static_cast<P*>(c.dbias);
+        const unsigned parameter_blocks = dweight || dbias ? unsigned(c.channels + 31) / 32 : 0;
+        const int fit = norm_vector<T>(c);
+        bool done = false;
+        with_vector<8, 4>(slab_vector(fit, sizeof(T), c.channels / c.groups), [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            if constexpr (V * sizeof(T) <= 16) {
+                NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+                const SlabPlan plan = slab_plan(s, V, sizeof(T), 2);
+                if (!plan.cluster) return;
+                add_call(s, c);
+                s.tile = plan.tile;
+                s.tiles = plan.tiles;
+                auto* channel_sums = static_cast<float2*>(c.workspace);
+                launch_slab<k_norm_slab_gradient<T, P, V>>(plan, s.instances, device, stream, grad, x, c.mean, c.rstd,
+                            weight, bias, dx, channel_sums, s, plan.slots);
+                if (parameter_blocks) {
+                    k_norm_parameters<P><<<parameter_blocks, NORM_THREADS, 0, stream>>>(dweight, dbias, channel_sums,
+                                                                                         s.instances, s.channels);
+                    CPDE_LAUNCHED();
+                }
+                done = true;
+            }
+        });
+        if (done) return;
+        with_norm_vector(fit, c.channels / c.groups, [&](auto width, auto one) {
+            constexpr int V = decltype(width)::value;
+            constexpr bool ONE = decltype(one)::value;
+            NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+            add_call(s, c);
+            auto* pieces = static_cast<float2*>(c.workspace);
+            auto* channel_sums = reinterpret_cast<float2*>(
+                static_cast<char*>(c.workspace) +
+                padded(size_t(s.instances) * s.splits * s.tiles * s.pieces * sizeof(Moments)));
+            const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
+            k_norm_sums<T, P, V, ONE><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
+                grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);
+            CPDE_LAUNCHED();
+            k_norm_input_gradient<T, P, V, ONE>
+                <<<dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
+                   size_t(s.pieces) * 8, stream>>>(grad, x, c.mean, c.rstd, weight, bias, dx, dweight, dbias,
+                                                    channel_sums, pieces, s);
+            CPDE_LAUNCHED();
+        });
     });
 }
 

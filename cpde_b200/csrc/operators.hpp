@@ -54,7 +54,7 @@ struct NormCall {
     void* workspace;
 };
 size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups);
-void group_norm(const NormCall& call, cudaStream_t stream);
-void group_norm_gradient(const NormCall& call, cudaStream_t stream);
+void group_norm(const NormCall& call, int device, cudaStream_t stream);
+void group_norm_gradient(const NormCall& call, int device, cudaStream_t stream);
 
 }  // namespace cpde::ops

@@ -7,7 +7,7 @@ namespace {
 using cpde::require;
 
 constexpr int64_t kMostIndexed = (int64_t(1) << 31) - 2;
-constexpr int64_t kMostChannels = int64_t(1) << 24;
+constexpr int64_t kMostChannels = int64_t(1) << 20;
 
 size_t type_bytes(int32_t type) {
     require(type == CPDE_F32 || type == CPDE_BF16 || type == CPDE_F16, "element type must be 0 (f32), 1 (bf16) or 2 (f16)");
@@ -27,7 +27,7 @@ void check_ids(int32_t id_type, const void* ids, int64_t tokens) {
 void check_embedding(int64_t tokens, int64_t rows, int64_t channels) {
     require(rows > 0 && rows <= kMostIndexed && tokens >= 0 && tokens <= kMostIndexed,
             "rows must be positive, tokens not negative, and both below 2^31 - 1");
-    require(channels > 0 && channels <= kMostChannels, "channels must be between 1 and 2^24");
+    require(channels > 0 && channels <= kMostChannels, "channels must be between 1 and 2^20");
 }
 
 void check_dropout(double rate) { require(rate >= 0 && rate <= 1, "the dropout rate must be between 0 and 1"); }
@@ -35,7 +35,7 @@ void check_dropout(double rate) { require(rate >= 0 && rate <= 1, "the dropout r
 void check_norm(int64_t instances, int64_t points, int64_t channels, int64_t groups) {
     require(instances >= 0 && points >= 0 && points <= kMostIndexed,
             "instances and points must not be negative, points below 2^31 - 1");
-    require(channels > 0 && channels <= kMostChannels, "channels must be between 1 and 2^24");
+    require(channels > 0 && channels <= kMostChannels, "channels must be between 1 and 2^20");
     require(groups > 0 && channels % groups == 0, "the group count must divide the channels");
     require(instances <= (int64_t(1) << 20), "instances must be at most 2^20");
 }
@@ -173,7 +173,7 @@ int cpde_group_norm(cpde_engine* h, int32_t type, const void* x, int64_t x_point
         if (instances && points)
             check_workspace(workspace, workspace_bytes,
                             cpde::ops::group_norm_workspace(instances, points, channels, groups));
-        cpde::ops::group_norm(c, stream_of(h, stream));
+        cpde::ops::group_norm(c, h->engine->device, stream_of(h, stream));
     });
 }
 
@@ -205,7 +205,7 @@ int cpde_group_norm_gradient(cpde_engine* h, int32_t type, const void* grad, int
             check_workspace(workspace, workspace_bytes,
                             cpde::ops::group_norm_workspace(instances, points, channels, groups));
         }
-        cpde::ops::group_norm_gradient(c, stream_of(h, stream));
+        cpde::ops::group_norm_gradient(c, h->engine->device, stream_of(h, stream));
     });
 }
 

@@ -202,7 +202,7 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
 /* out[t,:] = scale * table[ids[t],:] for `tokens` ids of type `id_type`. An id
  * outside [0, rows) is absent: its row of `out` is zero. `out_type` equals
  * `table_type`, or is a 16-bit type for an FP32 table. rows and tokens below
- * 2^31 - 1, channels up to 2^24. */
+ * 2^31 - 1, channels up to 2^20. */
 int cpde_embedding(cpde_engine* engine, int32_t table_type, const void* table, int64_t table_stride, int64_t rows,
                    int64_t channels, int32_t id_type, const void* ids, int64_t tokens, float scale, int32_t out_type,
                    void* out, void* stream);
