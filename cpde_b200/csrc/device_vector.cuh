@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 namespace cpde::ops {
 
@@ -70,6 +72,74 @@ __device__ __forceinline__ Vector<T, V> zeros() {
     Vector<T, V> v;
     memset(&v, 0, sizeof(v));
     return v;
+}
+
+// V values as pairs for the packed FP32 instructions (two operations an issue
+// slot); V = 1 leaves the second of its pair at zero.
+template <int V>
+struct Pairs {
+    static constexpr int N = (V + 1) / 2;
+    float2 p[N];
+    __device__ __forceinline__ float get(int j) const { return j % 2 ? p[j / 2].y : p[j / 2].x; }
+    __device__ __forceinline__ void set(int j, float v) { (j % 2 ? p[j / 2].y : p[j / 2].x) = v; }
+    __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = make_float2(v, v);
+    }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+template <class T, int V>
+__device__ __forceinline__ Pairs<V> unpack_pairs(const Vector<T, V>& v) {
+    Pairs<V> f;
+    if constexpr (V == 1) {
+        float e[1];
+        unpack<T, 1>(v, e);
+        f.p[0] = make_float2(e[0], 0.0f);
+    } else if constexpr (sizeof(T) == 4) {
+        memcpy(&f, &v, sizeof(f));
+    } else {
+        uint32_t w[V / 2];
+        memcpy(w, &v, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                f.p[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            } else {
+                __half2 h;
+                memcpy(&h, &w[i], 4);
+                f.p[i] = __half22float2(h);
+            }
+        }
+    }
+    return f;
+}
+
+template <class T, int V>
+__device__ __forceinline__ Vector<T, V> pack_pairs(const Pairs<V>& f) {
+    if constexpr (V == 1) {
+        const float e[1] = {f.p[0].x};
+        return pack<T, 1>(e);
+    } else {
+        Vector<T, V> v;
+        if constexpr (sizeof(T) == 4) {
+            memcpy(&v, &f, sizeof(v));
+        } else {
+            uint32_t w[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                    const __nv_bfloat162 h = __float22bfloat162_rn(f.p[i]);
+                    memcpy(&w[i], &h, 4);
+                } else {
+                    const __half2 h = __float22half2_rn(f.p[i]);
+                    memcpy(&w[i], &h, 4);
+                }
+            }
+            memcpy(&v, w, sizeof(v));
+        }
+        return v;
+    }
 }
 
 // Quotient of 31-bit integers by a divisor that is fixed for the launch

@@ -5,25 +5,6 @@
 
 namespace cpde::ops {
 
-// Philox4x32-10 (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw, "Parallel
-// random numbers: as easy as 1, 2, 3", SC 2011): ten rounds of two 32x32-bit
-// products over a 128-bit counter under a 64-bit key.
-__device__ __forceinline__ uint4 philox(uint64_t index, uint64_t offset, uint64_t seed) {
-    uint32_t c0 = uint32_t(index), c1 = uint32_t(index >> 32), c2 = uint32_t(offset), c3 = uint32_t(offset >> 32);
-    uint32_t k0 = uint32_t(seed), k1 = uint32_t(seed >> 32);
-#pragma unroll
-    for (int round = 0; round < 10; ++round) {
-        const uint64_t a = uint64_t(c0) * 0xD2511F53u, b = uint64_t(c2) * 0xCD9E8D57u;
-        c0 = uint32_t(b >> 32) ^ c1 ^ k0;
-        c1 = uint32_t(b);
-        c2 = uint32_t(a >> 32) ^ c3 ^ k1;
-        c3 = uint32_t(a);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-    return make_uint4(c0, c1, c2, c3);
-}
-
 // Which elements stay. Element i takes 16 of the 128 bits of counter i / 8
 // (word (i % 8) / 2, low half first) and stays when they are >= threshold =
 // round(65536 rate). 16 bits an element halve the integer work of 32: at 32 the
@@ -31,33 +12,73 @@ __device__ __forceinline__ uint4 philox(uint64_t index, uint64_t offset, uint64_
 // multiple of 1/65536, and `factor` is the exact inverse of that rate's keep
 // probability, so expectations are kept.
 struct DropoutRule {
-    uint64_t seed, offset;
+    uint64_t offset;
+    uint32_t key[20];    // the rounds' keys, from the seed: constants of the launch
     uint32_t threshold;  // 0: nothing is dropped
     float factor;
 };
 
-// Elements V * j .. V * j + V - 1 of the eight that `bits` decides (V <= 8).
-template <int V>
-__device__ __forceinline__ void drop(float (&f)[V], const uint4& bits, uint32_t first, const DropoutRule& rule) {
-    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        uint32_t w;
-        if constexpr (V == 8) {
-            w = word[i / 2];
-        } else {
-            const uint32_t at = (first + i) >> 1;
-            w = at == 0 ? word[0] : at == 1 ? word[1] : at == 2 ? word[2] : word[3];
-        }
-        const uint32_t half = V == 1 ? ((first & 1) ? w >> 16 : w & 0xffffu) : (i & 1) ? w >> 16 : w & 0xffffu;
-        f[i] = half >= rule.threshold ? f[i] * rule.factor : 0.0f;  // a dropped NaN or infinity is a zero
+// Philox4x32-10 (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw, "Parallel
+// random numbers: as easy as 1, 2, 3", SC 2011): ten rounds of two 32x32-bit
+// products over a 128-bit counter under a 64-bit key.
+inline DropoutRule keyed_rule(uint32_t threshold, float factor, uint64_t seed, uint64_t offset) {
+    DropoutRule rule = {offset, {}, threshold, factor};
+    uint32_t k0 = uint32_t(seed), k1 = uint32_t(seed >> 32);
+    for (int round = 0; round < 10; ++round) {
+        rule.key[2 * round] = k0;
+        rule.key[2 * round + 1] = k1;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
     }
+    return rule;
+}
+__device__ __forceinline__ uint4 philox(uint64_t index, const DropoutRule& rule) {
+    uint32_t c0 = uint32_t(index), c1 = uint32_t(index >> 32);
+    uint32_t c2 = uint32_t(rule.offset), c3 = uint32_t(rule.offset >> 32);
+#pragma unroll
+    for (int round = 0; round < 10; ++round) {
+        const uint64_t a = uint64_t(c0) * 0xD2511F53u, b = uint64_t(c2) * 0xCD9E8D57u;
+        c0 = uint32_t(b >> 32) ^ c1 ^ rule.key[2 * round];
+        c1 = uint32_t(b);
+        c2 = uint32_t(a >> 32) ^ c3 ^ rule.key[2 * round + 1];
+        c3 = uint32_t(a);
+    }
+    return make_uint4(c0, c1, c2, c3);
 }
 
-// V elements from logical index `index`, a multiple of V (V divides 8).
+// Zeros in the places of V elements that are dropped (a NaN or an infinity
+// there too); the others are left for the caller to scale. `index`, a multiple
+// of V, is the first one's; `bits` are its counter's.
 template <int V>
-__device__ __forceinline__ void drop_at(float (&f)[V], uint64_t index, const DropoutRule& rule) {
-    drop<V>(f, philox(index >> 3, rule.offset, rule.seed), uint32_t(index & 7), rule);
+__device__ __forceinline__ void drop(Pairs<V>& f, const uint4& bits, uint32_t index, const DropoutRule& rule) {
+    static_assert(V == 8 || V == 4 || V == 1);
+    if constexpr (V == 1) {
+        const uint32_t at = index & 7;
+        const uint32_t word = at < 4 ? (at < 2 ? bits.x : bits.y) : (at < 6 ? bits.z : bits.w);
+        const uint32_t half = at & 1 ? word >> 16 : word & 0xffffu;
+        if (half < rule.threshold) f.p[0].x = 0.0f;
+    } else {
+        const bool back = V == 4 && (index & 4);
+        const uint32_t word[4] = {back ? bits.z : bits.x, back ? bits.w : bits.y, bits.z, bits.w};
+        // Both halves against threshold - 1 in one instruction: `x > t - 1`.
+        const uint32_t least = (rule.threshold - 1) * 0x10001u;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            bool high, low;
+            __vibmax_u16x2(least, word[i], &high, &low);  // whether t - 1 >= x
+            if (low) f.p[i].x = 0.0f;
+            if (high) f.p[i].y = 0.0f;
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void drop_at(Pairs<V>& f, uint64_t index, const DropoutRule& rule) {
+    drop<V>(f, philox(index >> 3, rule), uint32_t(index), rule);
+}
+template <int V>
+__device__ __forceinline__ void scale(Pairs<V>& f, float by) {
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::N; ++i) f.p[i] = __fmul2_rn(f.p[i], both(by));
 }
 
 struct DropoutShape {
@@ -84,22 +105,24 @@ __global__ void __launch_bounds__(256) k_dropout(const T* __restrict__ x, const 
             rat = row * shape.residual_stride + column;
         }
         const auto vx = load<T, 8>(x + at);
-        float f[8];
-        unpack<T, 8>(vx, f);
-        if (random) {
-            bits = philox(uint64_t(group), rule.offset, rule.seed);
-            drop<8>(f, bits, 0, rule);
-        }
-        if (RESIDUAL) {
-            float r[8];
-            unpack<T, 8>(load<T, 8>(residual + rat), r);
+        Vector<T, 8> vr;
+        if (RESIDUAL) vr = load<T, 8>(residual + rat);
+        if (random) bits = philox(uint64_t(group), rule);
+        Pairs<8> f = unpack_pairs<T, 8>(vx);
+        if (random) drop<8>(f, bits, 0, rule);
+        // Rounded before the residual is added, so that the sum does not depend
+        // on whether a compiler joins the two operations.
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += r[i];
+        for (int j = 0; j < 8; ++j) f.set(j, __fmul_rn(f.get(j), rule.factor));
+        if (RESIDUAL) {
+            const Pairs<8> r = unpack_pairs<T, 8>(vr);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.p[i] = __fadd2_rn(f.p[i], r.p[i]);
         }
-        store<T, 8>(y + first, pack<T, 8>(f));
+        store<T, 8>(y + first, pack_pairs<T, 8>(f));
         return;
     }
-    if (random) bits = philox(uint64_t(group), rule.offset, rule.seed);
+    if (random) bits = philox(uint64_t(group), rule);
     for (int i = 0; i < 8 && first + i < count; ++i) {
         int64_t at = first + i, rat = at;
         if (VECTORS != 2) {
@@ -107,10 +130,10 @@ __global__ void __launch_bounds__(256) k_dropout(const T* __restrict__ x, const 
             at = row * shape.x_stride + column;
             rat = row * shape.residual_stride + column;
         }
-        float f[1] = {to_float(x[at])};
+        Pairs<1> f = {{make_float2(to_float(x[at]), 0.0f)}};
         if (random) drop<1>(f, bits, uint32_t(i), rule);
-        if (RESIDUAL) f[0] += to_float(residual[rat]);
-        y[first + i] = from_float<T>(f[0]);
+        const float kept = __fmul_rn(f.p[0].x, rule.factor);
+        y[first + i] = from_float<T>(RESIDUAL ? __fadd_rn(kept, to_float(residual[rat])) : kept);
     }
 }
 

@@ -43,50 +43,65 @@ __device__ __forceinline__ int32_t length_of(const NormShape& s, int32_t n) {
     return l < 0 ? 0 : l < s.points ? l : s.points;
 }
 
-// 1 / (1 + e^-z) from the special function unit's exponential and reciprocal
-// (a few 2^-23 off): an IEEE reciprocal alone would take as many instructions
-// as the rest of an element.
-__device__ __forceinline__ float sigmoid(float z) {
-    float e, f;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.0f + e));
+// 1 / (1 + e^-z) of V values, from the special function unit's exponential and
+// reciprocal (a few 2^-23 off): an IEEE reciprocal alone would take as many
+// instructions as the rest of an element.
+template <int V>
+__device__ __forceinline__ Pairs<V> sigmoid(const Pairs<V>& z) {
+    Pairs<V> f;
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::N; ++i) f.p[i] = __fmul2_rn(z.p[i], both(-1.4426950408889634f));
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(f.get(j)));
+        f.set(j, e);
+    }
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::N; ++i) f.p[i] = __fadd2_rn(f.p[i], both(1.0f));
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(f.get(j)));
+        f.set(j, r);
+    }
     return f;
 }
 
 template <int V>
-__device__ __forceinline__ void activate(float (&z)[V], int32_t activation) {
+__device__ __forceinline__ void activate(Pairs<V>& z, int32_t activation) {
+    constexpr int N = Pairs<V>::N;
     if (activation == SILU) {
+        const Pairs<V> f = sigmoid<V>(z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] *= sigmoid(z[i]);
+        for (int i = 0; i < N; ++i) z.p[i] = __fmul2_rn(z.p[i], f.p[i]);
     } else if (activation == SIGMOID) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = sigmoid(z[i]);
+        z = sigmoid<V>(z);
     } else if (activation == TANH) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = tanhf(z[i]);
+        for (int j = 0; j < V; ++j) z.set(j, tanhf(z.get(j)));
     }
 }
 
-// h *= act'(z).
+// h *= act'(z): f (1 + z (1 - f)), f (1 - f) or 1 - t^2.
 template <int V>
-__device__ __forceinline__ void activate_gradient(float (&h)[V], const float (&z)[V], int32_t activation) {
-    if (activation == SILU) {
+__device__ __forceinline__ void activate_gradient(Pairs<V>& h, const Pairs<V>& z, int32_t activation) {
+    constexpr int N = Pairs<V>::N;
+    if (activation == SILU || activation == SIGMOID) {
+        const Pairs<V> f = sigmoid<V>(z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float f = sigmoid(z[i]);
-            h[i] *= f * (1.0f + z[i] * (1.0f - f));
-        }
-    } else if (activation == SIGMOID) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float f = sigmoid(z[i]);
-            h[i] *= f * (1.0f - f);
+        for (int i = 0; i < N; ++i) {
+            const float2 back = __ffma2_rn(f.p[i], both(-1.0f), both(1.0f));
+            const float2 slope = activation == SILU
+                                     ? __ffma2_rn(f.p[i], __fmul2_rn(z.p[i], back), f.p[i])
+                                     : __fmul2_rn(f.p[i], back);
+            h.p[i] = __fmul2_rn(h.p[i], slope);
         }
     } else if (activation == TANH) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float t = tanhf(z[i]);
-            h[i] *= 1.0f - t * t;
+        for (int j = 0; j < V; ++j) {
+            const float t = tanhf(z.get(j));
+            h.set(j, h.get(j) * fmaf(-t, t, 1.0f));
         }
     }
 }
@@ -149,31 +164,35 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(const T* __restri
     if (active) {
         // Deviations from the thread's own first value: their squares cancel by
         // no more than the number of the thread's points.
-        float shift[V], s1[V], s2[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) shift[j] = s1[j] = s2[j] = 0.0f;
+        constexpr int N = Pairs<V>::N;
+        Pairs<V> shift, s1, s2;
+        shift.fill(0.0f);
+        s1.fill(0.0f);
+        s2.fill(0.0f);
         int32_t count = 0;
         const T* base = x + n * s.x_instance + t.first + tx * V;
-        if (lo + ty < hi) unpack<T, V>(load<T, V>(base + (lo + ty) * s.x_point), shift);
+        if (lo + ty < hi) {
+            shift = unpack_pairs<T, V>(load<T, V>(base + (lo + ty) * s.x_point));
+            scale<V>(shift, -1.0f);
+        }
 #pragma unroll 4
         for (int32_t p = lo + ty; p < hi; p += ys) {
-            float f[V];
-            unpack<T, V>(load<T, V>(base + p * s.x_point), f);
+            const Pairs<V> f = unpack_pairs<T, V>(load<T, V>(base + p * s.x_point));
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = f[j] - shift[j];
-                s1[j] += d;
-                s2[j] = fmaf(d, d, s2[j]);
+            for (int i = 0; i < N; ++i) {
+                const float2 d = __fadd2_rn(f.p[i], shift.p[i]);
+                s1.p[i] = __fadd2_rn(s1.p[i], d);
+                s2.p[i] = __ffma2_rn(d, d, s2.p[i]);
             }
             ++count;
         }
         const float inverse = count ? 1.0f / float(count) : 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float mean = s1[j] * inverse;
+            const float mean = s1.get(j) * inverse;
             float* to = norm_shared + 2 * (ty * width + tx * V + j);
-            to[0] = shift[j] + mean;
-            to[1] = fmaxf(s2[j] - s1[j] * mean, 0.0f);
+            to[0] = mean - shift.get(j);
+            to[1] = fmaxf(s2.get(j) - s1.get(j) * mean, 0.0f);
         }
     }
     __syncthreads();
@@ -195,23 +214,37 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(const T* __restri
     }
 }
 
-// Terms of a thread's vector by channel; ONE: its channels are of one group, so
-// that the statistics are two registers and not 2 V.
+// Terms of a thread's vector by channel. ONE: its channels are of one group, so
+// that what belongs to the group is two registers and not V.
 template <int V, bool ONE>
-struct Terms {
-    static constexpr int M = ONE ? 1 : V;
-    float mean[M], rstd[M], weight[V], bias[V];
-    __device__ __forceinline__ float mean_of(int j) const { return mean[ONE ? 0 : j]; }
-    __device__ __forceinline__ float rstd_of(int j) const { return rstd[ONE ? 0 : j]; }
+struct GroupTerms {
+    static constexpr int N = ONE ? 1 : Pairs<V>::N;
+    float2 p[N];
+    __device__ __forceinline__ const float2& of(int i) const { return p[ONE ? 0 : i]; }
+    __device__ __forceinline__ void set(int j, float v) {
+        if (ONE) p[0] = both(v);
+        else (j % 2 ? p[ONE ? 0 : j / 2].y : p[ONE ? 0 : j / 2].x) = v;
+    }
 };
 
-// drop(act((f - mean) weight + bias)), with rstd in the weight.
+// z = (x - mean) gain + bias, gain = weight rstd.
 template <int V, bool ONE>
-__device__ __forceinline__ void norm_value(float (&f)[V], const Terms<V, ONE>& k, uint64_t at, const NormShape& s) {
+struct Terms {
+    GroupTerms<V, ONE> minus_mean;
+    Pairs<V> gain, bias;
+};
+
+// factor drop(act(z)) of a vector of x.
+template <int V, bool ONE>
+__device__ __forceinline__ void norm_value(Pairs<V>& f, const Terms<V, ONE>& k, uint64_t at, const NormShape& s) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = fmaf(f[j] - k.mean_of(j), k.weight[j], k.bias[j]);
+    for (int i = 0; i < Pairs<V>::N; ++i)
+        f.p[i] = __ffma2_rn(__fadd2_rn(f.p[i], k.minus_mean.of(i)), k.gain.p[i], k.bias.p[i]);
     activate<V>(f, s.activation);
-    if (s.rule.threshold) drop_at<V>(f, at, s.rule);
+    if (s.rule.threshold) {
+        drop_at<V>(f, at, s.rule);
+        scale<V>(f, s.rule.factor);
+    }
 }
 
 // y = drop(act(norm(x))). The block first joins the moments of its groups'
@@ -254,12 +287,14 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
     if (ty >= ys || tx * V >= t.count) return;
     const int32_t channel = t.first + tx * V;
     Terms<V, ONE> k;
+    k.gain.fill(0.0f);
+    k.bias.fill(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int32_t g = (channel + j) / s.width - t.group;
-        if (!ONE || j == 0) k.mean[j] = norm_shared[2 * g];
-        k.weight[j] = parameter(weight, channel + j, 1.0f) * norm_shared[2 * g + 1];
-        k.bias[j] = parameter(bias, channel + j, 0.0f);
+        k.minus_mean.set(j, -norm_shared[2 * g]);
+        k.gain.set(j, parameter(weight, channel + j, 1.0f) * norm_shared[2 * g + 1]);
+        k.bias.set(j, parameter(bias, channel + j, 0.0f));
     }
     int32_t lo, hi;
     split_range(s.points, split, s.apply_splits, lo, hi);
@@ -273,43 +308,69 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
             store<T, V>(y + at, zeros<T, V>());
             continue;
         }
-        float f[V];
-        unpack<T, V>(load<T, V>(from + p * s.x_point), f);
+        Pairs<V> f = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
         norm_value<V, ONE>(f, k, uint64_t(at), s);
-        store<T, V>(y + at, pack<T, V>(f));
+        store<T, V>(y + at, pack_pairs<T, V>(f));
     }
 }
 
-// xhat and h of a thread's vector at one point.
-template <class T, int V, bool ONE>
-__device__ __forceinline__ void norm_adjoint(const Vector<T, V>& vx, const Vector<T, V>& vg, const Terms<V, ONE>& k,
-                                             uint64_t at, const NormShape& s, float (&xhat)[V], float (&h)[V]) {
-    float z[V];
-    unpack<T, V>(vx, xhat);
-    unpack<T, V>(vg, h);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        xhat[j] = (xhat[j] - k.mean_of(j)) * k.rstd_of(j);
-        z[j] = fmaf(xhat[j], k.weight[j], k.bias[j]);
-    }
-    if (s.rule.threshold) drop_at<V>(h, at, s.rule);
-    activate_gradient<V>(h, z, s.activation);
-}
+// Terms of the gradient: xhat = (x - mean) rstd, z = xhat weight + bias.
+template <int V, bool ONE>
+struct AdjointTerms {
+    GroupTerms<V, ONE> minus_mean, rstd;
+    Pairs<V> weight, bias;
+};
 
 template <class P, int V, bool ONE>
-__device__ __forceinline__ void load_terms(Terms<V, ONE>& k, const NormShape& s, int32_t n, int32_t channel,
+__device__ __forceinline__ void load_terms(AdjointTerms<V, ONE>& k, const NormShape& s, int32_t n, int32_t channel,
                                            const float* mean, const float* rstd, const P* weight, const P* bias) {
+    k.weight.fill(0.0f);
+    k.bias.fill(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t g = int64_t(n) * s.groups + (channel + j) / s.width;
         if (!ONE || j == 0) {
-            k.mean[j] = mean[g];
-            k.rstd[j] = rstd[g];
+            k.minus_mean.set(j, -mean[g]);
+            k.rstd.set(j, rstd[g]);
         }
-        k.weight[j] = parameter(weight, channel + j, 1.0f);
-        k.bias[j] = parameter(bias, channel + j, 0.0f);
+        k.weight.set(j, parameter(weight, channel + j, 1.0f));
+        k.bias.set(j, parameter(bias, channel + j, 0.0f));
     }
 }
+
+// xhat, and in h the kept gradients times act'(z), not yet scaled by the
+// dropout's factor.
+template <int V, bool ONE>
+__device__ __forceinline__ void norm_adjoint(Pairs<V>& xhat, Pairs<V>& h, const AdjointTerms<V, ONE>& k,
+                                             int32_t activation) {
+    Pairs<V> z;
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::N; ++i) {
+        xhat.p[i] = __fmul2_rn(__fadd2_rn(xhat.p[i], k.minus_mean.of(i)), k.rstd.of(i));
+        z.p[i] = __ffma2_rn(xhat.p[i], k.weight.p[i], k.bias.p[i]);
+    }
+    activate_gradient<V>(h, z, activation);
+}
+
+// dx = rstd (factor w h - (m1 + xhat m2)) as two products and sums.
+template <int V, bool ONE>
+struct InputTerms {
+    Pairs<V> gain;              // factor w rstd
+    GroupTerms<V, ONE> m1, m2;  // -rstd m1, -rstd m2
+    __device__ __forceinline__ void set(const AdjointTerms<V, ONE>& k, int j, float2 m, float factor) {
+        const float r = j % 2 ? k.rstd.of(j / 2).y : k.rstd.of(j / 2).x;
+        gain.set(j, factor * r * k.weight.get(j));
+        if (!ONE || j == 0) {
+            m1.set(j, -r * m.x);
+            m2.set(j, -r * m.y);
+        }
+    }
+    __device__ __forceinline__ void apply(Pairs<V>& h, const Pairs<V>& xhat) const {
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::N; ++i)
+            h.p[i] = __ffma2_rn(h.p[i], gain.p[i], __ffma2_rn(xhat.p[i], m2.of(i), m1.of(i)));
+    }
+};
 
 // Sums of h and h xhat over a block's points: per channel for dw and db
 // (channel_sums[instance][split][channel]), and times w per piece of a group
@@ -332,26 +393,30 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
     split_range(length_of(s, n), split, s.splits, lo, hi);
     if (ty < ys && tx * V < t.count) {
         const int32_t channel = t.first + tx * V;
-        Terms<V, ONE> k;
+        AdjointTerms<V, ONE> k;
         load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
-        float sh[V], sx[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) sh[j] = sx[j] = 0.0f;
+        Pairs<V> sh, sx;
+        sh.fill(0.0f);
+        sx.fill(0.0f);
         const T* from = x + n * s.x_instance + channel;
         const T* gfrom = grad + n * s.grad_instance + channel;
 #pragma unroll 2
         for (int32_t p = lo + ty; p < hi; p += ys) {
-            float xhat[V], h[V];
-            norm_adjoint<T, V, ONE>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k,
-                               uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s, xhat, h);
+            Pairs<V> xhat = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
+            Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
+            if (s.rule.threshold)
+                drop_at<V>(h, uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s.rule);
+            norm_adjoint<V, ONE>(xhat, h, k, s.activation);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                sh[j] += h[j];
-                sx[j] = fmaf(h[j], xhat[j], sx[j]);
+            for (int i = 0; i < Pairs<V>::N; ++i) {
+                sh.p[i] = __fadd2_rn(sh.p[i], h.p[i]);
+                sx.p[i] = __ffma2_rn(h.p[i], xhat.p[i], sx.p[i]);
             }
         }
+        scale<V>(sh, s.rule.factor);
+        scale<V>(sx, s.rule.factor);
 #pragma unroll
-        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = make_float2(sh[j], sx[j]);
+        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = make_float2(sh.get(j), sx.get(j));
     }
     __syncthreads();
     for (int32_t c = threadIdx.x; c < t.count; c += NORM_THREADS) {
@@ -458,16 +523,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const int32_t ty = threadIdx.x / s.tile, tx = threadIdx.x % s.tile;
     if (ty >= ys || tx * V >= t.count) return;
     const int32_t channel = t.first + tx * V;
-    Terms<V, ONE> k;
+    AdjointTerms<V, ONE> k;
     load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
-    constexpr int M = Terms<V, ONE>::M;
-    float m1[M], m2[M];
+    InputTerms<V, ONE> to_input;
+    to_input.gain.fill(0.0f);
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
-        const float2 m = shared[(channel + j) / s.width - t.group];
-        m1[j] = m.x;
-        m2[j] = m.y;
-    }
+    for (int j = 0; j < V; ++j) to_input.set(k, j, shared[(channel + j) / s.width - t.group], s.rule.factor);
     int32_t lo, hi;
     split_range(s.points, split, s.apply_splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
@@ -480,13 +541,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
             store<T, V>(dx + at, zeros<T, V>());
             continue;
         }
-        float xhat[V], h[V];
-        norm_adjoint<T, V, ONE>(load<T, V>(from + p * s.x_point), load<T, V>(gfrom + p * s.grad_point), k, uint64_t(at), s,
-                           xhat, h);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            h[j] = (h[j] * k.weight[j] - fmaf(xhat[j], m2[ONE ? 0 : j], m1[ONE ? 0 : j])) * k.rstd_of(j);
-        store<T, V>(dx + at, pack<T, V>(h));
+        Pairs<V> xhat = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
+        Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
+        if (s.rule.threshold) drop_at<V>(h, uint64_t(at), s.rule);
+        norm_adjoint<V, ONE>(xhat, h, k, s.activation);
+        to_input.apply(h, xhat);
+        store<T, V>(dx + at, pack_pairs<T, V>(h));
     }
 }
 

@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(NORM_THREADS, 3) k_norm_slab(const T* __restri
     if (at.active) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            k.weight[j] = parameter(weight, at.channel + j, 1.0f);
-            k.bias[j] = parameter(bias, at.channel + j, 0.0f);
+            k.gain.set(j, parameter(weight, at.channel + j, 1.0f));
+            k.bias.set(j, parameter(bias, at.channel + j, 0.0f));
         }
     }
     clear_tail<T, V>(y, at, s, rank, size);
@@ -109,20 +109,21 @@ __global__ void __launch_bounds__(NORM_THREADS, 3) k_norm_slab(const T* __restri
     if (at.active) {
         // Deviations from the thread's first value: their squares cancel by no
         // more than the number of the thread's values.
-        float shift = 0.0f, s1 = 0.0f, s2 = 0.0f;
+        float2 shift = both(0.0f), t1 = both(0.0f), t2 = both(0.0f);
+#pragma unroll 2
         for (int32_t i = 0; i < at.count; ++i) {
-            float f[V];
-            unpack<T, V>(data[i * NORM_THREADS + threadIdx.x], f);
-            if (i == 0) shift = f[0];
+            const Pairs<V> f = unpack_pairs<T, V>(data[i * NORM_THREADS + threadIdx.x]);
+            if (i == 0) shift = both(-f.p[0].x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = f[j] - shift;
-                s1 += d;
-                s2 = fmaf(d, d, s2);
+            for (int j = 0; j < Pairs<V>::N; ++j) {
+                const float2 d = __fadd2_rn(f.p[j], shift);
+                t1 = __fadd2_rn(t1, d);
+                t2 = __ffma2_rn(d, d, t2);
             }
         }
+        const float s1 = t1.x + t1.y, s2 = t2.x + t2.y;
         const float m = at.count ? s1 / float(at.count * V) : 0.0f;
-        shared.threads[threadIdx.x] = make_float2(shift + m, fmaxf(s2 - s1 * m, 0.0f));
+        shared.threads[threadIdx.x] = make_float2(m - shift.x, fmaxf(s2 - s1 * m, 0.0f));
     }
     __syncthreads();
     const int32_t per_group = s.width / V;  // vectors of a group
@@ -160,17 +161,15 @@ __global__ void __launch_bounds__(NORM_THREADS, 3) k_norm_slab(const T* __restri
     auto token = cluster.barrier_arrive();  // done with the other CTAs' memory
     if (at.active) {
         const float2 m = shared.statistics[at.tx / per_group];
-        k.mean[0] = m.x;
-#pragma unroll
-        for (int j = 0; j < V; ++j) k.weight[j] *= m.y;
+        k.minus_mean.set(0, -m.x);
+        scale<V>(k.gain, m.y);
         int64_t to = (int64_t(at.n) * s.points + at.lo + at.ty) * s.channels + at.channel;
         const int64_t step = int64_t(at.ys) * s.channels;
 #pragma unroll 2
         for (int32_t i = 0; i < at.count; ++i, to += step) {
-            float f[V];
-            unpack<T, V>(data[i * NORM_THREADS + threadIdx.x], f);
+            Pairs<V> f = unpack_pairs<T, V>(data[i * NORM_THREADS + threadIdx.x]);
             norm_value<V, true>(f, k, uint64_t(to), s);
-            store<T, V>(y + to, pack<T, V>(f));
+            store<T, V>(y + to, pack_pairs<T, V>(f));
         }
     }
     cluster.barrier_wait(std::move(token));
@@ -208,25 +207,35 @@ __global__ void __launch_bounds__(NORM_THREADS, 3) k_norm_slab_gradient(
         copy_async<sizeof(Slot)>(&data[i * NORM_THREADS + threadIdx.x], from + int64_t(i) * at.ys * s.x_point);
         copy_async<sizeof(Slot)>(&grads[i * NORM_THREADS + threadIdx.x], gfrom + int64_t(i) * at.ys * s.grad_point);
     }
-    Terms<V, true> k;
+    AdjointTerms<V, true> k;
     if (at.active) load_terms<P, V, true>(k, s, at.n, at.channel, mean, rstd, weight, bias);
     clear_tail<T, V>(dx, at, s, rank, size);
     copies_done();
     const int64_t first = (int64_t(at.n) * s.points + at.lo + at.ty) * s.channels + at.channel;
     const int64_t step = int64_t(at.ys) * s.channels;
-    float2 sum[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    Pairs<V> sh, sx;
+    sh.fill(0.0f);
+    sx.fill(0.0f);
+#pragma unroll 2
     for (int32_t i = 0; i < at.count; ++i) {
-        float xhat[V], h[V];
-        norm_adjoint<T, V, true>(data[i * NORM_THREADS + threadIdx.x], grads[i * NORM_THREADS + threadIdx.x], k,
-                                 uint64_t(first + i * step), s, xhat, h);
+        Slot& slot = grads[i * NORM_THREADS + threadIdx.x];
+        Pairs<V> xhat = unpack_pairs<T, V>(data[i * NORM_THREADS + threadIdx.x]), h = unpack_pairs<T, V>(slot);
+        if (s.rule.threshold) {
+            drop_at<V>(h, uint64_t(first + i * step), s.rule);
+            slot = pack_pairs<T, V>(h);  // exact; the second pass finds the zeros and need not draw again
+        }
+        norm_adjoint<V, true>(xhat, h, k, s.activation);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            sum[j].x += h[j];
-            sum[j].y = fmaf(h[j], xhat[j], sum[j].y);
+        for (int j = 0; j < Pairs<V>::N; ++j) {
+            sh.p[j] = __fadd2_rn(sh.p[j], h.p[j]);
+            sx.p[j] = __ffma2_rn(h.p[j], xhat.p[j], sx.p[j]);
         }
     }
+    scale<V>(sh, s.rule.factor);
+    scale<V>(sx, s.rule.factor);
+    float2 sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = make_float2(sh.get(j), sx.get(j));
     if (warps) {
         for (int32_t d = 16; d >= s.tile; d /= 2) {
 #pragma unroll
@@ -279,15 +288,17 @@ __global__ void __launch_bounds__(NORM_THREADS, 3) k_norm_slab_gradient(
     }
     __syncthreads();
     if (at.active) {
-        const float2 m = means[at.tx * V / s.width];
-        int64_t to = first;
-        for (int32_t i = 0; i < at.count; ++i, to += step) {
-            float xhat[V], h[V];
-            norm_adjoint<T, V, true>(data[i * NORM_THREADS + threadIdx.x], grads[i * NORM_THREADS + threadIdx.x], k,
-                                     uint64_t(to), s, xhat, h);
+        InputTerms<V, true> to_input;
 #pragma unroll
-            for (int j = 0; j < V; ++j) h[j] = (h[j] * k.weight[j] - fmaf(xhat[j], m.y, m.x)) * k.rstd[0];
-            store<T, V>(dx + to, pack<T, V>(h));
+        for (int j = 0; j < V; ++j) to_input.set(k, j, means[at.tx * V / s.width], s.rule.factor);
+        int64_t to = first;
+#pragma unroll 2
+        for (int32_t i = 0; i < at.count; ++i, to += step) {
+            Pairs<V> xhat = unpack_pairs<T, V>(data[i * NORM_THREADS + threadIdx.x]);
+            Pairs<V> h = unpack_pairs<T, V>(grads[i * NORM_THREADS + threadIdx.x]);
+            norm_adjoint<V, true>(xhat, h, k, s.activation);
+            to_input.apply(h, xhat);
+            store<T, V>(dx + to, pack_pairs<T, V>(h));
         }
     }
     cluster.barrier_wait(std::move(token));

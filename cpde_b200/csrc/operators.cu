@@ -251,7 +251,7 @@ namespace {
 
 DropoutRule dropout_rule(double rate, uint64_t seed, uint64_t offset) {
     const uint32_t threshold = uint32_t(std::lround(rate * 65536));
-    return {seed, offset, threshold, threshold < 65536 ? float(65536.0 / (65536.0 - threshold)) : 0.0f};
+    return keyed_rule(threshold, threshold < 65536 ? float(65536.0 / (65536.0 - threshold)) : 0.0f, seed, offset);
 }
 
 }  // namespace
