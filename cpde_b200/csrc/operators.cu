@@ -326,8 +326,8 @@ struct SlabPlan {
     int32_t slots;        // vectors of a thread, and array
     size_t shared;
 };
-constexpr size_t SLAB_TILE_BYTES = 128;                    // of a point, at least: whole lines of memory
-constexpr size_t SLAB_THREE = 72 << 10, SLAB_TWO = 108 << 10, SLAB_ONE = 220 << 10;  // shared memory of a CTA
+constexpr size_t SLAB_TILE_BYTES = 64;                    // of a point, at least: whole lines of memory
+constexpr size_t SLAB_SIX = 36 << 10, SLAB_THREE = 72 << 10, SLAB_TWO = 108 << 10, SLAB_ONE = 220 << 10;  // shared memory of a CTA
 
 // Vectors of at most 16 bytes (a copy's most) whose channels are of one group.
 int slab_vector(int fit, size_t element, int64_t width) {
@@ -343,20 +343,20 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, int arrays) {
     int64_t tile_groups = std::max<int64_t>(1, int64_t(SLAB_TILE_BYTES / vector_bytes) / group);
     tile_groups = std::min(tile_groups, groups);
     p.tile = int32_t(tile_groups * group);
-    if (p.tile > NORM_THREADS) return p;
+    if (p.tile > SLAB_THREADS) return p;
     p.tiles = int32_t((groups + tile_groups - 1) / tile_groups);
-    const int64_t ys = NORM_THREADS / p.tile;
+    const int64_t ys = SLAB_THREADS / p.tile;
     auto plan = [&](int32_t cluster) {
         const int64_t points = (int64_t(s.points) + cluster - 1) / cluster;
         const int64_t slots = (points + ys - 1) / ys;
         p.slots = int32_t(std::min<int64_t>(slots, 1 << 16));
-        const int64_t width = int64_t(p.tile) * v, rows = slab_rows_are_warps(p.tile) ? NORM_WARPS : ys;
-        p.shared = size_t(p.slots) * NORM_THREADS * vector_bytes * arrays +
+        const int64_t width = int64_t(p.tile) * v, rows = slab_rows_are_warps(p.tile) ? SLAB_WARPS : ys;
+        p.shared = size_t(p.slots) * SLAB_THREADS * vector_bytes * arrays +
                    (arrays == 1 ? sizeof(SlabMoments) : size_t((rows + 2) * width + tile_groups) * sizeof(float2));
         return p.shared;
     };
     int32_t cluster = 0;
-    for (size_t limit : {SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
+    for (size_t limit : {SLAB_SIX, SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
         for (int32_t c = 1; c <= 16 && !cluster; c *= 2)
             if (plan(c) <= limit) cluster = c;
         if (cluster) break;
@@ -370,6 +370,18 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, int arrays) {
     return p;
 }
 
+SlabShape slab_shape(const NormShape& norm, const SlabPlan& plan, int v, const NormCall& c, size_t parameter) {
+    const int32_t ys = SLAB_THREADS / plan.tile, group_vectors = norm.width / v;
+    auto by = [](int32_t d) { return Divisor(uint32_t(d)); };
+    SlabShape s = {norm, plan.cluster, plan.slots, ys, group_vectors, plan.tile * v, plan.tile / group_vectors,
+                   by(plan.cluster), by(plan.tiles), by(plan.tile), by(ys), by(group_vectors), false};
+    s.norm.tile = plan.tile;
+    s.norm.tiles = plan.tiles;
+    add_call(s.norm, c);
+    s.wide_parameters = Alignment().at(c.weight, parameter).at(c.bias, parameter).vector(v) == v;
+    return s;
+}
+
 template <auto kernel, class... A>
 void launch_slab(const SlabPlan& plan, int64_t instances, int device, cudaStream_t stream, A... arguments) {
     static std::atomic<uint64_t> ready{0};  // devices on which this kernel's limits are raised
@@ -380,7 +392,7 @@ void launch_slab(const SlabPlan& plan, int64_t instances, int device, cudaStream
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(instances * plan.tiles * plan.cluster));
-    config.blockDim = dim3(NORM_THREADS);
+    config.blockDim = dim3(SLAB_THREADS);
     config.dynamicSmemBytes = plan.shared;
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
@@ -452,14 +464,11 @@ void group_norm(const NormCall& c, int device, cudaStream_t stream) {
         with_vector<8, 4>(slab_vector(fit, sizeof(T), c.channels / c.groups), [&](auto width) {
             constexpr int V = decltype(width)::value;
             if constexpr (V * sizeof(T) <= 16) {
-                NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+                const NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
                 const SlabPlan plan = slab_plan(s, V, sizeof(T), 1);
                 if (!plan.cluster) return;
-                add_call(s, c);
-                s.tile = plan.tile;
-                s.tiles = plan.tiles;
                 launch_slab<k_norm_slab<T, P, V>>(plan, s.instances, device, stream, x, weight, bias, y, c.mean, c.rstd,
-                            s, plan.slots);
+                                                  slab_shape(s, plan, V, c, sizeof(P)));
                 done = true;
             }
         });
@@ -501,15 +510,13 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
         with_vector<8, 4>(slab_vector(fit, sizeof(T), c.channels / c.groups), [&](auto width) {
             constexpr int V = decltype(width)::value;
             if constexpr (V * sizeof(T) <= 16) {
-                NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
+                const NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
                 const SlabPlan plan = slab_plan(s, V, sizeof(T), 2);
                 if (!plan.cluster) return;
-                add_call(s, c);
-                s.tile = plan.tile;
-                s.tiles = plan.tiles;
                 auto* channel_sums = static_cast<float2*>(c.workspace);
                 launch_slab<k_norm_slab_gradient<T, P, V>>(plan, s.instances, device, stream, grad, x, c.mean, c.rstd,
-                            weight, bias, dx, channel_sums, s, plan.slots);
+                                                           weight, bias, dx, channel_sums,
+                                                           slab_shape(s, plan, V, c, sizeof(P)));
                 if (parameter_blocks) {
                     k_norm_parameters<P><<<parameter_blocks, NORM_THREADS, 0, stream>>>(dweight, dbias, channel_sums,
                                                                                          s.instances, s.channels);
