@@ -450,28 +450,21 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
 }
 
 // dw and db of 32 channels: sums over the rows of channel_sums in a fixed order.
-template <class P>
+template <class P, int WARPS>
 __device__ __forceinline__ void sum_parameters(P* __restrict__ dweight, P* __restrict__ dbias,
                                                const float2* __restrict__ channel_sums, int32_t rows,
                                                int32_t channels, int32_t block) {
-    __shared__ float2 shared[NORM_WARPS][32];
+    __shared__ float2 shared[WARPS][32];
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, channel = block * 32 + lane;
     float2 sum = make_float2(0.0f, 0.0f);
     if (channel < channels) {
-#pragma unroll 4
-        for (int32_t i = warp; i < rows; i += NORM_WARPS) {
-            const float2 v = channel_sums[int64_t(i) * channels + channel];
-            sum.x += v.x;
-            sum.y += v.y;
-        }
+#pragma unroll 8
+        for (int32_t i = warp; i < rows; i += WARPS) sum = __fadd2_rn(sum, channel_sums[int64_t(i) * channels + channel]);
     }
     shared[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && channel < channels) {
-        for (int w = 1; w < NORM_WARPS; ++w) {
-            sum.x += shared[w][lane].x;
-            sum.y += shared[w][lane].y;
-        }
+        for (int w = 1; w < WARPS; ++w) sum = __fadd2_rn(sum, shared[w][lane]);
         if (dbias) dbias[channel] = from_float<P>(sum.x);
         if (dweight) dweight[channel] = from_float<P>(sum.y);
     }
@@ -491,7 +484,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const int32_t n = blockIdx.x / s.apply_splits;
     if (n >= s.instances) {
         if (blockIdx.y == 0)
-            sum_parameters<P>(dweight, dbias, channel_sums, s.instances * s.splits, s.channels,
+            sum_parameters<P, NORM_WARPS>(dweight, dbias, channel_sums, s.instances * s.splits, s.channels,
                               blockIdx.x - s.instances * s.apply_splits);
         return;
     }

@@ -4,6 +4,9 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 #include "common.hpp"
 #include "kernels_dropout.cuh"
@@ -304,7 +307,9 @@ NormShape norm_shape(int64_t instances, int64_t points, int64_t channels, int64_
 
 size_t norm_workspace(const NormShape& s) {
     const size_t blocks = size_t(s.instances) * s.splits;
-    return padded(blocks * s.tiles * s.pieces * sizeof(Moments)) + padded(blocks * s.channels * sizeof(float2));
+    const size_t slabs = padded(4) + size_t(s.instances) * SLAB_CLUSTER * s.channels * sizeof(float2);
+    return std::max(slabs, padded(blocks * s.tiles * s.pieces * sizeof(Moments)) +
+                               padded(blocks * s.channels * sizeof(float2)));
 }
 
 // Strides, lengths and dropout of a call.
@@ -326,7 +331,6 @@ struct SlabPlan {
     int32_t slots;        // vectors of a thread, and array
     size_t shared;
 };
-constexpr size_t SLAB_TILE_BYTES = 64;                    // of a point, at least: whole lines of memory
 constexpr size_t SLAB_SIX = 36 << 10, SLAB_THREE = 72 << 10, SLAB_TWO = 108 << 10, SLAB_ONE = 220 << 10;  // shared memory of a CTA
 
 // Vectors of at most 16 bytes (a copy's most) whose channels are of one group.
@@ -336,11 +340,11 @@ int slab_vector(int fit, size_t element, int64_t width) {
     return v;
 }
 
-SlabPlan slab_plan(const NormShape& s, int v, size_t element, int arrays) {
+SlabPlan slab_plan(const NormShape& s, int v, size_t element, size_t parameter, int arrays) {
     SlabPlan p;
     const size_t vector_bytes = v * element;
     const int64_t group = s.width / v, groups = s.groups;
-    int64_t tile_groups = std::max<int64_t>(1, int64_t(SLAB_TILE_BYTES / vector_bytes) / group);
+    int64_t tile_groups = std::max<int64_t>(1, int64_t(SLAB_TILE_BYTES / vector_bytes) / group);  // whole lines
     tile_groups = std::min(tile_groups, groups);
     p.tile = int32_t(tile_groups * group);
     if (p.tile > SLAB_THREADS) return p;
@@ -351,47 +355,35 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, int arrays) {
         const int64_t slots = (points + ys - 1) / ys;
         p.slots = int32_t(std::min<int64_t>(slots, 1 << 16));
         const int64_t width = int64_t(p.tile) * v, rows = slab_rows_are_warps(p.tile) ? SLAB_WARPS : ys;
+        const size_t parameters = 2 * ((size_t(width) * parameter + 15) / 16 * 16) + 2 * SLAB_GROUPS * sizeof(float);
         p.shared = size_t(p.slots) * SLAB_THREADS * vector_bytes * arrays +
-                   (arrays == 1 ? sizeof(SlabMoments) : size_t((rows + 2) * width + tile_groups) * sizeof(float2));
+                   2 * SlabExchange::bytes(int32_t(tile_groups), cluster) + parameters +
+                   (arrays == 1 ? SLAB_THREADS : size_t((rows + 1) * width)) * sizeof(float2);
         return p.shared;
     };
     int32_t cluster = 0;
     for (size_t limit : {SLAB_SIX, SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
-        for (int32_t c = 1; c <= 16 && !cluster; c *= 2)
+        for (int32_t c = 1; c <= SLAB_CLUSTER && !cluster; c *= 2)
             if (plan(c) <= limit) cluster = c;
         if (cluster) break;
     }
     if (!cluster) return p;
     // Few instances: smaller shares, for more of the GPU.
-    while (cluster < 16 && int64_t(s.instances) * p.tiles * cluster < 2 * SMS && (plan(cluster), p.slots >= 4))
+    while (cluster < SLAB_CLUSTER && int64_t(s.instances) * p.tiles * cluster < 2 * SMS && (plan(cluster), p.slots >= 4))
         cluster *= 2;
     plan(cluster);
     p.cluster = cluster;
     return p;
 }
 
-SlabShape slab_shape(const NormShape& norm, const SlabPlan& plan, int v, const NormCall& c, size_t parameter) {
-    const int32_t ys = SLAB_THREADS / plan.tile, group_vectors = norm.width / v;
-    auto by = [](int32_t d) { return Divisor(uint32_t(d)); };
-    SlabShape s = {norm, plan.cluster, plan.slots, ys, group_vectors, plan.tile * v, plan.tile / group_vectors,
-                   by(plan.cluster), by(plan.tiles), by(plan.tile), by(ys), by(group_vectors), false};
-    s.norm.tile = plan.tile;
-    s.norm.tiles = plan.tiles;
-    add_call(s.norm, c);
-    s.wide_parameters = Alignment().at(c.weight, parameter).at(c.bias, parameter).vector(v) == v;
-    return s;
-}
-
+// Launches a slab kernel over the items of a call, with as many clusters as the
+// GPU holds at once; `counter` (four bytes) deals out the items behind those.
 template <auto kernel, class... A>
-void launch_slab(const SlabPlan& plan, int64_t instances, int device, cudaStream_t stream, A... arguments) {
-    static std::atomic<uint64_t> ready{0};  // devices on which this kernel's limits are raised
-    if (!(ready.load() >> (device & 63) & 1)) {
-        dynamic_shared(kernel, SLAB_ONE);
-        CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        ready.fetch_or(uint64_t(1) << (device & 63));
-    }
+void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormCall& c, size_t parameter,
+                 uint32_t* counter, int device, cudaStream_t stream, A... arguments) {
+    static std::mutex mutex;
+    static std::map<std::tuple<int, int32_t, size_t>, int32_t> resident;  // clusters by device, size and memory
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(instances * plan.tiles * plan.cluster));
     config.blockDim = dim3(SLAB_THREADS);
     config.dynamicSmemBytes = plan.shared;
     config.stream = stream;
@@ -401,7 +393,36 @@ void launch_slab(const SlabPlan& plan, int64_t instances, int device, cudaStream
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, arguments...));
+    int32_t clusters;
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        int32_t& known = resident[{device, plan.cluster, plan.shared}];
+        if (!known) {
+            dynamic_shared(kernel, SLAB_ONE);
+            CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            config.gridDim = dim3(plan.cluster);
+            int most = 0;
+            CPDE_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &config));
+            known = std::max(1, most);
+        }
+        clusters = known;
+    }
+    const int32_t ys = SLAB_THREADS / plan.tile, group_vectors = norm.width / v;
+    auto by = [](int32_t d) { return Divisor(uint32_t(d)); };
+    SlabShape s = {norm, plan.cluster, plan.slots, 0, norm.instances * plan.tiles, nullptr, ys, group_vectors,
+                   plan.tile * v, plan.tile / group_vectors, by(plan.cluster), by(plan.tiles), by(plan.tile), by(ys),
+                   by(group_vectors), false};
+    s.clusters = std::min(clusters, s.items);
+    s.norm.tile = plan.tile;
+    s.norm.tiles = plan.tiles;
+    add_call(s.norm, c);
+    s.wide_parameters = Alignment().at(c.weight, parameter).at(c.bias, parameter).vector(v) == v;
+    if (s.clusters < s.items) {
+        s.counter = counter;
+        CPDE_CUDA(cudaMemsetAsync(counter, 0, sizeof(*counter), stream));
+    }
+    config.gridDim = dim3(unsigned(s.clusters * plan.cluster));
+    CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, arguments..., s));
 }
 
 // The widest vectors that the call's addresses and strides allow.
@@ -465,10 +486,10 @@ void group_norm(const NormCall& c, int device, cudaStream_t stream) {
             constexpr int V = decltype(width)::value;
             if constexpr (V * sizeof(T) <= 16) {
                 const NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
-                const SlabPlan plan = slab_plan(s, V, sizeof(T), 1);
+                const SlabPlan plan = slab_plan(s, V, sizeof(T), sizeof(P), 1);
                 if (!plan.cluster) return;
-                launch_slab<k_norm_slab<T, P, V>>(plan, s.instances, device, stream, x, weight, bias, y, c.mean, c.rstd,
-                                                  slab_shape(s, plan, V, c, sizeof(P)));
+                launch_slab<k_norm_slab<T, P, V>>(plan, s, V, c, sizeof(P), static_cast<uint32_t*>(c.workspace), device,
+                                                  stream, x, weight, bias, y, c.mean, c.rstd);
                 done = true;
             }
         });
@@ -511,15 +532,15 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
             constexpr int V = decltype(width)::value;
             if constexpr (V * sizeof(T) <= 16) {
                 const NormShape s = norm_shape(c.instances, c.points, c.channels, c.groups, V);
-                const SlabPlan plan = slab_plan(s, V, sizeof(T), 2);
+                const SlabPlan plan = slab_plan(s, V, sizeof(T), sizeof(P), 2);
                 if (!plan.cluster) return;
-                auto* channel_sums = static_cast<float2*>(c.workspace);
-                launch_slab<k_norm_slab_gradient<T, P, V>>(plan, s.instances, device, stream, grad, x, c.mean, c.rstd,
-                                                           weight, bias, dx, channel_sums,
-                                                           slab_shape(s, plan, V, c, sizeof(P)));
+                auto* counter = static_cast<uint32_t*>(c.workspace);
+                auto* channel_sums = reinterpret_cast<float2*>(static_cast<char*>(c.workspace) + padded(4));
+                launch_slab<k_norm_slab_gradient<T, P, V>>(plan, s, V, c, sizeof(P), counter, device, stream, grad, x,
+                                                           c.mean, c.rstd, weight, bias, dx, channel_sums);
                 if (parameter_blocks) {
-                    k_norm_parameters<P><<<parameter_blocks, NORM_THREADS, 0, stream>>>(dweight, dbias, channel_sums,
-                                                                                         s.instances, s.channels);
+                    k_norm_parameters<P><<<parameter_blocks, 1024, 0, stream>>>(
+                        dweight, dbias, channel_sums, s.instances * plan.cluster, s.channels);
                     CPDE_LAUNCHED();
                 }
                 done = true;
