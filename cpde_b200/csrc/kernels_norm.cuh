@@ -43,18 +43,29 @@ __device__ __forceinline__ int32_t length_of(const NormShape& s, int32_t n) {
     return l < 0 ? 0 : l < s.points ? l : s.points;
 }
 
-// 1 / (1 + e^-z) of V values, from the special function unit's exponential and
-// reciprocal (a few 2^-23 off): an IEEE reciprocal alone would take as many
-// instructions as the rest of an element.
+// Calls f with the activation as a compile-time constant: the loops over points
+// hold no branch on it.
+template <class F>
+__device__ __forceinline__ void with_activation(int32_t activation, F&& f) {
+    if (activation == SILU) f(std::integral_constant<int32_t, SILU>{});
+    else if (activation == SIGMOID) f(std::integral_constant<int32_t, SIGMOID>{});
+    else if (activation == TANH) f(std::integral_constant<int32_t, TANH>{});
+    else f(std::integral_constant<int32_t, LINEAR>{});
+}
+
+constexpr float LOG2_E = 1.4426950408889634f;
+
+// 1 / (1 + 2^t) of V values, a sigmoid of z for t = -log2(e) z, from the special
+// function unit's exponential and reciprocal (a few 2^-23 off): an IEEE
+// reciprocal alone would take as many instructions as the rest of an element.
 template <int V>
-__device__ __forceinline__ Pairs<V> sigmoid(const Pairs<V>& z) {
+__device__ __forceinline__ Pairs<V> sigmoid2(const Pairs<V>& t) {
     Pairs<V> f;
-#pragma unroll
-    for (int i = 0; i < Pairs<V>::N; ++i) f.p[i] = __fmul2_rn(z.p[i], both(-1.4426950408889634f));
+    f.fill(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(f.get(j)));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t.get(j)));
         f.set(j, e);
     }
 #pragma unroll
@@ -68,40 +79,49 @@ __device__ __forceinline__ Pairs<V> sigmoid(const Pairs<V>& z) {
     return f;
 }
 
-template <int V>
-__device__ __forceinline__ void activate(Pairs<V>& z, int32_t activation) {
-    constexpr int N = Pairs<V>::N;
-    if (activation == SILU) {
-        const Pairs<V> f = sigmoid<V>(z);
+// What the weights and biases of z are scaled by, so that the activation's
+// argument comes out of the normalisation's own multiply-add: the forward's
+// sigmoid, and the gradients of both, want t.
+template <int32_t ACTIVATION, bool GRADIENT>
+__device__ constexpr float argument_scale() {
+    return ACTIVATION == SIGMOID || (GRADIENT && ACTIVATION == SILU) ? -LOG2_E : 1.0f;
+}
+
+// act(z) of z argument_scale.
+template <int32_t ACTIVATION, int V>
+__device__ __forceinline__ void activate(Pairs<V>& z) {
+    if constexpr (ACTIVATION == SILU) {
+        Pairs<V> t = z;
+        scale<V>(t, -LOG2_E);
+        t = sigmoid2<V>(t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) z.p[i] = __fmul2_rn(z.p[i], f.p[i]);
-    } else if (activation == SIGMOID) {
-        z = sigmoid<V>(z);
-    } else if (activation == TANH) {
+        for (int i = 0; i < Pairs<V>::N; ++i) z.p[i] = __fmul2_rn(z.p[i], t.p[i]);
+    } else if constexpr (ACTIVATION == SIGMOID) {
+        z = sigmoid2<V>(z);
+    } else if constexpr (ACTIVATION == TANH) {
 #pragma unroll
         for (int j = 0; j < V; ++j) z.set(j, tanhf(z.get(j)));
     }
 }
 
-// h *= act'(z): f (1 + z (1 - f)), f (1 - f) or 1 - t^2.
-template <int V>
-__device__ __forceinline__ void activate_gradient(Pairs<V>& h, const Pairs<V>& z, int32_t activation) {
-    constexpr int N = Pairs<V>::N;
-    if (activation == SILU || activation == SIGMOID) {
-        const Pairs<V> f = sigmoid<V>(z);
+// h *= act'(z), from t = z argument_scale: f + f (1 - f) z, f (1 - f) or 1 - tanh(z)^2.
+template <int32_t ACTIVATION, int V>
+__device__ __forceinline__ void activate_gradient(Pairs<V>& h, const Pairs<V>& t) {
+    if constexpr (ACTIVATION == SILU || ACTIVATION == SIGMOID) {
+        const Pairs<V> f = sigmoid2<V>(t);
+        constexpr float by = ACTIVATION == SILU ? -1.0f / LOG2_E : 1.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float2 back = __ffma2_rn(f.p[i], both(-1.0f), both(1.0f));
-            const float2 slope = activation == SILU
-                                     ? __ffma2_rn(f.p[i], __fmul2_rn(z.p[i], back), f.p[i])
-                                     : __fmul2_rn(f.p[i], back);
+        for (int i = 0; i < Pairs<V>::N; ++i) {
+            const float2 back = __ffma2_rn(f.p[i], both(-by), both(by));
+            const float2 slope = ACTIVATION == SILU ? __ffma2_rn(f.p[i], __fmul2_rn(t.p[i], back), f.p[i])
+                                                    : __fmul2_rn(f.p[i], back);
             h.p[i] = __fmul2_rn(h.p[i], slope);
         }
-    } else if (activation == TANH) {
+    } else if constexpr (ACTIVATION == TANH) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float t = tanhf(z.get(j));
-            h.set(j, h.get(j) * fmaf(-t, t, 1.0f));
+            const float y = tanhf(t.get(j));
+            h.set(j, h.get(j) * fmaf(-y, y, 1.0f));
         }
     }
 }
@@ -235,16 +255,25 @@ struct Terms {
 };
 
 // factor drop(act(z)) of a vector of x.
-template <int V, bool ONE>
-__device__ __forceinline__ void norm_value(Pairs<V>& f, const Terms<V, ONE>& k, uint64_t at, const NormShape& s) {
+template <int32_t ACTIVATION, bool DROPS, int V, bool ONE>
+__device__ __forceinline__ void norm_value(Pairs<V>& f, const Terms<V, ONE>& k, uint64_t at, const DropoutRule& rule) {
 #pragma unroll
     for (int i = 0; i < Pairs<V>::N; ++i)
         f.p[i] = __ffma2_rn(__fadd2_rn(f.p[i], k.minus_mean.of(i)), k.gain.p[i], k.bias.p[i]);
-    activate<V>(f, s.activation);
-    if (s.rule.threshold) {
-        drop_at<V>(f, at, s.rule);
-        scale<V>(f, s.rule.factor);
+    activate<ACTIVATION, V>(f);
+    if constexpr (DROPS) {
+        drop_at<V>(f, at, rule);
+        scale<V>(f, rule.factor);
     }
+}
+
+// Calls f(activation, whether there is dropout), both as constants.
+template <class F>
+__device__ __forceinline__ void with_tail(const NormShape& s, F&& f) {
+    with_activation(s.activation, [&](auto activation) {
+        if (s.rule.threshold) f(activation, std::true_type{});
+        else f(activation, std::false_type{});
+    });
 }
 
 // y = drop(act(norm(x))). The block first joins the moments of its groups'
@@ -301,30 +330,55 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict
     const T* from = x + n * s.x_instance + channel;
     const int64_t row = int64_t(n) * s.points;
     // From the back: the moments' pass has left the ends of the ranges in L2.
-#pragma unroll 4
-    for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
-        const int64_t at = (row + p) * s.channels + channel;
-        if (p >= length) {
-            store<T, V>(y + at, zeros<T, V>());
-            continue;
+    with_tail(s, [&](auto activation, auto drops) {
+        constexpr int32_t ACTIVATION = decltype(activation)::value;
+        Terms<V, ONE> scaled = k;
+        if constexpr (argument_scale<ACTIVATION, false>() != 1.0f) {
+            scale<V>(scaled.gain, argument_scale<ACTIVATION, false>());
+            scale<V>(scaled.bias, argument_scale<ACTIVATION, false>());
         }
-        Pairs<V> f = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
-        norm_value<V, ONE>(f, k, uint64_t(at), s);
-        store<T, V>(y + at, pack_pairs<T, V>(f));
-    }
+#pragma unroll 4
+        for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
+            const int64_t at = (row + p) * s.channels + channel;
+            if (p >= length) {
+                store<T, V>(y + at, zeros<T, V>());
+                continue;
+            }
+            Pairs<V> f = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
+            norm_value<ACTIVATION, decltype(drops)::value, V, ONE>(f, scaled, uint64_t(at), s.rule);
+            store<T, V>(y + at, pack_pairs<T, V>(f));
+        }
+    });
 }
 
-// Terms of the gradient: xhat = (x - mean) rstd, z = xhat weight + bias.
+// Terms of the gradient. With d = x - mean: z = d gain + bias, gain = weight rstd,
+// and xhat = d rstd stays unformed: rstd goes into what multiplies d.
 template <int V, bool ONE>
 struct AdjointTerms {
     GroupTerms<V, ONE> minus_mean, rstd;
-    Pairs<V> weight, bias;
+    Pairs<V> gain, bias;
+    __device__ __forceinline__ float rstd_of(int j) const { return j % 2 ? rstd.of(j / 2).y : rstd.of(j / 2).x; }
+    __device__ __forceinline__ void set_gain(const Pairs<V>& weight) {
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::N; ++i) gain.p[i] = __fmul2_rn(weight.p[i], rstd.of(i));
+    }
+    // For an activation's argument.
+    template <int32_t ACTIVATION>
+    __device__ __forceinline__ AdjointTerms scaled() const {
+        AdjointTerms k = *this;
+        if constexpr (argument_scale<ACTIVATION, true>() != 1.0f) {
+            scale<V>(k.gain, argument_scale<ACTIVATION, true>());
+            scale<V>(k.bias, argument_scale<ACTIVATION, true>());
+        }
+        return k;
+    }
 };
 
 template <class P, int V, bool ONE>
 __device__ __forceinline__ void load_terms(AdjointTerms<V, ONE>& k, const NormShape& s, int32_t n, int32_t channel,
                                            const float* mean, const float* rstd, const P* weight, const P* bias) {
-    k.weight.fill(0.0f);
+    Pairs<V> w;
+    w.fill(0.0f);
     k.bias.fill(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -333,42 +387,62 @@ __device__ __forceinline__ void load_terms(AdjointTerms<V, ONE>& k, const NormSh
             k.minus_mean.set(j, -mean[g]);
             k.rstd.set(j, rstd[g]);
         }
-        k.weight.set(j, parameter(weight, channel + j, 1.0f));
+        w.set(j, parameter(weight, channel + j, 1.0f));
         k.bias.set(j, parameter(bias, channel + j, 0.0f));
     }
+    k.set_gain(w);
 }
 
-// xhat, and in h the kept gradients times act'(z), not yet scaled by the
-// dropout's factor.
-template <int V, bool ONE>
-__device__ __forceinline__ void norm_adjoint(Pairs<V>& xhat, Pairs<V>& h, const AdjointTerms<V, ONE>& k,
-                                             int32_t activation) {
-    Pairs<V> z;
+// From x and the kept gradients in h: d, and h act'(z), not yet scaled by the
+// dropout's factor. `k` is scaled for the activation.
+template <int32_t ACTIVATION, int V, bool ONE>
+__device__ __forceinline__ void norm_adjoint(Pairs<V>& d, Pairs<V>& h, const AdjointTerms<V, ONE>& k) {
+    Pairs<V> t;
 #pragma unroll
     for (int i = 0; i < Pairs<V>::N; ++i) {
-        xhat.p[i] = __fmul2_rn(__fadd2_rn(xhat.p[i], k.minus_mean.of(i)), k.rstd.of(i));
-        z.p[i] = __ffma2_rn(xhat.p[i], k.weight.p[i], k.bias.p[i]);
+        d.p[i] = __fadd2_rn(d.p[i], k.minus_mean.of(i));
+        if constexpr (ACTIVATION != LINEAR) t.p[i] = __ffma2_rn(d.p[i], k.gain.p[i], k.bias.p[i]);
     }
-    activate_gradient<V>(h, z, activation);
+    if constexpr (ACTIVATION != LINEAR) activate_gradient<ACTIVATION, V>(h, t);
 }
+
+// A thread's sums of h and of h xhat by channel.
+template <int V, bool ONE>
+struct AdjointSums {
+    Pairs<V> h, hd;
+    __device__ __forceinline__ AdjointSums() {
+        h.fill(0.0f);
+        hd.fill(0.0f);
+    }
+    __device__ __forceinline__ void add(const Pairs<V>& d, const Pairs<V>& values) {
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::N; ++i) {
+            h.p[i] = __fadd2_rn(h.p[i], values.p[i]);
+            hd.p[i] = __ffma2_rn(values.p[i], d.p[i], hd.p[i]);
+        }
+    }
+    __device__ __forceinline__ float2 of(int j, const AdjointTerms<V, ONE>& k, float factor) const {
+        return make_float2(h.get(j) * factor, hd.get(j) * factor * k.rstd_of(j));
+    }
+};
 
 // dx = rstd (factor w h - (m1 + xhat m2)) as two products and sums.
 template <int V, bool ONE>
 struct InputTerms {
     Pairs<V> gain;              // factor w rstd
-    GroupTerms<V, ONE> m1, m2;  // -rstd m1, -rstd m2
+    GroupTerms<V, ONE> m1, m2;  // -rstd m1, -rstd^2 m2
     __device__ __forceinline__ void set(const AdjointTerms<V, ONE>& k, int j, float2 m, float factor) {
-        const float r = j % 2 ? k.rstd.of(j / 2).y : k.rstd.of(j / 2).x;
-        gain.set(j, factor * r * k.weight.get(j));
+        const float r = k.rstd_of(j);
+        gain.set(j, factor * k.gain.get(j));
         if (!ONE || j == 0) {
             m1.set(j, -r * m.x);
-            m2.set(j, -r * m.y);
+            m2.set(j, -r * r * m.y);
         }
     }
-    __device__ __forceinline__ void apply(Pairs<V>& h, const Pairs<V>& xhat) const {
+    __device__ __forceinline__ void apply(Pairs<V>& h, const Pairs<V>& d) const {
 #pragma unroll
         for (int i = 0; i < Pairs<V>::N; ++i)
-            h.p[i] = __ffma2_rn(h.p[i], gain.p[i], __ffma2_rn(xhat.p[i], m2.of(i), m1.of(i)));
+            h.p[i] = __ffma2_rn(h.p[i], gain.p[i], __ffma2_rn(d.p[i], m2.of(i), m1.of(i)));
     }
 };
 
@@ -395,28 +469,24 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict_
         const int32_t channel = t.first + tx * V;
         AdjointTerms<V, ONE> k;
         load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
-        Pairs<V> sh, sx;
-        sh.fill(0.0f);
-        sx.fill(0.0f);
+        AdjointSums<V, ONE> sums;
         const T* from = x + n * s.x_instance + channel;
         const T* gfrom = grad + n * s.grad_instance + channel;
+        with_tail(s, [&](auto activation, auto drops) {
+            constexpr int32_t ACTIVATION = decltype(activation)::value;
+            const auto scaled = k.template scaled<ACTIVATION>();
 #pragma unroll 2
-        for (int32_t p = lo + ty; p < hi; p += ys) {
-            Pairs<V> xhat = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
-            Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
-            if (s.rule.threshold)
-                drop_at<V>(h, uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s.rule);
-            norm_adjoint<V, ONE>(xhat, h, k, s.activation);
-#pragma unroll
-            for (int i = 0; i < Pairs<V>::N; ++i) {
-                sh.p[i] = __fadd2_rn(sh.p[i], h.p[i]);
-                sx.p[i] = __ffma2_rn(h.p[i], xhat.p[i], sx.p[i]);
+            for (int32_t p = lo + ty; p < hi; p += ys) {
+                Pairs<V> d = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
+                Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
+                if constexpr (decltype(drops)::value)
+                    drop_at<V>(h, uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s.rule);
+                norm_adjoint<ACTIVATION, V, ONE>(d, h, scaled);
+                sums.add(d, h);
             }
-        }
-        scale<V>(sh, s.rule.factor);
-        scale<V>(sx, s.rule.factor);
+        });
 #pragma unroll
-        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = make_float2(sh.get(j), sx.get(j));
+        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = sums.of(j, k, s.rule.factor);
     }
     __syncthreads();
     for (int32_t c = threadIdx.x; c < t.count; c += NORM_THREADS) {
@@ -527,20 +597,24 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
     const T* from = x + n * s.x_instance + channel;
     const T* gfrom = grad + n * s.grad_instance + channel;
     // From the back, as the forward.
+    with_tail(s, [&](auto activation, auto drops) {
+        constexpr int32_t ACTIVATION = decltype(activation)::value;
+        const auto scaled = k.template scaled<ACTIVATION>();
 #pragma unroll 2
-    for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
-        const int64_t at = (int64_t(n) * s.points + p) * s.channels + channel;
-        if (p >= length) {
-            store<T, V>(dx + at, zeros<T, V>());
-            continue;
+        for (int32_t p = hi - 1 - ty; p >= lo; p -= ys) {
+            const int64_t at = (int64_t(n) * s.points + p) * s.channels + channel;
+            if (p >= length) {
+                store<T, V>(dx + at, zeros<T, V>());
+                continue;
+            }
+            Pairs<V> d = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
+            Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
+            if constexpr (decltype(drops)::value) drop_at<V>(h, uint64_t(at), s.rule);
+            norm_adjoint<ACTIVATION, V, ONE>(d, h, scaled);
+            to_input.apply(h, d);
+            store<T, V>(dx + at, pack_pairs<T, V>(h));
         }
-        Pairs<V> xhat = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
-        Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
-        if (s.rule.threshold) drop_at<V>(h, uint64_t(at), s.rule);
-        norm_adjoint<V, ONE>(xhat, h, k, s.activation);
-        to_input.apply(h, xhat);
-        store<T, V>(dx + at, pack_pairs<T, V>(h));
-    }
+    });
 }
 
 }  // namespace cpde::ops

@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 
 constexpr int SLAB_THREADS = 128;
 constexpr int SLAB_WARPS = SLAB_THREADS / 32;
-constexpr int SLAB_BLOCKS = 6;  // CTAs of an SM
+constexpr int SLAB_BLOCKS = 6, SLAB_GRADIENT_BLOCKS = 3;  // CTAs of an SM
 
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* shared, const void* global) {
@@ -113,10 +113,11 @@ struct Item {
     }
 };
 
-template <class T, int V>
+template <class T, int V, int ARRAYS = 1>
 __device__ __forceinline__ void copy_points(Vector<T, V>* slots, const T* from, int64_t step, int32_t count) {
 #pragma unroll 4
-    for (int32_t i = 0; i < count; ++i, from += step, slots += SLAB_THREADS) copy_async<sizeof(T) * V>(slots, from);
+    for (int32_t i = 0; i < count; ++i, from += step, slots += ARRAYS * SLAB_THREADS)
+        copy_async<sizeof(T) * V>(slots, from);
 }
 
 // The tile's weights and biases in shared memory, and for the gradient its means
@@ -333,17 +334,25 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
             }
             k.minus_mean.set(0, -statistics.x);
             scale<V>(k.gain, statistics.y);
-            int64_t to = at.index(s, seat);
-#pragma unroll 2
-            for (int32_t i = 0; i < at.count; ++i, to += step, slot += SLAB_THREADS) {
-                Pairs<V> f = unpack_pairs<T, V>(*slot);
-                norm_value<V, true>(f, k, uint64_t(to), s.norm);
-                store<T, V>(y + to, pack_pairs<T, V>(f));
-                if (i < then.count) {
-                    copy_async<sizeof(Slot)>(slot, from);
-                    from += read_step;
+            with_tail(s.norm, [&](auto activation, auto drops) {
+                constexpr int32_t ACTIVATION = decltype(activation)::value;
+                if constexpr (argument_scale<ACTIVATION, false>() != 1.0f) {
+                    scale<V>(k.gain, argument_scale<ACTIVATION, false>());
+                    scale<V>(k.bias, argument_scale<ACTIVATION, false>());
                 }
-            }
+                const int64_t index = at.index(s, seat);
+                T* to = y + index;
+#pragma unroll 2
+                for (int32_t i = 0; i < at.count; ++i, to += step, slot += SLAB_THREADS) {
+                    Pairs<V> f = unpack_pairs<T, V>(*slot);
+                    norm_value<ACTIVATION, decltype(drops)::value, V, true>(f, k, uint64_t(to - y), s.norm.rule);
+                    store<T, V>(to, pack_pairs<T, V>(f));
+                    if (i < then.count) {
+                        copy_async<sizeof(Slot)>(slot, from);
+                        from += read_step;
+                    }
+                }
+            });
         }
         if (!more) break;
         copy_points<T, V>(slot, from, read_step, then.count - at.count);
@@ -357,14 +366,16 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
 __host__ __device__ inline bool slab_rows_are_warps(int32_t tile) { return tile <= 32 && (tile & (tile - 1)) == 0; }
 
 template <class T, class P, int V>
-__global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab_gradient(
+__global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_slab_gradient(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const P* __restrict__ weight, const P* __restrict__ bias, T* __restrict__ dx,
     float2* __restrict__ channel_sums, SlabShape s) {
     extern __shared__ __align__(16) unsigned char slab[];
     using Slot = Vector<T, V>;
+    // A slot of x and one of the gradient in turn.
     Slot* data = reinterpret_cast<Slot*>(slab) + threadIdx.x;
-    Slot* grads = data + size_t(s.slots) * SLAB_THREADS;
+    Slot* grads = data + SLAB_THREADS;
+    constexpr int32_t NEXT = 2 * SLAB_THREADS;
     const int32_t width = s.tile_channels;
     const bool warps = slab_rows_are_warps(s.norm.tile);
     const int32_t rows = warps ? SLAB_WARPS : s.ys;
@@ -389,8 +400,8 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab_gradien
     };
     Item<V> at(s, seat, seat.cluster, item_length(s, seat.cluster));
     fetch_parameters(at);
-    copy_points<T, V>(data, at.in(x, seat, s.norm.x_instance, s.norm.x_point), x_step, at.count);
-    copy_points<T, V>(grads, at.in(grad, seat, s.norm.grad_instance, s.norm.grad_point), grad_step, at.count);
+    copy_points<T, V, 2>(data, at.in(x, seat, s.norm.x_instance, s.norm.x_point), x_step, at.count);
+    copy_points<T, V, 2>(grads, at.in(grad, seat, s.norm.grad_instance, s.norm.grad_point), grad_step, at.count);
     cluster_arrive();
     bool started = false;
     for (int32_t turn = 0;; turn ^= 1) {
@@ -404,36 +415,33 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab_gradien
     AdjointTerms<V, true> k;
     k.minus_mean.set(0, at.active ? -tile.mean[seat.group] : 0.0f);
     k.rstd.set(0, at.active ? tile.rstd[seat.group] : 0.0f);
-    k.weight = stored_parameters<P, V>(tile.weight + seat.tx * V, weight, 1.0f);
+    k.set_gain(stored_parameters<P, V>(tile.weight + seat.tx * V, weight, 1.0f));
     k.bias = stored_parameters<P, V>(tile.bias + seat.tx * V, bias, 0.0f);
     const int32_t next_length = dealer ? item_length(s, next) : 0;
-    Pairs<V> sh, sx;
-    sh.fill(0.0f);
-    sx.fill(0.0f);
-    {
-        int64_t index = at.index(s, seat);
-        Slot *slot = data, *gslot = grads;
+    AdjointSums<V, true> sums_of;
+    with_tail(s.norm, [&](auto activation, auto drops) {
+        constexpr int32_t ACTIVATION = decltype(activation)::value;
+        const auto scaled = k.template scaled<ACTIVATION>();
+        uint64_t index = uint64_t(at.index(s, seat));
+        Slot* slot = data;
 #pragma unroll 2
-        for (int32_t i = 0; i < at.count; ++i, index += step, slot += SLAB_THREADS, gslot += SLAB_THREADS) {
-            Pairs<V> xhat = unpack_pairs<T, V>(*slot), h = unpack_pairs<T, V>(*gslot);
-            if (s.norm.rule.threshold) {
-                drop_at<V>(h, uint64_t(index), s.norm.rule);
-                *gslot = pack_pairs<T, V>(h);  // exact; the second pass finds the zeros and need not draw again
+        for (int32_t i = 0; i < at.count; ++i, index += step, slot += NEXT) {
+            Pairs<V> d = unpack_pairs<T, V>(slot[0]), h = unpack_pairs<T, V>(slot[SLAB_THREADS]);
+            if constexpr (decltype(drops)::value) {
+                drop_at<V>(h, index, s.norm.rule);
+                // Exact; the second pass finds the zeros and need not draw again.
+                slot[SLAB_THREADS] = pack_pairs<T, V>(h);
             }
-            norm_adjoint<V, true>(xhat, h, k, s.norm.activation);
-#pragma unroll
-            for (int j = 0; j < Pairs<V>::N; ++j) {
-                sh.p[j] = __fadd2_rn(sh.p[j], h.p[j]);
-                sx.p[j] = __ffma2_rn(h.p[j], xhat.p[j], sx.p[j]);
-            }
+            norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
+            sums_of.add(d, h);
         }
-    }
+    });
     // Sums over the points, by channel: within a warp where its lanes repeat the
     // tile's vectors (each step halves the values that a lane keeps), then over
     // the rows that are left.
     float2 sum[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = make_float2(sh.get(j), sx.get(j));
+    for (int j = 0; j < V; ++j) sum[j] = sums_of.of(j, k, s.norm.rule.factor);
     if (warps) {
         int32_t kept = 0;  // the first of the channels that the lane keeps
         int32_t d = 16;
@@ -461,11 +469,9 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab_gradien
         for (int j = 0; j < V; ++j) parts[seat.ty * width + seat.tx * V + j] = sum[j];
     }
     __syncthreads();
-    const float2 factor = both(s.norm.rule.factor);
     for (int32_t c = threadIdx.x; c < at.channels; c += SLAB_THREADS) {
         float2 v = parts[c];
         for (int32_t r = 1; r < rows; ++r) v = __fadd2_rn(v, parts[r * width + c]);
-        v = __fmul2_rn(v, factor);
         channel_sums[(int64_t(at.n) * s.cluster + seat.rank) * s.norm.channels + at.first_channel + c] = v;
         sums[c] = __fmul2_rn(v, both(weight ? to_float(tile.weight[c]) : 1.0f));
     }
@@ -494,31 +500,35 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab_gradien
     if (more) fetch_parameters(then);
     const T* from = then.in(x, seat, s.norm.x_instance, s.norm.x_point);
     const T* gfrom = then.in(grad, seat, s.norm.grad_instance, s.norm.grad_point);
-    Slot *slot = data, *gslot = grads;
+    Slot* slot = data;
     if (at.active) {
         const float inverse = at.length ? 1.0f / (float(at.length) * float(s.norm.width)) : 0.0f;
         means = __fmul2_rn(means, both(inverse));
         InputTerms<V, true> to_input;
 #pragma unroll
         for (int j = 0; j < V; ++j) to_input.set(k, j, means, s.norm.rule.factor);
-        int64_t to = at.index(s, seat);
+        with_activation(s.norm.activation, [&](auto activation) {
+            constexpr int32_t ACTIVATION = decltype(activation)::value;
+            const auto scaled = k.template scaled<ACTIVATION>();
+            T* to = dx + at.index(s, seat);
 #pragma unroll 2
-        for (int32_t i = 0; i < at.count; ++i, to += step, slot += SLAB_THREADS, gslot += SLAB_THREADS) {
-            Pairs<V> xhat = unpack_pairs<T, V>(*slot), h = unpack_pairs<T, V>(*gslot);
-            norm_adjoint<V, true>(xhat, h, k, s.norm.activation);
-            to_input.apply(h, xhat);
-            store<T, V>(dx + to, pack_pairs<T, V>(h));
-            if (i < then.count) {
-                copy_async<sizeof(Slot)>(slot, from);
-                copy_async<sizeof(Slot)>(gslot, gfrom);
-                from += x_step;
-                gfrom += grad_step;
+            for (int32_t i = 0; i < at.count; ++i, to += step, slot += NEXT) {
+                Pairs<V> d = unpack_pairs<T, V>(slot[0]), h = unpack_pairs<T, V>(slot[SLAB_THREADS]);
+                norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
+                to_input.apply(h, d);
+                store<T, V>(to, pack_pairs<T, V>(h));
+                if (i < then.count) {
+                    copy_async<sizeof(Slot)>(slot, from);
+                    copy_async<sizeof(Slot)>(slot + SLAB_THREADS, gfrom);
+                    from += x_step;
+                    gfrom += grad_step;
+                }
             }
-        }
+        });
     }
     if (!more) break;
-    copy_points<T, V>(slot, from, x_step, then.count - at.count);
-    copy_points<T, V>(gslot, gfrom, grad_step, then.count - at.count);
+    copy_points<T, V, 2>(slot, from, x_step, then.count - at.count);
+    copy_points<T, V, 2>(slot + SLAB_THREADS, gfrom, grad_step, then.count - at.count);
     at = then;
     }
 }

@@ -362,7 +362,7 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, size_t parameter, 
         return p.shared;
     };
     int32_t cluster = 0;
-    for (size_t limit : {SLAB_SIX, SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
+    for (size_t limit : {arrays == 1 ? SLAB_SIX : SLAB_THREE, SLAB_THREE, SLAB_TWO, SLAB_ONE}) {
         for (int32_t c = 1; c <= SLAB_CLUSTER && !cluster; c *= 2)
             if (plan(c) <= limit) cluster = c;
         if (cluster) break;
