@@ -18,6 +18,7 @@ enum Activation : int32_t { SIGMOID = 0, LINEAR = 1, TANH = 2, SILU = 3 };
 
 constexpr int NORM_THREADS = 256;
 constexpr int NORM_WARPS = NORM_THREADS / 32;
+constexpr int NORM_BLOCKS = 4;  // CTAs of an SM; a launch has as many as the GPU holds at once
 
 struct NormShape {
     int64_t x_point, x_instance, grad_point, grad_instance;  // strides in elements
@@ -170,7 +171,7 @@ __device__ __forceinline__ Tile tile_of(const NormShape& s, int32_t tile) {
 // Moments of each piece of a group in a block's points and channels.
 // pieces[instance][split][tile][piece] = (count, mean, m2).
 template <class T, int V>
-__global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(const T* __restrict__ x, NormShape s,
+__global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_moments(const T* __restrict__ x, NormShape s,
                                                                 Moments* __restrict__ pieces) {
     extern __shared__ float norm_shared[];  // [ty][channel of the tile] x (mean, m2)
     const int32_t split = blockIdx.x % s.splits, n = blockIdx.x / s.splits;
@@ -280,7 +281,7 @@ __device__ __forceinline__ void with_tail(const NormShape& s, F&& f) {
 // pieces; the first split of the tile that holds a group's first channel also
 // writes mean and rstd.
 template <class T, class P, int V, bool ONE>
-__global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(const T* __restrict__ x, const P* __restrict__ weight,
+__global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_apply(const T* __restrict__ x, const P* __restrict__ weight,
                                                               const P* __restrict__ bias, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd,
                                                               const Moments* __restrict__ pieces, NormShape s) {
@@ -450,7 +451,7 @@ struct InputTerms {
 // (channel_sums[instance][split][channel]), and times w per piece of a group
 // for dx (pieces[instance][split][tile][piece]).
 template <class T, class P, int V, bool ONE>
-__global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(const T* __restrict__ grad, const T* __restrict__ x,
+__global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T* __restrict__ grad, const T* __restrict__ x,
                                                              const float* __restrict__ mean,
                                                              const float* __restrict__ rstd,
                                                              const P* __restrict__ weight, const P* __restrict__ bias,
@@ -543,7 +544,7 @@ __device__ __forceinline__ void sum_parameters(P* __restrict__ dweight, P* __res
 // dx, and in the blocks behind those of the last instance dw and db: 32
 // channels each, summed over instances and splits in a fixed order.
 template <class T, class P, int V, bool ONE>
-__global__ void __launch_bounds__(NORM_THREADS) k_norm_input_gradient(
+__global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradient(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const P* __restrict__ weight, const P* __restrict__ bias, T* __restrict__ dx,
     P* __restrict__ dweight, P* __restrict__ dbias, const float2* __restrict__ channel_sums,
