@@ -47,30 +47,40 @@ __global__ void __launch_bounds__(256) k_embedding(const TI* __restrict__ table,
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 
-// Two buffers of (row, token) pairs that the passes of the sort alternate
-// between, pass p writing buffer p % 2.
-struct SortBuffers {
-    uint32_t* row[2];
-    uint32_t* token[2];
-};
-__host__ __device__ inline int sorted_buffer(int passes) { return (passes - 1) & 1; }
-
 // Row of a token; absent ids sort behind every row, as row `rows`.
 template <class Id>
 __device__ __forceinline__ uint32_t row_of(Id id, int64_t rows) {
     return uint32_t(int64_t(id) >= 0 && int64_t(id) < rows ? int64_t(id) : rows);
 }
 
-// What a pass of the sort reads: the ids themselves at first, then the pairs
-// that the pass before wrote.
+// (row, token) pairs. The passes of a sort alternate between two buffers, pass p
+// writing buffer p % 2; the first reads the ids themselves.
+__host__ __device__ inline int sorted_buffer(int passes) { return (passes - 1) & 1; }
 template <class Id>
 struct SortInput {
     const Id* ids;
     int64_t rows;
-    const uint32_t *row, *token;  // null in the first pass
-    __device__ __forceinline__ uint32_t row_at(uint32_t i) const { return row ? row[i] : row_of(ids[i], rows); }
-    __device__ __forceinline__ uint32_t token_at(uint32_t i) const { return row ? token[i] : i; }
+    const uint2* pairs;  // null in the first pass
+    __device__ __forceinline__ uint2 at(uint32_t i) const {
+        return pairs ? pairs[i] : make_uint2(row_of(ids[i], rows), i);
+    }
 };
+
+// The table's gradient is cleared where no token adds to it. Of a large one the
+// sort's launches clear the first words whole while memory idles, and the sums'
+// launch the rows behind those that have no bit in `present`.
+struct Clearing {
+    uint4* words;        // the table's gradient
+    int64_t whole;       // words that the sort clears
+    uint32_t* present;   // a bit for each row, or null: the sort clears all
+    uint32_t present_words;
+};
+__device__ __forceinline__ void clear_words(uint4* words, int64_t from, int64_t to, int64_t first, int64_t step) {
+    for (int64_t i = from + first; i < to; i += step) words[i] = make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void mark_present(const Clearing& clearing, uint32_t row, int64_t rows) {
+    if (clearing.present && row < rows) atomicOr(&clearing.present[row / 32], 1u << (row % 32));
+}
 
 // A pass is stable because each warp has a contiguous range of the pairs: a
 // pair's place is (smaller digits anywhere) + (its digit in the CTAs before) +
@@ -78,46 +88,46 @@ struct SortInput {
 // No order depends on timing. SORT_BATCH loads of a lane are in flight at once.
 constexpr int SORT_BATCH = 8;
 
-template <class Id>
+template <class Id, class F>
 __device__ __forceinline__ void count_digits(const SortInput<Id>& in, uint32_t lo, uint32_t hi, uint32_t step,
-                                             int shift, uint32_t mask, uint32_t* histogram) {
+                                             int shift, uint32_t mask, uint32_t* histogram, F&& each) {
     for (uint32_t at = lo; at < hi; at += SORT_BATCH * step) {
         uint32_t r[SORT_BATCH];
 #pragma unroll
-        for (int u = 0; u < SORT_BATCH; ++u) r[u] = at + u * step < hi ? in.row_at(at + u * step) : 0;
+        for (int u = 0; u < SORT_BATCH; ++u) r[u] = at + u * step < hi ? in.at(at + u * step).x : 0;
 #pragma unroll
         for (int u = 0; u < SORT_BATCH; ++u)
-            if (at + u * step < hi) atomicAdd(&histogram[(r[u] >> shift) & mask], 1u);
+            if (at + u * step < hi) {
+                atomicAdd(&histogram[(r[u] >> shift) & mask], 1u);
+                each(r[u]);
+            }
     }
 }
 
-// `place`: this warp's next place for each digit.
+// `place`: this warp's next place in `out` for each digit.
 template <class Id>
 __device__ __forceinline__ void place_pairs(const SortInput<Id>& in, uint32_t lo, uint32_t hi, int shift,
-                                            uint32_t mask, uint32_t* place, uint32_t* __restrict__ row_out,
-                                            uint32_t* __restrict__ token_out) {
+                                            uint32_t mask, uint32_t* place, uint2* out) {
     const uint32_t lane = threadIdx.x % 32;
     for (uint32_t at = lo; at < hi; at += SORT_BATCH * 32) {
-        uint32_t r[SORT_BATCH], token[SORT_BATCH];
+        uint2 pair[SORT_BATCH];
 #pragma unroll
         for (int u = 0; u < SORT_BATCH; ++u) {
             const uint32_t i = at + u * 32 + lane;
-            r[u] = i < hi ? in.row_at(i) : 0;
-            token[u] = i < hi ? in.token_at(i) : 0;
+            pair[u] = i < hi ? in.at(i) : make_uint2(0, 0);
         }
 #pragma unroll
         for (int u = 0; u < SORT_BATCH; ++u) {
             const bool active = at + u * 32 + lane < hi;
             const uint32_t lanes = __ballot_sync(~0u, active);
             if (active) {
-                const uint32_t digit = (r[u] >> shift) & mask;
+                const uint32_t digit = (pair[u].x >> shift) & mask;
                 const uint32_t peers = __match_any_sync(lanes, digit);
                 const uint32_t mine = __popc(peers & ((1u << lane) - 1));
                 const uint32_t to = place[digit] + mine;
                 __syncwarp(lanes);
                 if (mine == 0) place[digit] += __popc(peers);
-                row_out[to] = r[u];
-                token_out[to] = token[u];
+                out[to] = pair[u];
             }
             __syncwarp();
         }
@@ -125,15 +135,17 @@ __device__ __forceinline__ void place_pairs(const SortInput<Id>& in, uint32_t lo
 }
 
 // Exclusive prefix of the warps' counts by digit in shared memory, which become
-// places within the CTA; returns the CTA's count of digit threadIdx.x.
+// places within the digit; returns the CTA's count of digit threadIdx.x.
 __device__ __forceinline__ uint32_t prefix_warps(uint32_t* histogram, uint32_t bins) {
     uint32_t sum = 0;
-    if (threadIdx.x < bins)
+    if (threadIdx.x < bins) {
+#pragma unroll 8
         for (int w = 0; w < SORT_WARPS; ++w) {
             const uint32_t n = histogram[w * bins + threadIdx.x];
             histogram[w * bins + threadIdx.x] = sum;
             sum += n;
         }
+    }
     return sum;
 }
 
@@ -161,23 +173,18 @@ __device__ __forceinline__ uint32_t prefix_block(uint32_t value, uint32_t* warp_
     return scan - value + (warp ? warp_sums[warp - 1] : 0);
 }
 
-__device__ __forceinline__ void clear_words(uint4* words, int64_t from, int64_t to, int64_t first, int64_t step) {
-    for (int64_t i = from + first; i < to; i += step) words[i] = make_uint4(0, 0, 0, 0);
-}
-
 // Few tokens: all passes in one launch, by the first cluster of the grid, whose
 // CTAs exchange their counts through distributed shared memory; the other
-// clusters clear `fill` meanwhile.
+// clusters clear the table's gradient meanwhile.
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restrict__ ids, uint32_t tokens,
                                                                int64_t rows, int passes, int digit_bits,
-                                                               SortBuffers buffers, uint4* __restrict__ fill,
-                                                               int64_t fill_words) {
+                                                               uint2* pairs0, uint2* pairs1, Clearing clearing) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t size = cluster.num_blocks();
     if (blockIdx.x >= size) {
-        clear_words(fill, 0, fill_words, int64_t(blockIdx.x - size) * SORT_THREADS + threadIdx.x,
+        clear_words(clearing.words, 0, clearing.whole, int64_t(blockIdx.x - size) * SORT_THREADS + threadIdx.x,
                     int64_t(gridDim.x - size) * SORT_THREADS);
         return;
     }
@@ -188,16 +195,24 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
     __shared__ uint32_t warp_sums[SORT_WARPS];
     const uint32_t rank = cluster.block_rank();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, bin = threadIdx.x;
+    if (clearing.present) {
+        for (uint32_t i = rank * SORT_THREADS + threadIdx.x; i < clearing.present_words; i += size * SORT_THREADS)
+            clearing.present[i] = 0;
+        __threadfence();
+        cluster.sync();
+    }
     const uint32_t per_warp = (tokens + size * SORT_WARPS - 1) / (size * SORT_WARPS);
     const uint64_t start = uint64_t(rank * SORT_WARPS + warp) * per_warp;
     const uint32_t lo = uint32_t(start < tokens ? start : tokens);
     const uint32_t hi = uint32_t(start + per_warp < tokens ? start + per_warp : tokens);
     for (int pass = 0; pass < passes; ++pass) {
-        const int shift = pass * digit_bits, from = (pass + 1) & 1, to = pass & 1;
-        const SortInput<Id> in = {ids, rows, pass ? buffers.row[from] : nullptr, buffers.token[from]};
+        const int shift = pass * digit_bits;
+        const SortInput<Id> in = {ids, rows, pass == 0 ? nullptr : pass & 1 ? pairs0 : pairs1};
         for (uint32_t i = threadIdx.x; i < SORT_WARPS * bins; i += SORT_THREADS) histogram[i] = 0;
         __syncthreads();
-        count_digits(in, lo + lane, hi, 32, shift, bins - 1, histogram + warp * bins);
+        count_digits(in, lo + lane, hi, 32, shift, bins - 1, histogram + warp * bins, [&](uint32_t r) {
+            if (pass == 0) mark_present(clearing, r, rows);
+        });
         __syncthreads();
         const uint32_t mine = prefix_warps(histogram, bins);
         if (bin < bins) totals[bin] = mine;
@@ -210,10 +225,12 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
                 all += n;
             }
         const uint32_t base = prefix_block(all, warp_sums) + before;
-        if (bin < bins)
+        if (bin < bins) {
+#pragma unroll 8
             for (int w = 0; w < SORT_WARPS; ++w) histogram[w * bins + bin] += base;
+        }
         __syncthreads();
-        place_pairs(in, lo, hi, shift, bins - 1, histogram + warp * bins, buffers.row[to], buffers.token[to]);
+        place_pairs(in, lo, hi, shift, bins - 1, histogram + warp * bins, pass & 1 ? pairs1 : pairs0);
         // Orders this pass's pairs in global memory, and its reads of the other
         // CTAs' totals, before the next pass's.
         __threadfence();
@@ -221,102 +238,157 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
     }
 }
 
-// Many tokens: a pass is two launches over the whole GPU. The first counts the
+// Many tokens: a pass is three launches over the whole GPU. The first counts the
 // digits of each tile (a CTA's range of pairs).
 struct SortPass {
     uint32_t tokens, per_warp, bins;
     int shift;
-    int64_t fill_from, fill_to;  // the words of the output that this launch clears
+    int64_t from, to;  // the words of the table's gradient that this launch clears
 };
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in, SortPass s,
-                                                                uint32_t* __restrict__ counts,
-                                                                uint4* __restrict__ fill) {
+                                                                uint32_t* __restrict__ counts, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
-    clear_words(fill, s.fill_from, s.fill_to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
-                int64_t(gridDim.x) * SORT_THREADS);
+    const int64_t thread = int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x, threads = int64_t(gridDim.x) * SORT_THREADS;
+    clear_words(clearing.words, s.from, s.to, thread, threads);
+    if (clearing.present && !in.pairs)
+        for (int64_t i = thread; i < clearing.present_words; i += threads) clearing.present[i] = 0;
     if (threadIdx.x < s.bins) sort_shared[threadIdx.x] = 0;
     __syncthreads();
     const uint64_t per_tile = uint64_t(s.per_warp) * SORT_WARPS, start = blockIdx.x * per_tile;
     const uint32_t lo = uint32_t(start < s.tokens ? start : s.tokens);
     const uint32_t hi = uint32_t(start + per_tile < s.tokens ? start + per_tile : s.tokens);
-    count_digits(in, lo + threadIdx.x, hi, SORT_THREADS, s.shift, s.bins - 1, sort_shared);
+    count_digits(in, lo + threadIdx.x, hi, SORT_THREADS, s.shift, s.bins - 1, sort_shared, [](uint32_t) {});
     __syncthreads();
     if (threadIdx.x < s.bins) counts[blockIdx.x * s.bins + threadIdx.x] = sort_shared[threadIdx.x];
 }
 
-// The second sums the tiles' counts (each CTA all of them: they stay in L2) and
-// places the pairs.
+// The second replaces the tiles' counts of each digit by their exclusive prefix
+// over the tiles and writes the digits' totals behind them: a warp a digit. (Were
+// each CTA of the third to sum them itself, all of them would read 45 MB from L2
+// where 148 tiles have 512 digits, 9 us.)
+__global__ void __launch_bounds__(256) k_scan_counts(uint32_t* __restrict__ counts, uint32_t tiles, uint32_t bins) {
+    const uint32_t bin = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (bin >= bins) return;
+    uint32_t sum = 0;
+    for (uint32_t base = 0; base < tiles; base += 32 * 8) {
+        uint32_t n[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const uint32_t tile = base + u * 32 + lane;
+            n[u] = tile < tiles ? counts[tile * bins + bin] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            uint32_t scan = n[u];
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const uint32_t v = __shfl_up_sync(~0u, scan, d);
+                if (lane >= uint32_t(d)) scan += v;
+            }
+            const uint32_t tile = base + u * 32 + lane;
+            if (tile < tiles) counts[tile * bins + bin] = sum + scan - n[u];
+            sum += __shfl_sync(~0u, scan, 31);
+        }
+    }
+    if (lane == 0) counts[tiles * bins + bin] = sum;
+}
+
+// The third sorts its tile by the digit in shared memory and writes it out from
+// there, so that pairs of a digit leave side by side.
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in, SortPass s,
                                                                 const uint32_t* __restrict__ counts,
-                                                                uint32_t* __restrict__ row_out,
-                                                                uint32_t* __restrict__ token_out,
-                                                                uint4* __restrict__ fill) {
+                                                                uint2* __restrict__ out, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
-    __shared__ uint32_t warp_sums[SORT_WARPS], sums[2][SORT_THREADS];
-    uint32_t* histogram = sort_shared;  // [warp][bin]
-    clear_words(fill, s.fill_from, s.fill_to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
+    __shared__ uint32_t warp_sums[SORT_WARPS], shift_of[SORT_THREADS];
+    uint2* staged = reinterpret_cast<uint2*>(sort_shared);  // the tile
+    const uint32_t per_tile = s.per_warp * SORT_WARPS;
+    uint32_t* histogram = sort_shared + 2 * per_tile;  // [warp][bin]
+    clear_words(clearing.words, s.from, s.to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
                 int64_t(gridDim.x) * SORT_THREADS);
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, bin = threadIdx.x & (s.bins - 1);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, bin = threadIdx.x;
     for (uint32_t i = threadIdx.x; i < SORT_WARPS * s.bins; i += SORT_THREADS) histogram[i] = 0;
+    const uint32_t prefix = bin < s.bins ? counts[blockIdx.x * s.bins + bin] : 0;
+    const uint32_t total = bin < s.bins ? counts[gridDim.x * s.bins + bin] : 0;
     __syncthreads();
-    const uint64_t start = (uint64_t(blockIdx.x) * SORT_WARPS + warp) * s.per_warp;
+    const uint64_t tile = uint64_t(blockIdx.x) * per_tile, start = tile + uint64_t(warp) * s.per_warp;
     const uint32_t lo = uint32_t(start < s.tokens ? start : s.tokens);
     const uint32_t hi = uint32_t(start + s.per_warp < s.tokens ? start + s.per_warp : s.tokens);
-    count_digits(in, lo + lane, hi, 32, s.shift, s.bins - 1, histogram + warp * s.bins);
-    // Threads with equal bin share the tiles.
-    const uint32_t share = threadIdx.x / s.bins, shares = SORT_THREADS / s.bins;
-    uint32_t before = 0, all = 0;
-#pragma unroll 16
-    for (uint32_t tile = share; tile < gridDim.x; tile += shares) {
-        const uint32_t n = counts[tile * s.bins + bin];
-        before += tile < blockIdx.x ? n : 0;
-        all += n;
+    count_digits(in, lo + lane, hi, 32, s.shift, s.bins - 1, histogram + warp * s.bins, [&](uint32_t r) {
+        if (!in.pairs) mark_present(clearing, r, in.rows);
+    });
+    const uint32_t base = prefix_block(total, warp_sums) + prefix;  // where the tile's pairs of the digit go
+    __syncthreads();
+    const uint32_t mine = prefix_warps(histogram, s.bins);
+    const uint32_t local = prefix_block(mine, warp_sums);  // and where they are staged
+    if (bin < s.bins) {
+        shift_of[bin] = base - local;
+#pragma unroll 8
+        for (int w = 0; w < SORT_WARPS; ++w) histogram[w * s.bins + bin] += local;
     }
-    sums[0][threadIdx.x] = before;
-    sums[1][threadIdx.x] = all;
     __syncthreads();
-    prefix_warps(histogram, s.bins);
-    before = all = 0;
-    if (threadIdx.x < s.bins)
-        for (uint32_t i = threadIdx.x; i < SORT_THREADS; i += s.bins) {
-            before += sums[0][i];
-            all += sums[1][i];
-        }
-    const uint32_t base = prefix_block(all, warp_sums) + before;
-    if (threadIdx.x < s.bins)
-        for (int w = 0; w < SORT_WARPS; ++w) histogram[w * s.bins + threadIdx.x] += base;
+    place_pairs(in, lo, hi, s.shift, s.bins - 1, histogram + warp * s.bins, staged);
     __syncthreads();
-    place_pairs(in, lo, hi, s.shift, s.bins - 1, histogram + warp * s.bins, row_out, token_out);
+    const uint32_t count = tile < s.tokens ? uint32_t(s.tokens - tile < per_tile ? s.tokens - tile : per_tile) : 0;
+    for (uint32_t i = threadIdx.x; i < count; i += SORT_THREADS) {
+        const uint2 pair = staged[i];
+        out[i + shift_of[(pair.x >> s.shift) & (s.bins - 1)]] = pair;
+    }
 }
 
 constexpr uint32_t NO_ROW = 0xffffffffu;
 
-// Segmented sums over the sorted tokens. A group of `lanes` lanes has `chunk`
-// consecutive sorted tokens and `lanes` vectors of V channels, and adds the
-// gradients of a run of equal rows in FP32, in token order. A run inside the
-// chunk is written to the table's gradient; what a run that crosses a chunk's
-// border has in this chunk goes to partial[chunk][0] (runs that began before)
-// or partial[chunk][1] (runs that begin here and go on).
+// Segmented sums over the sorted tokens. A group of `lanes` lanes looks after
+// `chunk` consecutive sorted tokens and `lanes` vectors of V channels: it adds the
+// gradients of each run of equal rows that begins in the chunk, in FP32 and in
+// token order, on into the next chunk where the run ends there. A run that covers
+// a whole chunk behind the one in which it begins is long: each chunk writes
+// what it has of it to partial[chunk][0] (or [1] where it begins), and
+// k_join_chunks adds those.
 constexpr int SUM_BATCH = 8;
 struct SumShape {
     uint32_t tokens, rows, chunk, chunks, vectors, lanes, tiles;
+    uint32_t sum_blocks, clear_from;  // blocks that sum; the first row that the others clear
     int64_t channels, grad_stride;
 };
+
 template <class TI, class TO, int V>
-__global__ void __launch_bounds__(256) k_sum_tokens(const uint32_t* __restrict__ row, const uint32_t* __restrict__ token,
-                                                     const TI* __restrict__ grad, TO* __restrict__ out,
-                                                     float* __restrict__ partial, SumShape s, float scale) {
+__global__ void __launch_bounds__(256) k_sum_tokens(const uint2* __restrict__ pairs, const TI* __restrict__ grad,
+                                                     TO* __restrict__ out, float* __restrict__ partial, SumShape s,
+                                                     Clearing clearing, float scale) {
+    if (blockIdx.x >= s.sum_blocks) {
+        // Rows without a token, a warp a row.
+        const uint32_t warps = (gridDim.x - s.sum_blocks) * 8, lane = threadIdx.x % 32;
+        const int64_t row_words = s.channels * sizeof(TO) / 16;
+        for (uint32_t r = s.clear_from + (blockIdx.x - s.sum_blocks) * 8 + threadIdx.x / 32; r < s.rows; r += warps) {
+            if (clearing.present[r / 32] >> (r % 32) & 1) continue;
+            uint4* to = clearing.words + r * row_words;
+            for (int64_t i = lane; i < row_words; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
     const uint64_t group = (uint64_t(blockIdx.x) * 256 + threadIdx.x) / s.lanes;
     const uint32_t chunk = uint32_t(group / s.tiles), tile = uint32_t(group - uint64_t(chunk) * s.tiles);
     const uint32_t vector = tile * s.lanes + threadIdx.x % s.lanes;
     if (chunk >= s.chunks || vector >= s.vectors) return;
     const int64_t column = int64_t(vector) * V;
-    const uint32_t lo = chunk * s.chunk, hi = min(lo + s.chunk, s.tokens);
-    const uint32_t before = lo ? row[lo - 1] : NO_ROW, after = hi < s.tokens ? row[hi] : NO_ROW;
-    uint32_t current = row[lo];
-    bool continued = current == before;
+    const uint32_t lo = chunk * s.chunk, end = min(lo + s.chunk, s.tokens);
+    auto row_at = [&](uint32_t i) { return pairs[i].x; };
+    uint32_t current = row_at(lo);
+    if (current >= s.rows) return;
+    const uint32_t last = row_at(end - 1);
+    const bool continued = lo && row_at(lo - 1) == current;  // began in a chunk before
+    // Whether the run that ends the chunk, if it begins here, is long; and the one
+    // that begins the chunk, if it began before: it covers this chunk, or it
+    // covers the one before and began before that.
+    const bool tail_long = end + s.chunk <= s.tokens && row_at(end + s.chunk - 1) == last;
+    const bool head_long = continued && ((last == current && end - lo == s.chunk) ||
+                                         (lo > s.chunk && row_at(lo - s.chunk - 1) == current));
+    uint32_t stop = end;  // of what this group adds
+    if (!tail_long && end < s.tokens && last < s.rows && row_at(end) == last && !(continued && last == current))
+        stop = min(end + s.chunk, s.tokens);
+    int state = continued ? (head_long ? 1 : 2) : 0;  // of the run at hand: 1 to partial[0], 2 another's, 0 own
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0.0f;
@@ -324,70 +396,71 @@ __global__ void __launch_bounds__(256) k_sum_tokens(const uint32_t* __restrict__
         store<float, V>(partial + (int64_t(chunk) * 2 + which) * s.channels + column, pack<float, V>(sum));
     };
     auto flush = [&] {
-        if (continued) {
+        if (state == 1) {
             to_partial(0);
-        } else {
+        } else if (state == 0) {
             float f[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) f[j] = sum[j] * scale;
             store<TO, V>(out + int64_t(current) * s.channels + column, pack<TO, V>(f));
         }
     };
-    for (uint32_t at = lo; at < hi && current < s.rows; at += SUM_BATCH) {
+    bool done = false;
+    for (uint32_t at = lo; at < stop && !done; at += SUM_BATCH) {
         // `at` is a multiple of SUM_BATCH, and the buffers are padded to it.
         uint32_t r[SUM_BATCH], from[SUM_BATCH];
         Vector<TI, V> v[SUM_BATCH];
 #pragma unroll
-        for (int u = 0; u < SUM_BATCH; u += 4) {
-            const uint4 a = *reinterpret_cast<const uint4*>(row + at + u);
-            const uint4 b = *reinterpret_cast<const uint4*>(token + at + u);
-            r[u] = a.x, r[u + 1] = a.y, r[u + 2] = a.z, r[u + 3] = a.w;
-            from[u] = b.x, from[u + 1] = b.y, from[u + 2] = b.z, from[u + 3] = b.w;
+        for (int u = 0; u < SUM_BATCH; u += 2) {
+            const uint4 a = *reinterpret_cast<const uint4*>(pairs + at + u);
+            r[u] = a.x, from[u] = a.y, r[u + 1] = a.z, from[u + 1] = a.w;
         }
 #pragma unroll
         for (int u = 0; u < SUM_BATCH; ++u) {
-            if (at + u >= hi) r[u] = NO_ROW;
-            v[u] = r[u] < s.rows ? load<TI, V>(grad + int64_t(from[u]) * s.grad_stride + column) : zeros<TI, V>();
+            // Behind the chunk only its last run goes on.
+            if (at + u >= stop || (at + u >= end && r[u] != last)) r[u] = NO_ROW;
+            const bool wanted = r[u] < s.rows && !(state == 2 && r[u] == current);
+            v[u] = wanted ? load<TI, V>(grad + int64_t(from[u]) * s.grad_stride + column) : zeros<TI, V>();
         }
 #pragma unroll
         for (int u = 0; u < SUM_BATCH; ++u) {
-            if (r[u] == NO_ROW) break;
-            if (r[u] != current) {
-                flush();
-                current = r[u];
-                continued = false;
+            if (r[u] != current && !done) {
+                if (r[u] == NO_ROW) {
+                    done = true;
+                } else {
+                    flush();
+                    current = r[u];
+                    state = 0;
 #pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-                if (current >= s.rows) break;
+                    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+                    done = current >= s.rows;
+                }
             }
             float f[V];
             unpack<TI, V>(v[u], f);
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += f[j];
+            for (int j = 0; j < V; ++j) sum[j] += done ? 0.0f : f[j];
         }
     }
     if (current >= s.rows) return;
-    if (current == after && !continued)
+    if (state == 0 && tail_long && current == last)
         to_partial(1);
     else
         flush();
 }
 
-// Rows whose runs cross chunk borders. A warp looks after one chunk: where such
-// a run begins in it, it adds the run's partial sums in a tile of `lanes` times
-// V columns, its lanes sharing the chunks where the columns leave lanes over.
-// Runs of over JOIN_LONG chunks are shared by the block's warps. All orders are
-// fixed by the sizes and the ids.
-constexpr int JOIN_WARPS = 8;
+// Long runs: the block of the chunk in which such a run begins adds its partial
+// sums in a tile of `lanes` times V columns. A warp takes a run, its lanes
+// sharing the chunks where the columns leave lanes over; runs of over JOIN_LONG
+// chunks are shared by the block's warps. All orders are fixed by the sizes and
+// the ids.
+constexpr int JOIN_WARPS = 8, JOIN_CHUNKS = 32;
 constexpr uint32_t JOIN_LONG = 64;
-struct Run {
-    uint32_t row, last;  // the last chunk that begins with `row`
-};
 
 template <int V>
 __device__ __forceinline__ void add_chunks(const float* __restrict__ partial, int64_t channels, int64_t column,
                                            uint32_t first, uint32_t last, uint32_t step, float (&sum)[V]) {
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t c = first; c <= last; c += step) {
         float f[V];
         unpack<float, V>(load<float, V>(partial + int64_t(c) * 2 * channels + column), f);
@@ -397,36 +470,57 @@ __device__ __forceinline__ void add_chunks(const float* __restrict__ partial, in
 }
 
 template <class TO, int V>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint32_t* __restrict__ row,
+__global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __restrict__ pairs,
                                                                   TO* __restrict__ out,
                                                                   const float* __restrict__ partial, SumShape s,
                                                                   float scale) {
-    __shared__ Run runs[JOIN_WARPS];
+    __shared__ uint32_t starts[JOIN_CHUNKS], rows[JOIN_CHUNKS], lasts[JOIN_CHUNKS], found;
     __shared__ float sums[JOIN_WARPS][32 * V];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t chunk = blockIdx.x * JOIN_WARPS + warp;
-    Run run = {NO_ROW, 0};
-    if (chunk + 1 < s.chunks) {
-        const uint32_t lo = chunk * s.chunk, hi = lo + s.chunk, r = row[hi - 1];
-        if (r < s.rows && row[hi] == r && !(lo && row[lo] == r && row[lo - 1] == r)) {
-            uint32_t first = chunk + 1, last = chunk + 1;  // gallop, then halve
-            for (uint32_t step = 1; last + step < s.chunks && row[(last + step) * s.chunk] == r; step *= 2) last += step;
-            first = last;
-            uint32_t end = s.chunks - 1 - last < last - chunk + 1 ? s.chunks - 1 : last + (last - chunk + 1);
-            while (first < end) {
-                const uint32_t middle = first + (end - first + 1) / 2;
-                if (row[middle * s.chunk] == r) first = middle;
-                else end = middle - 1;
-            }
-            run = {r, first};
+    auto row_at = [&](uint32_t i) { return pairs[i].x; };
+    if (warp == 0) {  // a lane a chunk
+        const uint32_t chunk = blockIdx.x * JOIN_CHUNKS + lane, lo = chunk * s.chunk, end = lo + s.chunk;
+        uint32_t r = NO_ROW, last = chunk + 1;
+        if (chunk + 1 < s.chunks && end + s.chunk <= s.tokens) {
+            r = row_at(end - 1);
+            if (r >= s.rows || row_at(end + s.chunk - 1) != r || (lo && row_at(lo) == r && row_at(lo - 1) == r)) r = NO_ROW;
         }
+        if (r != NO_ROW) {
+            // The last chunk that begins with row r: by doubled steps, then by halving.
+            uint32_t step = 1;
+            while (last + step < s.chunks && row_at((last + step) * s.chunk) == r) {
+                last += step;
+                step *= 2;
+            }
+            uint32_t beyond = min(last + step, s.chunks);
+            while (beyond - last > 1) {
+                const uint32_t middle = last + (beyond - last) / 2;
+                if (row_at(middle * s.chunk) == r) last = middle;
+                else beyond = middle;
+            }
+        }
+        const uint32_t which = __ballot_sync(~0u, r != NO_ROW);
+        if (r != NO_ROW) {
+            const uint32_t at = __popc(which & ((1u << lane) - 1));
+            starts[at] = chunk;
+            rows[at] = r;
+            lasts[at] = last;
+        }
+        if (lane == 0) found = __popc(which);
     }
+    __syncthreads();
+    if (!found) return;
     const uint32_t x = lane % s.lanes, y = lane / s.lanes, ys = 32 / s.lanes;
     const uint32_t vector = blockIdx.y * s.lanes + x;
     const int64_t column = int64_t(vector) * V;
     const bool inside = vector < s.vectors;
-    const bool is_long = run.row != NO_ROW && run.last - chunk > JOIN_LONG;
     float sum[V];
+    auto start = [&](bool begins, uint32_t from) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+        if (begins && inside && y == 0)
+            unpack<float, V>(load<float, V>(partial + (int64_t(from) * 2 + 1) * s.channels + column), sum);
+    };
     auto write = [&](uint32_t r) {
         for (uint32_t d = 16; d >= s.lanes; d /= 2) {
 #pragma unroll
@@ -438,30 +532,17 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint32_t*
             store<TO, V>(out + int64_t(r) * s.channels + column, pack<TO, V>(sum));
         }
     };
-    auto start = [&](uint32_t from) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-        if (inside && y == 0)
-            unpack<float, V>(load<float, V>(partial + (int64_t(from) * 2 + 1) * s.channels + column), sum);
-    };
-    if (run.row != NO_ROW && !is_long) {
-        start(chunk);
-        if (inside) add_chunks<V>(partial, s.channels, column, chunk + 1 + y, run.last, ys, sum);
-        write(run.row);
+    for (uint32_t i = warp; i < found; i += JOIN_WARPS) {
+        if (lasts[i] - starts[i] > JOIN_LONG) continue;
+        start(true, starts[i]);
+        if (inside) add_chunks<V>(partial, s.channels, column, starts[i] + 1 + y, lasts[i], ys, sum);
+        write(rows[i]);
     }
-    if (lane == 0) runs[warp] = is_long ? run : Run{NO_ROW, 0};
-    __syncthreads();
-    for (uint32_t w = 0; w < JOIN_WARPS; ++w) {
-        const Run r = runs[w];
-        if (r.row == NO_ROW) continue;
-        const uint32_t from = blockIdx.x * JOIN_WARPS + w;
-        if (warp == 0) {
-            start(from);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-        }
-        if (inside) add_chunks<V>(partial, s.channels, column, from + 1 + warp * ys + y, r.last, JOIN_WARPS * ys, sum);
+    for (uint32_t i = 0; i < found; ++i) {
+        if (lasts[i] - starts[i] <= JOIN_LONG) continue;
+        start(warp == 0, starts[i]);
+        if (inside)
+            add_chunks<V>(partial, s.channels, column, starts[i] + 1 + warp * ys + y, lasts[i], JOIN_WARPS * ys, sum);
 #pragma unroll
         for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = sum[j];
         __syncthreads();
@@ -470,9 +551,69 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint32_t*
 #pragma unroll
                 for (int j = 0; j < V; ++j) sum[j] += sums[k][lane * V + j];
             }
-            write(r.row);
+            write(rows[i]);
         }
         __syncthreads();
+    }
+}
+
+// Few tokens and a small table: one launch. Each block sorts all (row, token)
+// keys in shared memory (a bitonic network; keys differ, so that the order is
+// the ids') and clears and sums its own columns, a group of lanes a run.
+constexpr int SMALL_TOKENS = 1024;
+constexpr int64_t SMALL_TABLE = 1 << 18;  // elements
+template <class TI, class TO, class Id, int V>
+__global__ void __launch_bounds__(512) k_small_gradient(const TI* __restrict__ grad, int64_t grad_stride,
+                                                         const Id* __restrict__ ids, uint32_t tokens, uint32_t size,
+                                                         int64_t rows, int64_t channels, uint32_t vectors,
+                                                         uint32_t lanes, TO* __restrict__ out, float scale) {
+    __shared__ uint64_t keys[SMALL_TOKENS];
+    const uint32_t vector = blockIdx.x * lanes + threadIdx.x % lanes;
+    const uint32_t group = threadIdx.x / lanes, groups = blockDim.x / lanes;
+    const bool inside = vector < vectors;
+    const int64_t column = int64_t(vector) * V;
+    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x)
+        keys[i] = i < tokens ? uint64_t(row_of(ids[i], rows)) << 32 | i : ~uint64_t(0);
+    if (inside)
+        for (int64_t r = group; r < rows; r += groups) store<TO, V>(out + r * channels + column, zeros<TO, V>());
+    for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j; j /= 2) {
+            __syncthreads();
+            for (uint32_t t = threadIdx.x; t < size / 2; t += blockDim.x) {
+                const uint32_t a = 2 * t - (t & (j - 1)), b = a + j;  // the pairs at distance j
+                const uint64_t x = keys[a], y = keys[b];
+                if ((x > y) == ((a & k) == 0)) {
+                    keys[a] = y;
+                    keys[b] = x;
+                }
+            }
+        }
+    __syncthreads();
+    if (!inside) return;
+    for (uint32_t i = group; i < tokens; i += groups) {
+        const uint32_t row = uint32_t(keys[i] >> 32);
+        if (row >= rows || (i && uint32_t(keys[i - 1] >> 32) == row)) continue;
+        float sum[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+        for (uint32_t at = i; at < tokens && uint32_t(keys[at] >> 32) == row; at += SUM_BATCH) {
+            Vector<TI, V> v[SUM_BATCH];
+#pragma unroll
+            for (int u = 0; u < SUM_BATCH; ++u) {
+                const bool mine = at + u < tokens && uint32_t(keys[at + u] >> 32) == row;
+                v[u] = mine ? load<TI, V>(grad + int64_t(uint32_t(keys[at + u])) * grad_stride + column) : zeros<TI, V>();
+            }
+#pragma unroll
+            for (int u = 0; u < SUM_BATCH; ++u) {
+                float f[V];
+                unpack<TI, V>(v[u], f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += f[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] *= scale;
+        store<TO, V>(out + int64_t(row) * channels + column, pack<TO, V>(sum));
     }
 }
 

@@ -76,7 +76,7 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // --- embedding -------------------------------------------------------------
 
-// Above this many tokens a sort takes the whole GPU, two launches a pass, and
+// Above this many tokens a sort takes the whole GPU, three launches a pass, and
 // below it one cluster in one launch.
 constexpr int64_t CLUSTER_TOKENS = 65536;
 
@@ -90,16 +90,20 @@ SortPlan sort_plan(int64_t tokens, int64_t rows) {
     int bits = 1;
     while ((int64_t(1) << bits) < rows + 1) ++bits;
     SortPlan p;
-    p.passes = (bits + 9) / 10;
+    const bool large = tokens > CLUSTER_TOKENS;
+    const int most = large ? 9 : 10;  // bits of a digit, from the shared memory of its warps' counts
+    p.passes = (bits + most - 1) / most;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
     p.cluster = std::min<uint32_t>(16, power_of_two_from((tokens + 2047) / 2048));
-    p.tiles = tokens > CLUSTER_TOKENS ? SMS : 0;
-    p.per_warp = p.tiles ? uint32_t((tokens + p.tiles * SORT_WARPS - 1) / (p.tiles * SORT_WARPS)) : 0;
+    // Tiles of at most 512 pairs a warp: 128 KB, beside 64 KB of counts.
+    const int64_t warps = SMS * SORT_WARPS, waves = std::max<int64_t>(1, (tokens + warps * 512 - 1) / (warps * 512));
+    p.tiles = large ? uint32_t(SMS * waves) : 0;
+    p.per_warp = large ? uint32_t((tokens + warps * waves - 1) / (warps * waves)) : 0;
     return p;
 }
 
 SumShape sum_shape(int64_t tokens, int64_t rows, int64_t channels, int v) {
-    SumShape s;
+    SumShape s = {};
     s.tokens = uint32_t(tokens);
     s.rows = uint32_t(rows);
     s.channels = channels;
@@ -109,41 +113,71 @@ SumShape sum_shape(int64_t tokens, int64_t rows, int64_t channels, int v) {
     s.chunk = 64;
     while (s.chunk > 8 && (tokens / s.chunk) * s.tiles * s.lanes / 32 < SMS * 12) s.chunk /= 2;
     s.chunks = uint32_t((tokens + s.chunk - 1) / s.chunk);
-    s.grad_stride = 0;
+    s.sum_blocks = uint32_t((uint64_t(s.chunks) * s.tiles * s.lanes + 255) / 256);
     return s;
 }
 
-// Sorts the tokens into buffer sorted_buffer(passes) and clears the output's words.
+// The parts of the workspace.
+struct GradientWorkspace {
+    uint2* pairs[2];
+    uint32_t *counts, *present;
+    float* partial;
+    size_t bytes;
+    GradientWorkspace(void* base, int64_t tokens, int64_t rows, int64_t channels) : bytes(0) {
+        auto take = [&](size_t n) {
+            char* p = static_cast<char*>(base) + bytes;
+            bytes += padded(n);
+            return p;
+        };
+        const SortPlan plan = sort_plan(tokens, rows);
+        for (auto& p : pairs) p = reinterpret_cast<uint2*>(take(size_t(tokens) * sizeof(uint2)));
+        counts = reinterpret_cast<uint32_t*>(take((size_t(plan.tiles + 1) << plan.digit_bits) * 4));
+        present = reinterpret_cast<uint32_t*>(take((size_t(rows) + 31) / 32 * 4));
+        size_t partials = 0;
+        for (int v : {8, 4, 2, 1})
+            if (channels % v == 0)
+                partials = std::max(partials, size_t(sum_shape(tokens, rows, channels, v).chunks) * 2 * channels);
+        partial = reinterpret_cast<float*>(take(partials * sizeof(float)));
+    }
+};
+
+// What the sort's launches clear while they leave memory idle: in the one launch
+// as much as it takes to sort (16 us for 32768 tokens), in each of the others a
+// few microseconds' worth.
+constexpr int64_t CLEARED_BY_CLUSTER = 72 << 20, CLEARED_BY_LAUNCH = 12 << 20;
+
+// Sorts the tokens into pairs[sorted_buffer(passes)] and clears the first
+// clearing.whole words of the output.
 template <class Id>
-void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, const SortBuffers& buffers,
-                 uint32_t* counts, int64_t fill_words, int device, cudaStream_t stream) {
+void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, const GradientWorkspace& w,
+                 const Clearing& clearing, int device, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};  // devices on which the kernels' limits are raised
     if (!(ready.load() >> (device & 63) & 1)) {
         dynamic_shared(k_sort_tokens<Id>, (size_t(SORT_WARPS) + 1) * 4096);
-        dynamic_shared(k_place_tokens<Id>, size_t(SORT_WARPS) * 4096);
+        dynamic_shared(k_place_tokens<Id>, SORT_WARPS * (512 * sizeof(uint2) + 512 * 4));
         CPDE_CUDA(cudaFuncSetAttribute(k_sort_tokens<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         ready.fetch_or(uint64_t(1) << (device & 63));
     }
-    uint4* fill = static_cast<uint4*>(c.out);
     if (plan.tiles) {
         SortPass s = {uint32_t(c.tokens), plan.per_warp, 1u << plan.digit_bits, 0, 0, 0};
-        const int launches = 2 * plan.passes;
-        for (int launch = 0; launch < launches; ++launch) {
-            const int pass = launch / 2, from = (pass + 1) & 1, to = pass & 1;
-            const SortInput<Id> in = {ids, c.rows, pass ? buffers.row[from] : nullptr, buffers.token[from]};
+        for (int pass = 0; pass < plan.passes; ++pass) {
+            const SortInput<Id> in = {ids, c.rows, pass ? w.pairs[(pass + 1) & 1] : nullptr};
             s.shift = pass * plan.digit_bits;
-            s.fill_from = fill_words * launch / launches;
-            s.fill_to = fill_words * (launch + 1) / launches;
-            if (launch % 2 == 0)
-                k_count_digits<Id><<<plan.tiles, SORT_THREADS, s.bins * 4, stream>>>(in, s, counts, fill);
-            else
-                k_place_tokens<Id><<<plan.tiles, SORT_THREADS, size_t(SORT_WARPS) * s.bins * 4, stream>>>(
-                    in, s, counts, buffers.row[to], buffers.token[to], fill);
+            s.from = clearing.whole * (2 * pass) / (2 * plan.passes);
+            s.to = clearing.whole * (2 * pass + 1) / (2 * plan.passes);
+            k_count_digits<Id><<<plan.tiles, SORT_THREADS, s.bins * 4, stream>>>(in, s, w.counts, clearing);
+            CPDE_LAUNCHED();
+            k_scan_counts<<<(s.bins + 7) / 8, 256, 0, stream>>>(w.counts, plan.tiles, s.bins);
+            CPDE_LAUNCHED();
+            s.from = s.to;
+            s.to = clearing.whole * (2 * pass + 2) / (2 * plan.passes);
+            const size_t shared = SORT_WARPS * (plan.per_warp * sizeof(uint2) + s.bins * 4);
+            k_place_tokens<Id><<<plan.tiles, SORT_THREADS, shared, stream>>>(in, s, w.counts, w.pairs[pass & 1], clearing);
             CPDE_LAUNCHED();
         }
         return;
     }
-    const int64_t fillers = std::min<int64_t>(112, (fill_words + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
+    const int64_t fillers = std::min<int64_t>(128, (clearing.whole + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(plan.cluster + (fillers + plan.cluster - 1) / plan.cluster * plan.cluster));
     config.blockDim = dim3(SORT_THREADS);
@@ -156,7 +190,11 @@ void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, co
     config.attrs = &attribute;
     config.numAttrs = 1;
     CPDE_CUDA(cudaLaunchKernelEx(&config, k_sort_tokens<Id>, ids, uint32_t(c.tokens), c.rows, plan.passes,
-                                 plan.digit_bits, buffers, fill, fill_words));
+                                 plan.digit_bits, w.pairs[0], w.pairs[1], clearing));
+}
+
+bool small_gradient(int64_t tokens, int64_t rows, int64_t channels) {
+    return tokens <= SMALL_TOKENS && rows * channels <= SMALL_TABLE;
 }
 
 }  // namespace
@@ -194,57 +232,81 @@ void embedding(const EmbeddingCall& c, cudaStream_t stream) {
 }
 
 size_t embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channels) {
-    size_t partials = 0;
-    for (int v : {8, 4, 2, 1})
-        if (channels % v == 0)
-            partials = std::max(partials, size_t(sum_shape(tokens, rows, channels, v).chunks) * 2 * channels);
-    const SortPlan plan = sort_plan(tokens, rows);
-    return 4 * padded(size_t(tokens) * 4) + padded(partials * 4) + padded((size_t(plan.tiles) << plan.digit_bits) * 4);
+    return GradientWorkspace(nullptr, tokens, rows, channels).bytes;
 }
 
 void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream) {
     const size_t out_bytes = size_t(c.rows) * c.channels * bytes_of(c.out_type);
-    const bool words = (reinterpret_cast<uintptr_t>(c.out) | out_bytes) % 16 == 0;
-    if (!c.tokens || !words) CPDE_CUDA(cudaMemsetAsync(c.out, 0, out_bytes, stream));
-    if (!c.tokens) return;
-
-    char* at = static_cast<char*>(c.workspace);
-    auto take = [&](size_t bytes) { char* p = at; at += padded(bytes); return p; };
-    SortBuffers buffers;
-    for (int i = 0; i < 2; ++i) {
-        buffers.row[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
-        buffers.token[i] = reinterpret_cast<uint32_t*>(take(size_t(c.tokens) * 4));
+    if (!c.tokens) {
+        CPDE_CUDA(cudaMemsetAsync(c.out, 0, out_bytes, stream));
+        return;
     }
+    // Calls f with the types and the vector width.
+    auto typed = [&](auto&& f) {
+        with_types<false>(c.in_type, c.out_type, [&](auto in, auto out) {
+            using TI = typename decltype(in)::type;
+            using TO = typename decltype(out)::type;
+            const int v = Alignment().at(c.in, sizeof(TI)).at(c.out, sizeof(TO)).stride(c.in_stride).stride(c.channels)
+                              .vector(16 / sizeof(TI));
+            with_vector<8, 4, 2, 1>(v, [&](auto width) {
+                if constexpr (decltype(width)::value * sizeof(TI) <= 16) f(in, out, width);
+            });
+        });
+    };
+    if (small_gradient(c.tokens, c.rows, c.channels)) {
+        typed([&](auto in, auto out, auto width) {
+            using TI = typename decltype(in)::type;
+            using TO = typename decltype(out)::type;
+            constexpr int V = decltype(width)::value;
+            const uint32_t vectors = uint32_t(c.channels / V), lanes = power_of_two_from(std::min<uint32_t>(vectors, 8));
+            const uint32_t blocks = (vectors + lanes - 1) / lanes, size = power_of_two_from(c.tokens);
+            auto launch = [&](auto* ids) {
+                k_small_gradient<TI, TO, std::remove_const_t<std::remove_pointer_t<decltype(ids)>>, V>
+                    <<<blocks, 512, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
+                                                 c.rows, c.channels, vectors, lanes, static_cast<TO*>(c.out), c.scale);
+            };
+            if (c.id_type) launch(static_cast<const int64_t*>(c.ids));
+            else launch(static_cast<const int32_t*>(c.ids));
+            CPDE_LAUNCHED();
+        });
+        return;
+    }
+    const GradientWorkspace w(c.workspace, c.tokens, c.rows, c.channels);
     const SortPlan plan = sort_plan(c.tokens, c.rows);
-    uint32_t* counts = reinterpret_cast<uint32_t*>(take((size_t(plan.tiles) << plan.digit_bits) * 4));
-    float* partial = reinterpret_cast<float*>(at);
-    const int64_t fill_words = words ? int64_t(out_bytes / 16) : 0;
-    if (c.id_type) sort_tokens(c, static_cast<const int64_t*>(c.ids), plan, buffers, counts, fill_words, device, stream);
-    else sort_tokens(c, static_cast<const int32_t*>(c.ids), plan, buffers, counts, fill_words, device, stream);
-
-    const uint32_t* row = buffers.row[sorted_buffer(plan.passes)];
-    const uint32_t* token = buffers.token[sorted_buffer(plan.passes)];
-    with_types<false>(c.in_type, c.out_type, [&](auto in, auto out) {
+    Clearing clearing = {static_cast<uint4*>(c.out), 0, nullptr, 0};
+    const size_t row_bytes = size_t(c.channels) * bytes_of(c.out_type);
+    uint32_t clear_from = uint32_t(c.rows);
+    if ((reinterpret_cast<uintptr_t>(c.out) | out_bytes) % 16) {
+        CPDE_CUDA(cudaMemsetAsync(c.out, 0, out_bytes, stream));
+    } else {
+        const int64_t idle = plan.tiles ? CLEARED_BY_LAUNCH * 2 * plan.passes : CLEARED_BY_CLUSTER;
+        clearing.whole = int64_t(out_bytes / 16);
+        if (row_bytes % 16 == 0 && int64_t(out_bytes) > 2 * idle) {
+            clear_from = uint32_t(idle / row_bytes);
+            clearing.whole = int64_t(clear_from * row_bytes / 16);
+            clearing.present = w.present;
+            clearing.present_words = uint32_t((c.rows + 31) / 32);
+        }
+    }
+    if (c.id_type) sort_tokens(c, static_cast<const int64_t*>(c.ids), plan, w, clearing, device, stream);
+    else sort_tokens(c, static_cast<const int32_t*>(c.ids), plan, w, clearing, device, stream);
+    const uint2* pairs = w.pairs[sorted_buffer(plan.passes)];
+    typed([&](auto in, auto out, auto width) {
         using TI = typename decltype(in)::type;
         using TO = typename decltype(out)::type;
-        const int v = Alignment().at(c.in, sizeof(TI)).at(c.out, sizeof(TO)).stride(c.in_stride).stride(c.channels)
-                          .vector(16 / sizeof(TI));
-        with_vector<8, 4, 2, 1>(v, [&](auto width) {
-            constexpr int V = decltype(width)::value;
-            if constexpr (V * sizeof(TI) <= 16) {
-                SumShape s = sum_shape(c.tokens, c.rows, c.channels, V);
-                s.grad_stride = c.in_stride;
-                const uint64_t threads = uint64_t(s.chunks) * s.tiles * s.lanes;
-                k_sum_tokens<TI, TO, V><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(
-                    row, token, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), partial, s, c.scale);
-                CPDE_LAUNCHED();
-                if (s.chunks > 1) {
-                    k_join_chunks<TO, V><<<dim3((s.chunks + JOIN_WARPS - 2) / JOIN_WARPS, s.tiles), JOIN_WARPS * 32, 0,
-                                           stream>>>(row, static_cast<TO*>(c.out), partial, s, c.scale);
-                    CPDE_LAUNCHED();
-                }
-            }
-        });
+        constexpr int V = decltype(width)::value;
+        SumShape s = sum_shape(c.tokens, c.rows, c.channels, V);
+        s.grad_stride = c.in_stride;
+        s.clear_from = clear_from;
+        const unsigned clear_blocks = clearing.present ? SMS * 4 : 0;
+        k_sum_tokens<TI, TO, V><<<s.sum_blocks + clear_blocks, 256, 0, stream>>>(
+            pairs, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), w.partial, s, clearing, c.scale);
+        CPDE_LAUNCHED();
+        if (c.tokens >= 2 * int64_t(s.chunk)) {  // else no run covers a chunk behind its first
+            k_join_chunks<TO, V><<<dim3((s.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, s.tiles), JOIN_WARPS * 32, 0, stream>>>(
+                pairs, static_cast<TO*>(c.out), w.partial, s, c.scale);
+            CPDE_LAUNCHED();
+        }
     });
 }
 
