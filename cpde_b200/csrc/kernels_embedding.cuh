@@ -84,8 +84,9 @@ __device__ __forceinline__ void mark_present(const Clearing& clearing, uint32_t 
 
 // A pass is stable because each warp has a contiguous range of the pairs: a
 // pair's place is (smaller digits anywhere) + (its digit in the CTAs before) +
-// (in the warps before) + (before it in its warp, from a match over the lanes).
-// No order depends on timing. SORT_BATCH loads of a lane are in flight at once.
+// (in the warps before) + (before it in its warp, from the lanes with the same
+// digit). No order depends on timing. SORT_BATCH loads of a lane are in flight at
+// once.
 constexpr int SORT_BATCH = 8;
 
 template <class Id, class F>
@@ -102,6 +103,17 @@ __device__ __forceinline__ void count_digits(const SortInput<Id>& in, uint32_t l
                 each(r[u]);
             }
     }
+}
+
+// The lanes of a warp whose digits of `bits` bits are equal to the caller's, by a
+// vote a bit: a warp's match instruction took 280 cycles here, nine votes 40.
+__device__ __forceinline__ uint32_t equal_lanes(uint32_t lanes, uint32_t digit, uint32_t mask) {
+    uint32_t equal = lanes;
+    for (uint32_t bit = 1; bit <= mask; bit *= 2) {
+        const uint32_t set = __ballot_sync(lanes, digit & bit);
+        equal &= digit & bit ? set : ~set;
+    }
+    return equal;
 }
 
 // `place`: this warp's next place in `out` for each digit.
@@ -122,7 +134,7 @@ __device__ __forceinline__ void place_pairs(const SortInput<Id>& in, uint32_t lo
             const uint32_t lanes = __ballot_sync(~0u, active);
             if (active) {
                 const uint32_t digit = (pair[u].x >> shift) & mask;
-                const uint32_t peers = __match_any_sync(lanes, digit);
+                const uint32_t peers = equal_lanes(lanes, digit, mask);
                 const uint32_t mine = __popc(peers & ((1u << lane) - 1));
                 const uint32_t to = place[digit] + mine;
                 __syncwarp(lanes);
@@ -139,14 +151,26 @@ __device__ __forceinline__ void place_pairs(const SortInput<Id>& in, uint32_t lo
 __device__ __forceinline__ uint32_t prefix_warps(uint32_t* histogram, uint32_t bins) {
     uint32_t sum = 0;
     if (threadIdx.x < bins) {
-#pragma unroll 8
+        uint32_t n[SORT_WARPS];
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; ++w) n[w] = histogram[w * bins + threadIdx.x];
+#pragma unroll
         for (int w = 0; w < SORT_WARPS; ++w) {
-            const uint32_t n = histogram[w * bins + threadIdx.x];
             histogram[w * bins + threadIdx.x] = sum;
-            sum += n;
+            sum += n[w];
         }
     }
     return sum;
+}
+
+// Adds the places' base to a digit's warps.
+__device__ __forceinline__ void add_to_warps(uint32_t* histogram, uint32_t bins, uint32_t base) {
+    if (threadIdx.x >= bins) return;
+    uint32_t n[SORT_WARPS];
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) n[w] = histogram[w * bins + threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) histogram[w * bins + threadIdx.x] = n[w] + base;
 }
 
 // Exclusive prefix over the block's threads.
@@ -225,10 +249,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
                 all += n;
             }
         const uint32_t base = prefix_block(all, warp_sums) + before;
-        if (bin < bins) {
-#pragma unroll 8
-            for (int w = 0; w < SORT_WARPS; ++w) histogram[w * bins + bin] += base;
-        }
+        add_to_warps(histogram, bins, base);
         __syncthreads();
         place_pairs(in, lo, hi, shift, bins - 1, histogram + warp * bins, pass & 1 ? pairs1 : pairs0);
         // Orders this pass's pairs in global memory, and its reads of the other
@@ -322,11 +343,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in,
     __syncthreads();
     const uint32_t mine = prefix_warps(histogram, s.bins);
     const uint32_t local = prefix_block(mine, warp_sums);  // and where they are staged
-    if (bin < s.bins) {
-        shift_of[bin] = base - local;
-#pragma unroll 8
-        for (int w = 0; w < SORT_WARPS; ++w) histogram[w * s.bins + bin] += local;
-    }
+    if (bin < s.bins) shift_of[bin] = base - local;
+    add_to_warps(histogram, s.bins, local);
     __syncthreads();
     place_pairs(in, lo, hi, s.shift, s.bins - 1, histogram + warp * s.bins, staged);
     __syncthreads();
@@ -455,7 +473,7 @@ __global__ void __launch_bounds__(256) k_sum_tokens(const uint2* __restrict__ pa
 // chunks are shared by the block's warps. All orders are fixed by the sizes and
 // the ids.
 constexpr int JOIN_WARPS = 8, JOIN_CHUNKS = 32;
-constexpr uint32_t JOIN_LONG = 64;
+constexpr uint32_t JOIN_LONG = 8;
 
 template <int V>
 __device__ __forceinline__ void add_chunks(const float* __restrict__ partial, int64_t channels, int64_t column,

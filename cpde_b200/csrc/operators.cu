@@ -177,7 +177,8 @@ void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, co
         }
         return;
     }
-    const int64_t fillers = std::min<int64_t>(128, (clearing.whole + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
+    // At most seven clusters of 16 beside the sort's: a GPC holds one of them.
+    const int64_t fillers = std::min<int64_t>(112, (clearing.whole + 4 * SORT_THREADS - 1) / (4 * SORT_THREADS));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(plan.cluster + (fillers + plan.cluster - 1) / plan.cluster * plan.cluster));
     config.blockDim = dim3(SORT_THREADS);
