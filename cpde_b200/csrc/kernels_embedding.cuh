@@ -68,18 +68,13 @@ struct SortInput {
 
 // The table's gradient is cleared where no token adds to it. Of a large one the
 // sort's launches clear the first words whole while memory idles, and the sums'
-// launch the rows behind those that have no bit in `present`.
+// launch those of the rows behind that the sorted tokens do not hold.
 struct Clearing {
-    uint4* words;        // the table's gradient
-    int64_t whole;       // words that the sort clears
-    uint32_t* present;   // a bit for each row, or null: the sort clears all
-    uint32_t present_words;
+    uint4* words;   // the table's gradient
+    int64_t whole;  // words that the sort clears
 };
 __device__ __forceinline__ void clear_words(uint4* words, int64_t from, int64_t to, int64_t first, int64_t step) {
     for (int64_t i = from + first; i < to; i += step) words[i] = make_uint4(0, 0, 0, 0);
-}
-__device__ __forceinline__ void mark_present(const Clearing& clearing, uint32_t row, int64_t rows) {
-    if (clearing.present && row < rows) atomicOr(&clearing.present[row / 32], 1u << (row % 32));
 }
 
 // A pass is stable because each warp has a contiguous range of the pairs: a
@@ -89,19 +84,16 @@ __device__ __forceinline__ void mark_present(const Clearing& clearing, uint32_t 
 // once.
 constexpr int SORT_BATCH = 8;
 
-template <class Id, class F>
+template <class Id>
 __device__ __forceinline__ void count_digits(const SortInput<Id>& in, uint32_t lo, uint32_t hi, uint32_t step,
-                                             int shift, uint32_t mask, uint32_t* histogram, F&& each) {
+                                             int shift, uint32_t mask, uint32_t* histogram) {
     for (uint32_t at = lo; at < hi; at += SORT_BATCH * step) {
         uint32_t r[SORT_BATCH];
 #pragma unroll
         for (int u = 0; u < SORT_BATCH; ++u) r[u] = at + u * step < hi ? in.at(at + u * step).x : 0;
 #pragma unroll
         for (int u = 0; u < SORT_BATCH; ++u)
-            if (at + u * step < hi) {
-                atomicAdd(&histogram[(r[u] >> shift) & mask], 1u);
-                each(r[u]);
-            }
+            if (at + u * step < hi) atomicAdd(&histogram[(r[u] >> shift) & mask], 1u);
     }
 }
 
@@ -219,12 +211,6 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
     __shared__ uint32_t warp_sums[SORT_WARPS];
     const uint32_t rank = cluster.block_rank();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, bin = threadIdx.x;
-    if (clearing.present) {
-        for (uint32_t i = rank * SORT_THREADS + threadIdx.x; i < clearing.present_words; i += size * SORT_THREADS)
-            clearing.present[i] = 0;
-        __threadfence();
-        cluster.sync();
-    }
     const uint32_t per_warp = (tokens + size * SORT_WARPS - 1) / (size * SORT_WARPS);
     const uint64_t start = uint64_t(rank * SORT_WARPS + warp) * per_warp;
     const uint32_t lo = uint32_t(start < tokens ? start : tokens);
@@ -234,20 +220,20 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
         const SortInput<Id> in = {ids, rows, pass == 0 ? nullptr : pass & 1 ? pairs0 : pairs1};
         for (uint32_t i = threadIdx.x; i < SORT_WARPS * bins; i += SORT_THREADS) histogram[i] = 0;
         __syncthreads();
-        count_digits(in, lo + lane, hi, 32, shift, bins - 1, histogram + warp * bins, [&](uint32_t r) {
-            if (pass == 0) mark_present(clearing, r, rows);
-        });
+        count_digits(in, lo + lane, hi, 32, shift, bins - 1, histogram + warp * bins);
         __syncthreads();
         const uint32_t mine = prefix_warps(histogram, bins);
         if (bin < bins) totals[bin] = mine;
         cluster.sync();
         uint32_t before = 0, all = 0;
-        if (bin < bins)
+        if (bin < bins) {
+#pragma unroll 8
             for (uint32_t c = 0; c < size; ++c) {
                 const uint32_t n = cluster.map_shared_rank(totals, c)[bin];
                 before += c < rank ? n : 0;
                 all += n;
             }
+        }
         const uint32_t base = prefix_block(all, warp_sums) + before;
         add_to_warps(histogram, bins, base);
         __syncthreads();
@@ -270,16 +256,14 @@ template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in, SortPass s,
                                                                 uint32_t* __restrict__ counts, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
-    const int64_t thread = int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x, threads = int64_t(gridDim.x) * SORT_THREADS;
-    clear_words(clearing.words, s.from, s.to, thread, threads);
-    if (clearing.present && !in.pairs)
-        for (int64_t i = thread; i < clearing.present_words; i += threads) clearing.present[i] = 0;
+    clear_words(clearing.words, s.from, s.to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
+                int64_t(gridDim.x) * SORT_THREADS);
     if (threadIdx.x < s.bins) sort_shared[threadIdx.x] = 0;
     __syncthreads();
     const uint64_t per_tile = uint64_t(s.per_warp) * SORT_WARPS, start = blockIdx.x * per_tile;
     const uint32_t lo = uint32_t(start < s.tokens ? start : s.tokens);
     const uint32_t hi = uint32_t(start + per_tile < s.tokens ? start + per_tile : s.tokens);
-    count_digits(in, lo + threadIdx.x, hi, SORT_THREADS, s.shift, s.bins - 1, sort_shared, [](uint32_t) {});
+    count_digits(in, lo + threadIdx.x, hi, SORT_THREADS, s.shift, s.bins - 1, sort_shared);
     __syncthreads();
     if (threadIdx.x < s.bins) counts[blockIdx.x * s.bins + threadIdx.x] = sort_shared[threadIdx.x];
 }
@@ -336,9 +320,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in,
     const uint64_t tile = uint64_t(blockIdx.x) * per_tile, start = tile + uint64_t(warp) * s.per_warp;
     const uint32_t lo = uint32_t(start < s.tokens ? start : s.tokens);
     const uint32_t hi = uint32_t(start + s.per_warp < s.tokens ? start + s.per_warp : s.tokens);
-    count_digits(in, lo + lane, hi, 32, s.shift, s.bins - 1, histogram + warp * s.bins, [&](uint32_t r) {
-        if (!in.pairs) mark_present(clearing, r, in.rows);
-    });
+    count_digits(in, lo + lane, hi, 32, s.shift, s.bins - 1, histogram + warp * s.bins);
     const uint32_t base = prefix_block(total, warp_sums) + prefix;  // where the tile's pairs of the digit go
     __syncthreads();
     const uint32_t mine = prefix_warps(histogram, s.bins);
@@ -376,13 +358,23 @@ __global__ void __launch_bounds__(256) k_sum_tokens(const uint2* __restrict__ pa
                                                      TO* __restrict__ out, float* __restrict__ partial, SumShape s,
                                                      Clearing clearing, float scale) {
     if (blockIdx.x >= s.sum_blocks) {
-        // Rows without a token, a warp a row.
-        const uint32_t warps = (gridDim.x - s.sum_blocks) * 8, lane = threadIdx.x % 32;
+        // Rows without a token: a lane looks for a row among the sorted tokens, then
+        // the warp clears those that are not there.
+        const uint32_t lane = threadIdx.x % 32, warps = (gridDim.x - s.sum_blocks) * 8;
         const int64_t row_words = s.channels * sizeof(TO) / 16;
-        for (uint32_t r = s.clear_from + (blockIdx.x - s.sum_blocks) * 8 + threadIdx.x / 32; r < s.rows; r += warps) {
-            if (clearing.present[r / 32] >> (r % 32) & 1) continue;
-            uint4* to = clearing.words + r * row_words;
-            for (int64_t i = lane; i < row_words; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+        for (uint32_t base = s.clear_from + ((blockIdx.x - s.sum_blocks) * 8 + threadIdx.x / 32) * 32; base < s.rows;
+             base += warps * 32) {
+            uint32_t lo = 0, hi = s.tokens;  // the first token whose row is not below
+            while (lo < hi) {
+                const uint32_t middle = lo + (hi - lo) / 2;
+                if (pairs[middle].x < base + lane) lo = middle + 1;
+                else hi = middle;
+            }
+            const bool absent = base + lane < s.rows && (lo == s.tokens || pairs[lo].x != base + lane);
+            for (uint32_t which = __ballot_sync(~0u, absent); which; which &= which - 1) {
+                uint4* to = clearing.words + int64_t(base + __ffs(which) - 1) * row_words;
+                for (int64_t i = lane; i < row_words; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+            }
         }
         return;
     }

@@ -120,7 +120,7 @@ SumShape sum_shape(int64_t tokens, int64_t rows, int64_t channels, int v) {
 // The parts of the workspace.
 struct GradientWorkspace {
     uint2* pairs[2];
-    uint32_t *counts, *present;
+    uint32_t* counts;
     float* partial;
     size_t bytes;
     GradientWorkspace(void* base, int64_t tokens, int64_t rows, int64_t channels) : bytes(0) {
@@ -132,7 +132,6 @@ struct GradientWorkspace {
         const SortPlan plan = sort_plan(tokens, rows);
         for (auto& p : pairs) p = reinterpret_cast<uint2*>(take(size_t(tokens) * sizeof(uint2)));
         counts = reinterpret_cast<uint32_t*>(take((size_t(plan.tiles + 1) << plan.digit_bits) * 4));
-        present = reinterpret_cast<uint32_t*>(take((size_t(rows) + 31) / 32 * 4));
         size_t partials = 0;
         for (int v : {8, 4, 2, 1})
             if (channels % v == 0)
@@ -274,7 +273,7 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
     }
     const GradientWorkspace w(c.workspace, c.tokens, c.rows, c.channels);
     const SortPlan plan = sort_plan(c.tokens, c.rows);
-    Clearing clearing = {static_cast<uint4*>(c.out), 0, nullptr, 0};
+    Clearing clearing = {static_cast<uint4*>(c.out), 0};
     const size_t row_bytes = size_t(c.channels) * bytes_of(c.out_type);
     uint32_t clear_from = uint32_t(c.rows);
     if ((reinterpret_cast<uintptr_t>(c.out) | out_bytes) % 16) {
@@ -285,8 +284,6 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
         if (row_bytes % 16 == 0 && int64_t(out_bytes) > 2 * idle) {
             clear_from = uint32_t(idle / row_bytes);
             clearing.whole = int64_t(clear_from * row_bytes / 16);
-            clearing.present = w.present;
-            clearing.present_words = uint32_t((c.rows + 31) / 32);
         }
     }
     if (c.id_type) sort_tokens(c, static_cast<const int64_t*>(c.ids), plan, w, clearing, device, stream);
@@ -299,7 +296,7 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
         SumShape s = sum_shape(c.tokens, c.rows, c.channels, V);
         s.grad_stride = c.in_stride;
         s.clear_from = clear_from;
-        const unsigned clear_blocks = clearing.present ? SMS * 4 : 0;
+        const unsigned clear_blocks = clear_from < s.rows ? SMS * 4 : 0;
         k_sum_tokens<TI, TO, V><<<s.sum_blocks + clear_blocks, 256, 0, stream>>>(
             pairs, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), w.partial, s, clearing, c.scale);
         CPDE_LAUNCHED();
