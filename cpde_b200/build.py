@@ -8,7 +8,8 @@ entry; fast_forward.cu, fast_backward.cu, fast_head.cu: the fast-tier
 dispatch and the kernels it instantiates; operators.cu: the device-tensor
 operators); the server is a host program
 linked against it with an $ORIGIN-relative rpath so the pair can be moved
-together.
+together. The operators' Python binding (csrc/binding.cpp) is an extension module
+over torch's C++ interface.
 """
 import os
 import subprocess
@@ -17,6 +18,7 @@ from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / 'csrc'
+BINDING = PACKAGE / '_operators.so'
 LIBRARY = PACKAGE / 'libcpde_b200.so'
 SERVER = PACKAGE / 'bin' / 'cpde_server'
 BUILD = PACKAGE / '_build'
@@ -70,7 +72,24 @@ def build(force=False, verbose_ptxas=False):
               CSRC / 'server_main.cpp', f'-L{PACKAGE}', '-lcpde_b200', f'-L{cuda / "lib64"}', '-lcudart',
               "-Wl,-rpath,$ORIGIN/..", f'-Wl,-rpath,{cuda / "lib64"}',
               '-Wl,--allow-shlib-undefined'])
+    _build_binding(force)
     return LIBRARY, SERVER
+
+
+def _build_binding(force):
+    sources = [CSRC / 'binding.cpp', PACKAGE.parent / 'include' / 'cpde_b200.h']
+    if not (force or _stale(BINDING, sources)):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(os.environ.get('CUDA_HOME', '/usr/local/cuda'))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_path('include'), cuda / 'include']
+    lib = Path(torch.__file__).parent / 'lib'
+    _run(['g++', '-std=c++17', '-O2', '-fPIC', '-shared', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}',
+          *[f'-isystem{p}' for p in includes], '-o', BINDING, CSRC / 'binding.cpp', f'-L{lib}', '-ltorch_python', '-ltorch',
+          '-ltorch_cpu', '-lc10', '-lc10_cuda', f'-L{cuda / "lib64"}', '-lcudart'])
 
 
 if __name__ == '__main__':
