@@ -569,7 +569,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __
 
 // Few tokens and a small table: one launch. Each block sorts all (row, token)
 // keys in shared memory (a bitonic network; keys differ, so that the order is
-// the ids') and clears and sums its own columns, a group of lanes a run.
+// the ids'), and clears and sums its own columns of the rows r with
+// r % gridDim.y = blockIdx.y, a group of lanes a run: most groups then wait for
+// one run's gradients instead of several in turn.
 constexpr int SMALL_TOKENS = 1024;
 constexpr int64_t SMALL_TABLE = 1 << 18;  // elements
 template <class TI, class TO, class Id, int V>
@@ -585,7 +587,8 @@ __global__ void __launch_bounds__(512) k_small_gradient(const TI* __restrict__ g
     for (uint32_t i = threadIdx.x; i < size; i += blockDim.x)
         keys[i] = i < tokens ? uint64_t(row_of(ids[i], rows)) << 32 | i : ~uint64_t(0);
     if (inside)
-        for (int64_t r = group; r < rows; r += groups) store<TO, V>(out + r * channels + column, zeros<TO, V>());
+        for (int64_t r = blockIdx.y + group * gridDim.y; r < rows; r += groups * gridDim.y)
+            store<TO, V>(out + r * channels + column, zeros<TO, V>());
     for (uint32_t k = 2; k <= size; k *= 2)
         for (uint32_t j = k / 2; j; j /= 2) {
             __syncthreads();
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(512) k_small_gradient(const TI* __restrict__ g
     if (!inside) return;
     for (uint32_t i = group; i < tokens; i += groups) {
         const uint32_t row = uint32_t(keys[i] >> 32);
-        if (row >= rows || (i && uint32_t(keys[i - 1] >> 32) == row)) continue;
+        if (row >= rows || row % gridDim.y != blockIdx.y || (i && uint32_t(keys[i - 1] >> 32) == row)) continue;
         float sum[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] = 0.0f;

@@ -260,9 +260,10 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
             constexpr int V = decltype(width)::value;
             const uint32_t vectors = uint32_t(c.channels / V), lanes = power_of_two_from(std::min<uint32_t>(vectors, 8));
             const uint32_t blocks = (vectors + lanes - 1) / lanes, size = power_of_two_from(c.tokens);
+            const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(16, uint32_t(c.tokens * lanes / 512)));
             auto launch = [&](auto* ids) {
                 k_small_gradient<TI, TO, std::remove_const_t<std::remove_pointer_t<decltype(ids)>>, V>
-                    <<<blocks, 512, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
+                    <<<dim3(blocks, shares), 512, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
                                                  c.rows, c.channels, vectors, lanes, static_cast<TO*>(c.out), c.scale);
             };
             if (c.id_type) launch(static_cast<const int64_t*>(c.ids));
