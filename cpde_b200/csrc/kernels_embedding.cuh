@@ -10,16 +10,16 @@ namespace cpde::ops {
 // gives a zero row. A thread has LOOKUPS vectors of V channels, a block's
 // vectors apart, so that its loads of ids and then of rows are in flight
 // together.
-constexpr int LOOKUPS = 4;
+constexpr int LOOKUPS = 4, LOOKUP_THREADS = 128;
 template <class TI, class TO, class Id, int V>
-__global__ void __launch_bounds__(256) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
+__global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
                                                     const Id* __restrict__ ids, TO* __restrict__ out,
                                                     int64_t channels, Divisor vectors, uint32_t count, float scale) {
-    const uint32_t base = blockIdx.x * (256 * LOOKUPS) + threadIdx.x;
+    const uint32_t base = blockIdx.x * (LOOKUP_THREADS * LOOKUPS) + threadIdx.x;
     int64_t source[LOOKUPS];
 #pragma unroll
     for (int u = 0; u < LOOKUPS; ++u) {
-        const uint32_t i = base + u * 256;
+        const uint32_t i = base + u * LOOKUP_THREADS;
         source[u] = -1;
         if (i < count) {
             const uint32_t t = vectors.quotient(i), k = i - t * vectors.divisor;
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) k_embedding(const TI* __restrict__ table,
     for (int u = 0; u < LOOKUPS; ++u) v[u] = source[u] >= 0 ? load<TI, V>(table + source[u]) : zeros<TI, V>();
 #pragma unroll
     for (int u = 0; u < LOOKUPS; ++u) {
-        const uint32_t i = base + u * 256;
+        const uint32_t i = base + u * LOOKUP_THREADS;
         if (i >= count) continue;
         float f[V];
         unpack<TI, V>(v[u], f);
@@ -567,54 +567,59 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __
     }
 }
 
-// Few tokens and a small table: one launch. Each block sorts all (row, token)
-// keys in shared memory (a bitonic network; keys differ, so that the order is
-// the ids'), and clears and sums its own columns of the rows r with
-// r % gridDim.y = blockIdx.y, a group of lanes a run: most groups then wait for
-// one run's gradients instead of several in turn.
-constexpr int SMALL_TOKENS = 1024;
-constexpr int64_t SMALL_TABLE = 1 << 18;  // elements
+// Few tokens and a small table: one launch. Each block sorts all tokens in shared
+// memory (a bitonic network over keys (row, token), a thread a key; keys differ,
+// so that the order is the ids'), and clears and sums its own columns of the rows
+// r with r % gridDim.y = blockIdx.y, a group of lanes a run: most groups then wait
+// for one run's gradients instead of several in turn.
+constexpr int SMALL_TOKENS = 1024, SMALL_BITS = 10;
+constexpr int64_t SMALL_TABLE = 1 << 18;  // elements; a row fits in the key's other 22 bits
 template <class TI, class TO, class Id, int V>
-__global__ void __launch_bounds__(512) k_small_gradient(const TI* __restrict__ grad, int64_t grad_stride,
-                                                         const Id* __restrict__ ids, uint32_t tokens, uint32_t size,
-                                                         int64_t rows, int64_t channels, uint32_t vectors,
-                                                         uint32_t lanes, TO* __restrict__ out, float scale) {
-    __shared__ uint64_t keys[SMALL_TOKENS];
+__global__ void __launch_bounds__(SMALL_TOKENS) k_small_gradient(const TI* __restrict__ grad, int64_t grad_stride,
+                                                                  const Id* __restrict__ ids, uint32_t tokens,
+                                                                  uint32_t size, int64_t rows, int64_t channels,
+                                                                  uint32_t vectors, uint32_t lanes,
+                                                                  TO* __restrict__ out, float scale) {
+    __shared__ uint32_t keys[2][SMALL_TOKENS];
     const uint32_t vector = blockIdx.x * lanes + threadIdx.x % lanes;
     const uint32_t group = threadIdx.x / lanes, groups = blockDim.x / lanes;
     const bool inside = vector < vectors;
     const int64_t column = int64_t(vector) * V;
-    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x)
-        keys[i] = i < tokens ? uint64_t(row_of(ids[i], rows)) << 32 | i : ~uint64_t(0);
+    const uint32_t t = threadIdx.x;
+    uint32_t key = t < tokens ? row_of(ids[t], rows) << SMALL_BITS | t : ~0u;
     if (inside)
         for (int64_t r = blockIdx.y + group * gridDim.y; r < rows; r += groups * gridDim.y)
             store<TO, V>(out + r * channels + column, zeros<TO, V>());
+    int buffer = 0;
     for (uint32_t k = 2; k <= size; k *= 2)
         for (uint32_t j = k / 2; j; j /= 2) {
-            __syncthreads();
-            for (uint32_t t = threadIdx.x; t < size / 2; t += blockDim.x) {
-                const uint32_t a = 2 * t - (t & (j - 1)), b = a + j;  // the pairs at distance j
-                const uint64_t x = keys[a], y = keys[b];
-                if ((x > y) == ((a & k) == 0)) {
-                    keys[a] = y;
-                    keys[b] = x;
-                }
+            uint32_t other;
+            if (j < 32) {
+                other = __shfl_xor_sync(~0u, key, j);
+            } else {  // between warps; the two buffers alternate, so that one barrier a step does
+                keys[buffer][t] = key;
+                __syncthreads();
+                other = keys[buffer][t ^ j];
+                buffer ^= 1;
             }
+            key = ((t & j) == 0) == ((t & k) == 0) ? min(key, other) : max(key, other);
         }
+    uint32_t* sorted = keys[buffer];
+    sorted[t] = key;
     __syncthreads();
     if (!inside) return;
     for (uint32_t i = group; i < tokens; i += groups) {
-        const uint32_t row = uint32_t(keys[i] >> 32);
-        if (row >= rows || row % gridDim.y != blockIdx.y || (i && uint32_t(keys[i - 1] >> 32) == row)) continue;
+        const uint32_t row = sorted[i] >> SMALL_BITS;
+        if (row >= rows || row % gridDim.y != blockIdx.y || (i && sorted[i - 1] >> SMALL_BITS == row)) continue;
         float sum[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-        for (uint32_t at = i; at < tokens && uint32_t(keys[at] >> 32) == row; at += SUM_BATCH) {
+        for (uint32_t at = i; at < tokens && sorted[at] >> SMALL_BITS == row; at += SUM_BATCH) {
             Vector<TI, V> v[SUM_BATCH];
 #pragma unroll
             for (int u = 0; u < SUM_BATCH; ++u) {
-                const bool mine = at + u < tokens && uint32_t(keys[at + u] >> 32) == row;
-                v[u] = mine ? load<TI, V>(grad + int64_t(uint32_t(keys[at + u])) * grad_stride + column) : zeros<TI, V>();
+                const bool mine = at + u < tokens && sorted[at + u] >> SMALL_BITS == row;
+                v[u] = mine ? load<TI, V>(grad + int64_t(sorted[at + u] % SMALL_TOKENS) * grad_stride + column) : zeros<TI, V>();
             }
 #pragma unroll
             for (int u = 0; u < SUM_BATCH; ++u) {

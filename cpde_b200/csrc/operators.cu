@@ -214,14 +214,14 @@ void embedding(const EmbeddingCall& c, cudaStream_t stream) {
                 const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / vectors);
                 for (int64_t t = 0; t < c.tokens; t += slab) {
                     const uint32_t count = uint32_t(std::min(slab, c.tokens - t) * vectors);
-                    const uint32_t blocks = (count + 256 * LOOKUPS - 1) / (256 * LOOKUPS);
+                    const uint32_t blocks = (count + LOOKUP_THREADS * LOOKUPS - 1) / (LOOKUP_THREADS * LOOKUPS);
                     TO* to = static_cast<TO*>(c.out) + t * c.channels;
                     if (c.id_type)
-                        k_embedding<TI, TO, int64_t, V><<<blocks, 256, 0, stream>>>(
+                        k_embedding<TI, TO, int64_t, V><<<blocks, LOOKUP_THREADS, 0, stream>>>(
                             static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int64_t*>(c.ids) + t,
                             to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
                     else
-                        k_embedding<TI, TO, int32_t, V><<<blocks, 256, 0, stream>>>(
+                        k_embedding<TI, TO, int32_t, V><<<blocks, LOOKUP_THREADS, 0, stream>>>(
                             static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int32_t*>(c.ids) + t,
                             to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
                     CPDE_LAUNCHED();
@@ -259,11 +259,11 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
             using TO = typename decltype(out)::type;
             constexpr int V = decltype(width)::value;
             const uint32_t vectors = uint32_t(c.channels / V), lanes = power_of_two_from(std::min<uint32_t>(vectors, 8));
-            const uint32_t blocks = (vectors + lanes - 1) / lanes, size = power_of_two_from(c.tokens);
-            const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(16, uint32_t(c.tokens * lanes / 512)));
+            const uint32_t blocks = (vectors + lanes - 1) / lanes, size = std::max(32u, power_of_two_from(c.tokens));
+            const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(16, uint32_t(lanes)));
             auto launch = [&](auto* ids) {
                 k_small_gradient<TI, TO, std::remove_const_t<std::remove_pointer_t<decltype(ids)>>, V>
-                    <<<dim3(blocks, shares), 512, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
+                    <<<dim3(blocks, shares), size, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
                                                  c.rows, c.channels, vectors, lanes, static_cast<TO*>(c.out), c.scale);
             };
             if (c.id_type) launch(static_cast<const int64_t*>(c.ids));
