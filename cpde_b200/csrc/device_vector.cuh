@@ -49,6 +49,14 @@ __device__ __forceinline__ void store(T* p, const Vector<T, V>& v) {
     for (int i = 0; i < Vector<T, V>::W::count; ++i) w[i] = v.word[i];
 }
 
+// For what this kernel will not read again.
+template <class T, int V>
+__device__ __forceinline__ void store_streaming(T* p, const Vector<T, V>& v) {
+    auto* w = reinterpret_cast<typename Vector<T, V>::Word*>(p);
+#pragma unroll
+    for (int i = 0; i < Vector<T, V>::W::count; ++i) __stcs(w + i, v.word[i]);
+}
+
 template <class T, int V>
 __device__ __forceinline__ void unpack(const Vector<T, V>& v, float (&f)[V]) {
     T e[V];

@@ -10,7 +10,7 @@ namespace cpde::ops {
 // gives a zero row. A thread has LOOKUPS vectors of V channels, a block's
 // vectors apart, so that its loads of ids and then of rows are in flight
 // together.
-constexpr int LOOKUPS = 4, LOOKUP_THREADS = 128;
+constexpr int LOOKUPS = 4, LOOKUP_THREADS = 64;
 template <class TI, class TO, class Id, int V>
 __global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
                                                     const Id* __restrict__ ids, TO* __restrict__ out,
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restri
         unpack<TI, V>(v[u], f);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = source[u] >= 0 ? f[j] * scale : 0.0f;
-        store<TO, V>(out + int64_t(i) * V, pack<TO, V>(f));
+        store_streaming<TO, V>(out + int64_t(i) * V, pack<TO, V>(f));  // the table stays in L2
     }
 }
 
