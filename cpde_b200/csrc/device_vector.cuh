@@ -11,6 +11,13 @@
 
 namespace cpde::ops {
 
+// A kernel that is launched as dependent (launch_dependent in operators.cu) may
+// begin before the launch ahead of it has ended: it waits here before it touches
+// what that one wrote, or anything that an earlier launch may still use.
+__device__ __forceinline__ void after_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the launch behind begin once every block has said so.
+__device__ __forceinline__ void next_launch_may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Bytes of V elements as one or more machine words.
 template <int BYTES> struct Words { using type = uint4; static constexpr int count = BYTES / 16; };
 template <> struct Words<8> { using type = uint2; static constexpr int count = 1; };

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
                                                                int64_t rows, int passes, int digit_bits,
                                                                uint2* pairs0, uint2* pairs1, Clearing clearing) {
     namespace cg = cooperative_groups;
+    next_launch_may_begin();
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t size = cluster.num_blocks();
     if (blockIdx.x >= size) {
@@ -256,6 +257,8 @@ template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in, SortPass s,
                                                                 uint32_t* __restrict__ counts, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
+    after_previous_launch();
+    next_launch_may_begin();
     clear_words(clearing.words, s.from, s.to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
                 int64_t(gridDim.x) * SORT_THREADS);
     if (threadIdx.x < s.bins) sort_shared[threadIdx.x] = 0;
@@ -274,6 +277,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in,
 // where 148 tiles have 512 digits, 9 us.)
 __global__ void __launch_bounds__(256) k_scan_counts(uint32_t* __restrict__ counts, uint32_t tiles, uint32_t bins) {
     const uint32_t bin = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    after_previous_launch();
+    next_launch_may_begin();
     if (bin >= bins) return;
     uint32_t sum = 0;
     for (uint32_t base = 0; base < tiles; base += 32 * 8) {
@@ -310,6 +315,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in,
     uint2* staged = reinterpret_cast<uint2*>(sort_shared);  // the tile
     const uint32_t per_tile = s.per_warp * SORT_WARPS;
     uint32_t* histogram = sort_shared + 2 * per_tile;  // [warp][bin]
+    after_previous_launch();
+    next_launch_may_begin();
     clear_words(clearing.words, s.from, s.to, int64_t(blockIdx.x) * SORT_THREADS + threadIdx.x,
                 int64_t(gridDim.x) * SORT_THREADS);
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, bin = threadIdx.x;
@@ -357,6 +364,8 @@ template <class TI, class TO, int V>
 __global__ void __launch_bounds__(256) k_sum_tokens(const uint2* __restrict__ pairs, const TI* __restrict__ grad,
                                                      TO* __restrict__ out, float* __restrict__ partial, SumShape s,
                                                      Clearing clearing, float scale) {
+    after_previous_launch();
+    next_launch_may_begin();
     if (blockIdx.x >= s.sum_blocks) {
         // Rows without a token: a lane looks for a row among the sorted tokens, then
         // the warp clears those that are not there.
@@ -486,6 +495,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __
                                                                   float scale) {
     __shared__ uint32_t starts[JOIN_CHUNKS], rows[JOIN_CHUNKS], lasts[JOIN_CHUNKS], found;
     __shared__ float sums[JOIN_WARPS][32 * V];
+    after_previous_launch();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     auto row_at = [&](uint32_t i) { return pairs[i].x; };
     if (warp == 0) {  // a lane a chunk

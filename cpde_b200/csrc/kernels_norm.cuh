@@ -174,6 +174,7 @@ template <class T, int V>
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_moments(const T* __restrict__ x, NormShape s,
                                                                 Moments* __restrict__ pieces) {
     extern __shared__ float norm_shared[];  // [ty][channel of the tile] x (mean, m2)
+    next_launch_may_begin();
     const int32_t split = blockIdx.x % s.splits, n = blockIdx.x / s.splits;
     const Tile t = tile_of<V>(s, blockIdx.y);
     const int32_t ys = NORM_THREADS / s.tile;
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_apply(const 
                                                               float* __restrict__ mean, float* __restrict__ rstd,
                                                               const Moments* __restrict__ pieces, NormShape s) {
     extern __shared__ float norm_shared[];  // [group of the tile] x (mean, rstd)
+    after_previous_launch();
     const int32_t split = blockIdx.x % s.apply_splits, n = blockIdx.x / s.apply_splits;
     const Tile t = tile_of<V>(s, blockIdx.y);
     const int32_t length = length_of(s, n);
@@ -458,6 +460,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
                                                              NormShape s, float2* __restrict__ channel_sums,
                                                              float2* __restrict__ pieces) {
     extern __shared__ float norm_shared[];  // [ty][channel of the tile] x (h, h xhat)
+    next_launch_may_begin();
     float2* shared = reinterpret_cast<float2*>(norm_shared);
     const int32_t split = blockIdx.x % s.splits, n = blockIdx.x / s.splits;
     const Tile t = tile_of<V>(s, blockIdx.y);
@@ -550,6 +553,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradie
     P* __restrict__ dweight, P* __restrict__ dbias, const float2* __restrict__ channel_sums,
     const float2* __restrict__ pieces, NormShape s) {
     extern __shared__ float norm_shared[];
+    after_previous_launch();
     float2* shared = reinterpret_cast<float2*>(norm_shared);
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int32_t n = blockIdx.x / s.apply_splits;

@@ -7,9 +7,9 @@
 // that the data needs no barrier and no registers while it is under way. A
 // cluster takes one item (an instance and a tile) after the other: as a thread
 // has written a slot's results it starts the next item's copy into that slot, so
-// that memory is read while it is written and while sums are joined. Where there
-// are more items than clusters, a counter deals them out, since point counts,
-// and with them times, differ from instance to instance.
+// that memory is read while it is written and while sums are joined. Where point
+// counts, and with them times, differ from instance to instance, a counter deals
+// the items out.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -52,7 +52,7 @@ struct SlabShape {
     NormShape norm;
     int32_t cluster, slots;  // CTAs of a cluster; vectors of a thread, and array
     int32_t clusters, items;
-    uint32_t* counter;       // items dealt out behind the first of each cluster; null if there are none
+    uint32_t* counter;       // deals out the items behind the first of each cluster; null: they go round
     int32_t ys;              // points that the block's threads cover at once
     int32_t group_vectors;   // vectors of a group
     int32_t tile_channels, tile_groups;
@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
         copy_parameters<P, V>(tile.weight + seat.tx * V, weight ? weight + item.channel : nullptr, s.wide_parameters);
         copy_parameters<P, V>(tile.bias + seat.tx * V, bias ? bias + item.channel : nullptr, s.wide_parameters);
     };
-    Item<V> at(s, seat, seat.cluster, item_length(s, seat.cluster));
+    int32_t item = seat.cluster;
+    Item<V> at(s, seat, item, item_length(s, item));
     fetch_parameters(at);
     copy_points<T, V>(data, at.in(x, seat, s.norm.x_instance, s.norm.x_point), read_step, at.count);
     cluster_arrive();
@@ -321,9 +322,10 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
             const float var = fmaxf(v.y - v.x * d, 0.0f) / count;
             return make_float2(pivot + d, count > 0.0f ? 1.0f / sqrtf(var + s.norm.eps) : 0.0f);
         });
-        const int2 coming = s.counter ? *exchange.next : make_int2(s.items, 0);
-        const bool more = coming.x < s.items;
-        const Item<V> then(s, seat, more ? coming.x : 0, more ? coming.y : 0);
+        const int2 coming = s.counter ? *exchange.next : make_int2(item + s.clusters, s.norm.points);
+        item = coming.x;
+        const bool more = item < s.items;
+        const Item<V> then(s, seat, more ? item : 0, more ? coming.y : 0);
         if (more) fetch_parameters(then);
         const T* from = then.in(x, seat, s.norm.x_instance, s.norm.x_point);
         Slot* slot = data;
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
     const float* __restrict__ rstd, const P* __restrict__ weight, const P* __restrict__ bias, T* __restrict__ dx,
     float2* __restrict__ channel_sums, SlabShape s) {
     extern __shared__ __align__(16) unsigned char slab[];
+    next_launch_may_begin();
     using Slot = Vector<T, V>;
     // A slot of x and one of the gradient in turn.
     Slot* data = reinterpret_cast<Slot*>(slab) + threadIdx.x;
@@ -398,7 +401,8 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
             copy_async<4>(tile.rstd + seat.group, rstd + g);
         }
     };
-    Item<V> at(s, seat, seat.cluster, item_length(s, seat.cluster));
+    int32_t item = seat.cluster;
+    Item<V> at(s, seat, item, item_length(s, item));
     fetch_parameters(at);
     copy_points<T, V, 2>(data, at.in(x, seat, s.norm.x_instance, s.norm.x_point), x_step, at.count);
     copy_points<T, V, 2>(grads, at.in(grad, seat, s.norm.grad_instance, s.norm.grad_point), grad_step, at.count);
@@ -494,9 +498,10 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
         for (int32_t i = s.cluster / 2; i; i /= 2) v = __fadd2_rn(v, shuffle_xor(v, i));
         return v;
     });
-    const int2 coming = s.counter ? *exchange.next : make_int2(s.items, 0);
-    const bool more = coming.x < s.items;
-    const Item<V> then(s, seat, more ? coming.x : 0, more ? coming.y : 0);
+    const int2 coming = s.counter ? *exchange.next : make_int2(item + s.clusters, s.norm.points);
+    item = coming.x;
+    const bool more = item < s.items;
+    const Item<V> then(s, seat, more ? item : 0, more ? coming.y : 0);
     if (more) fetch_parameters(then);
     const T* from = then.in(x, seat, s.norm.x_instance, s.norm.x_point);
     const T* gfrom = then.in(grad, seat, s.norm.grad_instance, s.norm.grad_point);
@@ -538,6 +543,7 @@ template <class P>
 __global__ void __launch_bounds__(1024) k_norm_parameters(P* __restrict__ dweight, P* __restrict__ dbias,
                                                                    const float2* __restrict__ channel_sums,
                                                                    int32_t rows, int32_t channels) {
+    after_previous_launch();
     sum_parameters<P, 32>(dweight, dbias, channel_sums, rows, channels, blockIdx.x);
 }
 

@@ -67,6 +67,24 @@ void with_vector(int v, F&& f) {
     ((v == VS ? f(std::integral_constant<int, VS>{}) : void()), ...);
 }
 
+// A launch that may begin before the launch ahead of it in the stream has ended:
+// for kernels that say after_previous_launch() first, behind one of this file's
+// kernels. It hides a launch's start, about a microsecond.
+template <class... P, class... A>
+void launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, A... arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
+}
+
 template <class K>
 void dynamic_shared(K kernel, size_t bytes) {
     CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
@@ -164,15 +182,18 @@ void sort_tokens(const EmbeddingCall& c, const Id* ids, const SortPlan& plan, co
             s.shift = pass * plan.digit_bits;
             s.from = clearing.whole * (2 * pass) / (2 * plan.passes);
             s.to = clearing.whole * (2 * pass + 1) / (2 * plan.passes);
-            k_count_digits<Id><<<plan.tiles, SORT_THREADS, s.bins * 4, stream>>>(in, s, w.counts, clearing);
-            CPDE_LAUNCHED();
-            k_scan_counts<<<(s.bins + 7) / 8, 256, 0, stream>>>(w.counts, plan.tiles, s.bins);
-            CPDE_LAUNCHED();
+            if (pass == 0) {
+                k_count_digits<Id><<<plan.tiles, SORT_THREADS, s.bins * 4, stream>>>(in, s, w.counts, clearing);
+                CPDE_LAUNCHED();
+            } else {
+                launch_dependent(k_count_digits<Id>, plan.tiles, SORT_THREADS, s.bins * 4, stream, in, s, w.counts, clearing);
+            }
+            launch_dependent(k_scan_counts, (s.bins + 7) / 8, 256, 0, stream, w.counts, plan.tiles, s.bins);
             s.from = s.to;
             s.to = clearing.whole * (2 * pass + 2) / (2 * plan.passes);
             const size_t shared = SORT_WARPS * (plan.per_warp * sizeof(uint2) + s.bins * 4);
-            k_place_tokens<Id><<<plan.tiles, SORT_THREADS, shared, stream>>>(in, s, w.counts, w.pairs[pass & 1], clearing);
-            CPDE_LAUNCHED();
+            launch_dependent(k_place_tokens<Id>, plan.tiles, SORT_THREADS, shared, stream, in, s, w.counts,
+                             w.pairs[pass & 1], clearing);
         }
         return;
     }
@@ -298,13 +319,11 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
         s.grad_stride = c.in_stride;
         s.clear_from = clear_from;
         const unsigned clear_blocks = clear_from < s.rows ? SMS * 4 : 0;
-        k_sum_tokens<TI, TO, V><<<s.sum_blocks + clear_blocks, 256, 0, stream>>>(
-            pairs, static_cast<const TI*>(c.in), static_cast<TO*>(c.out), w.partial, s, clearing, c.scale);
-        CPDE_LAUNCHED();
+        launch_dependent(k_sum_tokens<TI, TO, V>, s.sum_blocks + clear_blocks, 256, 0, stream, pairs,
+                         static_cast<const TI*>(c.in), static_cast<TO*>(c.out), w.partial, s, clearing, c.scale);
         if (c.tokens >= 2 * int64_t(s.chunk)) {  // else no run covers a chunk behind its first
-            k_join_chunks<TO, V><<<dim3((s.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, s.tiles), JOIN_WARPS * 32, 0, stream>>>(
-                pairs, static_cast<TO*>(c.out), w.partial, s, c.scale);
-            CPDE_LAUNCHED();
+            launch_dependent(k_join_chunks<TO, V>, dim3((s.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, s.tiles), JOIN_WARPS * 32,
+                             0, stream, pairs, static_cast<TO*>(c.out), w.partial, s, c.scale);
         }
     });
 }
@@ -478,7 +497,7 @@ void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormC
     s.norm.tiles = plan.tiles;
     add_call(s.norm, c);
     s.wide_parameters = Alignment().at(c.weight, parameter).at(c.bias, parameter).vector(v) == v;
-    if (s.clusters < s.items) {
+    if (s.clusters < s.items && c.lengths) {
         s.counter = counter;
         CPDE_CUDA(cudaMemsetAsync(counter, 0, sizeof(*counter), stream));
     }
@@ -570,10 +589,8 @@ void group_norm(const NormCall& c, int device, cudaStream_t stream) {
             k_norm_moments<T, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
                 x, s, pieces);
             CPDE_LAUNCHED();
-            k_norm_apply<T, P, V, decltype(one)::value>
-                <<<dim3(unsigned(s.instances) * s.apply_splits, s.tiles), NORM_THREADS, size_t(s.pieces) * 8, stream>>>(
-                    x, weight, bias, y, c.mean, c.rstd, pieces, s);
-            CPDE_LAUNCHED();
+            launch_dependent(k_norm_apply<T, P, V, decltype(one)::value>, dim3(unsigned(s.instances) * s.apply_splits, s.tiles),
+                             NORM_THREADS, size_t(s.pieces) * 8, stream, x, weight, bias, y, c.mean, c.rstd, pieces, s);
         });
     });
 }
@@ -606,9 +623,8 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
                 launch_slab<k_norm_slab_gradient<T, P, V>>(plan, s, V, c, sizeof(P), counter, device, stream, grad, x,
                                                            c.mean, c.rstd, weight, bias, dx, channel_sums);
                 if (parameter_blocks) {
-                    k_norm_parameters<P><<<parameter_blocks, 1024, 0, stream>>>(
-                        dweight, dbias, channel_sums, s.instances * plan.cluster, s.channels);
-                    CPDE_LAUNCHED();
+                    launch_dependent(k_norm_parameters<P>, parameter_blocks, 1024, 0, stream, dweight, dbias, channel_sums,
+                                     s.instances * plan.cluster, s.channels);
                 }
                 done = true;
             }
@@ -627,11 +643,10 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
             k_norm_sums<T, P, V, ONE><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
                 grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);
             CPDE_LAUNCHED();
-            k_norm_input_gradient<T, P, V, ONE>
-                <<<dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
-                   size_t(s.pieces) * 8, stream>>>(grad, x, c.mean, c.rstd, weight, bias, dx, dweight, dbias,
-                                                    channel_sums, pieces, s);
-            CPDE_LAUNCHED();
+            launch_dependent(k_norm_input_gradient<T, P, V, ONE>,
+                             dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
+                             size_t(s.pieces) * 8, stream, grad, x, c.mean, c.rstd, weight, bias, dx, dweight, dbias,
+                             channel_sums, pieces, s);
         });
     });
 }
