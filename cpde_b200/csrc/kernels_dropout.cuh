@@ -85,7 +85,9 @@ struct DropoutShape {
     int64_t rows, columns, x_stride, residual_stride;
 };
 
-// y = residual + drop(x). One thread has the eight elements of a counter.
+// y = residual + drop(x). One thread has the eight elements of a counter. Bound by
+// memory: 67M bf16 with a residual (403 MB) take 60 to 63 us, 6.4 to 6.7 TB/s;
+// with the halves of a word compared one by one and the keys in registers 74.
 // VECTORS: 2 rows are contiguous and aligned, 1 rows of a multiple of eight
 // columns at aligned strides, 0 anything.
 template <class T, bool RESIDUAL, int VECTORS>

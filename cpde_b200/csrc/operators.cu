@@ -497,7 +497,7 @@ void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormC
     s.norm.tiles = plan.tiles;
     add_call(s.norm, c);
     s.wide_parameters = Alignment().at(c.weight, parameter).at(c.bias, parameter).vector(v) == v;
-    if (s.clusters < s.items && c.lengths) {
+    if (s.clusters < s.items) {
         s.counter = counter;
         CPDE_CUDA(cudaMemsetAsync(counter, 0, sizeof(*counter), stream));
     }

@@ -67,6 +67,17 @@ void check_workspace(const void* workspace, size_t bytes, size_t needed) {
     check_array(workspace, 256, "workspace");
 }
 
+// As guard(), and the caller's current device stays what it was: these calls mix
+// with those of a program that has a device of its own.
+template <class F>
+int guard_operator(cpde_engine* h, F&& f) {
+    int before = 0;
+    const bool known = h && h->engine && cudaGetDevice(&before) == cudaSuccess;
+    const int status = guard(h, f);
+    if (known && before != h->engine->device) cudaSetDevice(before);
+    return status;
+}
+
 cudaStream_t stream_of(cpde_engine* h, void* stream) {
     return stream ? static_cast<cudaStream_t>(stream) : h->engine->stream;
 }
@@ -78,7 +89,7 @@ extern "C" {
 int cpde_embedding(cpde_engine* h, int32_t table_type, const void* table, int64_t table_stride, int64_t rows,
                    int64_t channels, int32_t id_type, const void* ids, int64_t tokens, float scale, int32_t out_type,
                    void* out, void* stream) {
-    return guard(h, [&] {
+    return guard_operator(h, [&] {
         const size_t element = type_bytes(table_type), out_element = type_bytes(out_type);
         require(out_type == table_type || table_type == CPDE_F32, "the output's type must be the table's, or the table f32");
         check_embedding(tokens, rows, channels);
@@ -108,7 +119,7 @@ int cpde_embedding_gradient(cpde_engine* h, int32_t grad_type, const void* grad,
                             int32_t id_type, const void* ids, int64_t tokens, int64_t rows, int64_t channels,
                             float scale, int32_t out_type, void* out, void* workspace, size_t workspace_bytes,
                             void* stream) {
-    return guard(h, [&] {
+    return guard_operator(h, [&] {
         const size_t element = type_bytes(grad_type), out_element = type_bytes(out_type);
         require(out_type == grad_type || out_type == CPDE_F32, "the output's type must be the gradient's or f32");
         check_embedding(tokens, rows, channels);
@@ -128,7 +139,7 @@ int cpde_embedding_gradient(cpde_engine* h, int32_t grad_type, const void* grad,
 int cpde_dropout(cpde_engine* h, int32_t type, const void* x, int64_t x_stride, const void* residual,
                  int64_t residual_stride, int64_t rows, int64_t columns, double rate, uint64_t seed, uint64_t offset,
                  void* y, void* stream) {
-    return guard(h, [&] {
+    return guard_operator(h, [&] {
         const size_t element = type_bytes(type);
         check_dropout(rate);
         require(rows >= 0 && columns >= 0, "rows and columns must not be negative");
@@ -160,7 +171,7 @@ int cpde_group_norm(cpde_engine* h, int32_t type, const void* x, int64_t x_point
                     int32_t parameter_type, const void* weight, const void* bias, double eps, int32_t activation,
                     const int32_t* lengths, double rate, uint64_t seed, uint64_t offset, void* y, float* mean,
                     float* rstd, void* workspace, size_t workspace_bytes, void* stream) {
-    return guard(h, [&] {
+    return guard_operator(h, [&] {
         cpde::ops::NormCall c = {};
         c.type = type, c.parameter_type = parameter_type, c.activation = activation;
         c.x = x, c.x_point = x_point_stride, c.x_instance = x_instance_stride;
@@ -184,7 +195,7 @@ int cpde_group_norm_gradient(cpde_engine* h, int32_t type, const void* grad, int
                              const void* weight, const void* bias, int32_t activation, const int32_t* lengths,
                              double rate, uint64_t seed, uint64_t offset, void* dx, void* dweight, void* dbias,
                              void* workspace, size_t workspace_bytes, void* stream) {
-    return guard(h, [&] {
+    return guard_operator(h, [&] {
         cpde::ops::NormCall c = {};
         c.type = type, c.parameter_type = parameter_type, c.activation = activation;
         c.x = x, c.x_point = x_point_stride, c.x_instance = x_instance_stride;

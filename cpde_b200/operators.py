@@ -11,6 +11,7 @@ Equal inputs give equal bits: no result depends on the order in which blocks run
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -96,6 +97,7 @@ class Embedding(torch.autograd.Function):
         return embedding(engine, table, ids, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         ids, = ctx.saved_tensors
         return None, embedding_gradient(ctx.engine, grad, ids, ctx.rows, ctx.scale), None, None
@@ -110,6 +112,7 @@ class Dropout(torch.autograd.Function):
         return dropout(engine, x, rate, seed, offset, residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         return (None, dropout_gradient(ctx.engine, grad, *ctx.rule), None, None, None,
                 grad if ctx.residual else None)
@@ -128,6 +131,7 @@ class GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, weight, bias, lengths, mean, rstd = ctx.saved_tensors
         groups, activation, rate, seed, offset = ctx.options
