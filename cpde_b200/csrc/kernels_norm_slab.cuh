@@ -415,131 +415,131 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
     cluster_arrive();
     bool started = false;
     for (int32_t turn = 0;; turn ^= 1) {
-    const SlabExchange exchange(s, behind, turn);
-    const bool dealer = s.counter && seat.rank == 0 && threadIdx.x == 0;
-    int32_t next = s.items;
-    if (dealer) next = s.clusters + atomicAdd(s.counter, 1u);
-    clear_tail<T, V>(dx, at, seat, s);
-    copies_done();
-    __syncthreads();
-    AdjointTerms<V, true> k;
-    k.minus_mean.set(0, at.active ? -tile.mean[seat.group] : 0.0f);
-    k.rstd.set(0, at.active ? tile.rstd[seat.group] : 0.0f);
-    k.set_gain(stored_parameters<P, V>(tile.weight + seat.tx * V, weight, 1.0f));
-    k.bias = stored_parameters<P, V>(tile.bias + seat.tx * V, bias, 0.0f);
-    const int32_t next_length = dealer ? item_length(s, next) : 0;
-    AdjointSums<V, true> sums_of;
-    with_tail(s.norm, [&](auto activation, auto drops) {
-        constexpr int32_t ACTIVATION = decltype(activation)::value;
-        const auto scaled = k.template scaled<ACTIVATION>();
-        uint64_t index = uint64_t(at.index(s, seat));
-        Slot* slot = data;
-#pragma unroll 1  // two vectors at once spill: 111 against 105 us
-        for (int32_t i = 0; i < at.count; ++i, index += step, slot += NEXT) {
-            Pairs<V> d = unpack_pairs<T, V>(slot[0]), h = unpack_pairs<T, V>(slot[SLAB_THREADS]);
-            if constexpr (decltype(drops)::value) {
-                drop_at<V>(h, index, s.norm.rule);
-                // Exact; the second pass finds the zeros and need not draw again.
-                slot[SLAB_THREADS] = pack_pairs<T, V>(h);
-            }
-            norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
-            sums_of.add(d, h);
-        }
-    });
-    // Sums over the points, by channel: within a warp where its lanes repeat the
-    // tile's vectors (each step halves the values that a lane keeps), then over
-    // the rows that are left.
-    float2 sum[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = sums_of.of(j, k, s.norm.rule.factor);
-    if (warps) {
-        int32_t kept = 0;  // the first of the channels that the lane keeps
-        int32_t d = 16;
-#pragma unroll
-        for (int half = V / 2; half; half /= 2) {
-            if (d >= s.norm.tile) {
-                const bool upper = lane & d;
-#pragma unroll
-                for (int j = 0; j < half; ++j) {
-                    const float2 send = upper ? sum[j] : sum[j + half], keep = upper ? sum[j + half] : sum[j];
-                    sum[j] = __fadd2_rn(keep, shuffle_xor(send, d));
-                }
-                if (upper) kept += half;
-                d /= 2;
-            } else {
-#pragma unroll
-                for (int j = 0; j < half; ++j) parts[warp * width + seat.tx * V + kept + half + j] = sum[j + half];
-            }
-        }
-        for (; d >= s.norm.tile; d /= 2)
-            sum[0] = __fadd2_rn(sum[0], shuffle_xor(sum[0], d));
-        parts[warp * width + seat.tx * V + kept] = sum[0];
-    } else if (seat.ty < rows) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) parts[seat.ty * width + seat.tx * V + j] = sum[j];
-    }
-    __syncthreads();
-    for (int32_t c = threadIdx.x; c < at.channels; c += SLAB_THREADS) {
-        float2 v = parts[c];
-        for (int32_t r = 1; r < rows; ++r) v = __fadd2_rn(v, parts[r * width + c]);
-        channel_sums[(int64_t(at.n) * s.cluster + seat.rank) * s.norm.channels + at.first_channel + c] = v;
-        sums[c] = __fmul2_rn(v, both(weight ? to_float(tile.weight[c]) : 1.0f));
-    }
-    __syncthreads();
-    if (!started) cluster_wait();  // every CTA runs, and its memory can be written
-    started = true;
-    for (int32_t g = warp; g < at.groups; g += SLAB_WARPS) {
-        float2 v = make_float2(0.0f, 0.0f);
-        for (int32_t c = g * s.norm.width + lane; c < (g + 1) * s.norm.width; c += 32) v = __fadd2_rn(v, sums[c]);
-#pragma unroll
-        for (int d = 16; d; d /= 2) v = __fadd2_rn(v, shuffle_xor(v, d));
-        if (lane < s.cluster)
-            cluster.map_shared_rank(exchange.groups, lane)[g * s.cluster + seat.rank] = make_float4(v.x, v.y, 0.0f, 0.0f);
-    }
-    deal(s, cluster, exchange, seat, next, next_length);
-    cluster_arrive();
-    cluster_wait();
-    float2 means = over_cluster(s, exchange, at.groups, seat.group, [&](const float4& m) {
-        float2 v = make_float2(m.x, m.y);
-        for (int32_t i = s.cluster / 2; i; i /= 2) v = __fadd2_rn(v, shuffle_xor(v, i));
-        return v;
-    });
-    const int2 coming = s.counter ? *exchange.next : make_int2(s.items, 0);
-    const bool more = coming.x < s.items;
-    const Item<V> then(s, seat, more ? coming.x : 0, more ? coming.y : 0);
-    if (more) fetch_parameters(then);
-    const T* from = then.in(x, seat, s.norm.x_instance, s.norm.x_point);
-    const T* gfrom = then.in(grad, seat, s.norm.grad_instance, s.norm.grad_point);
-    Slot* slot = data;
-    if (at.active) {
-        const float inverse = at.length ? 1.0f / (float(at.length) * float(s.norm.width)) : 0.0f;
-        means = __fmul2_rn(means, both(inverse));
-        InputTerms<V, true> to_input;
-#pragma unroll
-        for (int j = 0; j < V; ++j) to_input.set(k, j, means, s.norm.rule.factor);
-        with_activation(s.norm.activation, [&](auto activation) {
+        const SlabExchange exchange(s, behind, turn);
+        const bool dealer = s.counter && seat.rank == 0 && threadIdx.x == 0;
+        int32_t next = s.items;
+        if (dealer) next = s.clusters + atomicAdd(s.counter, 1u);
+        clear_tail<T, V>(dx, at, seat, s);
+        copies_done();
+        __syncthreads();
+        AdjointTerms<V, true> k;
+        k.minus_mean.set(0, at.active ? -tile.mean[seat.group] : 0.0f);
+        k.rstd.set(0, at.active ? tile.rstd[seat.group] : 0.0f);
+        k.set_gain(stored_parameters<P, V>(tile.weight + seat.tx * V, weight, 1.0f));
+        k.bias = stored_parameters<P, V>(tile.bias + seat.tx * V, bias, 0.0f);
+        const int32_t next_length = dealer ? item_length(s, next) : 0;
+        AdjointSums<V, true> sums_of;
+        with_tail(s.norm, [&](auto activation, auto drops) {
             constexpr int32_t ACTIVATION = decltype(activation)::value;
             const auto scaled = k.template scaled<ACTIVATION>();
-            T* to = dx + at.index(s, seat);
-#pragma unroll 1
-            for (int32_t i = 0; i < at.count; ++i, to += step, slot += NEXT) {
+            uint64_t index = uint64_t(at.index(s, seat));
+            Slot* slot = data;
+#pragma unroll 1  // two vectors at once spill: 111 against 105 us
+            for (int32_t i = 0; i < at.count; ++i, index += step, slot += NEXT) {
                 Pairs<V> d = unpack_pairs<T, V>(slot[0]), h = unpack_pairs<T, V>(slot[SLAB_THREADS]);
-                norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
-                to_input.apply(h, d);
-                store<T, V>(to, pack_pairs<T, V>(h));
-                if (i < then.count) {
-                    copy_async<sizeof(Slot)>(slot, from);
-                    copy_async<sizeof(Slot)>(slot + SLAB_THREADS, gfrom);
-                    from += x_step;
-                    gfrom += grad_step;
+                if constexpr (decltype(drops)::value) {
+                    drop_at<V>(h, index, s.norm.rule);
+                    // Exact; the second pass finds the zeros and need not draw again.
+                    slot[SLAB_THREADS] = pack_pairs<T, V>(h);
                 }
+                norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
+                sums_of.add(d, h);
             }
         });
-    }
-    if (!more) break;
-    copy_points<T, V, 2>(slot, from, x_step, then.count - at.count);
-    copy_points<T, V, 2>(slot + SLAB_THREADS, gfrom, grad_step, then.count - at.count);
-    at = then;
+        // Sums over the points, by channel: within a warp where its lanes repeat the
+        // tile's vectors (each step halves the values that a lane keeps), then over
+        // the rows that are left.
+        float2 sum[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = sums_of.of(j, k, s.norm.rule.factor);
+        if (warps) {
+            int32_t kept = 0;  // the first of the channels that the lane keeps
+            int32_t d = 16;
+#pragma unroll
+            for (int half = V / 2; half; half /= 2) {
+                if (d >= s.norm.tile) {
+                    const bool upper = lane & d;
+#pragma unroll
+                    for (int j = 0; j < half; ++j) {
+                        const float2 send = upper ? sum[j] : sum[j + half], keep = upper ? sum[j + half] : sum[j];
+                        sum[j] = __fadd2_rn(keep, shuffle_xor(send, d));
+                    }
+                    if (upper) kept += half;
+                    d /= 2;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < half; ++j) parts[warp * width + seat.tx * V + kept + half + j] = sum[j + half];
+                }
+            }
+            for (; d >= s.norm.tile; d /= 2)
+                sum[0] = __fadd2_rn(sum[0], shuffle_xor(sum[0], d));
+            parts[warp * width + seat.tx * V + kept] = sum[0];
+        } else if (seat.ty < rows) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) parts[seat.ty * width + seat.tx * V + j] = sum[j];
+        }
+        __syncthreads();
+        for (int32_t c = threadIdx.x; c < at.channels; c += SLAB_THREADS) {
+            float2 v = parts[c];
+            for (int32_t r = 1; r < rows; ++r) v = __fadd2_rn(v, parts[r * width + c]);
+            channel_sums[(int64_t(at.n) * s.cluster + seat.rank) * s.norm.channels + at.first_channel + c] = v;
+            sums[c] = __fmul2_rn(v, both(weight ? to_float(tile.weight[c]) : 1.0f));
+        }
+        __syncthreads();
+        if (!started) cluster_wait();  // every CTA runs, and its memory can be written
+        started = true;
+        for (int32_t g = warp; g < at.groups; g += SLAB_WARPS) {
+            float2 v = make_float2(0.0f, 0.0f);
+            for (int32_t c = g * s.norm.width + lane; c < (g + 1) * s.norm.width; c += 32) v = __fadd2_rn(v, sums[c]);
+#pragma unroll
+            for (int d = 16; d; d /= 2) v = __fadd2_rn(v, shuffle_xor(v, d));
+            if (lane < s.cluster)
+                cluster.map_shared_rank(exchange.groups, lane)[g * s.cluster + seat.rank] = make_float4(v.x, v.y, 0.0f, 0.0f);
+        }
+        deal(s, cluster, exchange, seat, next, next_length);
+        cluster_arrive();
+        cluster_wait();
+        float2 means = over_cluster(s, exchange, at.groups, seat.group, [&](const float4& m) {
+            float2 v = make_float2(m.x, m.y);
+            for (int32_t i = s.cluster / 2; i; i /= 2) v = __fadd2_rn(v, shuffle_xor(v, i));
+            return v;
+        });
+        const int2 coming = s.counter ? *exchange.next : make_int2(s.items, 0);
+        const bool more = coming.x < s.items;
+        const Item<V> then(s, seat, more ? coming.x : 0, more ? coming.y : 0);
+        if (more) fetch_parameters(then);
+        const T* from = then.in(x, seat, s.norm.x_instance, s.norm.x_point);
+        const T* gfrom = then.in(grad, seat, s.norm.grad_instance, s.norm.grad_point);
+        Slot* slot = data;
+        if (at.active) {
+            const float inverse = at.length ? 1.0f / (float(at.length) * float(s.norm.width)) : 0.0f;
+            means = __fmul2_rn(means, both(inverse));
+            InputTerms<V, true> to_input;
+#pragma unroll
+            for (int j = 0; j < V; ++j) to_input.set(k, j, means, s.norm.rule.factor);
+            with_activation(s.norm.activation, [&](auto activation) {
+                constexpr int32_t ACTIVATION = decltype(activation)::value;
+                const auto scaled = k.template scaled<ACTIVATION>();
+                T* to = dx + at.index(s, seat);
+#pragma unroll 1
+                for (int32_t i = 0; i < at.count; ++i, to += step, slot += NEXT) {
+                    Pairs<V> d = unpack_pairs<T, V>(slot[0]), h = unpack_pairs<T, V>(slot[SLAB_THREADS]);
+                    norm_adjoint<ACTIVATION, V, true>(d, h, scaled);
+                    to_input.apply(h, d);
+                    store<T, V>(to, pack_pairs<T, V>(h));
+                    if (i < then.count) {
+                        copy_async<sizeof(Slot)>(slot, from);
+                        copy_async<sizeof(Slot)>(slot + SLAB_THREADS, gfrom);
+                        from += x_step;
+                        gfrom += grad_step;
+                    }
+                }
+            });
+        }
+        if (!more) break;
+        copy_points<T, V, 2>(slot, from, x_step, then.count - at.count);
+        copy_points<T, V, 2>(slot + SLAB_THREADS, gfrom, grad_step, then.count - at.count);
+        at = then;
     }
 }
 
