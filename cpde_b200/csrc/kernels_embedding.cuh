@@ -10,18 +10,20 @@ namespace cpde::ops {
 // gives a zero row. A thread has LOOKUPS vectors of V channels, a block's
 // vectors apart, so that its loads of ids and then of rows are in flight
 // together. Bound by memory: 32768 rows of 2048 bf16 (181 MB) take 32.9 us, 5.5
-// TB/s; 2 lookups a thread 35.1, 8 36.9. Narrow rows wait for an id and then a
-// row: 1M rows of 8 f32 (40 MB) take 12.9 us, 14.3 with stores that stay in L2.
-constexpr int LOOKUPS = 4, LOOKUP_THREADS = 64;
-template <class TI, class TO, class Id, int V>
-__global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
+// TB/s, with four lookups a thread; with two 35.1, with eight 36.9. Rows of fewer
+// than four vectors wait for an id and then a row, and more threads hide that
+// better: 1M rows of 8 f32 (40 MB) take 12.3 us with two lookups, 14.3 with four.
+constexpr int lookup_threads(int lookups) { return 256 / lookups; }
+template <class TI, class TO, class Id, int V, int LOOKUPS>
+__global__ void __launch_bounds__(lookup_threads(LOOKUPS)) k_embedding(const TI* __restrict__ table, int64_t table_stride, int64_t rows,
                                                     const Id* __restrict__ ids, TO* __restrict__ out,
                                                     int64_t channels, Divisor vectors, uint32_t count, float scale) {
-    const uint32_t base = blockIdx.x * (LOOKUP_THREADS * LOOKUPS) + threadIdx.x;
+    constexpr int THREADS = lookup_threads(LOOKUPS);
+    const uint32_t base = blockIdx.x * (THREADS * LOOKUPS) + threadIdx.x;
     int64_t source[LOOKUPS];
 #pragma unroll
     for (int u = 0; u < LOOKUPS; ++u) {
-        const uint32_t i = base + u * LOOKUP_THREADS;
+        const uint32_t i = base + u * THREADS;
         source[u] = -1;
         if (i < count) {
             const uint32_t t = vectors.quotient(i), k = i - t * vectors.divisor;
@@ -34,7 +36,7 @@ __global__ void __launch_bounds__(LOOKUP_THREADS) k_embedding(const TI* __restri
     for (int u = 0; u < LOOKUPS; ++u) v[u] = source[u] >= 0 ? load<TI, V>(table + source[u]) : zeros<TI, V>();
 #pragma unroll
     for (int u = 0; u < LOOKUPS; ++u) {
-        const uint32_t i = base + u * LOOKUP_THREADS;
+        const uint32_t i = base + u * THREADS;
         if (i >= count) continue;
         float f[V];
         unpack<TI, V>(v[u], f);

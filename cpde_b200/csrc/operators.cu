@@ -235,16 +235,20 @@ void embedding(const EmbeddingCall& c, cudaStream_t stream) {
                 const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / vectors);
                 for (int64_t t = 0; t < c.tokens; t += slab) {
                     const uint32_t count = uint32_t(std::min(slab, c.tokens - t) * vectors);
-                    const uint32_t blocks = (count + LOOKUP_THREADS * LOOKUPS - 1) / (LOOKUP_THREADS * LOOKUPS);
                     TO* to = static_cast<TO*>(c.out) + t * c.channels;
-                    if (c.id_type)
-                        k_embedding<TI, TO, int64_t, V><<<blocks, LOOKUP_THREADS, 0, stream>>>(
-                            static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int64_t*>(c.ids) + t,
-                            to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
-                    else
-                        k_embedding<TI, TO, int32_t, V><<<blocks, LOOKUP_THREADS, 0, stream>>>(
-                            static_cast<const TI*>(c.in), c.in_stride, c.rows, static_cast<const int32_t*>(c.ids) + t,
-                            to, c.channels, Divisor(uint32_t(vectors)), count, c.scale);
+                    auto launch = [&](auto* ids, auto lookups) {
+                        constexpr int LOOKUPS = decltype(lookups)::value, THREADS = lookup_threads(LOOKUPS);
+                        const uint32_t blocks = (count + THREADS * LOOKUPS - 1) / (THREADS * LOOKUPS);
+                        k_embedding<TI, TO, std::remove_const_t<std::remove_pointer_t<decltype(ids)>>, V, LOOKUPS>
+                            <<<blocks, THREADS, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, c.rows, ids + t, to,
+                                                             c.channels, Divisor(uint32_t(vectors)), count, c.scale);
+                    };
+                    auto launch_ids = [&](auto lookups) {
+                        if (c.id_type) launch(static_cast<const int64_t*>(c.ids), lookups);
+                        else launch(static_cast<const int32_t*>(c.ids), lookups);
+                    };
+                    if (vectors < 4) launch_ids(std::integral_constant<int, 2>{});
+                    else launch_ids(std::integral_constant<int, 4>{});
                     CPDE_LAUNCHED();
                 }
             }
