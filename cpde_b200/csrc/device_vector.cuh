@@ -39,13 +39,26 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Inputs that the kernel never writes.
+// Inputs that nothing writes while the kernel runs: the read-only path, and loads
+// that a compiler may move freely.
 template <class T, int V>
 __device__ __forceinline__ Vector<T, V> load(const T* p) {
     Vector<T, V> v;
     const auto* w = reinterpret_cast<const typename Vector<T, V>::Word*>(p);
 #pragma unroll
     for (int i = 0; i < Vector<T, V>::W::count; ++i) v.word[i] = __ldg(w + i);
+    return v;
+}
+
+// What the launch ahead writes while this kernel may already be there: ordinary
+// loads, which stay behind after_previous_launch(). For the same reason a pointer to
+// such data is never __restrict__.
+template <class T, int V>
+__device__ __forceinline__ Vector<T, V> load_written(const T* p) {
+    Vector<T, V> v;
+    const auto* w = reinterpret_cast<const typename Vector<T, V>::Word*>(p);
+#pragma unroll
+    for (int i = 0; i < Vector<T, V>::W::count; ++i) v.word[i] = w[i];
     return v;
 }
 

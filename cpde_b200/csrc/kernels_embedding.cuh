@@ -262,7 +262,7 @@ struct SortPass {
 };
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in, SortPass s,
-                                                                uint32_t* __restrict__ counts, Clearing clearing) {
+                                                                uint32_t* counts, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
     after_previous_launch();
     next_launch_may_begin();
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_count_digits(SortInput<Id> in,
 // over the tiles and writes the digits' totals behind them: a warp a digit. (Were
 // each CTA of the third to sum them itself, all of them would read 45 MB from L2
 // where 148 tiles have 512 digits, 9 us.)
-__global__ void __launch_bounds__(256) k_scan_counts(uint32_t* __restrict__ counts, uint32_t tiles, uint32_t bins) {
+__global__ void __launch_bounds__(256) k_scan_counts(uint32_t* counts, uint32_t tiles, uint32_t bins) {
     const uint32_t bin = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
     after_previous_launch();
     next_launch_may_begin();
@@ -317,8 +317,7 @@ __global__ void __launch_bounds__(256) k_scan_counts(uint32_t* __restrict__ coun
 // their places, as two words, they took 27.
 template <class Id>
 __global__ void __launch_bounds__(SORT_THREADS) k_place_tokens(SortInput<Id> in, SortPass s,
-                                                                const uint32_t* __restrict__ counts,
-                                                                uint2* __restrict__ out, Clearing clearing) {
+                                                                const uint32_t* counts, uint2* out, Clearing clearing) {
     extern __shared__ uint32_t sort_shared[];
     __shared__ uint32_t warp_sums[SORT_WARPS], shift_of[SORT_THREADS];
     uint2* staged = reinterpret_cast<uint2*>(sort_shared);  // the tile
@@ -373,9 +372,8 @@ struct SumShape {
 };
 
 template <class TI, class TO, int V>
-__global__ void __launch_bounds__(256) k_sum_tokens(const uint2* __restrict__ pairs, const TI* __restrict__ grad,
-                                                     TO* __restrict__ out, float* __restrict__ partial, SumShape s,
-                                                     Clearing clearing, float scale) {
+__global__ void __launch_bounds__(256) k_sum_tokens(const uint2* pairs, const TI* __restrict__ grad, TO* out,
+                                                     float* partial, SumShape s, Clearing clearing, float scale) {
     after_previous_launch();
     next_launch_may_begin();
     if (blockIdx.x >= s.sum_blocks) {
@@ -489,22 +487,20 @@ constexpr int JOIN_WARPS = 8, JOIN_CHUNKS = 32;
 constexpr uint32_t JOIN_LONG = 8;
 
 template <int V>
-__device__ __forceinline__ void add_chunks(const float* __restrict__ partial, int64_t channels, int64_t column,
+__device__ __forceinline__ void add_chunks(const float* partial, int64_t channels, int64_t column,
                                            uint32_t first, uint32_t last, uint32_t step, float (&sum)[V]) {
 #pragma unroll 8
     for (uint32_t c = first; c <= last; c += step) {
         float f[V];
-        unpack<float, V>(load<float, V>(partial + int64_t(c) * 2 * channels + column), f);
+        unpack<float, V>(load_written<float, V>(partial + int64_t(c) * 2 * channels + column), f);
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] += f[j];
     }
 }
 
 template <class TO, int V>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __restrict__ pairs,
-                                                                  TO* __restrict__ out,
-                                                                  const float* __restrict__ partial, SumShape s,
-                                                                  float scale) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* pairs, TO* out, const float* partial,
+                                                                  SumShape s, float scale) {
     __shared__ uint32_t starts[JOIN_CHUNKS], rows[JOIN_CHUNKS], lasts[JOIN_CHUNKS], found;
     __shared__ float sums[JOIN_WARPS][32 * V];
     after_previous_launch();
@@ -551,7 +547,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_join_chunks(const uint2* __
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] = 0.0f;
         if (begins && inside && y == 0)
-            unpack<float, V>(load<float, V>(partial + (int64_t(from) * 2 + 1) * s.channels + column), sum);
+            unpack<float, V>(load_written<float, V>(partial + (int64_t(from) * 2 + 1) * s.channels + column), sum);
     };
     auto write = [&](uint32_t r) {
         for (uint32_t d = 16; d >= s.lanes; d /= 2) {

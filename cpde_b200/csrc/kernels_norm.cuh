@@ -293,7 +293,7 @@ template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_apply(const T* __restrict__ x, const P* __restrict__ weight,
                                                               const P* __restrict__ bias, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd,
-                                                              const Moments* __restrict__ pieces, NormShape s) {
+                                                              const Moments* pieces, NormShape s) {
     extern __shared__ float norm_shared[];  // [group of the tile] x (mean, rstd)
     after_previous_launch();
     const int32_t split = blockIdx.x % s.apply_splits, n = blockIdx.x / s.apply_splits;
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
 // dw and db of 32 channels: sums over the rows of channel_sums in a fixed order.
 template <class P, int WARPS>
 __device__ __forceinline__ void sum_parameters(P* __restrict__ dweight, P* __restrict__ dbias,
-                                               const float2* __restrict__ channel_sums, int32_t rows,
+                                               const float2* channel_sums, int32_t rows,
                                                int32_t channels, int32_t block) {
     __shared__ float2 shared[WARPS][32];
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, channel = block * 32 + lane;
@@ -558,8 +558,7 @@ template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradient(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const P* __restrict__ weight, const P* __restrict__ bias, T* __restrict__ dx,
-    P* __restrict__ dweight, P* __restrict__ dbias, const float2* __restrict__ channel_sums,
-    const float2* __restrict__ pieces, NormShape s) {
+    P* __restrict__ dweight, P* __restrict__ dbias, const float2* channel_sums, const float2* pieces, NormShape s) {
     extern __shared__ float norm_shared[];
     after_previous_launch();
     float2* shared = reinterpret_cast<float2*>(norm_shared);

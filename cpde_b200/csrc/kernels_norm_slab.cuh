@@ -546,8 +546,7 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
 // dw and db from the channels' sums by instance.
 template <class P>
 __global__ void __launch_bounds__(1024) k_norm_parameters(P* __restrict__ dweight, P* __restrict__ dbias,
-                                                                   const float2* __restrict__ channel_sums,
-                                                                   int32_t rows, int32_t channels) {
+                                                                   const float2* channel_sums, int32_t rows, int32_t channels) {
     after_previous_launch();
     sum_parameters<P, 32>(dweight, dbias, channel_sums, rows, channels, blockIdx.x);
 }
