@@ -60,14 +60,16 @@ __device__ __forceinline__ void drop(Pairs<V>& f, const uint4& bits, uint32_t in
     } else {
         const bool back = V == 4 && (index & 4);
         const uint32_t word[4] = {back ? bits.z : bits.x, back ? bits.w : bits.y, bits.z, bits.w};
-        // Both halves against threshold - 1 in one instruction: `x > t - 1`.
-        const uint32_t least = (rule.threshold - 1) * 0x10001u;
+        // A half is below the threshold where it, in the upper half of a word, is no more
+        // than the largest word below threshold << 16. (One instruction compares both
+        // halves and has two predicates as results; but with f16 values behind it the
+        // compiler lost one of the two, depending on how it placed registers, and dropped
+        // elements' neighbours became NaN.)
+        const uint32_t last = (rule.threshold << 16) - 1;
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            bool high, low;
-            __vibmax_u16x2(least, word[i], &high, &low);  // whether t - 1 >= x
-            if (low) f.p[i].x = 0.0f;
-            if (high) f.p[i].y = 0.0f;
+            if (word[i] << 16 <= last) f.p[i].x = 0.0f;
+            if (word[i] <= last) f.p[i].y = 0.0f;
         }
     }
 }
@@ -86,8 +88,8 @@ struct DropoutShape {
 };
 
 // y = residual + drop(x). One thread has the eight elements of a counter. Bound by
-// memory: 67M bf16 with a residual (403 MB) take 60 to 63 us, 6.4 to 6.7 TB/s;
-// with the halves of a word compared one by one and the keys in registers 74.
+// memory: 67M bf16 with a residual (403 MB) take 61 to 63 us, 6.4 to 6.6 TB/s;
+// with the keys in registers 74.
 // VECTORS: 2 rows are contiguous and aligned, 1 rows of a multiple of eight
 // columns at aligned strides, 0 anything.
 template <class T, bool RESIDUAL, int VECTORS>
