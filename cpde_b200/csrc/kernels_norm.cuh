@@ -437,17 +437,16 @@ struct AdjointSums {
     }
 };
 
-// dx = rstd (factor w h - (m1 + xhat m2)) as two products and sums.
+// dx = rstd (factor w h - (m1 + xhat m2)) as products and sums.
 template <int V, bool ONE>
 struct InputTerms {
     Pairs<V> gain;              // factor w rstd
     GroupTerms<V, ONE> m1, m2;  // -rstd m1, -rstd^2 m2
-    __device__ __forceinline__ void set(const AdjointTerms<V, ONE>& k, int j, float2 m, float factor) {
-        const float r = k.rstd_of(j);
-        gain.set(j, factor * k.gain.get(j));
+    __device__ __forceinline__ void set(int j, float channel_gain, float minus_m1, float minus_m2) {
+        gain.set(j, channel_gain);
         if (!ONE || j == 0) {
-            m1.set(j, -r * m.x);
-            m2.set(j, -r * r * m.y);
+            m1.set(j, minus_m1);
+            m2.set(j, minus_m2);
         }
     }
     __device__ __forceinline__ void apply(Pairs<V>& h, const Pairs<V>& d) const {
@@ -455,11 +454,23 @@ struct InputTerms {
         for (int i = 0; i < Pairs<V>::N; ++i)
             h.p[i] = __ffma2_rn(h.p[i], gain.p[i], __ffma2_rn(d.p[i], m2.of(i), m1.of(i)));
     }
+    // With the product rounded by itself, as it is in m1: a group of one value, whose
+    // m1 is that product, then gives exactly zero. (A compiler joins a packed product
+    // and sum, the products of single values it leaves apart.)
+    __device__ __forceinline__ void apply_apart(Pairs<V>& h, const Pairs<V>& d) const {
+#pragma unroll
+        for (int j = 0; j < V; ++j) h.set(j, __fmul_rn(h.get(j), gain.get(j)));
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::N; ++i) h.p[i] = __fadd2_rn(h.p[i], __ffma2_rn(d.p[i], m2.of(i), m1.of(i)));
+    }
 };
 
-// Sums of h and h xhat over a block's points: per channel for dw and db
-// (channel_sums[instance][split][channel]), and times w per piece of a group
-// for dx (pieces[instance][split][tile][piece]).
+// factor w rstd, rounded in one order wherever it is needed.
+__device__ __forceinline__ float input_gain(float weight_rstd, float factor) { return factor * weight_rstd; }
+
+// Sums of h and h d over a block's points: per channel as h and h xhat for dw and
+// db (channel_sums[instance][split][channel]), and times factor w rstd per piece of
+// a group for dx (pieces[instance][split][tile][piece]).
 template <class T, class P, int V, bool ONE>
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T* __restrict__ grad, const T* __restrict__ x,
                                                              const float* __restrict__ mean,
@@ -467,7 +478,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
                                                              const P* __restrict__ weight, const P* __restrict__ bias,
                                                              NormShape s, float2* __restrict__ channel_sums,
                                                              float2* __restrict__ pieces) {
-    extern __shared__ float norm_shared[];  // [ty][channel of the tile] x (h, h xhat)
+    extern __shared__ float norm_shared[];  // [ty][channel of the tile] x (h, h d)
     next_launch_may_begin();
     float2* shared = reinterpret_cast<float2*>(norm_shared);
     const int32_t split = blockIdx.x % s.splits, n = blockIdx.x / s.splits;
@@ -498,7 +509,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
             }
         });
 #pragma unroll
-        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = sums.of(j, k, s.rule.factor);
+        for (int j = 0; j < V; ++j) shared[ty * width + tx * V + j] = make_float2(sums.h.get(j), sums.hd.get(j));
     }
     __syncthreads();
     for (int32_t c = threadIdx.x; c < t.count; c += NORM_THREADS) {
@@ -508,9 +519,11 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
             sum.x += v.x;
             sum.y += v.y;
         }
-        channel_sums[int64_t(blockIdx.x) * s.channels + t.first + c] = sum;
-        const float w = parameter(weight, t.first + c, 1.0f);
-        shared[c] = make_float2(sum.x * w, sum.y * w);  // only this thread reads column c
+        const int32_t channel = t.first + c;
+        const float r = rstd[int64_t(n) * s.groups + channel / s.width];
+        channel_sums[int64_t(blockIdx.x) * s.channels + channel] = make_float2(sum.x * s.rule.factor, sum.y * s.rule.factor * r);
+        const float gain = input_gain(parameter(weight, channel, 1.0f) * r, s.rule.factor);
+        shared[c] = make_float2(sum.x * gain, sum.y * gain);  // only this thread reads column c
     }
     __syncthreads();
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -603,7 +616,11 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradie
     InputTerms<V, ONE> to_input;
     to_input.gain.fill(0.0f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) to_input.set(k, j, shared[(channel + j) / s.width - t.group], s.rule.factor);
+    for (int j = 0; j < V; ++j) {
+        const float2 m = shared[(channel + j) / s.width - t.group];
+        const float r = k.rstd_of(j);
+        to_input.set(j, input_gain(k.gain.get(j), s.rule.factor), -m.x, -r * r * m.y);
+    }
     int32_t lo, hi;
     split_range(s.points, split, s.apply_splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
@@ -623,7 +640,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradie
             Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
             if constexpr (decltype(drops)::value) drop_at<V>(h, uint64_t(at), s.rule);
             norm_adjoint<ACTIVATION, V, ONE>(d, h, scaled);
-            to_input.apply(h, d);
+            to_input.apply_apart(h, d);
             store<T, V>(dx + at, pack_pairs<T, V>(h));
         }
     });

@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_GRADIENT_BLOCKS) k_norm_sla
             means = __fmul2_rn(means, both(inverse));
             InputTerms<V, true> to_input;
 #pragma unroll
-            for (int j = 0; j < V; ++j) to_input.set(k, j, means, s.norm.rule.factor);
+            for (int j = 0; j < V; ++j)
+                to_input.set(j, input_gain(k.gain.get(j), s.norm.rule.factor), -k.rstd_of(j) * means.x,
+                             -k.rstd_of(j) * k.rstd_of(j) * means.y);
             with_activation(s.norm.activation, [&](auto activation) {
                 constexpr int32_t ACTIVATION = decltype(activation)::value;
                 const auto scaled = k.template scaled<ACTIVATION>();

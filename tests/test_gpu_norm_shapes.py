@@ -83,3 +83,19 @@ def test_every_type_with_dropout_and_lengths(engine, kind, activation, n, p, wid
     case.with_weight = case.with_bias = True
     inputs = case.inputs(250)
     check(case, *inputs, *run(engine, case, *inputs))
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('activation', ['linear', 'sigmoid', 'tanh', 'silu'])
+@pytest.mark.parametrize('p,channels', [(1, 16), (1, 7), (9, 16), (9, 5), (3000, 8)])
+def test_a_group_of_one_value_does_not_depend_on_it(engine, kind, activation, p, channels):
+    """One channel a group and one point: xhat is 0, dx and dweight are exactly 0, and dbias is the gradient's sum."""
+    case = Case(random.Random(5))
+    case.n, case.p, case.width, case.groups, case.kind, case.parameters = 40, p, 1, channels, kind, F32
+    case.activation, case.rate, case.lengths = activation, 0.1, None if p == 1 else [1] * 40
+    case.with_weight = case.with_bias = True
+    inputs = case.inputs(260)
+    y, mean, rstd, dx, dweight, dbias = run(engine, case, *inputs)
+    check(case, *inputs, y, mean, rstd, dx, dweight, dbias)
+    assert torch.equal(mean, inputs[0][:, 0].float())
+    assert not dx.any() and not dweight.any() and dbias.any()
