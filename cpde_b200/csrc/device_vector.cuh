@@ -170,6 +170,14 @@ __device__ __forceinline__ Vector<T, V> pack_pairs(const Pairs<V>& f) {
     }
 }
 
+// `v`, or zero where rounding has made it negative. A NaN stays one: fmaxf would make
+// it a zero too.
+__device__ __forceinline__ float not_negative(float v) { return v < 0.0f ? 0.0f : v; }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+// A value to take deviations from: one that is not finite would make a NaN of every
+// mean, also where the definition gives an infinity.
+__device__ __forceinline__ float finite_or_zero(float v) { return finite(v) ? v : 0.0f; }
+
 // Quotient of 31-bit integers by a divisor that is fixed for the launch
 // (multiply-high with a precomputed reciprocal; exact for n < 2^31).
 struct Divisor {

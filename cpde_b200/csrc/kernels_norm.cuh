@@ -145,7 +145,7 @@ __device__ __forceinline__ Moments merged(const Moments& a, const Moments& b) {
     if (b.count == 0.0f) return a;
     if (a.count == 0.0f) return b;
     const float delta = b.mean - a.mean, share = b.count / count;
-    return {count, a.mean + delta * share, a.m2 + b.m2 + delta * delta * a.count * share};
+    return {count, finite(delta) ? a.mean + delta * share : a.mean + b.mean, a.m2 + b.m2 + delta * delta * a.count * share};
 }
 __device__ __forceinline__ Moments warp_merged(Moments m) {
 #pragma unroll
@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_moments(cons
         const T* base = x + n * s.x_instance + t.first + tx * V;
         if (lo + ty < hi) {
             shift = unpack_pairs<T, V>(load<T, V>(base + (lo + ty) * s.x_point));
-            scale<V>(shift, -1.0f);
+#pragma unroll
+            for (int j = 0; j < V; ++j) shift.set(j, -finite_or_zero(shift.get(j)));
         }
 #pragma unroll 4
         for (int32_t p = lo + ty; p < hi; p += ys) {
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_moments(cons
             const float mean = s1.get(j) * inverse;
             float* to = norm_shared + 2 * (ty * width + tx * V + j);
             to[0] = mean - shift.get(j);
-            to[1] = fmaxf(s2.get(j) - s1.get(j) * mean, 0.0f);
+            to[1] = not_negative(s2.get(j) - s1.get(j) * mean);
         }
     }
     __syncthreads();

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
             float2 sum = f.p[0];
 #pragma unroll
             for (int j = 1; j < Pairs<V>::N; ++j) sum = __fadd2_rn(sum, f.p[j]);
-            return (sum.x + sum.y) * (1.0f / V);
+            return finite_or_zero((sum.x + sum.y) * (1.0f / V));
         };
         {
             const float2 shift = both(at.active ? -pivot_of(seat.group) : 0.0f);
@@ -312,14 +312,14 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
             const float count = float(at.hi - at.lo) * float(s.norm.width), d = count > 0.0f ? v.x / count : 0.0f;
             if (lane < s.cluster)
                 cluster.map_shared_rank(exchange.groups, lane)[g * s.cluster + seat.rank] =
-                    make_float4(count, pivot_of(g) + d, fmaxf(v.y - v.x * d, 0.0f), 0.0f);
+                    make_float4(count, pivot_of(g) + d, not_negative(v.y - v.x * d), 0.0f);
         }
         deal(s, cluster, exchange, seat, next, next_length);
         cluster_arrive();
         cluster_wait();
         const float2 statistics = over_cluster(s, exchange, at.groups, seat.group, [&](const float4& m) {
             // (count, mean, m2): sums by deviations from the first CTA's mean.
-            const float pivot = __shfl_sync(~0u, m.y, (lane / s.cluster) * s.cluster);
+            const float pivot = finite_or_zero(__shfl_sync(~0u, m.y, (lane / s.cluster) * s.cluster));
             float count = m.x, d = m.y - pivot;
             float2 v = make_float2(count * d, count > 0.0f ? fmaf(count * d, d, m.z) : 0.0f);
             for (int32_t i = s.cluster / 2; i; i /= 2) {
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
                 v = __fadd2_rn(v, shuffle_xor(v, i));
             }
             d = count > 0.0f ? v.x / count : 0.0f;
-            const float var = fmaxf(v.y - v.x * d, 0.0f) / count;
+            const float var = not_negative(v.y - v.x * d) / count;
             return make_float2(pivot + d, count > 0.0f ? 1.0f / sqrtf(var + s.norm.eps) : 0.0f);
         });
         const int2 coming = s.counter ? *exchange.next : make_int2(s.items, 0);
