@@ -19,6 +19,7 @@
 #pragma once
 #include "device_vector.cuh"
 #include "kernels_dropout.cuh"
+#include "point_range.hpp"
 
 namespace cpde::ops {
 
@@ -157,14 +158,6 @@ __device__ __forceinline__ Moments warp_merged(Moments m) {
     return m;
 }
 
-// The points [lo, hi) of split `split` of `splits`.
-__device__ __forceinline__ void split_range(int32_t length, int32_t split, int32_t splits, int32_t& lo, int32_t& hi) {
-    const int32_t per = (length + splits - 1) / splits;
-    const int64_t first = int64_t(split) * per;
-    lo = int32_t(first < length ? first : length);
-    hi = int32_t(first + per < length ? first + per : length);
-}
-
 // Channels [first, first + count) of the tile, and the groups they meet.
 struct Tile {
     int32_t first, count, group, groups;
@@ -200,14 +193,17 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_moments(cons
         s1.fill(0.0f);
         s2.fill(0.0f);
         int32_t count = 0;
-        const T* base = x + n * s.x_instance + t.first + tx * V;
-        if (lo + ty < hi) {
-            shift = unpack_pairs<T, V>(load<T, V>(base + (lo + ty) * s.x_point));
+        // Points are counted from lo: a thread's last step goes beyond hi, which may be
+        // 2^31 - 2.
+        const T* base = x + n * s.x_instance + lo * s.x_point + t.first + tx * V;
+        const int32_t points = hi - lo;
+        if (ty < points) {
+            shift = unpack_pairs<T, V>(load<T, V>(base + ty * s.x_point));
 #pragma unroll
             for (int j = 0; j < V; ++j) shift.set(j, -finite_or_zero(shift.get(j)));
         }
 #pragma unroll 4
-        for (int32_t p = lo + ty; p < hi; p += ys) {
+        for (int32_t p = ty; p < points; p += ys) {
             const Pairs<V> f = unpack_pairs<T, V>(load<T, V>(base + p * s.x_point));
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -494,17 +490,19 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_sums(const T
         AdjointTerms<V, ONE> k;
         load_terms<P, V, ONE>(k, s, n, channel, mean, rstd, weight, bias);
         AdjointSums<V, ONE> sums;
-        const T* from = x + n * s.x_instance + channel;
-        const T* gfrom = grad + n * s.grad_instance + channel;
+        const T* from = x + n * s.x_instance + lo * s.x_point + channel;
+        const T* gfrom = grad + n * s.grad_instance + lo * s.grad_point + channel;
+        const int64_t row = int64_t(n) * s.points + lo;
+        const int32_t points = hi - lo;  // counted from lo, as the moments
         with_tail(s, [&](auto activation, auto drops) {
             constexpr int32_t ACTIVATION = decltype(activation)::value;
             const auto scaled = k.template scaled<ACTIVATION>();
 #pragma unroll 2
-            for (int32_t p = lo + ty; p < hi; p += ys) {
+            for (int32_t p = ty; p < points; p += ys) {
                 Pairs<V> d = unpack_pairs<T, V>(load<T, V>(from + p * s.x_point));
                 Pairs<V> h = unpack_pairs<T, V>(load<T, V>(gfrom + p * s.grad_point));
                 if constexpr (decltype(drops)::value)
-                    drop_at<V>(h, uint64_t((int64_t(n) * s.points + p) * s.channels + channel), s.rule);
+                    drop_at<V>(h, uint64_t((row + p) * s.channels + channel), s.rule);
                 norm_adjoint<ACTIVATION, V, ONE>(d, h, scaled);
                 sums.add(d, h);
             }
