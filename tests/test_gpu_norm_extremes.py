@@ -95,3 +95,25 @@ def test_behind_the_length_it_does_not_count(engine, value):
     x[0, 30:], x[1] = value, value
     for a, b in zip(step(engine, x, grad, 8, None, None, lengths), before):
         assert (a is None and b is None) or torch.equal(a, b)
+
+
+@pytest.mark.parametrize('n,p,c,groups', [(2, 50, 16, 2), (2, 3000, 16, 2), (2, 40000, 16, 2), (3, 700, 21, 7), (1, 9000, 24, 8)])
+@pytest.mark.parametrize('level,outlier', [(1000.0, 0.0), (1000.0, 3000.0), (-300.0, 0.0)])
+@pytest.mark.parametrize('activation', ['linear', 'silu'])
+def test_level_far_above_the_spread(engine, n, p, c, groups, level, outlier, activation):
+    """The gradient against the formula with the kernel's own statistics, so that their error does not widen its bound; a first
+    point that is not like the others is what the deviations are taken from."""
+    x, grad = level + made(310, n, p, c), 1 + made(311, n, p, c)
+    x[:, 0] += outlier
+    weight, bias = 1 + 0.3 * made(312, c), 0.3 * made(313, c)
+    y, mean, rstd = operators.group_norm(engine, x, groups, weight, bias, activation=activation)
+    parts = operators.group_norm_gradient(engine, grad, x, mean, rstd, groups, weight, bias, activation=activation)
+    norm = norm_bounds.Norm(wide(x), groups, wide(weight), wide(bias), 1e-5, activation, None, 0.0, 0, 0)
+    want, want_rstd, off, off_rstd = norm.statistics()
+    assert (abs(wide(mean) - want) <= off).all() and (abs(wide(rstd) - want_rstd) <= off_rstd).all()
+    u = 2.0 ** -24
+    want, bound = norm.forward(wide(mean), wide(rstd), u, 2.0 ** -150)
+    assert (abs(wide(y) - want) <= bound).all()
+    for got, (want, bound) in zip(parts, norm.gradient(wide(grad), wide(mean), wide(rstd), u, 2.0 ** -150)):
+        assert np.linalg.norm(bound) < 0.05 * np.linalg.norm(want)  # the bound can fail
+        assert (abs(wide(got) - want) <= bound + u * abs(want)).all()
