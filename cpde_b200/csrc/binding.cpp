@@ -23,6 +23,7 @@ struct Entries {
     decltype(&cpde_embedding_gradient_workspace) embedding_gradient_workspace;
     decltype(&cpde_embedding_gradient) embedding_gradient;
     decltype(&cpde_dropout) dropout;
+    decltype(&cpde_group_norm_forward_workspace) group_norm_forward_workspace;
     decltype(&cpde_group_norm_workspace) group_norm_workspace;
     decltype(&cpde_group_norm) group_norm;
     decltype(&cpde_group_norm_gradient) group_norm_gradient;
@@ -218,7 +219,8 @@ struct Norm {
     double rate;
     uint64_t seed, offset;
     size_t bytes = 0;
-    Norm(Arguments& a, const Engine& e, const at::Tensor& x, int64_t groups) {
+    Norm(Arguments& a, const Engine& e, const at::Tensor& x, int64_t groups,
+         decltype(entries.group_norm_workspace) workspace) {
         weight = a.optional(e, "weight"), bias = a.optional(e, "bias");
         activation = int32_t(a.integer());
         lengths = a.optional(e, "lengths");
@@ -238,7 +240,7 @@ struct Norm {
         check(!lengths.defined() || (lengths.scalar_type() == at::kInt && lengths.dim() == 1 &&
                                      lengths.size(0) == x.size(0) && lengths.is_contiguous()),
               "lengths must be a contiguous int32 tensor with a value per instance");
-        check(entries.group_norm_workspace(x.size(0), x.size(1), x.size(2), groups, &bytes) == CPDE_OK,
+        check(workspace(x.size(0), x.size(1), x.size(2), groups, &bytes) == CPDE_OK,
               "invalid sizes, or a group count that does not divide the channels");
     }
     const int32_t* counts() const { return static_cast<const int32_t*>(pointer(lengths)); }
@@ -249,7 +251,7 @@ PyObject* group_norm(Arguments& a) {
     const Points x(a.tensor(e, "x"), "x must have shape (instances, points, channels)");
     const int64_t groups = a.integer();
     const double eps = a.number();
-    const Norm n(a, e, x.t, groups);
+    const Norm n(a, e, x.t, groups, entries.group_norm_forward_workspace);
     const at::Tensor y = made(x.t.sizes(), x.t, x.t.scalar_type());
     const at::Tensor mean = made({x.t.size(0), groups}, x.t, at::kFloat), rstd = made({x.t.size(0), groups}, x.t, at::kFloat);
     const at::Tensor workspace = made({int64_t(n.bytes)}, x.t, at::kByte);
@@ -269,7 +271,7 @@ PyObject* group_norm_gradient(Arguments& a) {
     const Points x(std::move(x_in), "x must have shape (instances, points, channels)");
     const at::Tensor mean = a.tensor(e, "mean"), rstd = a.tensor(e, "rstd");
     const int64_t groups = a.integer();
-    const Norm n(a, e, x.t, groups);
+    const Norm n(a, e, x.t, groups, entries.group_norm_workspace);
     for (const at::Tensor* t : {&mean, &rstd})
         check(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == x.t.size(0) && t->size(1) == groups &&
                   t->is_contiguous(),
@@ -309,6 +311,8 @@ PyObject* bind(Arguments& a) {
         reinterpret_cast<decltype(e.embedding_gradient_workspace)>(address("cpde_embedding_gradient_workspace"));
     e.embedding_gradient = reinterpret_cast<decltype(e.embedding_gradient)>(address("cpde_embedding_gradient"));
     e.dropout = reinterpret_cast<decltype(e.dropout)>(address("cpde_dropout"));
+    e.group_norm_forward_workspace =
+        reinterpret_cast<decltype(e.group_norm_forward_workspace)>(address("cpde_group_norm_forward_workspace"));
     e.group_norm_workspace = reinterpret_cast<decltype(e.group_norm_workspace)>(address("cpde_group_norm_workspace"));
     e.group_norm = reinterpret_cast<decltype(e.group_norm)>(address("cpde_group_norm"));
     e.group_norm_gradient = reinterpret_cast<decltype(e.group_norm_gradient)>(address("cpde_group_norm_gradient"));

@@ -389,11 +389,12 @@ NormShape norm_shape(int64_t instances, int64_t points, int64_t channels, int64_
     return s;
 }
 
-size_t norm_workspace(const NormShape& s) {
-    const size_t blocks = size_t(s.instances) * s.splits;
-    const size_t slabs = padded(4) + size_t(s.instances) * SLAB_CLUSTER * s.channels * sizeof(float2);
-    return std::max(slabs, padded(blocks * s.tiles * s.pieces * sizeof(Moments)) +
-                               padded(blocks * s.channels * sizeof(float2)));
+// The workspace of two passes: the groups' pieces, and the gradient's sums by channel.
+size_t piece_bytes(const NormShape& s, size_t piece) {
+    return padded(size_t(s.instances) * s.splits * s.tiles * s.pieces * piece);
+}
+size_t channel_sum_bytes(const NormShape& s, int64_t parts) {
+    return padded(size_t(s.instances) * parts * s.channels * sizeof(float2));
 }
 
 // Strides, lengths and dropout of a call.
@@ -549,11 +550,22 @@ void with_norm_vector(int v, int64_t width, F&& f) {
 
 }  // namespace
 
-size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups) {
-    size_t bytes = 0;
-    for (int v : {8, 4, 1})
-        if (channels % v == 0)
-            bytes = std::max(bytes, norm_workspace(norm_shape(instances, points, channels, groups, v)));
+size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, bool gradient) {
+    size_t bytes = padded(4);
+    for (int v : {8, 4, 1}) {
+        if (channels % v) continue;
+        const NormShape s = norm_shape(instances, points, channels, groups, v);
+        bytes = std::max(bytes, gradient ? piece_bytes(s, sizeof(float2)) + channel_sum_bytes(s, s.splits)
+                                         : piece_bytes(s, sizeof(Moments)));
+        if (!gradient || v == 1 || s.width % v) continue;
+        // Every plan that a call of these sizes can take.
+        const size_t types[][2] = {{4, 4}, {2, 4}, {2, 2}};  // bytes of an element and of a parameter
+        for (auto [element, parameter] : types) {
+            if (v * element > 16) continue;
+            const SlabPlan plan = slab_plan(s, v, element, parameter, 2);
+            if (plan.cluster) bytes = std::max(bytes, padded(4) + channel_sum_bytes(s, plan.cluster));
+        }
+    }
     return bytes;
 }
 
@@ -641,8 +653,7 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
             add_call(s, c);
             auto* pieces = static_cast<float2*>(c.workspace);
             auto* channel_sums = reinterpret_cast<float2*>(
-                static_cast<char*>(c.workspace) +
-                padded(size_t(s.instances) * s.splits * s.tiles * s.pieces * sizeof(Moments)));
+                static_cast<char*>(c.workspace) + piece_bytes(s, sizeof(float2)));
             const size_t shared = size_t(NORM_THREADS / s.tile) * s.tile * V * 8;
             k_norm_sums<T, P, V, ONE><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
                 grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);

@@ -53,7 +53,7 @@ struct NormCall {
     void *dweight, *dbias;
     void* workspace;
 };
-size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups);
+size_t group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, bool gradient);
 void group_norm(const NormCall& call, int device, cudaStream_t stream);
 void group_norm_gradient(const NormCall& call, int device, cudaStream_t stream);
 

@@ -2,6 +2,8 @@
 // launches of operators.cu.
 #include "operators.hpp"
 
+#include <algorithm>
+
 namespace {
 
 using cpde::require;
@@ -78,6 +80,22 @@ int guard_operator(cpde_engine* h, F&& f) {
     return status;
 }
 
+// A workspace size for a caller.
+template <class F>
+int query(size_t* bytes, F&& f) {
+    if (!bytes) return CPDE_REJECTED;
+    try {
+        *bytes = f();
+        return CPDE_OK;
+    } catch (...) {
+        return CPDE_REJECTED;
+    }
+}
+
+size_t norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, bool gradient) {
+    return instances && points ? cpde::ops::group_norm_workspace(instances, points, channels, groups, gradient) : 0;
+}
+
 cudaStream_t stream_of(cpde_engine* h, void* stream) {
     return stream ? static_cast<cudaStream_t>(stream) : h->engine->stream;
 }
@@ -105,14 +123,10 @@ int cpde_embedding(cpde_engine* h, int32_t table_type, const void* table, int64_
 }
 
 int cpde_embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channels, size_t* bytes) {
-    try {
+    return query(bytes, [&] {
         check_embedding(tokens, rows, channels);
-        if (!bytes) return CPDE_REJECTED;
-        *bytes = cpde::ops::embedding_gradient_workspace(tokens, rows, channels);
-        return CPDE_OK;
-    } catch (...) {
-        return CPDE_REJECTED;
-    }
+        return cpde::ops::embedding_gradient_workspace(tokens, rows, channels);
+    });
 }
 
 int cpde_embedding_gradient(cpde_engine* h, int32_t grad_type, const void* grad, int64_t grad_stride,
@@ -156,14 +170,18 @@ int cpde_dropout(cpde_engine* h, int32_t type, const void* x, int64_t x_stride, 
 }
 
 int cpde_group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, size_t* bytes) {
-    try {
+    return query(bytes, [&] {
         check_norm(instances, points, channels, groups);
-        if (!bytes) return CPDE_REJECTED;
-        *bytes = instances && points ? cpde::ops::group_norm_workspace(instances, points, channels, groups) : 0;
-        return CPDE_OK;
-    } catch (...) {
-        return CPDE_REJECTED;
-    }
+        return std::max(norm_workspace(instances, points, channels, groups, false),
+                        norm_workspace(instances, points, channels, groups, true));
+    });
+}
+
+int cpde_group_norm_forward_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, size_t* bytes) {
+    return query(bytes, [&] {
+        check_norm(instances, points, channels, groups);
+        return norm_workspace(instances, points, channels, groups, false);
+    });
 }
 
 int cpde_group_norm(cpde_engine* h, int32_t type, const void* x, int64_t x_point_stride,
@@ -181,9 +199,7 @@ int cpde_group_norm(cpde_engine* h, int32_t type, const void* x, int64_t x_point
         c.out = y, c.mean = mean, c.rstd = rstd, c.workspace = workspace;
         check_norm_call(c);
         require(eps > 0, "eps must be positive");
-        if (instances && points)
-            check_workspace(workspace, workspace_bytes,
-                            cpde::ops::group_norm_workspace(instances, points, channels, groups));
+        check_workspace(workspace, workspace_bytes, norm_workspace(instances, points, channels, groups, false));
         cpde::ops::group_norm(c, h->engine->device, stream_of(h, stream));
     });
 }
@@ -213,8 +229,7 @@ int cpde_group_norm_gradient(cpde_engine* h, int32_t type, const void* grad, int
             check_array(grad, type_bytes(type), "grad");
             require(grad_point_stride >= channels || points == 1, "the gradient's point stride must be at least the channels");
             require(grad_instance_stride >= 0, "the gradient's instance stride must not be negative");
-            check_workspace(workspace, workspace_bytes,
-                            cpde::ops::group_norm_workspace(instances, points, channels, groups));
+            check_workspace(workspace, workspace_bytes, norm_workspace(instances, points, channels, groups, true));
         }
         cpde::ops::group_norm_gradient(c, h->engine->device, stream_of(h, stream));
     });

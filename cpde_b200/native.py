@@ -64,6 +64,7 @@ SIGNATURES = {
     'cpde_embedding_gradient': (I32, [P, I32, P, I64, I32, P, I64, I64, I64, F32, I32, P, P, SZ, P]),
     'cpde_dropout': (I32, [P, I32, P, I64, P, I64, I64, I64, F64, U64, U64, P, P]),
     'cpde_group_norm_workspace': (I32, [I64, I64, I64, I64, ctypes.POINTER(SZ)]),
+    'cpde_group_norm_forward_workspace': (I32, [I64, I64, I64, I64, ctypes.POINTER(SZ)]),
     'cpde_group_norm': (I32, [P, I32, P, I64, I64, I64, I64, I64, I64, I32, P, P, F64, I32, P, F64, U64, U64, P, P, P,
                               P, SZ, P]),
     'cpde_group_norm_gradient': (I32, [P, I32, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I32, P, P, I32, P,

@@ -25,7 +25,8 @@ ACTIVATIONS = {'sigmoid': 0, 'linear': 1, 'tanh': 2, 'silu': 3}
 _operators.bind(native.EngineError, {
     name: ctypes.cast(getattr(native.load(), name), ctypes.c_void_p).value
     for name in ('cpde_last_error', 'cpde_embedding', 'cpde_embedding_gradient_workspace', 'cpde_embedding_gradient',
-                 'cpde_dropout', 'cpde_group_norm_workspace', 'cpde_group_norm', 'cpde_group_norm_gradient')})
+                 'cpde_dropout', 'cpde_group_norm_forward_workspace', 'cpde_group_norm_workspace', 'cpde_group_norm',
+                 'cpde_group_norm_gradient')})
 
 
 def _handle(engine, tensor):

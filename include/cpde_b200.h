@@ -237,8 +237,11 @@ int cpde_dropout(cpde_engine* engine, int32_t type, const void* x, int64_t x_str
  * clamp(lengths[n], 0, points) points: the others are not read and y is zero
  * there; an instance without points has mean = rstd = 0. `rate`, `seed` and
  * `offset` are those of cpde_dropout over y's elements. mean and rstd are FP32
- * (instances x groups). The group count divides channels. */
+ * (instances x groups). The group count divides channels. The first workspace
+ * size serves the forward and the gradient; the second, for the forward alone, is
+ * that of the groups' moments, without the gradient's sums by channel. */
 int cpde_group_norm_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, size_t* bytes);
+int cpde_group_norm_forward_workspace(int64_t instances, int64_t points, int64_t channels, int64_t groups, size_t* bytes);
 int cpde_group_norm(cpde_engine* engine, int32_t type, const void* x, int64_t x_point_stride,
                     int64_t x_instance_stride, int64_t instances, int64_t points, int64_t channels, int64_t groups,
                     int32_t parameter_type, const void* weight, const void* bias, double eps, int32_t activation,

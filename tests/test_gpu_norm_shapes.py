@@ -99,3 +99,35 @@ def test_a_group_of_one_value_does_not_depend_on_it(engine, kind, activation, p,
     check(case, *inputs, y, mean, rstd, dx, dweight, dbias)
     assert torch.equal(mean, inputs[0][:, 0].float())
     assert not dx.any() and not dweight.any() and dbias.any()
+
+
+@pytest.mark.parametrize('kind,parameters', [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize('n,p,c,groups', [(1, 30000, 64, 8), (1, 3000, 512, 8), (300, 33, 64, 16), (3, 5000, 96, 4), (70, 90, 192, 12),
+                                          (2, 2000, 1024, 2), (1, 60000, 24, 8), (9, 700, 21, 7), (600, 3, 64, 64), (1, 1, 8, 2)])
+def test_nothing_is_written_behind_the_workspace(engine, kind, parameters, n, p, c, groups):
+    """The queried sizes, forward and gradient, and 64 KB behind them that stay as they were."""
+    case = Case(random.Random(6))
+    case.n, case.p, case.width, case.groups, case.kind, case.parameters = n, p, c // groups, groups, kind, parameters
+    x, grad, weight, bias = case.inputs(270)
+    code, parameter = {F32: 0, BF16: 1}[kind], {F32: 0, BF16: 1}[parameters]
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    mean, rstd = torch.empty((n, groups), device='cuda'), torch.empty((n, groups), device='cuda')
+    dweight, dbias = torch.empty_like(weight), torch.empty_like(bias)
+    size = ctypes.c_size_t()
+    for query, entry, arguments in (
+            (engine.lib.cpde_group_norm_forward_workspace, engine.lib.cpde_group_norm,
+             lambda: (code, x.data_ptr(), c, p * c, n, p, c, groups, parameter, weight.data_ptr(), bias.data_ptr(), 1e-5, 3, None,
+                      0.1, 1, 2, y.data_ptr(), mean.data_ptr(), rstd.data_ptr())),
+            (engine.lib.cpde_group_norm_workspace, engine.lib.cpde_group_norm_gradient,
+             lambda: (code, grad.data_ptr(), c, p * c, x.data_ptr(), c, p * c, mean.data_ptr(), rstd.data_ptr(), n, p, c, groups,
+                      parameter, weight.data_ptr(), bias.data_ptr(), 3, None, 0.1, 1, 2, dx.data_ptr(), dweight.data_ptr(),
+                      dbias.data_ptr()))):
+        assert query(n, p, c, groups, ctypes.byref(size)) == native.OK
+        workspace = torch.full((size.value + 65536,), 0xA5, dtype=torch.uint8, device='cuda')
+        assert entry(engine.handle, *arguments(), workspace.data_ptr(), size.value, LEGACY) == native.OK
+        assert bool((workspace[size.value:] == 0xA5).all())
+    options = dict(activation='silu', rate=0.1, seed=1, offset=2)
+    want, m, r = operators.group_norm(engine, x, groups, weight, bias, **options)
+    assert torch.equal(y, want) and torch.equal(mean, m) and torch.equal(rstd, r)
+    for got, want in zip((dx, dweight, dbias), operators.group_norm_gradient(engine, grad, x, m, r, groups, weight, bias, **options)):
+        assert torch.equal(got, want)
