@@ -417,6 +417,7 @@ struct SlabPlan {
     size_t shared;
 };
 constexpr size_t SLAB_SIX = 36 << 10, SLAB_THREE = 72 << 10, SLAB_TWO = 108 << 10, SLAB_ONE = 220 << 10;  // shared memory of a CTA
+constexpr int64_t MOST_ITEMS = int64_t(1) << 30;  // items of a launch are counted in 31 bits
 
 // Vectors of at most 16 bytes (a copy's most) whose channels are of one group.
 int slab_vector(int fit, size_t element, int64_t width) {
@@ -434,6 +435,7 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, size_t parameter, 
     p.tile = int32_t(tile_groups * group);
     if (p.tile > SLAB_THREADS) return p;
     p.tiles = int32_t((groups + tile_groups - 1) / tile_groups);
+    if (int64_t(s.instances) * p.tiles > MOST_ITEMS) return p;
     const int64_t ys = SLAB_THREADS / p.tile;
     auto plan = [&](int32_t cluster) {
         const int64_t points = (int64_t(s.points) + cluster - 1) / cluster;

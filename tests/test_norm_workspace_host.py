@@ -43,3 +43,10 @@ def test_wrong_sizes_are_refused():
     for bad in ((1, 10, 8, 3), (1, 10, 8, 0), (-1, 10, 8, 2), (1, -1, 8, 2), (1, 10, 0, 1), ((1 << 20) + 1, 1, 8, 2)):
         assert lib.cpde_group_norm_forward_workspace(*bad, ctypes.byref(size)) == native.REJECTED
     assert lib.cpde_group_norm_forward_workspace(1, 10, 8, 2, None) == native.REJECTED
+
+
+def test_more_items_than_a_launch_counts_take_two_passes():
+    """2^20 instances of 2^18 groups: 2^38 items of the one-pass kernel, whose sums of eight CTAs would be asked for."""
+    n, p, c, groups = 1 << 20, 3000, 1 << 20, 1 << 18
+    _, both = sizes(n, p, c, groups)
+    assert both < 4 * 8 * n * c
