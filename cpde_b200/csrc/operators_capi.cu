@@ -198,7 +198,7 @@ int cpde_group_norm(cpde_engine* h, int32_t type, const void* x, int64_t x_point
         c.eps = eps, c.rate = rate, c.seed = seed, c.offset = offset;
         c.out = y, c.mean = mean, c.rstd = rstd, c.workspace = workspace;
         check_norm_call(c);
-        require(eps > 0, "eps must be positive");
+        require(float(eps) > 0, "eps must be positive, also in FP32");
         check_workspace(workspace, workspace_bytes, norm_workspace(instances, points, channels, groups, false));
         cpde::ops::group_norm(c, h->engine->device, stream_of(h, stream));
     });

@@ -117,3 +117,15 @@ def test_level_far_above_the_spread(engine, n, p, c, groups, level, outlier, act
     for got, (want, bound) in zip(parts, norm.gradient(wide(grad), wide(mean), wide(rstd), u, 2.0 ** -150)):
         assert np.linalg.norm(bound) < 0.05 * np.linalg.norm(want)  # the bound can fail
         assert (abs(wide(got) - want) <= bound + u * abs(want)).all()
+
+
+def test_eps_is_positive_in_fp32(engine):
+    """1e-60 is zero in FP32, in which the kernels add it: groups without variance would be NaN."""
+    x = torch.full((2, 40, 64), 2.5, device='cuda')
+    for eps in (1e-60, 1e-46, 0.0, -1.0):
+        with pytest.raises(native.EngineError, match='eps') as error:
+            operators.group_norm(engine, x, 8, eps=eps)
+        assert error.value.status == native.REJECTED
+    for shape in (x, x[:, :, :21]):
+        y, _, rstd = operators.group_norm(engine, shape, 1, eps=1e-40)
+        assert not y.any() and torch.allclose(rstd.double(), torch.full_like(rstd, 1e20).double(), rtol=1e-4)
