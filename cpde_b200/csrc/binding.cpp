@@ -6,6 +6,7 @@
 // The entry points' addresses come from Python (bind), so that this module uses
 // the library that cpde_b200.native has loaded.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -96,6 +97,9 @@ struct Arguments {
         check(THPVariable_Check(o), (std::string(name) + " must be a tensor").c_str());
         at::Tensor t = THPVariable_Unpack(o);
         check(t.is_cuda() && t.get_device() == e.device, "every tensor must be on the engine's device");
+        // The result would be detached in silence.
+        check(!t.requires_grad() || !at::GradMode::is_enabled(),
+              "a tensor requires gradients: use operators.Embedding, Dropout or GroupNorm, or torch.no_grad()");
         return t;
     }
     // An element type, or `none` for None.

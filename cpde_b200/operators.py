@@ -2,9 +2,13 @@
 with an activation (channels last), each with its gradient.
 
 Every function takes the :class:`cpde_b200.native.Engine` of the tensors' device, launches on torch's current stream of
-that device and returns new contiguous tensors; nothing synchronises. The classes at the end are the same operators for
-torch's autograd. Wrong arguments raise ``ValueError`` here or :class:`cpde_b200.native.EngineError` in the library. As
-with any kernel launch, a tensor that another stream made has to be ordered before the current stream by the caller.
+that device and returns new contiguous tensors; nothing synchronises. Wrong arguments raise ``ValueError`` here or
+:class:`cpde_b200.native.EngineError` in the library. As with any kernel launch, a tensor that another stream made has to be
+ordered before the current stream by the caller.
+
+The functions compute values only, and refuse a tensor that requires gradients while torch records them. The classes at the
+end are the same operators for torch's autograd, with first derivatives in reverse mode; forward mode, vmap, tracing and
+higher derivatives are not supported.
 
 Equal inputs give equal bits: no result depends on the order in which blocks run.
 """
@@ -101,6 +105,8 @@ class Embedding(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         ids, = ctx.saved_tensors
+        if not ctx.needs_input_grad[1]:
+            return (None,) * 4
         return None, embedding_gradient(ctx.engine, grad, ids, ctx.rows, ctx.scale), None, None
 
 
@@ -115,7 +121,7 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return (None, dropout_gradient(ctx.engine, grad, *ctx.rule), None, None, None,
+        return (None, dropout_gradient(ctx.engine, grad, *ctx.rule) if ctx.needs_input_grad[1] else None, None, None, None,
                 grad if ctx.residual else None)
 
 
