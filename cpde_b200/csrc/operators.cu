@@ -469,7 +469,9 @@ template <auto kernel, class... A>
 void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormCall& c, size_t parameter,
                  uint32_t* counter, int device, cudaStream_t stream, A... arguments) {
     static std::mutex mutex;
-    static std::map<std::tuple<int, int32_t, size_t>, int32_t> resident;  // clusters by device, size and memory
+    // Clusters that a device holds at once, by its number, their size and their memory in
+    // KB: a property of the kernel, looked up once; at most 5 x 220 a device.
+    static std::map<std::tuple<int, int32_t, int32_t>, int32_t> resident;
     cudaLaunchConfig_t config = {};
     config.blockDim = dim3(SLAB_THREADS);
     config.dynamicSmemBytes = plan.shared;
@@ -483,13 +485,16 @@ void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormC
     int32_t clusters;
     {
         std::lock_guard<std::mutex> lock(mutex);
-        int32_t& known = resident[{device, plan.cluster, plan.shared}];
+        const int32_t kilobytes = int32_t((plan.shared + 1023) / 1024);
+        int32_t& known = resident[{device, plan.cluster, kilobytes}];
         if (!known) {
             dynamic_shared(kernel, SLAB_ONE);
             CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             config.gridDim = dim3(plan.cluster);
+            config.dynamicSmemBytes = size_t(kilobytes) * 1024;
             int most = 0;
             CPDE_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &config));
+            config.dynamicSmemBytes = plan.shared;
             known = std::max(1, most);
         }
         clusters = known;

@@ -186,7 +186,8 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
  *  - All arrays are device memory of the engine's device, aligned to their
  *    element type; 16-byte aligned addresses and strides take the fast kernels.
  *    Strides are in elements. Outputs are contiguous and do not overlap inputs.
- *  - Nothing is allocated and nothing is kept between calls. Where a workspace
+ *  - No device memory is allocated and no data is kept between calls (what a
+ *    kernel's launch may take of the device is looked up once). Where a workspace
  *    is asked for, it is 256-byte aligned device memory of at least the queried
  *    size, contents undefined, that no other call in flight uses.
  *  - Calls are asynchronous on `stream` (NULL: the engine's stream) and may be
