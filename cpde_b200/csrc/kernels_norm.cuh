@@ -35,7 +35,7 @@ struct NormShape {
     int32_t vectors;                                         // channels / V
     int32_t tile, tiles;                                     // vectors of a block, blocks across the channels
     int32_t pieces;                                          // most groups that a tile meets
-    int32_t splits, apply_splits;                            // blocks along the points
+    int32_t splits;                                          // blocks along the points
     int32_t activation;
     float eps;
     const int32_t* lengths;
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_apply(const 
                                                               const Moments* pieces, NormShape s) {
     extern __shared__ float norm_shared[];  // [group of the tile] x (mean, rstd)
     after_previous_launch();
-    const int32_t split = blockIdx.x % s.apply_splits, n = blockIdx.x / s.apply_splits;
+    const int32_t split = blockIdx.x % s.splits, n = blockIdx.x / s.splits;
     const Tile t = tile_of<V>(s, blockIdx.y);
     const int32_t length = length_of(s, n);
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_apply(const 
         k.bias.set(j, parameter(bias, channel + j, 0.0f));
     }
     int32_t lo, hi;
-    split_range(s.points, split, s.apply_splits, lo, hi);
+    split_range(s.points, split, s.splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
     const int64_t row = int64_t(n) * s.points;
     // From the back: the moments' pass has left the ends of the ranges in L2.
@@ -575,14 +575,14 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradie
     after_previous_launch();
     float2* shared = reinterpret_cast<float2*>(norm_shared);
     const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int32_t n = blockIdx.x / s.apply_splits;
+    const int32_t n = blockIdx.x / s.splits;
     if (n >= s.instances) {
         if (blockIdx.y == 0)
             sum_parameters<P, NORM_WARPS>(dweight, dbias, channel_sums, s.instances * s.splits, s.channels,
-                              blockIdx.x - s.instances * s.apply_splits);
+                              blockIdx.x - s.instances * s.splits);
         return;
     }
-    const int32_t split = blockIdx.x % s.apply_splits;
+    const int32_t split = blockIdx.x % s.splits;
     const Tile t = tile_of<V>(s, blockIdx.y);
     const int32_t length = length_of(s, n);
     for (int32_t g = warp; g < t.groups; g += NORM_WARPS) {
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS) k_norm_input_gradie
         to_input.set(j, input_gain(k.gain.get(j), s.rule.factor), -m.x, -r * r * m.y);
     }
     int32_t lo, hi;
-    split_range(s.points, split, s.apply_splits, lo, hi);
+    split_range(s.points, split, s.splits, lo, hi);
     const T* from = x + n * s.x_instance + channel;
     const T* gfrom = grad + n * s.grad_instance + channel;
     // From the back, as the forward.

@@ -132,19 +132,23 @@ __device__ __forceinline__ void copy_points(Vector<T, V>* slots, const T* from, 
 // The tile's weights and biases in shared memory, and for the gradient its means
 // and reciprocal deviations. They are copied with the points: a load of its own
 // would wait behind the points' in the queue to memory, once more an item.
+__host__ __device__ constexpr size_t tile_parameter_array(int64_t channels, size_t parameter) {
+    return (size_t(channels) * parameter + 15) / 16 * 16;
+}
+__host__ __device__ constexpr size_t tile_parameter_bytes(int64_t channels, size_t parameter) {
+    return 2 * tile_parameter_array(channels, parameter) + 2 * SLAB_GROUPS * sizeof(float);
+}
 template <class P>
 struct TileParameters {
     P *weight, *bias;
     float *mean, *rstd;
-    __host__ __device__ static constexpr size_t array(int32_t channels) {
-        return (size_t(channels) * sizeof(P) + 15) / 16 * 16;
+    __device__ __forceinline__ TileParameters(unsigned char* at, int32_t channels) {
+        const size_t array = tile_parameter_array(channels, sizeof(P));
+        weight = reinterpret_cast<P*>(at);
+        bias = reinterpret_cast<P*>(at + array);
+        mean = reinterpret_cast<float*>(at + 2 * array);
+        rstd = mean + SLAB_GROUPS;
     }
-    __host__ __device__ static constexpr size_t bytes(int32_t channels) {
-        return 2 * array(channels) + 2 * SLAB_GROUPS * sizeof(float);
-    }
-    __device__ __forceinline__ TileParameters(unsigned char* at, int32_t channels)
-        : weight(reinterpret_cast<P*>(at)), bias(reinterpret_cast<P*>(at + array(channels))),
-          mean(reinterpret_cast<float*>(at + 2 * array(channels))), rstd(mean + SLAB_GROUPS) {}
 };
 
 template <class P, int V>
@@ -271,8 +275,8 @@ __global__ void __launch_bounds__(SLAB_THREADS, SLAB_BLOCKS) k_norm_slab(const T
         k.gain = stored_parameters<P, V>(tile.weight + seat.tx * V, weight, 1.0f);
         k.bias = stored_parameters<P, V>(tile.bias + seat.tx * V, bias, 0.0f);
         // Deviations from a pivot, the mean of the group's first vector of values:
-        // what their squares lose to cancellation is bounded by the number of
-        // values over V^2 however far off that vector lies.
+        // however far off that vector lies, its own share of the variance bounds what the
+        // squares' sum loses to cancellation by the number of values over V.
         auto pivot_of = [&](int32_t g) {
             if (at.hi <= at.lo) return 0.0f;
             const Pairs<V> f = unpack_pairs<T, V>(reinterpret_cast<const Slot*>(slab)[g * s.group_vectors]);

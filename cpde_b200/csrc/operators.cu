@@ -285,10 +285,9 @@ void embedding_gradient(const EmbeddingCall& c, int device, cudaStream_t stream)
             constexpr int V = decltype(width)::value;
             const uint32_t vectors = uint32_t(c.channels / V), lanes = power_of_two_from(std::min<uint32_t>(vectors, 8));
             const uint32_t blocks = (vectors + lanes - 1) / lanes, size = std::max(32u, power_of_two_from(c.tokens));
-            const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(16, uint32_t(lanes)));
             auto launch = [&](auto* ids) {
                 k_small_gradient<TI, TO, std::remove_const_t<std::remove_pointer_t<decltype(ids)>>, V>
-                    <<<dim3(blocks, shares), size, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
+                    <<<dim3(blocks, lanes), size, 0, stream>>>(static_cast<const TI*>(c.in), c.in_stride, ids, uint32_t(c.tokens), size,
                                                  c.rows, c.channels, vectors, lanes, static_cast<TO*>(c.out), c.scale);
             };
             if (c.id_type) launch(static_cast<const int64_t*>(c.ids));
@@ -385,7 +384,6 @@ NormShape norm_shape(int64_t instances, int64_t points, int64_t channels, int64_
     const int64_t ys = NORM_THREADS / s.tile, blocks = instances * s.tiles;
     s.splits = int32_t(std::max<int64_t>(1, std::min(std::max<int64_t>(1, SMS * NORM_BLOCKS / blocks), (points + ys * 4 - 1) / (ys * 4))));
     s.splits = int32_t(std::max<int64_t>(s.splits, (points + ys * 512 - 1) / (ys * 512)));
-    s.apply_splits = s.splits;
     return s;
 }
 
@@ -442,7 +440,7 @@ SlabPlan slab_plan(const NormShape& s, int v, size_t element, size_t parameter, 
         const int64_t slots = (points + ys - 1) / ys;
         p.slots = int32_t(std::min<int64_t>(slots, 1 << 16));
         const int64_t width = int64_t(p.tile) * v, rows = slab_rows_are_warps(p.tile) ? SLAB_WARPS : ys;
-        const size_t parameters = 2 * ((size_t(width) * parameter + 15) / 16 * 16) + 2 * SLAB_GROUPS * sizeof(float);
+        const size_t parameters = tile_parameter_bytes(width, parameter);
         p.shared = size_t(p.slots) * SLAB_THREADS * vector_bytes * arrays +
                    2 * SlabExchange::bytes(int32_t(tile_groups), cluster) + parameters +
                    (arrays == 1 ? SLAB_THREADS : size_t((rows + 1) * width)) * sizeof(float2);
@@ -612,7 +610,7 @@ void group_norm(const NormCall& c, int device, cudaStream_t stream) {
             k_norm_moments<T, V><<<dim3(unsigned(s.instances) * s.splits, s.tiles), NORM_THREADS, shared, stream>>>(
                 x, s, pieces);
             CPDE_LAUNCHED();
-            launch_dependent(k_norm_apply<T, P, V, decltype(one)::value>, dim3(unsigned(s.instances) * s.apply_splits, s.tiles),
+            launch_dependent(k_norm_apply<T, P, V, decltype(one)::value>, dim3(unsigned(s.instances) * s.splits, s.tiles),
                              NORM_THREADS, size_t(s.pieces) * 8, stream, x, weight, bias, y, c.mean, c.rstd, pieces, s);
         });
     });
@@ -666,7 +664,7 @@ void group_norm_gradient(const NormCall& c, int device, cudaStream_t stream) {
                 grad, x, c.mean, c.rstd, weight, bias, s, channel_sums, pieces);
             CPDE_LAUNCHED();
             launch_dependent(k_norm_input_gradient<T, P, V, ONE>,
-                             dim3(unsigned(s.instances) * s.apply_splits + parameter_blocks, s.tiles), NORM_THREADS,
+                             dim3(unsigned(s.instances) * s.splits + parameter_blocks, s.tiles), NORM_THREADS,
                              size_t(s.pieces) * 8, stream, grad, x, c.mean, c.rstd, weight, bias, dx, dweight, dbias,
                              channel_sums, pieces, s);
         });

@@ -10,7 +10,7 @@ The functions compute values only, and refuse a tensor that requires gradients w
 end are the same operators for torch's autograd, with first derivatives in reverse mode; forward mode, vmap, tracing and
 higher derivatives are not supported.
 
-Equal inputs give equal bits: no result depends on the order in which blocks run.
+Equal calls on equally laid out inputs give equal bits: no result depends on the order in which blocks run.
 """
 import ctypes
 

@@ -184,7 +184,8 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
  * that condition the point networks above (a latent code per instance, features
  * per cell, normalised and regularised trunk layers).
  *  - All arrays are device memory of the engine's device, aligned to their
- *    element type; 16-byte aligned addresses and strides take the fast kernels.
+ *    element type. Addresses and strides of whole 16 bytes take the fast kernels;
+ *    FP32 dropout and FP32-to-16-bit lookups want 32 bytes on their FP32 side.
  *    Strides are in elements. Outputs are contiguous and do not overlap inputs.
  *  - No device memory is allocated and no data is kept between calls (what a
  *    kernel's launch may take of the device is looked up once). Where a workspace
@@ -192,7 +193,8 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
  *    size, contents undefined, that no other call in flight uses.
  *  - Calls are asynchronous on `stream` (NULL: the engine's stream) and may be
  *    captured into a CUDA graph. Results do not depend on the order in which
- *    blocks run: equal inputs give equal bits.
+ *    blocks run: equal calls (sizes, types, strides, alignments, values) give
+ *    equal bits.
  *  - Computation and sums are in FP32, rounded once to the output's type. */
 #define CPDE_F32 0
 #define CPDE_BF16 1
@@ -210,7 +212,7 @@ int cpde_embedding(cpde_engine* engine, int32_t table_type, const void* table, i
 /* out[r,:] = scale * (sum of grad[t,:] over the tokens t with ids[t] == r), for
  * every row of the table (rows that no token names are zeros); absent ids add
  * nothing. The tokens are sorted by row and each row's are added in an order
- * that depends on the ids alone. `out_type` equals `grad_type` or is CPDE_F32. */
+ * that the ids, the sizes, the types and the alignment fix. `out_type` equals `grad_type` or is CPDE_F32. */
 int cpde_embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t channels, size_t* bytes);
 int cpde_embedding_gradient(cpde_engine* engine, int32_t grad_type, const void* grad, int64_t grad_stride,
                             int32_t id_type, const void* ids, int64_t tokens, int64_t rows, int64_t channels,
