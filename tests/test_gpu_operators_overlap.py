@@ -143,3 +143,31 @@ def test_group_norms_in_two_passes(engine, n, p, c, groups, kind):
     case.with_weight = case.with_bias = True
     first, other = case.inputs(230), case.inputs(240)
     check(case, *first, *queued(lambda: run(engine, case, *other), lambda: run(engine, case, *first)))
+
+
+def test_streams_with_inputs_of_their_own(engine):
+    """Three streams at once, each with its own inputs: workspaces, counters and statistics stay apart."""
+    case = Case(random.Random(7))
+    case.n, case.p, case.groups, case.width, case.kind, case.parameters = 20, 900, 8, 8, BF16, F32
+    case.activation, case.rate, case.lengths = 'silu', 0.1, [900 - 40 * i for i in range(20)]
+    case.with_weight = case.with_bias = True
+    inputs = [case.inputs(400 + 10 * i) for i in range(3)]
+    lookups = [(made(440 + i, 70001, 8), some_ids(450 + i, 70001, 30000, absent=True)) for i in range(3)]
+
+    def step(i):
+        return (*run(engine, case, *inputs[i]), operators.embedding_gradient(engine, *lookups[i], 30000))
+
+    want = [step(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [[] for _ in range(3)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(2000000)
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in range(3):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
