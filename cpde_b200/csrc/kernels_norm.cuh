@@ -11,8 +11,8 @@
 //
 // The kernels of this file take two passes over memory, for point sets that no
 // cluster holds (kernels_norm_slab.cuh). Both directions are bound by memory: a
-// million points of 64 f32 channels take 169 us forward (805 MB in two passes) and
-// 237 us for the gradient (1.34 GB, 5.7 TB/s). The second pass goes from the back
+// million points of 64 f32 channels take 160 us forward (805 MB in two passes, 5.0
+// TB/s) and 238 us for the gradient (1.34 GB, 5.6 TB/s). The second pass goes from the back
 // because the first leaves the ends of the blocks' ranges in L2. FP32 arithmetic
 // is in packed pairs: an issue slot then has two operations, and issue slots are
 // what an activation and a generator run short of.

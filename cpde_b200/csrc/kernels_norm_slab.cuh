@@ -4,9 +4,9 @@
 // distributed shared memory, and write the result from what they hold.
 //
 // Measured on 32 instances of 4096 points and 512 bf16 channels in 32 groups, SiLU:
-// forward 63 us for 268 MB (two passes: 131; the copies alone, without sums and
+// forward 65 us for 268 MB (two passes: 131; the copies alone, without sums and
 // arithmetic, 48), where the special function unit's two operations an element
-// are busy for 30 us; the gradient with dropout and half of the points 105 us for
+// are busy for 30 us; the gradient with dropout and half of the points 106 us for
 // 268 MB (two passes: 177), bound by issue at 10 to 11 warps an SM, the most that
 // the slabs leave room for. A tile is 64 bytes of a point: with 128, a cluster has
 // twice the CTAs to wait for (76 us forward), with 32 memory is read in half lines.

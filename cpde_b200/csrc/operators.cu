@@ -516,9 +516,9 @@ void launch_slab(const SlabPlan& plan, const NormShape& norm, int v, const NormC
 }
 
 // The widest vectors that the call's addresses and strides allow. The forward
-// takes eight channels of any type (169 us against 177 for a million points of 64
-// f32 channels in two passes), the gradient one access of 16 bytes an array (241
-// against 250 us).
+// takes eight channels of any type (160 us against 169 for a million points of 64
+// f32 channels in two passes), the gradient one access of 16 bytes an array (234
+// us; with eight channels 232, within what the sums' registers allow).
 template <class T>
 int norm_vector(const NormCall& c) {
     Alignment a;

@@ -1,5 +1,5 @@
-"""Operators on CUDA tensors for networks that condition the point networks: embedding lookup, dropout and group norm
-with an activation (channels last), each with its gradient.
+"""Operators on CUDA tensors for torch networks beside the engine's, such as one that learns a family of its solutions:
+embedding lookup, dropout and group norm with an activation (channels last), each with its gradient.
 
 Every function takes the :class:`cpde_b200.native.Engine` of the tensors' device, launches on torch's current stream of
 that device and returns new contiguous tensors; nothing synchronises. Wrong arguments raise ``ValueError`` here or

@@ -181,8 +181,9 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
 /* --- Operators on caller-owned device arrays (no reference counterpart) ---
  *
  * Embedding lookup, dropout and group norm with their gradients, for networks
- * that condition the point networks above (a latent code per instance, features
- * per cell, normalised and regularised trunk layers).
+ * that a caller trains beside the point networks above, such as one that learns a
+ * family of their solutions (a latent code per instance, features per cell,
+ * normalised and regularised trunk layers).
  *  - All arrays are device memory of the engine's device, aligned to their
  *    element type. Addresses and strides of whole 16 bytes take the fast kernels;
  *    FP32 dropout and FP32-to-16-bit lookups want 32 bytes on their FP32 side.
