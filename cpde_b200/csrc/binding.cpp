@@ -13,6 +13,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/cpde_b200.h"
 
@@ -28,6 +29,14 @@ struct Entries {
     decltype(&cpde_group_norm_workspace) group_norm_workspace;
     decltype(&cpde_group_norm) group_norm;
     decltype(&cpde_group_norm_gradient) group_norm_gradient;
+    decltype(&cpde_linear_workspace) linear_workspace;
+    decltype(&cpde_linear) linear;
+    decltype(&cpde_linear_gradient_workspace) linear_gradient_workspace;
+    decltype(&cpde_linear_gradient) linear_gradient;
+    decltype(&cpde_orthogonalize_workspace) orthogonalize_workspace;
+    decltype(&cpde_orthogonalize) orthogonalize;
+    decltype(&cpde_muon_workspace) muon_workspace;
+    decltype(&cpde_muon) muon;
 } entries = {};
 PyObject* engine_error = nullptr;  // cpde_b200.native.EngineError
 
@@ -99,7 +108,7 @@ struct Arguments {
         check(t.is_cuda() && t.get_device() == e.device, "every tensor must be on the engine's device");
         // The result would be detached in silence.
         check(!t.requires_grad() || !at::GradMode::is_enabled(),
-              "a tensor requires gradients: use operators.Embedding, Dropout or GroupNorm, or torch.no_grad()");
+              "a tensor requires gradients: use operators.Embedding, Dropout, GroupNorm or Linear, or torch.no_grad()");
         return t;
     }
     // An element type, or `none` for None.
@@ -125,6 +134,12 @@ const void* pointer(const at::Tensor& t) { return t.defined() ? t.const_data_ptr
 
 at::Tensor made(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
     return at::empty(sizes, like.options().dtype(type).requires_grad(false));
+}
+
+PyObject* wrapped(const at::Tensor& t) {
+    if (t.defined()) return THPVariable_Wrap(t);
+    Py_INCREF(Py_None);
+    return Py_None;
 }
 
 // A matrix of rows with adjacent channels and their stride; other layouts
@@ -291,12 +306,169 @@ PyObject* group_norm_gradient(Arguments& a) {
         x.t.size(2), groups, n.parameter, pointer(n.weight), pointer(n.bias), n.activation, n.counts(), n.rate, n.seed,
         n.offset, dx.mutable_data_ptr(), const_cast<void*>(pointer(dweight)), const_cast<void*>(pointer(dbias)),
         workspace.mutable_data_ptr(), n.bytes, e.stream()));
-    auto wrap = [](const at::Tensor& t) {
-        if (t.defined()) return THPVariable_Wrap(t);
-        Py_INCREF(Py_None);
-        return Py_None;
-    };
-    return Py_BuildValue("NNN", wrap(dx), wrap(dweight), wrap(dbias));
+    return Py_BuildValue("NNN", wrapped(dx), wrapped(dweight), wrapped(dbias));
+}
+
+// A bias of a value per output, FP32 or of x's type; its type's code.
+int32_t bias_code(const at::Tensor& bias, const at::Tensor& x, int64_t outputs) {
+    if (!bias.defined()) return CPDE_F32;
+    check(bias.dim() == 1 && bias.size(0) == outputs && bias.is_contiguous(), "bias must be a contiguous tensor with a value per output");
+    check(bias.scalar_type() == at::kFloat || bias.scalar_type() == x.scalar_type(), "bias must be float32 or of x's type");
+    return type_code(bias.scalar_type(), "bias must be float32 or of x's type");
+}
+
+// x (..., inputs) and weight (outputs, inputs) of one type.
+int32_t layer_code(const at::Tensor& x, const at::Tensor& weight) {
+    check(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
+          "x must have shape (..., inputs) and weight (outputs, inputs)");
+    check(weight.size(0) > 0 && weight.size(1) > 0, "inputs and outputs must be positive");
+    check(x.scalar_type() == weight.scalar_type(), "x and weight must have one type");
+    return type_code(x.scalar_type(), "x must be float32, bfloat16 or float16");
+}
+
+PyObject* linear(Arguments& a) {
+    const Engine e = a.engine();
+    at::Tensor x_in = a.tensor(e, "x"), weight_in = a.tensor(e, "weight"), bias = a.optional(e, "bias");
+    const int32_t activation = int32_t(a.integer());
+    at::Tensor residual = a.optional(e, "residual");
+    const bool keep = a.integer() != 0;
+    const int32_t kind = layer_code(x_in, weight_in);
+    at::DimVector sizes(x_in.sizes());
+    sizes.back() = weight_in.size(0);
+    const int32_t bias_kind = bias_code(bias, x_in, sizes.back());
+    check(!residual.defined() || (residual.sizes() == at::IntArrayRef(sizes) && residual.scalar_type() == x_in.scalar_type()),
+          "residual must have the result's shape and x's type");
+    const at::Tensor y = made(sizes, x_in, x_in.scalar_type());
+    at::Tensor z;
+    if (keep) z = made(sizes, x_in, x_in.scalar_type());
+    const Rows x(std::move(x_in)), weight(std::move(weight_in));
+    int64_t residual_stride = 0;
+    if (residual.defined()) {
+        const Rows r(std::move(residual));
+        residual = r.t, residual_stride = r.stride;
+    }
+    size_t bytes = 0;
+    check(entries.linear_workspace(kind, pointer(x.t), x.stride, x.rows, x.columns, weight.rows, pointer(weight.t), weight.stride,
+                                   &bytes) == CPDE_OK,
+          "invalid points, inputs or outputs");
+    const at::Tensor workspace = made({int64_t(bytes)}, x.t, at::kByte);
+    e.done(entries.linear(e.handle, kind, pointer(x.t), x.stride, x.rows, x.columns, weight.rows, pointer(weight.t), weight.stride,
+                          bias_kind, pointer(bias), activation, pointer(residual), residual_stride, y.mutable_data_ptr(),
+                          keep ? z.mutable_data_ptr() : nullptr, workspace.mutable_data_ptr(), bytes, e.stream()));
+    return Py_BuildValue("NN", THPVariable_Wrap(y), wrapped(z));
+}
+
+PyObject* linear_gradient(Arguments& a) {
+    const Engine e = a.engine();
+    at::Tensor grad_in = a.tensor(e, "grad"), x_in = a.tensor(e, "x"), weight_in = a.tensor(e, "weight"),
+               bias = a.optional(e, "bias");
+    const int32_t activation = int32_t(a.integer());
+    at::Tensor z = a.optional(e, "z");
+    const bool want_x = a.integer() != 0, want_weight = a.integer() != 0;
+    const int32_t kind = layer_code(x_in, weight_in);
+    at::DimVector sizes(x_in.sizes());
+    sizes.back() = weight_in.size(0);
+    int32_t bias_kind = bias_code(bias, x_in, sizes.back());
+    check(grad_in.sizes() == at::IntArrayRef(sizes) && grad_in.scalar_type() == x_in.scalar_type(),
+          "grad must have the result's shape and x's type");
+    check(activation == 1 || z.defined(), "z is needed: call linear with keep=True");
+    check(!z.defined() || (z.sizes() == at::IntArrayRef(sizes) && z.scalar_type() == x_in.scalar_type()),
+          "z must have the result's shape and x's type");
+    const at::ScalarType weight_type = a.type(weight_in.scalar_type()), bias_type = weight_type == at::kFloat || !bias.defined()
+                                                                                       ? at::kFloat : bias.scalar_type();
+    const char* message = "dtype must be float32 or x's type";
+    check(weight_type == at::kFloat || weight_type == x_in.scalar_type(), message);
+    const int32_t weight_kind = type_code(weight_type, message);
+    bias_kind = type_code(bias_type, message);
+    at::Tensor dx, dweight, dbias;
+    if (want_x) dx = made(x_in.sizes(), x_in, x_in.scalar_type());
+    if (want_weight) dweight = made(weight_in.sizes(), x_in, weight_type);
+    if (bias.defined()) dbias = made(bias.sizes(), x_in, bias_type);
+    const Rows grad(std::move(grad_in)), x(std::move(x_in)), weight(std::move(weight_in));
+    int64_t z_stride = 0;
+    if (z.defined()) {
+        const Rows r(std::move(z));
+        z = r.t, z_stride = r.stride;
+    }
+    size_t bytes = 0;
+    check(entries.linear_gradient_workspace(kind, pointer(grad.t), grad.stride, activation, pointer(x.t), x.stride, x.rows,
+                                            x.columns, weight.rows, pointer(weight.t), weight.stride,
+                                            want_x + 2 * want_weight + 4 * bias.defined(), &bytes) == CPDE_OK,
+          "invalid points, inputs or outputs");
+    const at::Tensor workspace = made({int64_t(bytes)}, x.t, at::kByte);
+    e.done(entries.linear_gradient(e.handle, kind, pointer(grad.t), grad.stride, pointer(z), z_stride, activation, pointer(x.t),
+                                   x.stride, x.rows, x.columns, weight.rows, pointer(weight.t), weight.stride,
+                                   const_cast<void*>(pointer(dx)), weight_kind, const_cast<void*>(pointer(dweight)), bias_kind,
+                                   const_cast<void*>(pointer(dbias)), workspace.mutable_data_ptr(), bytes, e.stream()));
+    return Py_BuildValue("NNN", wrapped(dx), wrapped(dweight), wrapped(dbias));
+}
+
+// Steps, coefficients and eps of the Newton-Schulz iteration.
+struct Steps {
+    int32_t count;
+    std::vector<double> coefficients;
+    double eps;
+    explicit Steps(Arguments& a) {
+        count = int32_t(a.integer());
+        PyObject* items = a.take();
+        check(PyTuple_Check(items), "coefficients must be triples");
+        for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(items); ++i) {
+            coefficients.push_back(PyFloat_AsDouble(PyTuple_GET_ITEM(items, i)));
+            if (PyErr_Occurred()) throw Raised();
+        }
+        eps = a.number();
+    }
+    int32_t triples() const { return int32_t(coefficients.size() / 3); }
+};
+
+PyObject* orthogonalize(Arguments& a) {
+    const Engine e = a.engine();
+    at::Tensor x = a.tensor(e, "x");
+    const Steps steps(a);
+    check(x.dim() == 2 || x.dim() == 3, "x must have shape (rows, columns) or (matrices, rows, columns)");
+    const int32_t kind = type_code(x.scalar_type(), "x must be float32, bfloat16 or float16");
+    const int64_t matrices = x.dim() == 3 ? x.size(0) : 1, rows = x.size(-2), columns = x.size(-1);
+    const at::Tensor out = made(x.sizes(), x, x.scalar_type());
+    size_t bytes = 0;
+    check(entries.orthogonalize_workspace(kind, matrices, rows, columns, &bytes) == CPDE_OK, "invalid matrices, rows or columns");
+    const at::Tensor workspace = made({int64_t(bytes)}, x, at::kByte);
+    x = x.contiguous();
+    e.done(entries.orthogonalize(e.handle, kind, pointer(x), matrices, rows, columns, steps.count, steps.coefficients.data(),
+                                 steps.triples(), steps.eps, out.mutable_data_ptr(), workspace.mutable_data_ptr(), bytes,
+                                 e.stream()));
+    return THPVariable_Wrap(out);
+}
+
+PyObject* muon(Arguments& a) {
+    const Engine e = a.engine();
+    at::Tensor weight = a.tensor(e, "weight"), grad = a.tensor(e, "grad"), momentum = a.tensor(e, "momentum");
+    const double rate = a.number(), beta = a.number();
+    const int32_t nesterov = int32_t(a.integer());
+    const double decay = a.number(), scale = a.number();
+    const Steps steps(a);
+    const bool inplace = a.integer() != 0;
+    check(weight.dim() == 2, "weight must have shape (rows, columns)");
+    check(grad.sizes() == weight.sizes() && momentum.sizes() == weight.sizes(), "grad and momentum must have weight's shape");
+    const int32_t kind = type_code(weight.scalar_type(), "weight must be float32, bfloat16 or float16");
+    check(grad.scalar_type() == weight.scalar_type(), "grad must have weight's type");
+    const char* message = "momentum must be float32 or of weight's type";
+    check(momentum.scalar_type() == at::kFloat || momentum.scalar_type() == weight.scalar_type(), message);
+    const int32_t momentum_kind = type_code(momentum.scalar_type(), message);
+    check(!inplace || (weight.is_contiguous() && momentum.is_contiguous()), "weight and momentum must be contiguous to be updated in place");
+    size_t bytes = 0;
+    check(entries.muon_workspace(kind, weight.size(0), weight.size(1), &bytes) == CPDE_OK, "invalid rows or columns");
+    const at::Tensor workspace = made({int64_t(bytes)}, weight, at::kByte);
+    weight = weight.contiguous(), grad = grad.contiguous(), momentum = momentum.contiguous();
+    const at::Tensor new_weight = inplace ? weight : made(weight.sizes(), weight, weight.scalar_type());
+    const at::Tensor new_momentum = inplace ? momentum : made(weight.sizes(), weight, momentum.scalar_type());
+    e.done(entries.muon(e.handle, kind, pointer(weight), pointer(grad), momentum_kind, pointer(momentum), weight.size(0),
+                        weight.size(1), rate, beta, nesterov, decay, scale, steps.count, steps.coefficients.data(),
+                        steps.triples(), steps.eps, new_weight.mutable_data_ptr(), new_momentum.mutable_data_ptr(),
+                        workspace.mutable_data_ptr(), bytes, e.stream()));
+    if (inplace)  // a graph that saved the old values must find that they are gone
+        for (const at::Tensor* t : {&new_weight, &new_momentum})
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return Py_BuildValue("NN", THPVariable_Wrap(new_weight), THPVariable_Wrap(new_momentum));
 }
 
 // bind(EngineError, {name: address}).
@@ -320,6 +492,15 @@ PyObject* bind(Arguments& a) {
     e.group_norm_workspace = reinterpret_cast<decltype(e.group_norm_workspace)>(address("cpde_group_norm_workspace"));
     e.group_norm = reinterpret_cast<decltype(e.group_norm)>(address("cpde_group_norm"));
     e.group_norm_gradient = reinterpret_cast<decltype(e.group_norm_gradient)>(address("cpde_group_norm_gradient"));
+    e.linear_workspace = reinterpret_cast<decltype(e.linear_workspace)>(address("cpde_linear_workspace"));
+    e.linear = reinterpret_cast<decltype(e.linear)>(address("cpde_linear"));
+    e.linear_gradient_workspace =
+        reinterpret_cast<decltype(e.linear_gradient_workspace)>(address("cpde_linear_gradient_workspace"));
+    e.linear_gradient = reinterpret_cast<decltype(e.linear_gradient)>(address("cpde_linear_gradient"));
+    e.orthogonalize_workspace = reinterpret_cast<decltype(e.orthogonalize_workspace)>(address("cpde_orthogonalize_workspace"));
+    e.orthogonalize = reinterpret_cast<decltype(e.orthogonalize)>(address("cpde_orthogonalize"));
+    e.muon_workspace = reinterpret_cast<decltype(e.muon_workspace)>(address("cpde_muon_workspace"));
+    e.muon = reinterpret_cast<decltype(e.muon)>(address("cpde_muon"));
     entries = e;
     Py_XDECREF(engine_error);
     Py_INCREF(error);
@@ -347,6 +528,8 @@ PyMethodDef method(const char* name) {
 PyMethodDef methods[] = {method<bind>("bind"), method<embedding>("embedding"),
                          method<embedding_gradient>("embedding_gradient"), method<dropout>("dropout"),
                          method<group_norm>("group_norm"), method<group_norm_gradient>("group_norm_gradient"),
+                         method<linear>("linear"), method<linear_gradient>("linear_gradient"),
+                         method<orthogonalize>("orthogonalize"), method<muon>("muon"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,147 @@
+// Launches of kernels_gemm.cuh: tensor maps, tiles and splits.
+#pragma once
+#include <algorithm>
+#include <atomic>
+
+#include "common.hpp"
+#include "expression.hpp"
+#include "kernels_gemm.cuh"
+
+namespace cpde::ops {
+
+constexpr int GEMM_SMS = 148;
+
+// A launch that may begin before the one ahead in the stream has ended: every kernel
+// behind it says after_previous_launch() before it touches memory. CLUSTER CTAs each.
+template <class... P, class... A>
+void launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, int cluster, cudaStream_t stream,
+                  A&&... arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    CPDE_CUDA(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
+}
+
+// A 16-bit operand: `planes` arrays (parts, batches) of rows of `pitch` elements.
+struct Operand {
+    const void* base;
+    int64_t pitch, rows, columns, planes, plane;  // `plane` elements from one array to the next
+    int each;                                     // arrays a batch
+};
+
+// Boxes of 64 columns and `box` rows; what lies outside the array is read as zeros.
+inline CUtensorMap operand_map(const Operand& o, int box, bool bf16) {
+    CUtensorMap map;
+    // The stride of a single row or array is never used, but has to be a valid one.
+    const int64_t pitch = o.rows > 1 ? o.pitch : (o.columns + 7) / 8 * 8, plane = o.planes > 1 ? o.plane : 8;
+    cuuint64_t dims[3] = {cuuint64_t(o.columns), cuuint64_t(o.rows), cuuint64_t(o.planes)};
+    cuuint64_t strides[2] = {cuuint64_t(pitch) * 2, cuuint64_t(plane) * 2};
+    cuuint32_t boxes[3] = {GEMM_SLAB, cuuint32_t(box), 1};
+    cuuint32_t element_strides[3] = {1, 1, 1};
+    driver_check(driver_api().encode_tiled(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                           const_cast<void*>(o.base), dims, strides, boxes, element_strides,
+                                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                 "cuTensorMapEncodeTiled");
+    return map;
+}
+
+// Which tile a product takes, and into how many parts its contraction is split.
+struct GemmPlan {
+    int ctas, bn, splits, split_slabs;
+};
+
+// Tiles that products of P parts have (GemmTile).
+struct GemmChoice {
+    int ctas, bn;
+};
+template <int P> constexpr GemmChoice GEMM_CHOICES[3] = {{2, 128}, {1, 64}, {0, 0}};
+template <> constexpr GemmChoice GEMM_CHOICES<1>[3] = {{2, 256}, {2, 128}, {1, 64}};
+
+inline int64_t lower_tiles(int64_t tiles_m, int64_t tiles_n, int64_t ratio) {
+    int64_t sum = 0;
+    for (int64_t m = 0; m < tiles_m; ++m) sum += std::min(tiles_n, ratio * (m + 1));
+    return sum;
+}
+
+// The choice of the shortest estimate: waves of tiles, a slab at the rate of the MMAs or
+// of what L2 brings (64 bytes a clock an SM), some clocks around each tile, and what
+// splitting costs (its partial sums' way through memory and a launch).
+template <int P>
+GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, int64_t batches, bool lower, bool may_split) {
+    const int64_t slabs = (k + GEMM_SLAB - 1) / GEMM_SLAB;
+    GemmPlan best = {};
+    double least = 1e300;
+    for (const GemmChoice& c : GEMM_CHOICES<P>) {
+        if (!c.ctas) continue;
+        const int64_t bm = 128 * c.ctas, tm = (m + bm - 1) / bm, tn = (n + c.bn - 1) / c.bn;
+        const int64_t tiles = (lower ? lower_tiles(tm, tn, bm / c.bn) : tm * tn) * batches, slots = GEMM_SMS / c.ctas;
+        const double bytes = P * (128 + c.bn / c.ctas) * 128.0, clocks = Products<P>::COUNT * 4 * (c.bn / 2);
+        const double slab = std::max(clocks, bytes / 64);
+        const int64_t fill = std::max<int64_t>(1, slots / std::max<int64_t>(tiles, 1));
+        const int64_t most = may_split ? std::min(slabs / 2, 4 * fill) : 1;
+        for (int64_t want : {int64_t(1), int64_t(2), int64_t(3), int64_t(4), int64_t(6), int64_t(8), fill, 2 * fill}) {
+            if (want > 1 && want > most) continue;
+            const int64_t each = (slabs + want - 1) / want, splits = (slabs + each - 1) / each;
+            double time = double((tiles * splits + slots - 1) / slots) * (each * slab + 1500);
+            if (splits > 1) time += 5000 + double(splits) * m * n * 8 / 4000;
+            if (time < least) least = time, best = {c.ctas, c.bn, int(splits), int(each)};
+        }
+    }
+    return best;
+}
+
+template <class C, class E>
+void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k, int64_t batches, bool bf16, bool lower,
+                 const GemmPlan& plan, const E& epilogue, int* error, cudaStream_t stream) {
+    GemmShape s = {};
+    s.m = int(m), s.n = int(n);
+    s.slabs = int((k + GEMM_SLAB - 1) / GEMM_SLAB);
+    s.splits = plan.splits, s.split_slabs = plan.split_slabs;
+    s.tiles_m = int((m + C::BM - 1) / C::BM), s.tiles_n = int((n + C::BN - 1) / C::BN);
+    s.tiles = int(lower ? lower_tiles(s.tiles_m, s.tiles_n, C::BM / C::BN) : int64_t(s.tiles_m) * s.tiles_n);
+    s.batches = int(batches);
+    s.a_planes = a.each, s.b_planes = b.each;
+    s.lower = lower;
+    // A single tile of few rows loads no more of them than there are; what the other
+    // lanes compute from old bytes is never read.
+    const bool few = !C::A_ROWS && C::CTAS == 1 && m < GEMM_ROWS;
+    const int a_box = C::A_ROWS ? 64 : few ? int((m + 7) / 8 * 8) : GEMM_ROWS;
+    const int b_box = C::B_ROWS ? 64 : C::B_PART;
+    s.stage_bytes = uint32_t(C::CTAS * C::P * ((few ? a_box * 128 : C::A_BYTES) + C::B_BYTES));
+    const uint32_t kind = bf16 ? 1 : 0;
+    s.instruction = 1u << 4 | kind << 7 | kind << 10 | uint32_t(C::A_ROWS) << 15 | uint32_t(C::B_ROWS) << 16 |
+                    uint32_t(C::BN >> 3) << 17 | uint32_t(C::BM >> 4) << 24;
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limit is raised
+    int device = 0;
+    CPDE_CUDA(cudaGetDevice(&device));
+    if (!(ready.load() >> (device & 63) & 1)) {
+        CPDE_CUDA(cudaFuncSetAttribute(k_gemm<C, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHARED));
+        ready.fetch_or(uint64_t(1) << (device & 63));
+    }
+    const int64_t items = int64_t(s.tiles) * s.splits * s.batches;
+    const int clusters = int(std::min<int64_t>(items, GEMM_SMS / C::CTAS));
+    launch_early(k_gemm<C, E>, dim3(clusters * C::CTAS), C::THREADS, C::SHARED, C::CTAS, stream, operand_map(a, a_box, bf16),
+                 operand_map(b, b_box, bf16), s, epilogue, error);
+}
+
+// The tile of the plan as a type.
+template <int P, bool A_ROWS, bool B_ROWS, class F>
+void with_tile(const GemmPlan& plan, F&& f) {
+    if constexpr (P == 1)
+        if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS>{});
+    if (plan.bn == 128) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS>{});
+    f(GemmTile<1, 64, P, A_ROWS, B_ROWS>{});
+}
+
+}  // namespace cpde::ops

@@ -1,0 +1,427 @@
+// Matrix products of 16-bit operands on the tensor cores, D = A B' with FP32
+// accumulators in tensor memory; what becomes of D is an epilogue's.
+//
+// An operand is an array of rows of 64-element slabs that TMA brings into shared
+// memory in the 128-byte swizzle. The contraction runs along a row (K-major) or
+// over the rows (MN-major): the bytes in shared memory are the same, only the
+// descriptors differ, so that no operand is ever transposed.
+//
+// An operand of P > 1 parts is the sum of P arrays of 16-bit numbers, each part
+// the rest that the parts before leave: two FP16 parts hold 22 bits, three BF16
+// parts the 24 of FP32 with its exponents. Of the products of parts those are
+// taken that are not below the last part's own rounding: 3 for two parts, 6 for
+// three, the small ones first. The tensor core rounds its sums toward zero, which
+// adds up over a long contraction (a sum of K terms of one sign falls short by up
+// to K/16 2^-24): with P > 1 the accumulator is therefore taken out after each
+// slab and the slabs are added in registers, rounded to nearest. Over 65,536
+// terms that leaves the error of an FP32 sum.
+//
+// A tile of 128 x BN of one CTA, or 256 x BN of a cluster of two whose CTAs hold
+// half of each operand (cta_group::2), by three roles that are two accumulators
+// ahead of each other: a thread that issues the loads, one that issues the MMAs,
+// and warps that take the accumulators out. CTAs go through the tiles in strides.
+// Every wait is bounded: a role that gives up raises the CTA's abort flag, the
+// loads in flight are waited for, tensor memory is released and `error` is set.
+#pragma once
+#include "device_vector.cuh"
+#include "tc.cuh"
+
+namespace cpde::ops {
+
+constexpr int GEMM_ROWS = 128;   // rows of a CTA's tile: the lanes of tensor memory
+constexpr int GEMM_SLAB = 64;    // elements of a slab: 128 bytes, one swizzled row
+constexpr int GEMM_PIECE = 32;   // columns that an epilogue warp handles at a time
+constexpr int GEMM_STRIDE = GEMM_PIECE + 4;  // floats between its rows in shared memory: no bank conflicts
+constexpr long long GEMM_WAIT = 2000000000LL;  // clocks, about a second
+
+struct GemmShape {
+    int m, n;                        // rows and columns of the result
+    int slabs, splits, split_slabs;  // slabs of the contraction, and how they are split
+    int tiles_m, tiles_n, tiles, batches;
+    int a_planes, b_planes;          // arrays of an operand a batch (of which P are read)
+    uint32_t stage_bytes;            // what a slab's loads bring, of all CTAs of the cluster
+    uint32_t instruction;            // the MMA's descriptor
+    bool lower;                      // only tiles that reach the diagonal or below
+};
+
+// What a CTA holds. A_ROWS and B_ROWS: the contraction runs over the rows of the operand's array.
+template <int CTAS_, int BN_, int P_, bool A_ROWS_, bool B_ROWS_>
+struct GemmTile {
+    static constexpr int CTAS = CTAS_, BN = BN_, P = P_;
+    static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_;
+    static constexpr int BM = GEMM_ROWS * CTAS;
+    static constexpr int B_PART = BN / CTAS;  // columns of the tile whose operand this CTA loads
+    static constexpr int A_BYTES = GEMM_ROWS * 128, B_BYTES = B_PART * 128;
+    static constexpr int STAGE = P * (A_BYTES + B_BYTES);
+    static constexpr int WARPS = BN > 128 || P == 1 ? 4 : 8;  // of the epilogue
+    static constexpr int COLUMNS = BN / (WARPS / 4);  // of an epilogue warp
+    static constexpr int THREADS = 64 + 32 * WARPS;
+    static constexpr int PIECES = WARPS * 32 * GEMM_STRIDE * 4;
+    static constexpr int ROOM = (227 * 1024 - 1024 - 256 - PIECES) / STAGE;
+    static constexpr int STAGES = ROOM > 8 ? 8 : ROOM;
+    static constexpr int SHARED = 1024 + STAGES * STAGE + PIECES + 256;
+    static constexpr uint32_t TMEM = BN * 2 <= 32 ? 32 : BN * 2 <= 64 ? 64 : BN * 2 <= 128 ? 128 : BN * 2 <= 256 ? 256 : 512;
+    static_assert(STAGES >= 2 && BN * 2 <= 512 && BN % 32 == 0 && COLUMNS % GEMM_PIECE == 0);
+    static_assert(!B_ROWS || B_PART % 64 == 0, "boxes of rows are 64 columns wide");
+};
+
+namespace gemm {
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc::smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// A box into this CTA's memory; its bytes count at `bar`, for two CTAs that of the first.
+template <int CTAS>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    if constexpr (CTAS == 2)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                     "[%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y),
+                     "r"(z)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                     "[%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y),
+                     "r"(z)
+                     : "memory");
+}
+
+template <int CTAS>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    if constexpr (CTAS == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                     "r"(instruction), "r"(uint32_t(accumulate))
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                     "r"(instruction), "r"(uint32_t(accumulate))
+                     : "memory");
+}
+// Arrives at `bar`, in every CTA of the cluster, when this thread's MMAs have ended.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         tc::smem_u32(bar)),
+                     "h"(uint16_t(3))
+                     : "memory");
+    else
+        tc::mma_commit(bar);
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_take(uint32_t* slot, uint32_t columns) {
+    if constexpr (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tc::tmem_alloc(slot, columns);
+        tc::tmem_relinquish();
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_release(uint32_t base, uint32_t columns) {
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
+    else
+        tc::tmem_dealloc(base, columns);
+}
+
+// 32 columns of a warp's lanes: thread i gets lane i's.
+__device__ __forceinline__ void tmem_piece(uint32_t at, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    tc::tmem_landed(v);
+}
+
+// Descriptors of a tile in shared memory, 128-byte swizzle, 8-row groups 1024 bytes
+// apart. K-major: the groups follow each other along M or N. MN-major: they follow
+// each other along K, and blocks of 64 along M or N are 64 rows apart.
+template <bool ROWS>
+__device__ __forceinline__ uint64_t descriptor(uint32_t at) {
+    return uint64_t((at >> 4) & 0x3FFFu) | uint64_t(ROWS ? 8192u >> 4 : 1u) << 16 | uint64_t(1024u >> 4) << 32 |
+           uint64_t(1u) << 46 | uint64_t(2u) << 61;
+}
+// Bytes from one MMA's 16 elements of the contraction to the next one's.
+template <bool ROWS> constexpr uint32_t STEP = ROWS ? 16 * 128 : 32;
+
+struct Work {
+    int tile_m, tile_n, split, batch, from, to;  // and its slabs
+};
+// Work items in an order that keeps the operands of neighbours in L2: bands of 8
+// tiles high, batch after batch and split after split.
+template <class C>
+__device__ __forceinline__ Work work_at(const GemmShape& s, int64_t at) {
+    Work w;
+    const int each = s.tiles * s.splits;
+    w.batch = int(at / each);
+    const int rest = int(at % each), tile = rest % s.tiles;
+    w.split = rest / s.tiles;
+    if (s.lower) {
+        constexpr int RATIO = C::BM / C::BN;  // tiles of a band up to the diagonal, a band
+        int left = tile, m = 0, wide;
+        while (left >= (wide = min(s.tiles_n, RATIO * (m + 1)))) left -= wide, ++m;
+        w.tile_m = m, w.tile_n = left;
+    } else {
+        const int band = tile / (8 * s.tiles_n), high = min(8, s.tiles_m - 8 * band), in = tile - band * 8 * s.tiles_n;
+        w.tile_m = 8 * band + in % high, w.tile_n = in / high;
+    }
+    w.from = w.split * s.split_slabs;
+    w.to = min(s.slabs, w.from + s.split_slabs);
+    return w;
+}
+
+template <class C>
+struct Shared {
+    uint8_t* stages;
+    float* pieces;
+    uint64_t *full, *empty, *ready, *taken;  // of the stages; of the two accumulators
+    volatile int* abort;
+    uint32_t* slot;
+    __device__ explicit Shared(uint8_t* raw) {
+        stages = raw + (1024 - (tc::smem_u32(raw) & 1023)) % 1024;
+        pieces = reinterpret_cast<float*>(stages + C::STAGES * C::STAGE);
+        full = reinterpret_cast<uint64_t*>(stages + C::STAGES * C::STAGE + C::PIECES);
+        empty = full + 8, ready = empty + 8, taken = ready + 2;
+        slot = reinterpret_cast<uint32_t*>(taken + 2);
+        abort = reinterpret_cast<volatile int*>(slot + 1);
+    }
+};
+
+}  // namespace gemm
+
+// The products of parts (A's, B's), the small ones first.
+template <int P> struct Products;
+template <> struct Products<1> {
+    static constexpr int COUNT = 1;
+    __device__ static constexpr int a(int) { return 0; }
+    __device__ static constexpr int b(int) { return 0; }
+};
+template <> struct Products<2> {
+    static constexpr int COUNT = 3;
+    __device__ static constexpr int a(int i) { return i == 0; }
+    __device__ static constexpr int b(int i) { return i == 1; }
+};
+template <> struct Products<3> {
+    static constexpr int COUNT = 6;
+    __device__ static constexpr int a(int i) { return i == 0 ? 2 : i == 2 || i == 3; }
+    __device__ static constexpr int b(int i) { return i == 1 ? 2 : i == 2 || i == 4; }
+};
+
+// The epilogue E gets every element of a tile once, as float4 of neighbouring
+// columns (put), after what it reads for them has been fetched (fetch); `direct` sees
+// them before that by lanes, a row a thread. Columns behind n are the epilogue's to skip.
+template <class C, class E>
+__global__ void __launch_bounds__(C::THREADS, 1)
+    k_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const GemmShape s, const E epilogue,
+           int* error) {
+    using namespace gemm;
+    extern __shared__ uint8_t raw_shared[];
+    const Shared<C> sh(raw_shared);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = C::CTAS == 2 ? cluster_rank() : 0;
+    const int first = blockIdx.x / C::CTAS, stride = gridDim.x / C::CTAS;
+    const int64_t items = int64_t(s.tiles) * s.splits * s.batches;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; ++i) tc::mbar_init(sh.full + i, 1), tc::mbar_init(sh.empty + i, 1);
+        for (int i = 0; i < 2; ++i) tc::mbar_init(sh.ready + i, 1), tc::mbar_init(sh.taken + i, C::CTAS * C::WARPS);
+        *sh.abort = 0;
+        tc::fence_barrier_init();
+    }
+    if (warp == 1) tmem_take<C::CTAS>(sh.slot, C::TMEM);
+    tc::tc_fence_before();
+    if constexpr (C::CTAS == 2) cluster_sync();
+    else __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *sh.slot;
+    next_launch_may_begin();
+    after_previous_launch();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int64_t at = first; at < items && !*sh.abort; at += stride) {
+                const Work w = work_at<C>(s, at);
+                const int m0 = w.tile_m * C::BM + rank * GEMM_ROWS, n0 = w.tile_n * C::BN + rank * C::B_PART;
+                for (int slab = w.from; slab < w.to; ++slab, ++it) {
+                    const int st = it % C::STAGES;
+                    if (!tc::mbar_wait_or_abort(sh.empty + st, ((it / C::STAGES) & 1) ^ 1, GEMM_WAIT, sh.abort)) break;
+                    if (rank == 0) tc::mbar_expect_tx(sh.full + st, s.stage_bytes);
+                    const uint32_t bar = C::CTAS == 2 ? at_rank(sh.full + st, 0) : tc::smem_u32(sh.full + st);
+                    uint32_t to = tc::smem_u32(sh.stages + st * C::STAGE);
+#pragma unroll
+                    for (int p = 0; p < C::P; ++p, to += C::A_BYTES) {
+                        const int z = w.batch * s.a_planes + p;
+                        if constexpr (C::A_ROWS) {
+                            load_box<C::CTAS>(to, &a_map, bar, m0, slab * GEMM_SLAB, z);
+                            load_box<C::CTAS>(to + 8192, &a_map, bar, m0 + 64, slab * GEMM_SLAB, z);
+                        } else {
+                            load_box<C::CTAS>(to, &a_map, bar, slab * GEMM_SLAB, m0, z);
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < C::P; ++p, to += C::B_BYTES) {
+                        const int z = w.batch * s.b_planes + p;
+                        if constexpr (C::B_ROWS) {
+#pragma unroll
+                            for (int j = 0; j < C::B_PART; j += 64)
+                                load_box<C::CTAS>(to + j * 128, &b_map, bar, n0 + j, slab * GEMM_SLAB, z);
+                        } else {
+                            load_box<C::CTAS>(to, &b_map, bar, slab * GEMM_SLAB, n0, z);
+                        }
+                    }
+                }
+            }
+            // No load may be in flight when the CTA ends, also where a role gave up, nor a
+            // commit under way to the other CTA's barriers.
+            for (uint32_t k = it - min(it, uint32_t(C::STAGES)); k < it; ++k) {
+                const uint32_t parity = (k / C::STAGES) & 1;
+                if (rank == 0 && !tc::mbar_wait(sh.full + k % C::STAGES, parity, GEMM_WAIT)) *sh.abort = 1;
+                if (!*sh.abort) tc::mbar_wait_or_abort(sh.empty + k % C::STAGES, parity, GEMM_WAIT, sh.abort);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, unit = 0;
+            bool ok = true;
+            for (int64_t at = first; ok && at < items; at += stride) {
+                const Work w = work_at<C>(s, at);
+                for (int slab = w.from; ok && slab < w.to; ++slab, ++it) {
+                    const bool begins = C::P > 1 || slab == w.from, ends = C::P > 1 || slab + 1 == w.to;
+                    const uint32_t d = tmem + (unit & 1) * C::BN;
+                    if (begins) ok = tc::mbar_wait_or_abort(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, GEMM_WAIT, sh.abort);
+                    const int st = it % C::STAGES;
+                    ok = ok && tc::mbar_wait_or_abort(sh.full + st, (it / C::STAGES) & 1, GEMM_WAIT, sh.abort);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t a0 = tc::smem_u32(sh.stages + st * C::STAGE), b0 = a0 + C::P * C::A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < Products<C::P>::COUNT; ++i) {
+                        const uint64_t a = descriptor<C::A_ROWS>(a0 + Products<C::P>::a(i) * C::A_BYTES);
+                        const uint64_t b = descriptor<C::B_ROWS>(b0 + Products<C::P>::b(i) * C::B_BYTES);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma<C::CTAS>(d, a + k * (STEP<C::A_ROWS> >> 4), b + k * (STEP<C::B_ROWS> >> 4), s.instruction,
+                                         !(begins && i == 0 && k == 0));
+                    }
+                    commit<C::CTAS>(sh.empty + st);
+                    if (ends) commit<C::CTAS>(sh.ready + (unit & 1)), ++unit;
+                }
+            }
+        }
+    } else {
+        const int e = warp - 2, quarter = warp % 4;  // the lanes that a warp may read
+        const int c0 = e / 4 * C::COLUMNS;
+        float* piece = sh.pieces + e * 32 * GEMM_STRIDE;
+        uint32_t unit = 0;
+        // Waits for an accumulator; false where a role gave up.
+        auto wait = [&] {
+            const bool ok = tc::mbar_wait_or_abort(sh.ready + (unit & 1), (unit >> 1) & 1, GEMM_WAIT, sh.abort);
+            tc::tc_fence_after();
+            return __all_sync(~0u, ok);
+        };
+        auto taken = [&] {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (C::CTAS == 2) arrive_at(at_rank(sh.taken + (unit & 1), 0));
+                else tc::mbar_arrive(sh.taken + (unit & 1));
+            }
+            ++unit;
+        };
+        auto put = [&](const float (&v)[32], int row, int column, const Work& w) {
+            if (row >= s.m || column >= s.n) return;
+            epilogue.direct(v, row + lane, column, w.batch, C::BM, C::BN, s);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(piece + lane * GEMM_STRIDE + 4 * i) =
+                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            __syncwarp();
+            const int c = lane % 8 * 4;
+            typename E::Fetched got[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 8;
+                if (row + r < s.m && column + c < s.n) epilogue.fetch(got[i], row + r, column + c, w.batch, s);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 8;
+                if (row + r < s.m && column + c < s.n)
+                    epilogue.put(*reinterpret_cast<const float4*>(piece + r * GEMM_STRIDE + c), got[i], row + r, column + c,
+                                 w.batch, w.split, s);
+            }
+        };
+        bool ok = true;
+        for (int64_t at = first; ok && at < items; at += stride) {
+            const Work w = work_at<C>(s, at);
+            const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column = w.tile_n * C::BN + c0;
+            const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + c0;
+            if constexpr (C::P == 1) {
+                if (!(ok = wait())) break;
+                const uint32_t from = lanes + (unit & 1) * C::BN;
+#pragma unroll 1
+                for (int c = 0; c < C::COLUMNS; c += 32) {
+                    float v[32];
+                    tmem_piece(from + c, v);
+                    if (c + 32 == C::COLUMNS) taken();
+                    put(v, row, column + c, w);
+                }
+            } else {
+                float sum[C::COLUMNS / 32][32] = {};
+                for (int slab = w.from; ok && slab < w.to; ++slab) {
+                    if (!(ok = wait())) break;
+#pragma unroll
+                    for (int c = 0; c < C::COLUMNS / 32; ++c) {
+                        float v[32];
+                        tmem_piece(lanes + (unit & 1) * C::BN + 32 * c, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[c][i] += v[i];
+                    }
+                    taken();
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < C::COLUMNS / 32; ++c) put(sum[c], row, column + 32 * c, w);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncwarp();
+    if constexpr (C::CTAS == 2) cluster_sync();
+    else __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tmem_release<C::CTAS>(tmem, C::TMEM);
+    }
+    if (threadIdx.x == 0 && *sh.abort) atomicExch(error, 3);
+}
+
+}  // namespace cpde::ops

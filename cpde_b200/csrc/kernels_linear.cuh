@@ -1,0 +1,236 @@
+// Linear layers: what stands before and behind the matrix products of
+// kernels_gemm.cuh.
+//
+// z = x W' + b, y = r + act(z); from dy: dz = dy act'(z), dx = dz W, dW = dz' x,
+// db = sum of dz over the points.
+#pragma once
+#include "kernels_gemm.cuh"
+
+namespace cpde::ops {
+
+// 1 / (1 + e^-z) from the special function unit's 2^x and 1/x.
+__device__ __forceinline__ float layer_sigmoid(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * z));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
+// The activations by their codes: 0 sigmoid, 1 linear, 2 tanh, 3 SiLU.
+__device__ __forceinline__ float layer_activation(float z, int32_t activation) {
+    if (activation == 1) return z;
+    if (activation == 2) return tanhf(z);
+    const float f = layer_sigmoid(z);
+    return activation == 3 ? z * f : f;
+}
+__device__ __forceinline__ float layer_slope(float z, int32_t activation) {
+    if (activation == 1) return 1.0f;
+    if (activation == 2) {
+        const float t = tanhf(z);
+        return fmaf(-t, t, 1.0f);
+    }
+    const float f = layer_sigmoid(z);
+    return activation == 3 ? fmaf(f, z * (1.0f - f), f) : f * (1.0f - f);
+}
+
+// Up to V elements of a row that has `left` of them from here on.
+template <class T, int V>
+__device__ __forceinline__ void load_some(const T* p, float (&f)[V], int64_t left, bool whole) {
+    if (whole) {
+        unpack<T, V>(load_written<T, V>(p), f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = i < left ? to_float(p[i]) : 0.0f;
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_some(T* p, const float (&f)[V], int64_t left, bool whole) {
+    if (whole) {
+        store<T, V>(p, pack<T, V>(f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = from_float<T>(f[i]);
+    }
+}
+
+// Bias, activation and residual in the product's epilogue, or plain results, or the
+// partial sums of a split contraction.
+template <class T>
+struct LinearEpilogue {
+    const void* bias;       // of FP32 or T, or null
+    const T* residual;      // or null
+    T* z;                   // or null
+    void* y;                // of FP32 or T
+    float* partial;         // where the contraction is split: (split, row, column) sums, pitch n rounded up to 4
+    int64_t residual_stride;
+    int32_t activation;
+    bool bias_wide, y_wide;
+    bool whole;             // four elements at a time are there and aligned in every array
+
+    struct Fetched {
+        float bias[4], residual[4];
+    };
+    __device__ void direct(const float (&)[32], int, int, int, int, int, const GemmShape&) const {}
+    __device__ __forceinline__ void fetch(Fetched& f, int64_t row, int column, int, const GemmShape& s) const {
+        if (partial) return;
+        const int64_t left = s.n - column;
+        if (bias) {
+            if (bias_wide) load_some<float, 4>(static_cast<const float*>(bias) + column, f.bias, left, whole);
+            else load_some<T, 4>(static_cast<const T*>(bias) + column, f.bias, left, whole);
+        }
+        if (residual) load_some<T, 4>(residual + row * residual_stride + column, f.residual, left, whole);
+    }
+    __device__ __forceinline__ void put(const float4& d, const Fetched& f, int64_t row, int column, int, int split,
+                                        const GemmShape& s) const {
+        if (partial) {
+            const int64_t pitch = (s.n + 3) / 4 * 4;
+            *reinterpret_cast<float4*>(partial + (split * int64_t(s.m) + row) * pitch + column) = d;
+            return;
+        }
+        float v[4] = {d.x, d.y, d.z, d.w};
+        const int64_t left = s.n - column, at = row * s.n + column;
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += f.bias[i];
+        }
+        if (z) store_some<T, 4>(z + at, v, left, whole);
+        if (activation != 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = layer_activation(v[i], activation);
+        }
+        if (residual) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += f.residual[i];
+        }
+        if (y_wide) store_some<float, 4>(static_cast<float*>(y) + at, v, left, whole);
+        else store_some<T, 4>(static_cast<T*>(y) + at, v, left, whole);
+    }
+};
+
+// Joins the partial sums of a split contraction, in the order of the splits, and ends them as the epilogue does.
+template <class T>
+__global__ void __launch_bounds__(256) k_join(LinearEpilogue<T> epilogue, GemmShape s) {
+    after_previous_launch();
+    const float* partial = epilogue.partial;
+    epilogue.partial = nullptr;
+    const int64_t fours = (s.n + 3) / 4, all = s.m * fours;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < all; i += gridDim.x * int64_t(256)) {
+        const int64_t row = i / fours;
+        const int column = int(i % fours) * 4;
+        typename LinearEpilogue<T>::Fetched f;
+        epilogue.fetch(f, row, column, 0, s);
+        float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+        for (int split = 0; split < s.splits; ++split) {
+            const float4 v = *reinterpret_cast<const float4*>(partial + (split * all + i) * 4);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        epilogue.put(sum, f, row, column, 0, 0, s);
+    }
+}
+
+// An operand's parts from an array: part after part, rows of `pitch`. With z, the
+// array is multiplied by the activation's slope there. `sums` takes the column sums
+// of each chunk of rows.
+template <class T>
+struct PartsCall {
+    const T* x;
+    const T* z;
+    void* out;         // or null: sums alone
+    float* sums;       // (chunk, column), or null
+    int64_t x_stride, z_stride, rows, chunk;
+    int32_t columns, pitch, activation;
+    int32_t lanes;     // threads of a row, eight columns each: a power of two up to 32
+    bool whole;        // x and z can be read in eights
+};
+
+// T's parts: FP32 as three BF16, what each leaves going to the next (24 bits, all
+// exponents); the 16-bit types as they are.
+template <class T> struct Parts { using type = T; static constexpr int count = 1; };
+template <> struct Parts<float> { using type = __nv_bfloat16; static constexpr int count = 3; };
+
+// The part of v, and in v the rest. A value that rounds to infinity is cut to the
+// largest finite one, and an infinity's rest is nothing.
+__device__ __forceinline__ float next_part(float& v) {
+    float h = __bfloat162float(__float2bfloat16_rn(v));
+    if (!finite(h) && finite(v)) h = copysignf(__uint_as_float(0x7f7f0000u), v);
+    v = finite(h) ? v - h : 0.0f;
+    return h;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
+    using O = typename Parts<T>::type;
+    __shared__ float shared[256 * 8];
+    next_launch_may_begin();
+    after_previous_launch();
+    const int lane = threadIdx.x % c.lanes, high = 256 / c.lanes;
+    const int column = (blockIdx.x * c.lanes + lane) * 8;
+    const int64_t from = blockIdx.y * c.chunk, to = min(c.rows, from + c.chunk);
+    float sum[8] = {};
+    if (column < c.columns) {
+        const int left = c.columns - column;
+        const bool whole = c.whole && left >= 8;
+#pragma unroll 2
+        for (int64_t row = from + threadIdx.x / c.lanes; row < to; row += high) {
+            float v[8];
+            load_some<T, 8>(c.x + row * c.x_stride + column, v, left, whole);
+            if (c.z) {
+                float z[8];
+                load_some<T, 8>(c.z + row * c.z_stride + column, z, left, whole);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < left) v[i] *= layer_slope(z[i], c.activation);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[i];
+            if (c.out) {
+                O* out = static_cast<O*>(c.out) + row * c.pitch + column;
+                if constexpr (Parts<T>::count == 1) {
+                    store<O, 8>(out, pack<O, 8>(v));
+                } else {
+#pragma unroll
+                    for (int p = 0; p < Parts<T>::count; ++p, out += c.rows * c.pitch) {
+                        float h[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) h[i] = next_part(v[i]);
+                        store<O, 8>(out, pack<O, 8>(h));
+                    }
+                }
+            }
+        }
+    }
+    if (!c.sums) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) shared[(threadIdx.x * 8) + i] = sum[i];
+    __syncthreads();
+    // The rows of threads are added in their order.
+    const int wide = c.lanes * 8;
+    for (int i = threadIdx.x; i < wide; i += 256) {
+        float total = 0.0f;
+        for (int r = 0; r < high; ++r) total += shared[r * wide + i];
+        const int at = blockIdx.x * wide + i;
+        if (at < c.columns) c.sums[blockIdx.y * int64_t(c.columns) + at] = total;
+    }
+}
+
+// Column sums over the chunks: 32 columns a block, whose eight warps take every eighth chunk.
+template <class O>
+__global__ void __launch_bounds__(256) k_column_sums(const float* sums, int32_t chunks, int32_t columns, O* out) {
+    __shared__ float shared[8][32];
+    after_previous_launch();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+    if (column < columns) {
+#pragma unroll 8
+        for (int i = warp; i < chunks; i += 8) sum += sums[i * int64_t(columns) + column];
+    }
+    shared[warp][lane] = sum;
+    __syncthreads();
+    if (warp || column >= columns) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += shared[i][lane];
+    out[column] = from_float<O>(sum);
+}
+
+}  // namespace cpde::ops

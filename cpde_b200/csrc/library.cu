@@ -3,3 +3,4 @@
 #include "capi.cu"
 #include "noalloc.cu"
 #include "operators_capi.cu"
+#include "layers_capi.cu"

@@ -1,5 +1,6 @@
 """Operators on CUDA tensors for torch networks beside the engine's, such as one that learns a family of its solutions:
-embedding lookup, dropout and group norm with an activation (channels last), each with its gradient.
+embedding lookup, dropout, group norm with an activation (channels last) and linear layers, each with its gradient;
+orthogonalised matrices and the optimiser step that takes them.
 
 Every function takes the :class:`cpde_b200.native.Engine` of the tensors' device, launches on torch's current stream of
 that device and returns new contiguous tensors; nothing synchronises. Wrong arguments raise ``ValueError`` here or
@@ -30,7 +31,9 @@ _operators.bind(native.EngineError, {
     name: ctypes.cast(getattr(native.load(), name), ctypes.c_void_p).value
     for name in ('cpde_last_error', 'cpde_embedding', 'cpde_embedding_gradient_workspace', 'cpde_embedding_gradient',
                  'cpde_dropout', 'cpde_group_norm_forward_workspace', 'cpde_group_norm_workspace', 'cpde_group_norm',
-                 'cpde_group_norm_gradient')})
+                 'cpde_group_norm_gradient', 'cpde_linear_workspace', 'cpde_linear', 'cpde_linear_gradient_workspace',
+                 'cpde_linear_gradient', 'cpde_orthogonalize_workspace', 'cpde_orthogonalize', 'cpde_muon_workspace',
+                 'cpde_muon')})
 
 
 def _handle(engine, tensor):
@@ -90,6 +93,58 @@ def group_norm_gradient(engine, grad, x, mean, rstd, groups, weight=None, bias=N
                                           _activation(activation), lengths, rate, seed, offset)
 
 
+def linear(engine, x, weight, bias=None, activation='linear', residual=None, keep=False):
+    """``(y, z)`` of ``y = residual + act(x @ weight.T + bias)`` over x of shape (..., inputs) and weight of shape
+    (outputs, inputs). z, the sums before the activation that :func:`linear_gradient` takes, is None unless ``keep``.
+
+    The products of 16-bit types are summed in FP32; those of float32 have the error of FP32 products."""
+    return _operators.linear(_handle(engine, x), engine.device, x, weight, bias, _activation(activation), residual, keep)
+
+
+def linear_gradient(engine, grad, x, weight, bias=None, activation='linear', z=None, need=(True, True), dtype=None):
+    """``(dx, dweight, dbias)`` of :func:`linear` from the gradient of y, its inputs and z (not needed for a linear
+    activation); the residual's gradient is ``grad`` itself. ``need`` says which of dx and dweight are computed, the others
+    are None, and so is dbias without a bias. ``dtype`` of dweight and dbias (default: the parameters') may be float32 for
+    a 16-bit weight."""
+    need_x, need_weight = need
+    return _operators.linear_gradient(_handle(engine, x), engine.device, grad, x, weight, bias, _activation(activation), z,
+                                      need_x, need_weight, dtype)
+
+
+QUINTIC = (3.4445, -4.775, 2.0315)
+
+
+def _coefficients(coefficients):
+    """A triple, or a sequence of triples, as one tuple."""
+    flat = coefficients if isinstance(coefficients[0], (int, float)) else [v for triple in coefficients for v in triple]
+    if len(flat) % 3:
+        raise ValueError('coefficients must be triples')
+    return tuple(flat)
+
+
+def orthogonalize(engine, x, steps=5, coefficients=QUINTIC, eps=1e-7):
+    """Each matrix of x, of shape (rows, columns) or (matrices, rows, columns), with its singular values taken near one:
+    ``X = x / (|x| + eps)`` with the Frobenius norm, then ``steps`` times ``X = a X + b (X X') X + c (X X')^2 X``.
+    ``coefficients`` is a triple (a, b, c), or one for each step (the last counts for the steps behind it).
+
+    Values are held in 22 bits. Products take all of them for float32, whose result is good to about 1e-6 of its norm, and
+    11 for the 16-bit types, which leaves less than their rounding to bfloat16 adds."""
+    return _operators.orthogonalize(_handle(engine, x), engine.device, x, steps, _coefficients(coefficients), eps)
+
+
+def muon(engine, weight, grad, momentum, rate, beta=0.95, nesterov=True, decay=0.0, scale=None, steps=5,
+         coefficients=QUINTIC, eps=1e-7, inplace=False):
+    """``(weight, momentum)`` after an optimiser step of a weight matrix whose update is orthogonalised (Muon):
+    ``m = beta momentum + (1 - beta) grad``, ``u = beta m + (1 - beta) grad`` (m itself without ``nesterov``) and
+    ``(1 - rate decay) weight - rate scale O``, O being u as :func:`orthogonalize` gives it and the scale by default
+    ``max(1, rows / columns) ** 0.5``. momentum is float32 or of the weight's type. With ``inplace`` the given tensors
+    are written and returned."""
+    if scale is None:
+        scale = max(1.0, weight.shape[0] / weight.shape[-1]) ** 0.5
+    return _operators.muon(_handle(engine, weight), engine.device, weight, grad, momentum, rate, beta, nesterov, decay, scale,
+                           steps, _coefficients(coefficients), eps, inplace)
+
+
 # --- autograd --------------------------------------------------------------
 
 class Embedding(torch.autograd.Function):
@@ -145,3 +200,62 @@ class GroupNorm(torch.autograd.Function):
         dx, dweight, dbias = group_norm_gradient(ctx.engine, grad, x, mean, rstd, groups, weight, bias, activation,
                                                  lengths, rate, seed, offset)
         return None, dx, dweight, dbias, *(None,) * 7
+
+
+class Linear(torch.autograd.Function):
+    """``Linear.apply(engine, x, weight, bias, activation, residual)``: :func:`linear`'s y with its gradients."""
+
+    @staticmethod
+    def forward(ctx, engine, x, weight, bias=None, activation='linear', residual=None):
+        keep = activation != 'linear' and any(ctx.needs_input_grad[1:4])
+        y, z = linear(engine, x, weight, bias, activation, residual, keep)
+        ctx.save_for_backward(x, weight, bias, z)
+        ctx.engine, ctx.activation = engine, activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, z = ctx.saved_tensors
+        _, need_x, need_weight, need_bias, _, need_residual = ctx.needs_input_grad
+        dx = dweight = dbias = None
+        if need_x or need_weight or need_bias:
+            dx, dweight, dbias = linear_gradient(ctx.engine, grad, x, weight, bias if need_bias else None, ctx.activation, z,
+                                                 (need_x, need_weight))
+        return None, dx, dweight, dbias, None, grad if need_residual else None
+
+
+# --- optimiser -------------------------------------------------------------
+
+class Muon(torch.optim.Optimizer):
+    """Steps of :func:`muon`, in place, for the weight matrices of hidden layers; other parameters (biases, embeddings,
+    heads) are for another optimiser."""
+
+    def __init__(self, engine, params, lr=0.02, beta=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=QUINTIC,
+                 eps=1e-7):
+        self.engine = engine
+        super().__init__(params, dict(lr=lr, beta=beta, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if any(p.dim() != 2 for p in self.param_groups[-1]['params']):
+            self.param_groups.pop()
+            raise ValueError('Muon takes matrices alone')
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if 'momentum' not in state:
+                    state['momentum'] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                muon(self.engine, p, p.grad, state['momentum'], group['lr'], group['beta'], group['nesterov'],
+                     group['weight_decay'], None, group['steps'], group['coefficients'], group['eps'], inplace=True)
+        return loss

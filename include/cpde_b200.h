@@ -261,6 +261,57 @@ int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad
                              double rate, uint64_t seed, uint64_t offset, void* dx, void* dweight, void* dbias,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* Linear layer over `points` rows: y = residual + act(x weight' + bias), with
+ * `weight` rows of inputs, one an output. `activation` counts as above. x, weight,
+ * residual (or NULL), y and z are of `type`; `bias` (or NULL) is FP32 or of it. z
+ * (or NULL) takes the sums before the activation, for the gradient. Products of
+ * the 16-bit types are exact and summed in FP32; those of FP32 arrays are of
+ * three BF16 parts each (24 bits), so that they have the error of FP32 products; a
+ * row with an infinity gives infinities or NaNs. 16-bit arrays whose address and
+ * stride are whole 16 bytes are read in place; others, and FP32, go through the
+ * workspace, whose query therefore takes the addresses too. */
+int cpde_linear_workspace(int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs,
+                          const void* weight, int64_t weight_stride, size_t* bytes);
+int cpde_linear(cpde_engine* engine, int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs,
+                int64_t outputs, const void* weight, int64_t weight_stride, int32_t bias_type, const void* bias,
+                int32_t activation, const void* residual, int64_t residual_stride, void* y, void* z, void* workspace,
+                size_t workspace_bytes, void* stream);
+/* Its gradient from that of y: dz = grad act'(z), dx = dz weight, dweight = dz' x,
+ * dbias = sum of dz; the residual's gradient is grad. z is the forward's (any
+ * pointer where the activation is linear). Gradients that are NULL are not
+ * computed, and what only they need (x, weight) is not read. dweight is FP32 or of
+ * `type`, and so is dbias. For the 16-bit types dz is rounded to the type where the
+ * activation is not linear. `want` of the query: 1 dx, 2 dweight, 4 dbias, added. */
+int cpde_linear_gradient_workspace(int32_t type, const void* grad, int64_t grad_stride, int32_t activation, const void* x,
+                                   int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs, const void* weight,
+                                   int64_t weight_stride, int32_t want, size_t* bytes);
+int cpde_linear_gradient(cpde_engine* engine, int32_t type, const void* grad, int64_t grad_stride, const void* z,
+                         int64_t z_stride, int32_t activation, const void* x, int64_t x_stride, int64_t points,
+                         int64_t inputs, int64_t outputs, const void* weight, int64_t weight_stride, void* dx,
+                         int32_t weight_type, void* dweight, int32_t bias_type, void* dbias, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Newton-Schulz steps on contiguous matrices: X = x / (|x| + eps) with the
+ * Frobenius norm, then X <- a X + b (X X') X + c (X X')^2 X, `steps` times. Step k
+ * takes the k-th of `triples` (a, b, c) at `coefficients` (host memory), or the
+ * last. Coefficients with which a singular value may pass 1024 are refused. Values
+ * are held in 22 bits; products take all of them for FP32 matrices and 11 bits for
+ * the 16-bit types. Entries of X below 2^-40 of the bound on the singular values
+ * are lost. */
+int cpde_orthogonalize_workspace(int32_t type, int64_t matrices, int64_t rows, int64_t columns, size_t* bytes);
+int cpde_orthogonalize(cpde_engine* engine, int32_t type, const void* x, int64_t matrices, int64_t rows, int64_t columns,
+                       int32_t steps, const double* coefficients, int32_t triples, double eps, void* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+/* Optimiser step of one weight matrix: m' = beta m + (1 - beta) g, u = m', or
+ * beta m' + (1 - beta) g with `nesterov`, O = u orthogonalised as above,
+ * weight' = (1 - rate decay) weight - rate scale O. grad and weight are of `type`,
+ * momentum FP32 or of it. The new arrays may be the old ones. */
+int cpde_muon_workspace(int32_t type, int64_t rows, int64_t columns, size_t* bytes);
+int cpde_muon(cpde_engine* engine, int32_t type, const void* weight, const void* grad, int32_t momentum_type,
+              const void* momentum, int64_t rows, int64_t columns, double rate, double beta, int32_t nesterov,
+              double decay, double scale, int32_t steps, const double* coefficients, int32_t triples, double eps,
+              void* new_weight, void* new_momentum, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Host-only schema compiler (no device needed): Leibniz jet tables for the
  * given rows x variables count matrix, packed as documented in schema.hpp. */
 int cpde_jet_plan(const int32_t* counts, int32_t rows, int32_t variables, int32_t* packed, size_t capacity,
