@@ -31,7 +31,7 @@ namespace cpde::ops {
 constexpr int GEMM_ROWS = 128;   // rows of a CTA's tile: the lanes of tensor memory
 constexpr int GEMM_SLAB = 64;    // elements of a slab: 128 bytes, one swizzled row
 constexpr int GEMM_PIECE = 32;   // columns that an epilogue warp handles at a time
-constexpr int GEMM_STRIDE = GEMM_PIECE + 4;  // floats between its rows in shared memory: no bank conflicts
+constexpr int GEMM_STRIDE = 9;  // floats between rows of 8 columns in shared memory: no bank conflicts
 constexpr long long GEMM_WAIT = 2000000000LL;  // clocks, about a second
 
 struct GemmShape {
@@ -53,7 +53,9 @@ struct GemmTile {
     static constexpr int B_PART = BN / CTAS;  // columns of the tile whose operand this CTA loads
     static constexpr int A_BYTES = GEMM_ROWS * 128, B_BYTES = B_PART * 128;
     static constexpr int STAGE = P * (A_BYTES + B_BYTES);
-    static constexpr int WARPS = BN > 128 || P == 1 ? 4 : 8;  // of the epilogue
+    // Of the epilogue. Its loads, conversions and stores are long chains, of which a
+    // scheduler needs two warps' at least: four warps took twice the time.
+    static constexpr int WARPS = 8;
     static constexpr int COLUMNS = BN / (WARPS / 4);  // of an epilogue warp
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int PIECES = WARPS * 32 * GEMM_STRIDE * 4;
@@ -234,9 +236,52 @@ template <> struct Products<3> {
     __device__ static constexpr int b(int i) { return i == 1 ? 2 : i == 2 || i == 4; }
 };
 
-// The epilogue E gets every element of a tile once, as float4 of neighbouring
-// columns (put), after what it reads for them has been fetched (fetch); `direct` sees
-// them before that by lanes, a row a thread. Columns behind n are the epilogue's to skip.
+// 32 bytes that one thread moves, 32-byte aligned: whole sectors, also where every
+// thread of a warp is in a row of its own.
+struct Wide {
+    uint32_t w[8];
+};
+__device__ __forceinline__ Wide load_wide(const void* p) {
+    Wide v;
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void store_wide(void* p, const Wide& v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]),
+                 "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+                 : "memory");
+}
+
+// 16 elements of T as one or two of them.
+template <class T>
+struct Sixteen {
+    static constexpr int COUNT = sizeof(T) / 2;
+    Wide part[COUNT];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) part[i] = load_wide(reinterpret_cast<const char*>(p) + 32 * i);
+    }
+    __device__ __forceinline__ void get(float (&f)[16]) const {
+        Vector<T, 16> v;
+        memcpy(&v, part, sizeof(v));
+        unpack<T, 16>(v, f);
+    }
+    __device__ __forceinline__ static void store(T* p, const float (&f)[16]) {
+        const Vector<T, 16> v = pack<T, 16>(f);
+        Wide w[COUNT];
+        memcpy(w, &v, sizeof(v));
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) store_wide(reinterpret_cast<char*>(p) + 32 * i, w[i]);
+    }
+};
+
+// The epilogue E gets a tile in pieces of 32 rows and 32 columns. Where its arrays have
+// rows of whole 32 bytes (`whole`), a thread keeps the row of its lane: `fetch` reads what
+// belongs to half a piece, 16 columns, ahead of `half`, which ends them. Otherwise the
+// piece goes through shared memory, so that neighbouring threads have neighbouring
+// columns, and `one` ends each element.
 template <class C, class E>
 __global__ void __launch_bounds__(C::THREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const GemmShape s, const E epilogue,
@@ -355,28 +400,38 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             }
             ++unit;
         };
-        auto put = [&](const float (&v)[32], int row, int column, const Work& w) {
+        // What a piece needs beside D, read ahead.
+        struct Ahead {
+            typename E::Fetched half[2];
+        };
+        auto fetch = [&](Ahead& got, int row, int column, const Work& w) {
+            if (!epilogue.whole || row + lane >= s.m) return;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (column + 16 * h < s.n) epilogue.fetch(got.half[h], row + lane, column + 16 * h, w.batch, s);
+        };
+        auto put = [&](float (&v)[32], const Ahead& got, int row, int column, const Work& w) {
             if (row >= s.m || column >= s.n) return;
-            epilogue.direct(v, row + lane, column, w.batch, C::BM, C::BN, s);
-            __syncwarp();
+            if (epilogue.whole) {
+                if (row + lane >= s.m) return;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(piece + lane * GEMM_STRIDE + 4 * i) =
-                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            __syncwarp();
-            const int c = lane % 8 * 4;
-            typename E::Fetched got[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + lane / 8;
-                if (row + r < s.m && column + c < s.n) epilogue.fetch(got[i], row + r, column + c, w.batch, s);
+                for (int h = 0; h < 2; ++h)
+                    if (column + 16 * h < s.n)
+                        epilogue.half(*reinterpret_cast<float(*)[16]>(v + 16 * h), got.half[h], row + lane, column + 16 * h,
+                                      w.batch, w.split, C::BM, C::BN, s);
+                return;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + lane / 8;
-                if (row + r < s.m && column + c < s.n)
-                    epilogue.put(*reinterpret_cast<const float4*>(piece + r * GEMM_STRIDE + c), got[i], row + r, column + c,
-                                 w.batch, w.split, s);
+            for (int h = 0; h < 4; ++h) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) piece[lane * GEMM_STRIDE + i] = v[8 * h + i];
+                __syncwarp();
+                const int c = column + 8 * h + lane % 8;
+                if (c >= s.n) continue;
+#pragma unroll 4
+                for (int r = lane / 8; r < 32; r += 4)
+                    if (row + r < s.m) epilogue.one(piece[r * GEMM_STRIDE + lane % 8], row + r, c, w.batch, w.split, s);
             }
         };
         bool ok = true;
@@ -385,14 +440,18 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column = w.tile_n * C::BN + c0;
             const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + c0;
             if constexpr (C::P == 1) {
+                Ahead got;
+                fetch(got, row, column, w);
                 if (!(ok = wait())) break;
                 const uint32_t from = lanes + (unit & 1) * C::BN;
 #pragma unroll 1
                 for (int c = 0; c < C::COLUMNS; c += 32) {
                     float v[32];
                     tmem_piece(from + c, v);
+                    const Ahead now = got;
                     if (c + 32 == C::COLUMNS) taken();
-                    put(v, row, column + c, w);
+                    else fetch(got, row, column + c + 32, w);
+                    put(v, now, row, column + c, w);
                 }
             } else {
                 float sum[C::COLUMNS / 32][32] = {};
@@ -409,7 +468,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < C::COLUMNS / 32; ++c) put(sum[c], row, column + 32 * c, w);
+                for (int c = 0; c < C::COLUMNS / 32; ++c) {
+                    Ahead got;
+                    fetch(got, row, column + 32 * c, w);
+                    put(sum[c], got, row, column + 32 * c, w);
+                }
             }
         }
     }

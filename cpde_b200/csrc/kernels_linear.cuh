@@ -53,6 +53,21 @@ __device__ __forceinline__ void store_some(T* p, const float (&f)[V], int64_t le
     }
 }
 
+template <int V>
+__device__ __forceinline__ void activate_all(float (&v)[V], int32_t activation) {
+    if (activation == 1) return;
+    if (activation == 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 2);
+    } else if (activation == 3) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 3);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 0);
+    }
+}
+
 // Bias, activation and residual in the product's epilogue, or plain results, or the
 // partial sums of a split contraction.
 template <class T>
@@ -61,71 +76,96 @@ struct LinearEpilogue {
     const T* residual;      // or null
     T* z;                   // or null
     void* y;                // of FP32 or T
-    float* partial;         // where the contraction is split: (split, row, column) sums, pitch n rounded up to 4
+    float* partial;         // where the contraction is split: (split, row, column) sums, pitch n rounded up to 16
     int64_t residual_stride;
     int32_t activation;
     bool bias_wide, y_wide;
-    bool whole;             // four elements at a time are there and aligned in every array
+    bool whole;             // 16 elements at a time are there and in whole 32 bytes, in every array
+    bool fours;             // four at a time are, for the joining of partial sums
 
-    struct Fetched {
-        float bias[4], residual[4];
-    };
-    __device__ void direct(const float (&)[32], int, int, int, int, int, const GemmShape&) const {}
-    __device__ __forceinline__ void fetch(Fetched& f, int64_t row, int column, int, const GemmShape& s) const {
-        if (partial) return;
-        const int64_t left = s.n - column;
-        if (bias) {
-            if (bias_wide) load_some<float, 4>(static_cast<const float*>(bias) + column, f.bias, left, whole);
-            else load_some<T, 4>(static_cast<const T*>(bias) + column, f.bias, left, whole);
-        }
-        if (residual) load_some<T, 4>(residual + row * residual_stride + column, f.residual, left, whole);
+    using Fetched = Sixteen<T>;  // the residual
+    __device__ static int64_t partial_pitch(const GemmShape& s) { return (s.n + 15) / 16 * 16; }
+
+    __device__ __forceinline__ void fetch(Fetched& f, int64_t row, int column, int, const GemmShape&) const {
+        if (residual && !partial) f.load(residual + row * residual_stride + column);
     }
-    __device__ __forceinline__ void put(const float4& d, const Fetched& f, int64_t row, int column, int, int split,
-                                        const GemmShape& s) const {
+    __device__ __forceinline__ void half(float (&v)[16], const Fetched& f, int64_t row, int column, int, int split, int, int,
+                                         const GemmShape& s) const {
         if (partial) {
-            const int64_t pitch = (s.n + 3) / 4 * 4;
-            *reinterpret_cast<float4*>(partial + (split * int64_t(s.m) + row) * pitch + column) = d;
+            Sixteen<float>::store(partial + (split * int64_t(s.m) + row) * partial_pitch(s) + column, v);
             return;
         }
-        float v[4] = {d.x, d.y, d.z, d.w};
-        const int64_t left = s.n - column, at = row * s.n + column;
         if (bias) {
+            float b[16];
+            if (bias_wide) load_some<float, 16>(static_cast<const float*>(bias) + column, b, 16, true);
+            else load_some<T, 16>(static_cast<const T*>(bias) + column, b, 16, true);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += f.bias[i];
+            for (int i = 0; i < 16; ++i) v[i] += b[i];
         }
-        if (z) store_some<T, 4>(z + at, v, left, whole);
-        if (activation != 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = layer_activation(v[i], activation);
-        }
+        const int64_t at = row * s.n + column;
+        if (z) Sixteen<T>::store(z + at, v);
+        activate_all<16>(v, activation);
         if (residual) {
+            float r[16];
+            f.get(r);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += f.residual[i];
+            for (int i = 0; i < 16; ++i) v[i] += r[i];
         }
-        if (y_wide) store_some<float, 4>(static_cast<float*>(y) + at, v, left, whole);
-        else store_some<T, 4>(static_cast<T*>(y) + at, v, left, whole);
+        if (y_wide) Sixteen<float>::store(static_cast<float*>(y) + at, v);
+        else Sixteen<T>::store(static_cast<T*>(y) + at, v);
+    }
+    // V elements, whatever the arrays' alignment if V is 1.
+    template <int V>
+    __device__ __forceinline__ void some(float (&v)[V], int64_t row, int column, const GemmShape& s) const {
+        const int64_t at = row * s.n + column;
+        if (bias) {
+            float b[V];
+            if (bias_wide) load_some<float, V>(static_cast<const float*>(bias) + column, b, V, true);
+            else load_some<T, V>(static_cast<const T*>(bias) + column, b, V, true);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] += b[i];
+        }
+        if (z) store<T, V>(z + at, pack<T, V>(v));
+        activate_all<V>(v, activation);
+        if (residual) {
+            float r[V];
+            load_some<T, V>(residual + row * residual_stride + column, r, V, true);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] += r[i];
+        }
+        if (y_wide) store<float, V>(static_cast<float*>(y) + at, pack<float, V>(v));
+        else store<T, V>(static_cast<T*>(y) + at, pack<T, V>(v));
+    }
+    __device__ __forceinline__ void one(float d, int64_t row, int column, int, int split, const GemmShape& s) const {
+        if (partial) {
+            partial[(split * int64_t(s.m) + row) * partial_pitch(s) + column] = d;
+            return;
+        }
+        float v[1] = {d};
+        some<1>(v, row, column, s);
     }
 };
 
-// Joins the partial sums of a split contraction, in the order of the splits, and ends them as the epilogue does.
-template <class T>
+// Joins the partial sums of a split contraction, in the order of the splits, and ends
+// them as the epilogue does.
+template <class T, int V>
 __global__ void __launch_bounds__(256) k_join(LinearEpilogue<T> epilogue, GemmShape s) {
     after_previous_launch();
     const float* partial = epilogue.partial;
     epilogue.partial = nullptr;
-    const int64_t fours = (s.n + 3) / 4, all = s.m * fours;
+    const int64_t pitch = LinearEpilogue<T>::partial_pitch(s), across = (s.n + V - 1) / V, all = s.m * across;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < all; i += gridDim.x * int64_t(256)) {
-        const int64_t row = i / fours;
-        const int column = int(i % fours) * 4;
-        typename LinearEpilogue<T>::Fetched f;
-        epilogue.fetch(f, row, column, 0, s);
-        float4 sum = make_float4(0, 0, 0, 0);
+        const int64_t row = i / across;
+        const int column = int(i % across) * V;
+        float sum[V] = {};
 #pragma unroll 8
         for (int split = 0; split < s.splits; ++split) {
-            const float4 v = *reinterpret_cast<const float4*>(partial + (split * all + i) * 4);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            float v[V];
+            load_some<float, V>(partial + (split * int64_t(s.m) + row) * pitch + column, v, V, true);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += v[j];
         }
-        epilogue.put(sum, f, row, column, 0, 0, s);
+        epilogue.template some<V>(sum, row, column, s);
     }
 }
 

@@ -27,97 +27,79 @@ struct OrthogonalEpilogue {
     __half* out;            // OUT parts a batch
     T* final;               // OUT == 0: contiguous
     const T* weight;        // or null
-    int64_t pitch, plane;   // of the parts
+    int64_t pitch, plane;   // of the parts: rows of whole 32 bytes
     int in_planes, out_planes;
     float scale_d, scale_in, keep, rate;
-    bool whole;             // four elements of the result at a time
+    bool whole;             // the result has rows of whole 32 bytes, or there are parts alone
 
     struct Fetched {
-        uint2 in[IN ? IN : 1];
-        float weight[4];
+        Sixteen<__half> in[IN ? IN : 1];
+        Sixteen<T> weight;
     };
-    __device__ __forceinline__ static float4 halves(const uint2& w) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    // The mirrored elements, where no tile computes them: lanes along a row.
-    __device__ __forceinline__ void direct(const float (&d)[32], int row, int column, int batch, int bm, int bn,
-                                           const GemmShape& s) const {
-        if constexpr (MIRROR) {
-            const int first = row - int(threadIdx.x % 32);  // the piece's first row; pieces do not cross tiles
-            if (first / bn * bn < (column / bm + 1) * bm) return;
-            const __half* from = in + int64_t(batch) * in_planes * plane;
-            __half* to = out + int64_t(batch) * out_planes * plane;
-            if (row >= s.m) return;
-#pragma unroll 4
-            for (int i = 0; i < 32; ++i) {
-                const int64_t at = (column + i) * pitch + row;
-                float v = scale_d * d[i];
-                if constexpr (IN > 0) {
-                    float x = __half2float(from[at]);
-                    if constexpr (IN > 1) x += __half2float(from[plane + at]);
-                    v = fmaf(scale_in, x, v);
-                }
-                const __half h = __float2half_rn(v);
-                to[at] = h;
-                if constexpr (OUT > 1) to[plane + at] = __float2half_rn(v - __half2float(h));
-            }
-        }
-    }
     __device__ __forceinline__ void fetch(Fetched& f, int64_t row, int column, int batch, const GemmShape& s) const {
         if constexpr (IN > 0) {
             const __half* from = in + int64_t(batch) * in_planes * plane + row * pitch + column;
 #pragma unroll
-            for (int p = 0; p < IN; ++p) f.in[p] = *reinterpret_cast<const uint2*>(from + p * plane);
+            for (int p = 0; p < IN; ++p) f.in[p].load(from + p * plane);
         }
-        if constexpr (OUT == 0) {
-            if (!weight) return;
-            const T* w = weight + (int64_t(batch) * s.m + row) * s.n + column;
-            if (whole) unpack<T, 4>(load_written<T, 4>(w), f.weight);
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f.weight[i] = column + i < s.n ? to_float(w[i]) : 0.0f;
-        }
+        if constexpr (OUT == 0)
+            if (weight) f.weight.load(weight + (int64_t(batch) * s.m + row) * s.n + column);
     }
-    __device__ __forceinline__ void put(const float4& d, const Fetched& f, int64_t row, int column, int batch, int,
-                                        const GemmShape& s) const {
-        float v[4] = {scale_d * d.x, scale_d * d.y, scale_d * d.z, scale_d * d.w};
+    __device__ __forceinline__ void half(float (&v)[16], const Fetched& f, int64_t row, int column, int batch, int, int bm, int bn,
+                                         const GemmShape& s) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= scale_d;
         if constexpr (IN > 0) {
-            float4 x = halves(f.in[0]);
+            float x[16], rest[16];
+            f.in[0].get(x);
             if constexpr (IN > 1) {
-                const float4 rest = halves(f.in[1]);
-                x.x += rest.x, x.y += rest.y, x.z += rest.z, x.w += rest.w;
+                f.in[1].get(rest);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] += rest[i];
             }
-            v[0] = fmaf(scale_in, x.x, v[0]), v[1] = fmaf(scale_in, x.y, v[1]);
-            v[2] = fmaf(scale_in, x.z, v[2]), v[3] = fmaf(scale_in, x.w, v[3]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = fmaf(scale_in, x[i], v[i]);
         }
         if constexpr (OUT > 0) {
-            __half* to = out + int64_t(batch) * out_planes * plane + row * pitch + column;
+            __half* to = out + int64_t(batch) * out_planes * plane;
+            // The tile on the other side of the diagonal, where none is computed. Pieces lie in one tile.
+            const bool mirror = MIRROR && int(row) / bn * bn >= (column / bm + 1) * bm;
 #pragma unroll
-            for (int p = 0; p < OUT; ++p) {
-                const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-                uint2 w;
-                memcpy(&w.x, &a, 4), memcpy(&w.y, &b, 4);
-                *reinterpret_cast<uint2*>(to + p * plane) = w;
-                if (p + 1 < OUT) {
-                    const float2 x = __half22float2(a), y = __half22float2(b);
-                    v[0] -= x.x, v[1] -= x.y, v[2] -= y.x, v[3] -= y.y;
+            for (int p = 0; p < OUT; ++p, to += plane) {
+                __half h[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    h[i] = __float2half_rn(v[i]);
+                    v[i] -= __half2float(h[i]);
+                }
+                Wide w;
+                memcpy(&w, h, sizeof(w));
+                store_wide(to + row * pitch + column, w);
+                if (MIRROR && mirror) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) to[(column + i) * pitch + row] = h[i];
                 }
             }
         } else {
-            T* to = final + (int64_t(batch) * s.m + row) * s.n + column;
             if (weight) {
+                float w[16];
+                f.weight.get(w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = fmaf(-rate, v[i], keep * f.weight[i]);
+                for (int i = 0; i < 16; ++i) v[i] = fmaf(-rate, v[i], keep * w[i]);
             }
-            if (whole) {
-                store<T, 4>(to, pack<T, 4>(v));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (column + i < s.n) to[i] = from_float<T>(v[i]);
-            }
+            Sixteen<T>::store(final + (int64_t(batch) * s.m + row) * s.n + column, v);
+        }
+    }
+    __device__ __forceinline__ void one(float d, int64_t row, int column, int batch, int, const GemmShape& s) const {
+        if constexpr (OUT == 0) {
+            float v = scale_d * d;
+            const __half* from = in + int64_t(batch) * in_planes * plane + row * pitch + column;
+            float x = __half2float(from[0]);
+            if constexpr (IN > 1) x += __half2float(from[plane]);
+            v = fmaf(scale_in, x, v);
+            const int64_t at = (int64_t(batch) * s.m + row) * s.n + column;
+            if (weight) v = fmaf(-rate, v, keep * to_float(weight[at]));
+            final[at] = from_float<T>(v);
         }
     }
 };
@@ -190,7 +172,7 @@ __global__ void __launch_bounds__(256) k_update_norm(const UpdateCall<T, M> c) {
     c.sums[blockIdx.y * c.blocks + blockIdx.x] = sum;
 }
 
-// Divides by norm + eps and splits into parts, with zeros in the rows' padding.
+// Divides by norm + eps and splits into parts.
 template <class V>
 __global__ void __launch_bounds__(256)
     k_normalise(const V* x, const double* sums, __half* out, int64_t rows, int64_t pitch, int64_t plane, int32_t columns,
@@ -208,7 +190,7 @@ __global__ void __launch_bounds__(256)
     const float by = float(scale / (sqrt(sum) + eps));
     const int lane = threadIdx.x % lanes, high = 256 / lanes, wide = lanes * 8;
     for (int64_t row = blockIdx.x * int64_t(high) + threadIdx.x / lanes; row < rows; row += int64_t(gridDim.x) * high)
-        for (int column = lane * 8; column < columns; column += wide) {
+        for (int column = lane * 8; column < columns; column += wide) {  // the padding behind is never read
             const V* p = x + (blockIdx.y * rows + row) * columns + column;
             float v[8], h[8];
             if (whole) unpack<V, 8>(load_written<V, 8>(p), v);

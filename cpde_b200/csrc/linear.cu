@@ -74,21 +74,34 @@ void product(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k
              LinearEpilogue<T> epilogue, float* partial, int* error, cudaStream_t stream) {
     constexpr int P = Parts<T>::count;
     constexpr bool bf16 = !std::is_same_v<T, __half>;
-    if (plan.splits > 1) epilogue.partial = partial;
+    // Partial sums have whole rows, whatever the result's are.
+    if (plan.splits > 1) epilogue.partial = partial, epilogue.whole = true;
     with_tile<P, A_ROWS, B_ROWS>(plan, [&](auto tile) {
         launch_gemm<decltype(tile)>(a, b, m, n, k, 1, bf16, false, plan, epilogue, error, stream);
     });
-    if (plan.splits > 1) {
-        GemmShape s = {};
-        s.m = int(m), s.n = int(n), s.splits = plan.splits;
-        const int64_t fours = m * ((n + 3) / 4);
-        launch_early(k_join<T>, dim3(unsigned(std::min<int64_t>((fours + 255) / 256, GEMM_SMS * 8))), 256, 0, 1, stream, epilogue,
-                     s);
-    }
+    if (plan.splits == 1) return;
+    GemmShape s = {};
+    s.m = int(m), s.n = int(n), s.splits = plan.splits;
+    const int64_t threads = m * (epilogue.fours ? n / 4 : n);
+    const dim3 grid(unsigned(std::min<int64_t>((threads + 255) / 256, GEMM_SMS * 8)));
+    if (epilogue.fours) launch_early(k_join<T, 4>, grid, 256, 0, 1, stream, epilogue, s);
+    else launch_early(k_join<T, 1>, grid, 256, 0, 1, stream, epilogue, s);
+}
+
+// Whether rows of `n` elements at these addresses take the wide accesses of the epilogue, and those of fours.
+template <class T>
+void set_widths(LinearEpilogue<T>& e, int64_t n) {
+    auto all = [&](int count) {
+        const int64_t own = count * sizeof(T), wide = count * 4;
+        auto fits = [](const void* p, int64_t bytes) { return aligned(p, std::min<int64_t>(bytes, 32)); };
+        return n % count == 0 && fits(e.y, e.y_wide ? wide : own) && fits(e.z, own) && fits(e.bias, e.bias_wide ? wide : own) &&
+               fits(e.residual, own) && (!e.residual || e.residual_stride % count == 0);
+    };
+    e.whole = all(16), e.fours = all(4);
 }
 
 size_t partial_count(const GemmPlan& plan, int64_t m, int64_t n) {
-    return plan.splits > 1 ? size_t(plan.splits) * m * ((n + 3) / 4 * 4) : 0;
+    return plan.splits > 1 ? size_t(plan.splits) * m * ((n + 15) / 16 * 16) : 0;
 }
 
 template <class T>
@@ -112,9 +125,7 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     e.residual = static_cast<const T*>(c.residual), e.residual_stride = c.residual_stride;
     e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
     e.activation = c.activation;
-    const int64_t four = 4 * sizeof(T);
-    e.whole = c.outputs % 4 == 0 && aligned(c.y, four) && aligned(c.z, four) && aligned(c.bias, e.bias_wide ? 16 : 8) &&
-              (!c.residual || (aligned(c.residual, four) && c.residual_stride % 4 == 0));
+    set_widths(e, c.outputs);
     product<T, false, false>(a, b, c.points, c.outputs, c.inputs, plan, e, partial, error, stream);
     return room.bytes;
 }
@@ -161,14 +172,14 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
         const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
                                    : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
         e.y = c.dx, e.y_wide = c.type == F32;
-        e.whole = c.inputs % 4 == 0 && aligned(c.dx, 4 * sizeof(T));
+        set_widths(e, c.inputs);
         product<T, false, true>(dz, b, c.points, c.inputs, c.outputs, dx_plan, e, partial, error, stream);
     }
     if (c.dweight) {
         const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
                                    : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
         e.y = c.dweight, e.y_wide = c.weight_type == F32;
-        e.whole = c.inputs % 4 == 0 && aligned(c.dweight, e.y_wide ? 16 : 8);
+        set_widths(e, c.inputs);
         product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw_plan, e, partial, error, stream);
     }
     return room.bytes;

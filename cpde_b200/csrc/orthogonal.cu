@@ -76,7 +76,7 @@ size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const int64_t m = c.rows, n = c.columns, side = std::min(m, n), batch = c.matrices;
     const bool tall = m > n;
-    const int64_t pitch = (n + 7) / 8 * 8, gram_pitch = (side + 7) / 8 * 8;
+    const int64_t pitch = (n + 15) / 16 * 16, gram_pitch = (side + 15) / 16 * 16;
     const int lanes = row_lanes(n), high = 256 / lanes;
     const int blocks = int(std::max<int64_t>(
         1, std::min<int64_t>({(m + high - 1) / high, (GEMM_SMS * 8 + batch - 1) / batch, 1024})));
@@ -119,6 +119,7 @@ size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch
         const Operand in = {x[k & 1], pitch, m, n, 2 * batch, plane, 2};
         OrthogonalEpilogue<true, 0, P, T> to_gram = {};
         to_gram.out = gram, to_gram.pitch = gram_pitch, to_gram.plane = gram_plane, to_gram.out_planes = P;
+        to_gram.whole = true;
         to_gram.scale_d = std::ldexp(1.0f, s.gram - 2 * s.x);
         if (tall)
             with_tile<P, true, true>(gram_plan, [&](auto tile) {
@@ -130,6 +131,7 @@ size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch
             });
         OrthogonalEpilogue<true, P, P, T> to_poly = {};
         to_poly.in = gram, to_poly.out = poly, to_poly.pitch = gram_pitch, to_poly.plane = gram_plane;
+        to_poly.whole = true;
         to_poly.in_planes = to_poly.out_planes = P;
         to_poly.scale_in = float(std::ldexp(s.b, s.poly - s.gram)), to_poly.scale_d = float(std::ldexp(s.c, s.poly - 2 * s.gram));
         with_tile<P, false, false>(square_plan, [&](auto tile) {
@@ -150,13 +152,13 @@ size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch
         };
         if (k + 1 < c.steps) {
             OrthogonalEpilogue<false, 2, 2, T> e = {};
-            e.out = x[(k + 1) & 1];
+            e.out = x[(k + 1) & 1], e.whole = true;
             step(e, steps[k + 1].x);
         } else {
             OrthogonalEpilogue<false, 2, 0, T> e = {};
             e.final = static_cast<T*>(c.out);
             if (c.step) e.weight = static_cast<const T*>(c.weight), e.keep = float(c.keep), e.rate = float(c.rate);
-            e.whole = n % 4 == 0 && aligned(c.out, 4 * sizeof(T)) && aligned(e.weight, 4 * sizeof(T));
+            e.whole = n % 16 == 0 && aligned(c.out, 32) && aligned(e.weight, 32);
             step(e, 0);
         }
     }
