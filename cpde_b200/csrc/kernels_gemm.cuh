@@ -69,6 +69,19 @@ struct GemmTile {
 
 namespace gemm {
 
+// As tc::mbar_wait_or_abort, without a clock where there is nothing to wait for.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return tc::mbar_try_wait(bar, parity) || tc::mbar_wait_or_abort(bar, parity, GEMM_WAIT, abort);
+}
+
+// One thread of the warp. The loads and MMAs take their operands from registers of the
+// whole warp: a thread that the compiler knows to be the only one issues them directly.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -299,6 +312,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         *sh.abort = 0;
         tc::fence_barrier_init();
     }
+    if (threadIdx.x == 32 * 2) {
+        for (const CUtensorMap* map : {&a_map, &b_map})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+    }
     if (warp == 1) tmem_take<C::CTAS>(sh.slot, C::TMEM);
     tc::tc_fence_before();
     if constexpr (C::CTAS == 2) cluster_sync();
@@ -309,63 +326,71 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     after_previous_launch();
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
+        if (elected()) {
+            int st = 0;
+            uint32_t parity = 1, loaded = 0;
+            // The barriers that the bytes count at, and the boxes' places.
+            const uint32_t bars = C::CTAS == 2 ? at_rank(sh.full, 0) : tc::smem_u32(sh.full);
+            const uint32_t stages = tc::smem_u32(sh.stages);
             for (int64_t at = first; at < items && !*sh.abort; at += stride) {
                 const Work w = work_at<C>(s, at);
                 const int m0 = w.tile_m * C::BM + rank * GEMM_ROWS, n0 = w.tile_n * C::BN + rank * C::B_PART;
-                for (int slab = w.from; slab < w.to; ++slab, ++it) {
-                    const int st = it % C::STAGES;
-                    if (!tc::mbar_wait_or_abort(sh.empty + st, ((it / C::STAGES) & 1) ^ 1, GEMM_WAIT, sh.abort)) break;
+                const int za = w.batch * s.a_planes, zb = w.batch * s.b_planes;
+                for (int slab = w.from; slab < w.to; ++slab, ++loaded) {
+                    if (!wait_for(sh.empty + st, parity, sh.abort)) break;
                     if (rank == 0) tc::mbar_expect_tx(sh.full + st, s.stage_bytes);
-                    const uint32_t bar = C::CTAS == 2 ? at_rank(sh.full + st, 0) : tc::smem_u32(sh.full + st);
-                    uint32_t to = tc::smem_u32(sh.stages + st * C::STAGE);
+                    const uint32_t bar = bars + 8 * st;
+                    uint32_t to = stages + st * C::STAGE;
+                    const int k0 = slab * GEMM_SLAB;
 #pragma unroll
                     for (int p = 0; p < C::P; ++p, to += C::A_BYTES) {
-                        const int z = w.batch * s.a_planes + p;
                         if constexpr (C::A_ROWS) {
-                            load_box<C::CTAS>(to, &a_map, bar, m0, slab * GEMM_SLAB, z);
-                            load_box<C::CTAS>(to + 8192, &a_map, bar, m0 + 64, slab * GEMM_SLAB, z);
+                            load_box<C::CTAS>(to, &a_map, bar, m0, k0, za + p);
+                            load_box<C::CTAS>(to + 8192, &a_map, bar, m0 + 64, k0, za + p);
                         } else {
-                            load_box<C::CTAS>(to, &a_map, bar, slab * GEMM_SLAB, m0, z);
+                            load_box<C::CTAS>(to, &a_map, bar, k0, m0, za + p);
                         }
                     }
 #pragma unroll
                     for (int p = 0; p < C::P; ++p, to += C::B_BYTES) {
-                        const int z = w.batch * s.b_planes + p;
                         if constexpr (C::B_ROWS) {
 #pragma unroll
-                            for (int j = 0; j < C::B_PART; j += 64)
-                                load_box<C::CTAS>(to + j * 128, &b_map, bar, n0 + j, slab * GEMM_SLAB, z);
+                            for (int j = 0; j < C::B_PART; j += 64) load_box<C::CTAS>(to + j * 128, &b_map, bar, n0 + j, k0, zb + p);
                         } else {
-                            load_box<C::CTAS>(to, &b_map, bar, slab * GEMM_SLAB, n0, z);
+                            load_box<C::CTAS>(to, &b_map, bar, k0, n0, zb + p);
                         }
                     }
+                    if (++st == C::STAGES) st = 0, parity ^= 1;
                 }
             }
             // No load may be in flight when the CTA ends, also where a role gave up, nor a
             // commit under way to the other CTA's barriers.
-            for (uint32_t k = it - min(it, uint32_t(C::STAGES)); k < it; ++k) {
-                const uint32_t parity = (k / C::STAGES) & 1;
-                if (rank == 0 && !tc::mbar_wait(sh.full + k % C::STAGES, parity, GEMM_WAIT)) *sh.abort = 1;
-                if (!*sh.abort) tc::mbar_wait_or_abort(sh.empty + k % C::STAGES, parity, GEMM_WAIT, sh.abort);
+            for (uint32_t k = loaded - min(loaded, uint32_t(C::STAGES)); k < loaded; ++k) {
+                const uint32_t round = (k / C::STAGES) & 1;
+                if (rank == 0 && !tc::mbar_wait(sh.full + k % C::STAGES, round, GEMM_WAIT)) *sh.abort = 1;
+                if (!*sh.abort) wait_for(sh.empty + k % C::STAGES, round, sh.abort);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0, unit = 0;
-            bool ok = true;
+        if (rank == 0 && elected()) {
+            // The stage, its round's parity, and whether it was there when the one before
+            // was issued: asking takes longer than the tensor core has work queued.
+            int st = 0;
+            uint32_t parity = 0, unit = 0;
+            bool ok = true, there = false;
             for (int64_t at = first; ok && at < items; at += stride) {
                 const Work w = work_at<C>(s, at);
-                for (int slab = w.from; ok && slab < w.to; ++slab, ++it) {
+                for (int slab = w.from; slab < w.to; ++slab) {
                     const bool begins = C::P > 1 || slab == w.from, ends = C::P > 1 || slab + 1 == w.to;
                     const uint32_t d = tmem + (unit & 1) * C::BN;
-                    if (begins) ok = tc::mbar_wait_or_abort(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, GEMM_WAIT, sh.abort);
-                    const int st = it % C::STAGES;
-                    ok = ok && tc::mbar_wait_or_abort(sh.full + st, (it / C::STAGES) & 1, GEMM_WAIT, sh.abort);
+                    if (begins) ok = wait_for(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, sh.abort);
+                    ok = ok && (there || wait_for(sh.full + st, parity, sh.abort));
                     if (!ok) break;
                     tc::tc_fence_after();
                     const uint32_t a0 = tc::smem_u32(sh.stages + st * C::STAGE), b0 = a0 + C::P * C::A_BYTES;
+                    const int next = st + 1 == C::STAGES ? 0 : st + 1;
+                    const uint32_t next_parity = parity ^ (next == 0);
+                    there = tc::mbar_try_wait(sh.full + next, next_parity);
 #pragma unroll
                     for (int i = 0; i < Products<C::P>::COUNT; ++i) {
                         const uint64_t a = descriptor<C::A_ROWS>(a0 + Products<C::P>::a(i) * C::A_BYTES);
@@ -377,6 +402,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                     }
                     commit<C::CTAS>(sh.empty + st);
                     if (ends) commit<C::CTAS>(sh.ready + (unit & 1)), ++unit;
+                    st = next, parity = next_parity;
                 }
             }
         }
@@ -385,11 +411,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const int c0 = e / 4 * C::COLUMNS;
         float* piece = sh.pieces + e * 32 * GEMM_STRIDE;
         uint32_t unit = 0;
-        // Waits for an accumulator; false where a role gave up.
+        // Waits for an accumulator, one lane for all; false where a role gave up.
         auto wait = [&] {
-            const bool ok = tc::mbar_wait_or_abort(sh.ready + (unit & 1), (unit >> 1) & 1, GEMM_WAIT, sh.abort);
+            const bool ok = lane || wait_for(sh.ready + (unit & 1), (unit >> 1) & 1, sh.abort);
+            const bool all = __all_sync(~0u, ok);
             tc::tc_fence_after();
-            return __all_sync(~0u, ok);
+            return all;
         };
         auto taken = [&] {
             tc::tc_fence_before();
