@@ -61,12 +61,13 @@ struct GemmPlan {
     int ctas, bn, splits, split_slabs;
 };
 
-// Tiles that products of P parts have (GemmTile).
+// The tiles (GemmTile), and the clocks that an MMA of theirs was measured to take in a
+// long contraction: only the largest has the rate of the tensor core, the others are
+// bound by what an MMA reads of shared memory.
 struct GemmChoice {
-    int ctas, bn;
+    int ctas, bn, clocks;
 };
-template <int P> constexpr GemmChoice GEMM_CHOICES[3] = {{2, 128}, {1, 64}, {0, 0}};
-template <> constexpr GemmChoice GEMM_CHOICES<1>[3] = {{2, 256}, {2, 128}, {1, 64}};
+constexpr GemmChoice GEMM_CHOICES[3] = {{2, 256, 130}, {2, 128, 100}, {1, 64, 70}};
 
 inline int64_t lower_tiles(int64_t tiles_m, int64_t tiles_n, int64_t ratio) {
     int64_t sum = 0;
@@ -82,11 +83,10 @@ GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, int64_t batches, bool lower,
     const int64_t slabs = (k + GEMM_SLAB - 1) / GEMM_SLAB;
     GemmPlan best = {};
     double least = 1e300;
-    for (const GemmChoice& c : GEMM_CHOICES<P>) {
-        if (!c.ctas) continue;
+    for (const GemmChoice& c : GEMM_CHOICES) {
         const int64_t bm = 128 * c.ctas, tm = (m + bm - 1) / bm, tn = (n + c.bn - 1) / c.bn;
         const int64_t tiles = (lower ? lower_tiles(tm, tn, bm / c.bn) : tm * tn) * batches, slots = GEMM_SMS / c.ctas;
-        const double bytes = P * (128 + c.bn / c.ctas) * 128.0, clocks = Products<P>::COUNT * 4 * (c.bn / 2);
+        const double bytes = P * (128 + c.bn / c.ctas) * 128.0, clocks = PRODUCTS<P> * 4 * c.clocks;
         const double slab = std::max(clocks, bytes / 64);
         const int64_t fill = std::max<int64_t>(1, slots / std::max<int64_t>(tiles, 1));
         const int64_t most = may_split ? std::min(slabs / 2, 4 * fill) : 1;
@@ -118,7 +118,7 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
     const bool few = !C::A_ROWS && C::CTAS == 1 && m < GEMM_ROWS;
     const int a_box = C::A_ROWS ? 64 : few ? int((m + 7) / 8 * 8) : GEMM_ROWS;
     const int b_box = C::B_ROWS ? 64 : C::B_PART;
-    s.stage_bytes = uint32_t(C::CTAS * C::P * ((few ? a_box * 128 : C::A_BYTES) + C::B_BYTES));
+    s.stage_bytes = uint32_t(C::CTAS * ((few ? a_box * 128 : C::A_BYTES) + C::B_BYTES));
     const uint32_t kind = bf16 ? 1 : 0;
     s.instruction = 1u << 4 | kind << 7 | kind << 10 | uint32_t(C::A_ROWS) << 15 | uint32_t(C::B_ROWS) << 16 |
                     uint32_t(C::BN >> 3) << 17 | uint32_t(C::BM >> 4) << 24;
@@ -138,8 +138,7 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
 // The tile of the plan as a type.
 template <int P, bool A_ROWS, bool B_ROWS, class F>
 void with_tile(const GemmPlan& plan, F&& f) {
-    if constexpr (P == 1)
-        if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS>{});
+    if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS>{});
     if (plan.bn == 128) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS>{});
     f(GemmTile<1, 64, P, A_ROWS, B_ROWS>{});
 }

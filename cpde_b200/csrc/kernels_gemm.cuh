@@ -39,7 +39,7 @@ struct GemmShape {
     int slabs, splits, split_slabs;  // slabs of the contraction, and how they are split
     int tiles_m, tiles_n, tiles, batches;
     int a_planes, b_planes;          // arrays of an operand a batch (of which P are read)
-    uint32_t stage_bytes;            // what a slab's loads bring, of all CTAs of the cluster
+    uint32_t stage_bytes;            // what a stage's loads bring, of all CTAs of the cluster
     uint32_t instruction;            // the MMA's descriptor
     bool lower;                      // only tiles that reach the diagonal or below
 };
@@ -52,18 +52,22 @@ struct GemmTile {
     static constexpr int BM = GEMM_ROWS * CTAS;
     static constexpr int B_PART = BN / CTAS;  // columns of the tile whose operand this CTA loads
     static constexpr int A_BYTES = GEMM_ROWS * 128, B_BYTES = B_PART * 128;
-    static constexpr int STAGE = P * (A_BYTES + B_BYTES);
+    static constexpr int STAGE = A_BYTES + B_BYTES;  // one part of a slab of both operands
     // Of the epilogue. Its loads, conversions and stores are long chains, of which a
     // scheduler needs two warps' at least: four warps took twice the time.
     static constexpr int WARPS = 8;
+    // Slabs that are summed in the accumulator before it is taken out. The way from the
+    // last MMA to the epilogue and back takes 1.4 us a slab with two CTAs of 256 columns:
+    // less than the six products of three parts (1.7), more than the three of two (0.83).
+    static constexpr int UNIT = P == 1 ? 1 << 30 : P == 2 ? 2 : 1;
     static constexpr int COLUMNS = BN / (WARPS / 4);  // of an epilogue warp
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int PIECES = WARPS * 32 * GEMM_STRIDE * 4;
     static constexpr int ROOM = (227 * 1024 - 1024 - 256 - PIECES) / STAGE;
-    static constexpr int STAGES = ROOM > 8 ? 8 : ROOM;
+    static constexpr int STAGES = ROOM > 12 ? 12 : ROOM;
     static constexpr int SHARED = 1024 + STAGES * STAGE + PIECES + 256;
     static constexpr uint32_t TMEM = BN * 2 <= 32 ? 32 : BN * 2 <= 64 ? 64 : BN * 2 <= 128 ? 128 : BN * 2 <= 256 ? 256 : 512;
-    static_assert(STAGES >= 2 && BN * 2 <= 512 && BN % 32 == 0 && COLUMNS % GEMM_PIECE == 0);
+    static_assert(STAGES > P && BN * 2 <= 512 && BN % 32 == 0 && COLUMNS % GEMM_PIECE == 0);
     static_assert(!B_ROWS || B_PART % 64 == 0, "boxes of rows are 64 columns wide");
 };
 
@@ -223,7 +227,7 @@ struct Shared {
         stages = raw + (1024 - (tc::smem_u32(raw) & 1023)) % 1024;
         pieces = reinterpret_cast<float*>(stages + C::STAGES * C::STAGE);
         full = reinterpret_cast<uint64_t*>(stages + C::STAGES * C::STAGE + C::PIECES);
-        empty = full + 8, ready = empty + 8, taken = ready + 2;
+        empty = full + 12, ready = empty + 12, taken = ready + 2;
         slot = reinterpret_cast<uint32_t*>(taken + 2);
         abort = reinterpret_cast<volatile int*>(slot + 1);
     }
@@ -231,23 +235,8 @@ struct Shared {
 
 }  // namespace gemm
 
-// The products of parts (A's, B's), the small ones first.
-template <int P> struct Products;
-template <> struct Products<1> {
-    static constexpr int COUNT = 1;
-    __device__ static constexpr int a(int) { return 0; }
-    __device__ static constexpr int b(int) { return 0; }
-};
-template <> struct Products<2> {
-    static constexpr int COUNT = 3;
-    __device__ static constexpr int a(int i) { return i == 0; }
-    __device__ static constexpr int b(int i) { return i == 1; }
-};
-template <> struct Products<3> {
-    static constexpr int COUNT = 6;
-    __device__ static constexpr int a(int i) { return i == 0 ? 2 : i == 2 || i == 3; }
-    __device__ static constexpr int b(int i) { return i == 1 ? 2 : i == 2 || i == 4; }
-};
+// Products of parts: all but those below the last part's own rounding.
+template <int P> constexpr int PRODUCTS = P * (P + 1) / 2;
 
 // 32 bytes that one thread moves, 32-byte aligned: whole sectors, also where every
 // thread of a warp is in a row of its own.
@@ -336,31 +325,30 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 const Work w = work_at<C>(s, at);
                 const int m0 = w.tile_m * C::BM + rank * GEMM_ROWS, n0 = w.tile_n * C::BN + rank * C::B_PART;
                 const int za = w.batch * s.a_planes, zb = w.batch * s.b_planes;
-                for (int slab = w.from; slab < w.to; ++slab, ++loaded) {
-                    if (!wait_for(sh.empty + st, parity, sh.abort)) break;
-                    if (rank == 0) tc::mbar_expect_tx(sh.full + st, s.stage_bytes);
-                    const uint32_t bar = bars + 8 * st;
-                    uint32_t to = stages + st * C::STAGE;
+                bool ok = true;
+                for (int slab = w.from; ok && slab < w.to; ++slab) {
                     const int k0 = slab * GEMM_SLAB;
 #pragma unroll
-                    for (int p = 0; p < C::P; ++p, to += C::A_BYTES) {
+                    for (int i = 0; i < C::P; ++i, ++loaded) {  // the last part first: it is the first to be done with
+                        const int p = C::P - 1 - i;
+                        if (!(ok = wait_for(sh.empty + st, parity, sh.abort))) break;
+                        if (rank == 0) tc::mbar_expect_tx(sh.full + st, s.stage_bytes);
+                        const uint32_t bar = bars + 8 * st;
+                        const uint32_t a = stages + st * C::STAGE, b = a + C::A_BYTES;
                         if constexpr (C::A_ROWS) {
-                            load_box<C::CTAS>(to, &a_map, bar, m0, k0, za + p);
-                            load_box<C::CTAS>(to + 8192, &a_map, bar, m0 + 64, k0, za + p);
+                            load_box<C::CTAS>(a, &a_map, bar, m0, k0, za + p);
+                            load_box<C::CTAS>(a + 8192, &a_map, bar, m0 + 64, k0, za + p);
                         } else {
-                            load_box<C::CTAS>(to, &a_map, bar, k0, m0, za + p);
+                            load_box<C::CTAS>(a, &a_map, bar, k0, m0, za + p);
                         }
-                    }
-#pragma unroll
-                    for (int p = 0; p < C::P; ++p, to += C::B_BYTES) {
                         if constexpr (C::B_ROWS) {
 #pragma unroll
-                            for (int j = 0; j < C::B_PART; j += 64) load_box<C::CTAS>(to + j * 128, &b_map, bar, n0 + j, k0, zb + p);
+                            for (int j = 0; j < C::B_PART; j += 64) load_box<C::CTAS>(b + j * 128, &b_map, bar, n0 + j, k0, zb + p);
                         } else {
-                            load_box<C::CTAS>(to, &b_map, bar, k0, n0, zb + p);
+                            load_box<C::CTAS>(b, &b_map, bar, k0, n0, zb + p);
                         }
+                        if (++st == C::STAGES) st = 0, parity ^= 1;
                     }
-                    if (++st == C::STAGES) st = 0, parity ^= 1;
                 }
             }
             // No load may be in flight when the CTA ends, also where a role gave up, nor a
@@ -373,36 +361,56 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         }
     } else if (warp == 1) {
         if (rank == 0 && elected()) {
-            // The stage, its round's parity, and whether it was there when the one before
-            // was issued: asking takes longer than the tensor core has work queued.
+            const uint32_t stages = tc::smem_u32(sh.stages);
             int st = 0;
             uint32_t parity = 0, unit = 0;
-            bool ok = true, there = false;
+            bool ok = true;
             for (int64_t at = first; ok && at < items; at += stride) {
                 const Work w = work_at<C>(s, at);
-                for (int slab = w.from; slab < w.to; ++slab) {
-                    const bool begins = C::P > 1 || slab == w.from, ends = C::P > 1 || slab + 1 == w.to;
+                for (int slab = w.from; ok && slab < w.to; ++slab) {
+                    const bool begins = (slab - w.from) % C::UNIT == 0, ends = (slab - w.from) % C::UNIT == C::UNIT - 1 || slab + 1 == w.to;
                     const uint32_t d = tmem + (unit & 1) * C::BN;
                     if (begins) ok = wait_for(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, sh.abort);
-                    ok = ok && (there || wait_for(sh.full + st, parity, sh.abort));
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    const uint32_t a0 = tc::smem_u32(sh.stages + st * C::STAGE), b0 = a0 + C::P * C::A_BYTES;
-                    const int next = st + 1 == C::STAGES ? 0 : st + 1;
-                    const uint32_t next_parity = parity ^ (next == 0);
-                    there = tc::mbar_try_wait(sh.full + next, next_parity);
+                    // The slab's stages, by part.
+                    int stage[C::P];
+                    uint32_t round[C::P];
 #pragma unroll
-                    for (int i = 0; i < Products<C::P>::COUNT; ++i) {
-                        const uint64_t a = descriptor<C::A_ROWS>(a0 + Products<C::P>::a(i) * C::A_BYTES);
-                        const uint64_t b = descriptor<C::B_ROWS>(b0 + Products<C::P>::b(i) * C::B_BYTES);
+                    for (int p = C::P - 1; p >= 0; --p) {
+                        stage[p] = st, round[p] = parity;
+                        if (++st == C::STAGES) st = 0, parity ^= 1;
+                    }
+                    auto there = [&](int p) { ok = ok && wait_for(sh.full + stage[p], round[p], sh.abort); };
+                    auto multiply = [&](int pa, int pb, bool first_of_all) {
+                        const uint64_t a = descriptor<C::A_ROWS>(stages + stage[pa] * C::STAGE);
+                        const uint64_t b = descriptor<C::B_ROWS>(stages + stage[pb] * C::STAGE + C::A_BYTES);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mma<C::CTAS>(d, a + k * (STEP<C::A_ROWS> >> 4), b + k * (STEP<C::B_ROWS> >> 4), s.instruction,
-                                         !(begins && i == 0 && k == 0));
+                                         !(first_of_all && k == 0));
+                    };
+                    there(0);
+                    if constexpr (C::P > 1) there(C::P - 1);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    if constexpr (C::P == 3) {
+                        multiply(2, 0, begins);
+                        multiply(0, 2, false);
+                        commit<C::CTAS>(sh.empty + stage[2]);
+                        there(1);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        multiply(1, 1, false);
+                        multiply(1, 0, false);
+                        multiply(0, 1, false);
+                        commit<C::CTAS>(sh.empty + stage[1]);
+                    } else if constexpr (C::P == 2) {
+                        multiply(1, 0, begins);
+                        multiply(0, 1, false);
+                        commit<C::CTAS>(sh.empty + stage[1]);
                     }
-                    commit<C::CTAS>(sh.empty + st);
+                    multiply(0, 0, C::P == 1 && begins);
+                    commit<C::CTAS>(sh.empty + stage[0]);
                     if (ends) commit<C::CTAS>(sh.ready + (unit & 1)), ++unit;
-                    st = next, parity = next_parity;
                 }
             }
         }
@@ -482,7 +490,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 }
             } else {
                 float sum[C::COLUMNS / 32][32] = {};
-                for (int slab = w.from; ok && slab < w.to; ++slab) {
+                for (int slab = w.from; ok && slab < w.to; slab += C::UNIT) {
                     if (!(ok = wait())) break;
 #pragma unroll
                     for (int c = 0; c < C::COLUMNS / 32; ++c) {
@@ -496,9 +504,20 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 if (!ok) break;
 #pragma unroll
                 for (int c = 0; c < C::COLUMNS / 32; ++c) {
-                    Ahead got;
-                    fetch(got, row, column + 32 * c, w);
-                    put(sum[c], got, row, column + 32 * c, w);
+                    if (epilogue.whole) {  // as in put, without reading ahead, for which there are no registers
+                        if (row + lane >= s.m) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int at_column = column + 32 * c + 16 * h;
+                            if (at_column >= s.n) continue;
+                            typename E::Fetched got;
+                            epilogue.fetch(got, row + lane, at_column, w.batch, s);
+                            epilogue.half(*reinterpret_cast<float(*)[16]>(sum[c] + 16 * h), got, row + lane, at_column, w.batch,
+                                          w.split, C::BM, C::BN, s);
+                        }
+                    } else {
+                        put(sum[c], {}, row, column + 32 * c, w);
+                    }
                 }
             }
         }
