@@ -238,6 +238,27 @@ struct Shared {
 // Products of parts: all but those below the last part's own rounding.
 template <int P> constexpr int PRODUCTS = P * (P + 1) / 2;
 
+// Up to V elements of a row that has `left` of them from here on.
+template <class T, int V>
+__device__ __forceinline__ void load_some(const T* p, float (&f)[V], int64_t left, bool whole) {
+    if (whole) {
+        unpack<T, V>(load_written<T, V>(p), f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = i < left ? to_float(p[i]) : 0.0f;
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_some(T* p, const float (&f)[V], int64_t left, bool whole) {
+    if (whole) {
+        store<T, V>(p, pack<T, V>(f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = from_float<T>(f[i]);
+    }
+}
+
 // 32 bytes that one thread moves, 32-byte aligned: whole sectors, also where every
 // thread of a warp is in a row of its own.
 struct Wide {

@@ -32,27 +32,6 @@ __device__ __forceinline__ float layer_slope(float z, int32_t activation) {
     return activation == 3 ? fmaf(f, z * (1.0f - f), f) : f * (1.0f - f);
 }
 
-// Up to V elements of a row that has `left` of them from here on.
-template <class T, int V>
-__device__ __forceinline__ void load_some(const T* p, float (&f)[V], int64_t left, bool whole) {
-    if (whole) {
-        unpack<T, V>(load_written<T, V>(p), f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = i < left ? to_float(p[i]) : 0.0f;
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_some(T* p, const float (&f)[V], int64_t left, bool whole) {
-    if (whole) {
-        store<T, V>(p, pack<T, V>(f));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = from_float<T>(f[i]);
-    }
-}
-
 template <int V>
 __device__ __forceinline__ void activate_all(float (&v)[V], int32_t activation) {
     if (activation == 1) return;

@@ -3,7 +3,7 @@
 #include <vector>
 
 #include "gemm_launch.hpp"
-#include "kernels_orthogonal.cuh"
+#include "kernels_orthogonal_small.cuh"
 #include "layers.hpp"
 
 namespace cpde::ops {
@@ -71,8 +71,57 @@ int row_lanes(int64_t columns) {
     return lanes;
 }
 
+// Whether one CTA holds a matrix.
+bool small(const OrthogonalCall& c) {
+    return std::min(c.rows, c.columns) <= SMALL_SIDE && std::max(c.rows, c.columns) <= SMALL_LENGTH;
+}
+
+template <class T, class M>
+void run_small(const OrthogonalCall& c, int* error, cudaStream_t stream) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    std::vector<Step> steps;
+    plan_steps(c, steps);
+    SmallCall<T, M> s = {};
+    s.x = static_cast<const T*>(c.x);
+    s.out = static_cast<T*>(c.out);
+    if (c.step) {
+        s.momentum = static_cast<const M*>(c.momentum), s.new_momentum = static_cast<M*>(c.new_momentum);
+        s.weight = static_cast<const T*>(c.weight);
+        s.beta = float(c.beta), s.rest = float(1 - c.beta), s.keep = float(c.keep), s.rate = float(c.rate);
+        s.nesterov = c.nesterov;
+    }
+    s.rows = int(c.rows), s.columns = int(c.columns), s.steps = c.steps;
+    s.whole = c.columns % 8 == 0;
+    for (const void* p : {c.x, static_cast<const void*>(c.out), s.weight ? c.weight : nullptr, s.momentum ? c.momentum : nullptr,
+                          static_cast<const void*>(s.new_momentum)})
+        s.whole = s.whole && aligned(p, 16);
+    s.scale = std::ldexp(1.0f, steps[0].x), s.eps = c.eps;
+    for (int k = 0; k < c.steps; ++k) {
+        const Step& v = steps[k];
+        const int next = k + 1 < c.steps ? steps[k + 1].x : 0;
+        s.step[k] = {std::ldexp(1.0f, v.gram - 2 * v.x), float(std::ldexp(v.b, v.poly - v.gram)),
+                     float(std::ldexp(v.c, v.poly - 2 * v.gram)), float(std::ldexp(v.a, next - v.x)),
+                     float(std::ldexp(1.0, next - v.x - v.poly))};
+    }
+    const int64_t side = std::min(c.rows, c.columns), length = std::max(c.rows, c.columns);
+    const size_t shared = 1024 + ((length + 63) / 64 * 2 + (side + 63) / 64 * P) * SMALL_BLOCK;
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limit is raised
+    int device = 0;
+    CPDE_CUDA(cudaGetDevice(&device));
+    if (!(ready.load() >> (device & 63) & 1)) {
+        CPDE_CUDA(cudaFuncSetAttribute(k_orthogonal_small<P, T, M>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       1024 + (8 + 2 * P) * SMALL_BLOCK));
+        ready.fetch_or(uint64_t(1) << (device & 63));
+    }
+    launch_early(k_orthogonal_small<P, T, M>, dim3(unsigned(c.matrices)), SMALL_THREADS, shared, 1, stream, s, error);
+}
+
 template <class T, class M>
 size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch) {
+    if (small(c)) {
+        if (launch) run_small<T, M>(c, error, stream);
+        return 0;
+    }
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const int64_t m = c.rows, n = c.columns, side = std::min(m, n), batch = c.matrices;
     const bool tall = m > n;

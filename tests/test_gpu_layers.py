@@ -204,7 +204,7 @@ def close(got, x, kind, **options):
                                                               float(bound / want.norm()))
 
 
-MATRICES = [(1, 1), (1, 7), (7, 1), (3, 5), (20, 128), (128, 20), (64, 64), (65, 64), (128, 128), (130, 257), (500, 129),
+MATRICES = [(1, 1), (1, 7), (7, 1), (3, 5), (24, 40), (40, 24), (20, 128), (128, 20), (64, 64), (128, 256), (250, 120), (72, 200), (65, 64), (128, 128), (130, 257), (500, 129),
             (77, 1000), (256, 256), (512, 384), (1024, 320)]
 
 
@@ -273,7 +273,7 @@ def test_orthogonalize_zeros_and_bad_values(engine, kind):
 # --- the optimiser step ------------------------------------------------------------
 
 @pytest.mark.parametrize('kind,momentum_kind', [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
-@pytest.mark.parametrize('rows,columns', [(1, 1), (20, 128), (128, 20), (128, 128), (33, 515), (640, 256)])
+@pytest.mark.parametrize('rows,columns', [(1, 1), (24, 40), (20, 128), (128, 20), (128, 128), (200, 72), (33, 515), (640, 256)])
 def test_muon(engine, kind, momentum_kind, rows, columns):
     weight, grad = made(50, rows, columns, dtype=kind), update(51, rows, columns, dtype=kind)
     momentum = update(54, rows, columns, dtype=momentum_kind)
@@ -416,6 +416,26 @@ def test_workspace_is_not_read(engine):
         assert status == native.OK
         assert (y[:128] == 7).all() and (y[128 + p * o:] == 7).all()
         assert same_bits(y[128:128 + p * o].view(p, o), operators.linear(engine, x, weight, None, 'tanh')[0])
+
+
+@pytest.mark.parametrize('rows,columns', [(24, 40), (40, 24), (128, 128), (100, 77), (16, 250), (140, 136), (300, 50)])
+def test_orthogonalize_writes_its_own(engine, rows, columns):
+    """The C entry between guards, with a workspace full of NaNs, for one matrix and for three."""
+    lib, coefficients = engine.lib, (ctypes.c_double * 3)(*oracle.QUINTIC)
+    for matrices in (1, 3):
+        x = update(132, matrices, rows, columns)
+        count, size = x.numel(), ctypes.c_size_t()
+        assert lib.cpde_orthogonalize_workspace(0, matrices, rows, columns, ctypes.byref(size)) == native.OK
+        work = torch.full((size.value // 4 + 64,), float('nan'), device='cuda')
+        out = torch.full((count + 256,), 7.0, device='cuda')
+        status = lib.cpde_orthogonalize(engine.handle, 0, x.data_ptr(), matrices, rows, columns, 5, coefficients, 1, 1e-7,
+                                        out[128:].data_ptr(), work.data_ptr(), size.value,
+                                        torch.cuda.current_stream().cuda_stream or 1)
+        assert status == native.OK
+        assert (out[:128] == 7).all() and (out[128 + count:] == 7).all()
+        assert same_bits(out[128:128 + count].view(x.shape), operators.orthogonalize(engine, x))
+        for part, matrix in zip(out[128:128 + count].view(x.shape), x):
+            close(part, matrix, F32)
 
 
 def test_refusals(engine):
