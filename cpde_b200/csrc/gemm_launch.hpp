@@ -56,9 +56,11 @@ inline CUtensorMap operand_map(const Operand& o, int box, bool bf16) {
     return map;
 }
 
-// Which tile a product takes, and into how many parts its contraction is split.
+// Which tile a product takes, into how many parts its contraction is split, and the
+// clocks that it is estimated to take.
 struct GemmPlan {
     int ctas, bn, splits, split_slabs;
+    double clocks;
 };
 
 // The tiles (GemmTile), and the clocks that an MMA of theirs was measured to take in a
@@ -75,60 +77,79 @@ inline int64_t lower_tiles(int64_t tiles_m, int64_t tiles_n, int64_t ratio) {
     return sum;
 }
 
+// Clocks around a tile; those of a launch, and of joining a split contraction besides its
+// partial sums' way through memory.
+constexpr double TILE_CLOCKS = 1500, LAUNCH_CLOCKS = 3000, JOIN_CLOCKS = 5000;
+
+// Takes the tile into `best` if it is estimated to be faster, with its best split.
+inline void consider(GemmPlan& best, int ctas, int bn, double slab, int64_t m, int64_t n, int64_t k, int64_t batches, bool lower,
+                     bool may_split) {
+    const int64_t slabs = (k + GEMM_SLAB - 1) / GEMM_SLAB;
+    const int64_t bm = 128 * ctas, tm = (m + bm - 1) / bm, tn = (n + bn - 1) / bn;
+    const int64_t tiles = (lower ? lower_tiles(tm, tn, bm / bn) : tm * tn) * batches, slots = GEMM_SMS / ctas;
+    const int64_t fill = std::max<int64_t>(1, slots / std::max<int64_t>(tiles, 1));
+    const int64_t most = may_split ? std::min(slabs / 2, 4 * fill) : 1;
+    for (int64_t want : {int64_t(1), int64_t(2), int64_t(3), int64_t(4), int64_t(6), int64_t(8), fill, 2 * fill}) {
+        if (want > 1 && want > most) continue;
+        const int64_t each = (slabs + want - 1) / want, splits = (slabs + each - 1) / each;
+        double time = double((tiles * splits + slots - 1) / slots) * (each * slab + TILE_CLOCKS);
+        if (splits > 1) time += JOIN_CLOCKS + double(splits) * m * n * 8 / 4000;
+        if (!best.ctas || time < best.clocks) best = {ctas, bn, int(splits), int(each), time};
+    }
+}
+
 // The choice of the shortest estimate: waves of tiles, a slab at the rate of the MMAs or
-// of what L2 brings (64 bytes a clock an SM), some clocks around each tile, and what
-// splitting costs (its partial sums' way through memory and a launch).
+// of what L2 brings (64 bytes a clock an SM).
 template <int P>
 GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, int64_t batches, bool lower, bool may_split) {
-    const int64_t slabs = (k + GEMM_SLAB - 1) / GEMM_SLAB;
     GemmPlan best = {};
-    double least = 1e300;
     for (const GemmChoice& c : GEMM_CHOICES) {
-        const int64_t bm = 128 * c.ctas, tm = (m + bm - 1) / bm, tn = (n + c.bn - 1) / c.bn;
-        const int64_t tiles = (lower ? lower_tiles(tm, tn, bm / c.bn) : tm * tn) * batches, slots = GEMM_SMS / c.ctas;
-        const double bytes = P * (128 + c.bn / c.ctas) * 128.0, clocks = PRODUCTS<P> * 4 * c.clocks;
-        const double slab = std::max(clocks, bytes / 64);
-        const int64_t fill = std::max<int64_t>(1, slots / std::max<int64_t>(tiles, 1));
-        const int64_t most = may_split ? std::min(slabs / 2, 4 * fill) : 1;
-        for (int64_t want : {int64_t(1), int64_t(2), int64_t(3), int64_t(4), int64_t(6), int64_t(8), fill, 2 * fill}) {
-            if (want > 1 && want > most) continue;
-            const int64_t each = (slabs + want - 1) / want, splits = (slabs + each - 1) / each;
-            double time = double((tiles * splits + slots - 1) / slots) * (each * slab + 1500);
-            if (splits > 1) time += 5000 + double(splits) * m * n * 8 / 4000;
-            if (time < least) least = time, best = {c.ctas, c.bn, int(splits), int(each)};
-        }
+        const double bytes = P * (128 + c.bn / c.ctas) * 128.0;
+        consider(best, c.ctas, c.bn, std::max(PRODUCTS<P> * 4.0 * c.clocks, bytes / 64), m, n, k, batches, lower, may_split);
     }
     return best;
+}
+
+inline GemmShape gemm_shape(int64_t m, int64_t n, int64_t k, int64_t batches, int bm, int bn, bool lower, const GemmPlan& plan) {
+    GemmShape s = {};
+    s.m = int(m), s.n = int(n);
+    s.slabs = int((k + GEMM_SLAB - 1) / GEMM_SLAB);
+    s.splits = plan.splits, s.split_slabs = plan.split_slabs;
+    s.tiles_m = int((m + bm - 1) / bm), s.tiles_n = int((n + bn - 1) / bn);
+    s.tiles = int(lower ? lower_tiles(s.tiles_m, s.tiles_n, bm / bn) : int64_t(s.tiles_m) * s.tiles_n);
+    s.batches = int(batches);
+    s.lower = lower;
+    return s;
+}
+inline uint32_t mma_instruction(int m, int n, bool a_rows, bool b_rows, bool bf16) {
+    const uint32_t kind = bf16 ? 1 : 0;
+    return 1u << 4 | kind << 7 | kind << 10 | uint32_t(a_rows) << 15 | uint32_t(b_rows) << 16 | uint32_t(n >> 3) << 17 |
+           uint32_t(m >> 4) << 24;
+}
+// Raises the kernel's limit of shared memory, once a device.
+template <class K>
+void allow_shared(K kernel, int bytes, std::atomic<uint64_t>& ready) {
+    int device = 0;
+    CPDE_CUDA(cudaGetDevice(&device));
+    if (ready.load() >> (device & 63) & 1) return;
+    CPDE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(uint64_t(1) << (device & 63));
 }
 
 template <class C, class E>
 void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k, int64_t batches, bool bf16, bool lower,
                  const GemmPlan& plan, const E& epilogue, int* error, cudaStream_t stream) {
-    GemmShape s = {};
-    s.m = int(m), s.n = int(n);
-    s.slabs = int((k + GEMM_SLAB - 1) / GEMM_SLAB);
-    s.splits = plan.splits, s.split_slabs = plan.split_slabs;
-    s.tiles_m = int((m + C::BM - 1) / C::BM), s.tiles_n = int((n + C::BN - 1) / C::BN);
-    s.tiles = int(lower ? lower_tiles(s.tiles_m, s.tiles_n, C::BM / C::BN) : int64_t(s.tiles_m) * s.tiles_n);
-    s.batches = int(batches);
+    GemmShape s = gemm_shape(m, n, k, batches, C::BM, C::BN, lower, plan);
     s.a_planes = a.each, s.b_planes = b.each;
-    s.lower = lower;
     // A single tile of few rows loads no more of them than there are; what the other
     // lanes compute from old bytes is never read.
     const bool few = !C::A_ROWS && C::CTAS == 1 && m < GEMM_ROWS;
     const int a_box = C::A_ROWS ? 64 : few ? int((m + 7) / 8 * 8) : GEMM_ROWS;
     const int b_box = C::B_ROWS ? 64 : C::B_PART;
     s.stage_bytes = uint32_t(C::CTAS * ((few ? a_box * 128 : C::A_BYTES) + C::B_BYTES));
-    const uint32_t kind = bf16 ? 1 : 0;
-    s.instruction = 1u << 4 | kind << 7 | kind << 10 | uint32_t(C::A_ROWS) << 15 | uint32_t(C::B_ROWS) << 16 |
-                    uint32_t(C::BN >> 3) << 17 | uint32_t(C::BM >> 4) << 24;
-    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limit is raised
-    int device = 0;
-    CPDE_CUDA(cudaGetDevice(&device));
-    if (!(ready.load() >> (device & 63) & 1)) {
-        CPDE_CUDA(cudaFuncSetAttribute(k_gemm<C, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHARED));
-        ready.fetch_or(uint64_t(1) << (device & 63));
-    }
+    s.instruction = mma_instruction(C::BM, C::BN, C::A_ROWS, C::B_ROWS, bf16);
+    static std::atomic<uint64_t> ready{0};
+    allow_shared(k_gemm<C, E>, C::SHARED, ready);
     const int64_t items = int64_t(s.tiles) * s.splits * s.batches;
     const int clusters = int(std::min<int64_t>(items, GEMM_SMS / C::CTAS));
     launch_early(k_gemm<C, E>, dim3(clusters * C::CTAS), C::THREADS, C::SHARED, C::CTAS, stream, operand_map(a, a_box, bf16),

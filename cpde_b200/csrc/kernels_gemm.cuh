@@ -45,27 +45,31 @@ struct GemmShape {
 };
 
 // What a CTA holds. A_ROWS and B_ROWS: the contraction runs over the rows of the operand's array.
-template <int CTAS_, int BN_, int P_, bool A_ROWS_, bool B_ROWS_>
+// RESIDENT: the whole of B stays in shared memory, HELD parts of slabs at most.
+template <int CTAS_, int BN_, int P_, bool A_ROWS_, bool B_ROWS_, bool RESIDENT_ = false>
 struct GemmTile {
     static constexpr int CTAS = CTAS_, BN = BN_, P = P_;
-    static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_;
+    static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, RESIDENT = RESIDENT_;
     static constexpr int BM = GEMM_ROWS * CTAS;
     static constexpr int B_PART = BN / CTAS;  // columns of the tile whose operand this CTA loads
     static constexpr int A_BYTES = GEMM_ROWS * 128, B_BYTES = B_PART * 128;
-    static constexpr int STAGE = A_BYTES + B_BYTES;  // one part of a slab of both operands
+    static constexpr int HELD = RESIDENT ? 6 : 0;
+    static constexpr int STAGE = A_BYTES + (RESIDENT ? 0 : B_BYTES);  // one part of a slab of both operands
     // Of the epilogue. Its loads, conversions and stores are long chains, of which a
     // scheduler needs two warps' at least: four warps took twice the time.
-    static constexpr int WARPS = 8;
+    static constexpr int WARPS = RESIDENT ? 4 : 8;
     // Slabs that are summed in the accumulator before it is taken out. The way from the
     // last MMA to the epilogue and back takes 1.4 us a slab with two CTAs of 256 columns:
     // less than the six products of three parts (1.7), more than the three of two (0.83).
-    static constexpr int UNIT = P == 1 ? 1 << 30 : P == 2 ? 2 : 1;
+    // A resident B's few slabs are one unit, whose large products come last.
+    static constexpr bool WHOLE = P == 1 || RESIDENT;
+    static constexpr int UNIT = WHOLE ? 1 << 30 : P == 2 ? 2 : 1;
     static constexpr int COLUMNS = BN / (WARPS / 4);  // of an epilogue warp
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int PIECES = WARPS * 32 * GEMM_STRIDE * 4;
-    static constexpr int ROOM = (227 * 1024 - 1024 - 256 - PIECES) / STAGE;
+    static constexpr int ROOM = (227 * 1024 - 1024 - 256 - PIECES - HELD * B_BYTES) / STAGE;
     static constexpr int STAGES = ROOM > 12 ? 12 : ROOM;
-    static constexpr int SHARED = 1024 + STAGES * STAGE + PIECES + 256;
+    static constexpr int SHARED = 1024 + STAGES * STAGE + HELD * B_BYTES + PIECES + 256;
     static constexpr uint32_t TMEM = BN * 2 <= 32 ? 32 : BN * 2 <= 64 ? 64 : BN * 2 <= 128 ? 128 : BN * 2 <= 256 ? 256 : 512;
     static_assert(STAGES > P && BN * 2 <= 512 && BN % 32 == 0 && COLUMNS % GEMM_PIECE == 0);
     static_assert(!B_ROWS || B_PART % 64 == 0, "boxes of rows are 64 columns wide");
@@ -220,15 +224,17 @@ template <class C>
 struct Shared {
     uint8_t* stages;
     float* pieces;
-    uint64_t *full, *empty, *ready, *taken;  // of the stages; of the two accumulators
+    uint64_t *full, *empty, *ready, *taken, *held;  // of the stages; of the two accumulators; of a resident B
     volatile int* abort;
     uint32_t* slot;
     __device__ explicit Shared(uint8_t* raw) {
         stages = raw + (1024 - (tc::smem_u32(raw) & 1023)) % 1024;
-        pieces = reinterpret_cast<float*>(stages + C::STAGES * C::STAGE);
-        full = reinterpret_cast<uint64_t*>(stages + C::STAGES * C::STAGE + C::PIECES);
+        uint8_t* behind = stages + C::STAGES * C::STAGE + C::HELD * C::B_BYTES;
+        pieces = reinterpret_cast<float*>(behind);
+        full = reinterpret_cast<uint64_t*>(behind + C::PIECES);
         empty = full + 12, ready = empty + 12, taken = ready + 2;
-        slot = reinterpret_cast<uint32_t*>(taken + 2);
+        held = taken + 2;
+        slot = reinterpret_cast<uint32_t*>(held + 1);
         abort = reinterpret_cast<volatile int*>(slot + 1);
     }
 };
@@ -299,6 +305,196 @@ struct Sixteen {
         for (int i = 0; i < COUNT; ++i) store_wide(reinterpret_cast<char*>(p) + 32 * i, w[i]);
     }
 };
+
+namespace gemm {
+
+// The MMAs of this cluster's work, by the one thread that calls this.
+template <class C>
+__device__ __forceinline__ void issue(const Shared<C>& sh, const GemmShape& s, uint32_t tmem, int first, int stride, int64_t items) {
+    const uint32_t stages = tc::smem_u32(sh.stages), held = stages + C::STAGES * C::STAGE;
+    if (C::RESIDENT && !wait_for(sh.held, 0, sh.abort)) return;
+    int st = 0;
+    uint32_t parity = 0, unit = 0;
+    int waiting = 0;  // the first part's stage of a resident unit's slab before
+    bool ok = true;
+    for (int64_t at = first; ok && at < items; at += stride) {
+        const Work w = work_at<C>(s, at);
+        for (int slab = w.from; ok && slab < w.to; ++slab) {
+            const int in = (slab - w.from) % C::UNIT;
+            const bool begins = in == 0, ends = in == C::UNIT - 1 || slab + 1 == w.to;
+            const uint32_t d = tmem + (unit & 1) * C::BN;
+            if (begins) ok = wait_for(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, sh.abort);
+            // The slab's stages, by part.
+            int stage[C::P];
+            uint32_t round[C::P];
+#pragma unroll
+            for (int p = C::P - 1; p >= 0; --p) {
+                stage[p] = st, round[p] = parity;
+                if (++st == C::STAGES) st = 0, parity ^= 1;
+            }
+            auto there = [&](int p) { ok = ok && wait_for(sh.full + stage[p], round[p], sh.abort); };
+            auto multiply_at = [&](int a_stage, uint32_t b_at, bool accumulate) {
+                const uint64_t a = descriptor<C::A_ROWS>(stages + a_stage * C::STAGE), b = descriptor<C::B_ROWS>(b_at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mma<C::CTAS>(d, a + k * (STEP<C::A_ROWS> >> 4), b + k * (STEP<C::B_ROWS> >> 4), s.instruction,
+                                 accumulate || k > 0);
+            };
+            auto multiply = [&](int pa, int pb, bool accumulate) {
+                multiply_at(stage[pa], C::RESIDENT ? held + (slab * C::P + pb) * C::B_BYTES : stages + stage[pb] * C::STAGE + C::A_BYTES,
+                            accumulate);
+            };
+            there(0);
+            if constexpr (C::P > 1) there(C::P - 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+            if constexpr (C::P == 3) {
+                multiply(2, 0, !begins);
+                multiply(0, 2, true);
+                commit<C::CTAS>(sh.empty + stage[2]);
+                there(1);
+                if (!ok) break;
+                tc::tc_fence_after();
+                multiply(1, 1, true);
+                multiply(1, 0, true);
+                multiply(0, 1, true);
+                commit<C::CTAS>(sh.empty + stage[1]);
+            } else if constexpr (C::P == 2) {
+                multiply(1, 0, !begins);
+                multiply(0, 1, true);
+                commit<C::CTAS>(sh.empty + stage[1]);
+            }
+            if constexpr (C::RESIDENT && C::P > 1) {
+                // Sums are cut toward zero at their size: the large products of a unit, of
+                // two slabs at most, follow when all of the small ones are in.
+                if (!ends) {
+                    waiting = stage[0];
+                    continue;
+                }
+                if (!begins) {
+                    multiply_at(waiting, held + (slab - 1) * C::P * C::B_BYTES, true);
+                    commit<C::CTAS>(sh.empty + waiting);
+                }
+            }
+            multiply(0, 0, C::P > 1 || !begins);
+            commit<C::CTAS>(sh.empty + stage[0]);
+            if (ends) commit<C::CTAS>(sh.ready + (unit & 1)), ++unit;
+        }
+    }
+}
+
+// The accumulators' way out, by epilogue warp e whose lanes are those of `quarter`.
+template <class C, class E>
+__device__ __forceinline__ void finish(const Shared<C>& sh, const GemmShape& s, const E& epilogue, uint32_t tmem, int e, int quarter,
+                                       uint32_t rank, int first, int stride, int64_t items) {
+    const int lane = threadIdx.x % 32, c0 = e / 4 * C::COLUMNS;
+    float* piece = sh.pieces + e * 32 * GEMM_STRIDE;
+    uint32_t unit = 0;
+    // Waits for an accumulator, one lane for all; false where a role gave up.
+    auto wait = [&] {
+        const bool ok = lane || wait_for(sh.ready + (unit & 1), (unit >> 1) & 1, sh.abort);
+        const bool all = __all_sync(~0u, ok);
+        tc::tc_fence_after();
+        return all;
+    };
+    auto taken = [&] {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            if constexpr (C::CTAS == 2) arrive_at(at_rank(sh.taken + (unit & 1), 0));
+            else tc::mbar_arrive(sh.taken + (unit & 1));
+        }
+        ++unit;
+    };
+    // What a piece needs beside D, read ahead.
+    struct Ahead {
+        typename E::Fetched half[2];
+    };
+    auto fetch = [&](Ahead& got, int row, int column, const Work& w) {
+        if (!epilogue.whole || row + lane >= s.m) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (column + 16 * h < s.n) epilogue.fetch(got.half[h], row + lane, column + 16 * h, w.batch, s);
+    };
+    auto put = [&](float (&v)[32], const Ahead& got, int row, int column, const Work& w) {
+        if (row >= s.m || column >= s.n) return;
+        if (epilogue.whole) {
+            if (row + lane >= s.m) return;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (column + 16 * h < s.n)
+                    epilogue.half(*reinterpret_cast<float(*)[16]>(v + 16 * h), got.half[h], row + lane, column + 16 * h, w.batch,
+                                  w.split, C::BM, C::BN, s);
+            return;
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) piece[lane * GEMM_STRIDE + i] = v[8 * h + i];
+            __syncwarp();
+            const int c = column + 8 * h + lane % 8;
+            if (c >= s.n) continue;
+#pragma unroll 4
+            for (int r = lane / 8; r < 32; r += 4)
+                if (row + r < s.m) epilogue.one(piece[r * GEMM_STRIDE + lane % 8], row + r, c, w.batch, w.split, s);
+        }
+    };
+    bool ok = true;
+    for (int64_t at = first; ok && at < items; at += stride) {
+        const Work w = work_at<C>(s, at);
+        const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column = w.tile_n * C::BN + c0;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + c0;
+        if constexpr (C::WHOLE) {
+            Ahead got;
+            fetch(got, row, column, w);
+            if (!(ok = wait())) break;
+            const uint32_t from = lanes + (unit & 1) * C::BN;
+#pragma unroll 1
+            for (int c = 0; c < C::COLUMNS; c += 32) {
+                float v[32];
+                tmem_piece(from + c, v);
+                const Ahead now = got;
+                if (c + 32 == C::COLUMNS) taken();
+                else fetch(got, row, column + c + 32, w);
+                put(v, now, row, column + c, w);
+            }
+        } else {
+            float sum[C::COLUMNS / 32][32] = {};
+            for (int slab = w.from; ok && slab < w.to; slab += C::UNIT) {
+                if (!(ok = wait())) break;
+#pragma unroll
+                for (int c = 0; c < C::COLUMNS / 16; ++c) {  // few registers at a time: the sums take most of them
+                    float v[16];
+                    tc::tmem_read<16>(lanes + (unit & 1) * C::BN + 16 * c, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[c / 2][c % 2 * 16 + i] += v[i];
+                }
+                taken();
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < C::COLUMNS / 32; ++c) {
+                if (!epilogue.whole) {
+                    put(sum[c], {}, row, column + 32 * c, w);
+                    continue;
+                }
+                if (row + lane >= s.m) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // as in put, without reading ahead, for which there are no registers
+                    const int at_column = column + 32 * c + 16 * h;
+                    if (at_column >= s.n) continue;
+                    typename E::Fetched got;
+                    epilogue.fetch(got, row + lane, at_column, w.batch, s);
+                    epilogue.half(*reinterpret_cast<float(*)[16]>(sum[c] + 16 * h), got, row + lane, at_column, w.batch, w.split,
+                                  C::BM, C::BN, s);
+                }
+            }
+        }
+    }
+}
+
+}  // namespace gemm
 
 // The epilogue E gets a tile in pieces of 32 rows and 32 columns. Where its arrays have
 // rows of whole 32 bytes (`whole`), a thread keeps the row of its lane: `fetch` reads what
@@ -381,167 +577,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (rank == 0 && elected()) {
-            const uint32_t stages = tc::smem_u32(sh.stages);
-            int st = 0;
-            uint32_t parity = 0, unit = 0;
-            bool ok = true;
-            for (int64_t at = first; ok && at < items; at += stride) {
-                const Work w = work_at<C>(s, at);
-                for (int slab = w.from; ok && slab < w.to; ++slab) {
-                    const bool begins = (slab - w.from) % C::UNIT == 0, ends = (slab - w.from) % C::UNIT == C::UNIT - 1 || slab + 1 == w.to;
-                    const uint32_t d = tmem + (unit & 1) * C::BN;
-                    if (begins) ok = wait_for(sh.taken + (unit & 1), ((unit >> 1) & 1) ^ 1, sh.abort);
-                    // The slab's stages, by part.
-                    int stage[C::P];
-                    uint32_t round[C::P];
-#pragma unroll
-                    for (int p = C::P - 1; p >= 0; --p) {
-                        stage[p] = st, round[p] = parity;
-                        if (++st == C::STAGES) st = 0, parity ^= 1;
-                    }
-                    auto there = [&](int p) { ok = ok && wait_for(sh.full + stage[p], round[p], sh.abort); };
-                    auto multiply = [&](int pa, int pb, bool first_of_all) {
-                        const uint64_t a = descriptor<C::A_ROWS>(stages + stage[pa] * C::STAGE);
-                        const uint64_t b = descriptor<C::B_ROWS>(stages + stage[pb] * C::STAGE + C::A_BYTES);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<C::CTAS>(d, a + k * (STEP<C::A_ROWS> >> 4), b + k * (STEP<C::B_ROWS> >> 4), s.instruction,
-                                         !(first_of_all && k == 0));
-                    };
-                    there(0);
-                    if constexpr (C::P > 1) there(C::P - 1);
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    if constexpr (C::P == 3) {
-                        multiply(2, 0, begins);
-                        multiply(0, 2, false);
-                        commit<C::CTAS>(sh.empty + stage[2]);
-                        there(1);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        multiply(1, 1, false);
-                        multiply(1, 0, false);
-                        multiply(0, 1, false);
-                        commit<C::CTAS>(sh.empty + stage[1]);
-                    } else if constexpr (C::P == 2) {
-                        multiply(1, 0, begins);
-                        multiply(0, 1, false);
-                        commit<C::CTAS>(sh.empty + stage[1]);
-                    }
-                    multiply(0, 0, C::P == 1 && begins);
-                    commit<C::CTAS>(sh.empty + stage[0]);
-                    if (ends) commit<C::CTAS>(sh.ready + (unit & 1)), ++unit;
-                }
-            }
-        }
+        if (rank == 0 && elected()) issue<C>(sh, s, tmem, first, stride, items);
     } else {
-        const int e = warp - 2, quarter = warp % 4;  // the lanes that a warp may read
-        const int c0 = e / 4 * C::COLUMNS;
-        float* piece = sh.pieces + e * 32 * GEMM_STRIDE;
-        uint32_t unit = 0;
-        // Waits for an accumulator, one lane for all; false where a role gave up.
-        auto wait = [&] {
-            const bool ok = lane || wait_for(sh.ready + (unit & 1), (unit >> 1) & 1, sh.abort);
-            const bool all = __all_sync(~0u, ok);
-            tc::tc_fence_after();
-            return all;
-        };
-        auto taken = [&] {
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (C::CTAS == 2) arrive_at(at_rank(sh.taken + (unit & 1), 0));
-                else tc::mbar_arrive(sh.taken + (unit & 1));
-            }
-            ++unit;
-        };
-        // What a piece needs beside D, read ahead.
-        struct Ahead {
-            typename E::Fetched half[2];
-        };
-        auto fetch = [&](Ahead& got, int row, int column, const Work& w) {
-            if (!epilogue.whole || row + lane >= s.m) return;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (column + 16 * h < s.n) epilogue.fetch(got.half[h], row + lane, column + 16 * h, w.batch, s);
-        };
-        auto put = [&](float (&v)[32], const Ahead& got, int row, int column, const Work& w) {
-            if (row >= s.m || column >= s.n) return;
-            if (epilogue.whole) {
-                if (row + lane >= s.m) return;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (column + 16 * h < s.n)
-                        epilogue.half(*reinterpret_cast<float(*)[16]>(v + 16 * h), got.half[h], row + lane, column + 16 * h,
-                                      w.batch, w.split, C::BM, C::BN, s);
-                return;
-            }
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) piece[lane * GEMM_STRIDE + i] = v[8 * h + i];
-                __syncwarp();
-                const int c = column + 8 * h + lane % 8;
-                if (c >= s.n) continue;
-#pragma unroll 4
-                for (int r = lane / 8; r < 32; r += 4)
-                    if (row + r < s.m) epilogue.one(piece[r * GEMM_STRIDE + lane % 8], row + r, c, w.batch, w.split, s);
-            }
-        };
-        bool ok = true;
-        for (int64_t at = first; ok && at < items; at += stride) {
-            const Work w = work_at<C>(s, at);
-            const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column = w.tile_n * C::BN + c0;
-            const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + c0;
-            if constexpr (C::P == 1) {
-                Ahead got;
-                fetch(got, row, column, w);
-                if (!(ok = wait())) break;
-                const uint32_t from = lanes + (unit & 1) * C::BN;
-#pragma unroll 1
-                for (int c = 0; c < C::COLUMNS; c += 32) {
-                    float v[32];
-                    tmem_piece(from + c, v);
-                    const Ahead now = got;
-                    if (c + 32 == C::COLUMNS) taken();
-                    else fetch(got, row, column + c + 32, w);
-                    put(v, now, row, column + c, w);
-                }
-            } else {
-                float sum[C::COLUMNS / 32][32] = {};
-                for (int slab = w.from; ok && slab < w.to; slab += C::UNIT) {
-                    if (!(ok = wait())) break;
-#pragma unroll
-                    for (int c = 0; c < C::COLUMNS / 32; ++c) {
-                        float v[32];
-                        tmem_piece(lanes + (unit & 1) * C::BN + 32 * c, v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) sum[c][i] += v[i];
-                    }
-                    taken();
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int c = 0; c < C::COLUMNS / 32; ++c) {
-                    if (epilogue.whole) {  // as in put, without reading ahead, for which there are no registers
-                        if (row + lane >= s.m) continue;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int at_column = column + 32 * c + 16 * h;
-                            if (at_column >= s.n) continue;
-                            typename E::Fetched got;
-                            epilogue.fetch(got, row + lane, at_column, w.batch, s);
-                            epilogue.half(*reinterpret_cast<float(*)[16]>(sum[c] + 16 * h), got, row + lane, at_column, w.batch,
-                                          w.split, C::BM, C::BN, s);
-                        }
-                    } else {
-                        put(sum[c], {}, row, column + 32 * c, w);
-                    }
-                }
-            }
-        }
+        finish<C>(sh, s, epilogue, tmem, warp - 2, warp % 4, rank, first, stride, items);
     }
     tc::tc_fence_before();
     __syncwarp();

@@ -1,10 +1,10 @@
 // Linear layers: what stands before and behind the matrix products of
-// kernels_gemm.cuh.
+// kernels_gemm.cuh and kernels_gather.cuh.
 //
 // z = x W' + b, y = r + act(z); from dy: dz = dy act'(z), dx = dz W, dW = dz' x,
 // db = sum of dz over the points.
 #pragma once
-#include "kernels_gemm.cuh"
+#include "kernels_gather.cuh"
 
 namespace cpde::ops {
 
@@ -125,26 +125,34 @@ struct LinearEpilogue {
     }
 };
 
-// Joins the partial sums of a split contraction, in the order of the splits, and ends
-// them as the epilogue does.
+// Joins the partial sums of a split contraction and ends them as the epilogue does. A
+// result's splits are shared by `share` neighbouring threads (1 or 8), each of which adds
+// every share-th in order; their sums are added in order too.
 template <class T, int V>
-__global__ void __launch_bounds__(256) k_join(LinearEpilogue<T> epilogue, GemmShape s) {
+__global__ void __launch_bounds__(256) k_join(LinearEpilogue<T> epilogue, GemmShape s, int32_t share) {
+    next_launch_may_begin();
     after_previous_launch();
     const float* partial = epilogue.partial;
     epilogue.partial = nullptr;
     const int64_t pitch = LinearEpilogue<T>::partial_pitch(s), across = (s.n + V - 1) / V, all = s.m * across;
-    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < all; i += gridDim.x * int64_t(256)) {
-        const int64_t row = i / across;
-        const int column = int(i % across) * V;
+    const int mine = threadIdx.x % share;
+    // Whole warps go round together.
+    const int64_t step = gridDim.x * int64_t(256 / share);
+    for (int64_t begin = blockIdx.x * int64_t(256 / share); begin < all; begin += step) {
+        const int64_t i = begin + threadIdx.x / share, row = min(i, all - 1) / across;
+        const int column = int(min(i, all - 1) % across) * V;
         float sum[V] = {};
 #pragma unroll 8
-        for (int split = 0; split < s.splits; ++split) {
+        for (int split = mine; split < s.splits; split += share) {
             float v[V];
             load_some<float, V>(partial + (split * int64_t(s.m) + row) * pitch + column, v, V, true);
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += v[j];
         }
-        epilogue.template some<V>(sum, row, column, s);
+        for (int o = 1; o < share; o *= 2)
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += __shfl_xor_sync(~0u, sum[j], o);
+        if (mine == 0 && i < all) epilogue.template some<V>(sum, row, column, s);
     }
 }
 
@@ -162,20 +170,6 @@ struct PartsCall {
     int32_t lanes;     // threads of a row, eight columns each: a power of two up to 32
     bool whole;        // x and z can be read in eights
 };
-
-// T's parts: FP32 as three BF16, what each leaves going to the next (24 bits, all
-// exponents); the 16-bit types as they are.
-template <class T> struct Parts { using type = T; static constexpr int count = 1; };
-template <> struct Parts<float> { using type = __nv_bfloat16; static constexpr int count = 3; };
-
-// The part of v, and in v the rest. A value that rounds to infinity is cut to the
-// largest finite one, and an infinity's rest is nothing.
-__device__ __forceinline__ float next_part(float& v) {
-    float h = __bfloat162float(__float2bfloat16_rn(v));
-    if (!finite(h) && finite(v)) h = copysignf(__uint_as_float(0x7f7f0000u), v);
-    v = finite(h) ? v - h : 0.0f;
-    return h;
-}
 
 template <class T>
 __global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
@@ -205,17 +199,10 @@ __global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
             for (int i = 0; i < 8; ++i) sum[i] += v[i];
             if (c.out) {
                 O* out = static_cast<O*>(c.out) + row * c.pitch + column;
-                if constexpr (Parts<T>::count == 1) {
-                    store<O, 8>(out, pack<O, 8>(v));
-                } else {
+                uint4 part[Parts<T>::count];
+                split_eight<T>(v, part);
 #pragma unroll
-                    for (int p = 0; p < Parts<T>::count; ++p, out += c.rows * c.pitch) {
-                        float h[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) h[i] = next_part(v[i]);
-                        store<O, 8>(out, pack<O, 8>(h));
-                    }
-                }
+                for (int p = 0; p < Parts<T>::count; ++p, out += c.rows * c.pitch) *reinterpret_cast<uint4*>(out) = part[p];
             }
         }
     }
@@ -233,23 +220,24 @@ __global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
     }
 }
 
-// Column sums over the chunks: 32 columns a block, whose eight warps take every eighth chunk.
+// Column sums over the chunks: 32 columns a block, whose 32 warps take every 32nd chunk.
 template <class O>
-__global__ void __launch_bounds__(256) k_column_sums(const float* sums, int32_t chunks, int32_t columns, O* out) {
-    __shared__ float shared[8][32];
+__global__ void __launch_bounds__(1024) k_column_sums(const float* sums, int32_t chunks, int32_t columns, O* out) {
+    __shared__ float shared[32][33];
+    next_launch_may_begin();
     after_previous_launch();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = blockIdx.x * 32 + lane;
     float sum = 0.0f;
     if (column < columns) {
 #pragma unroll 8
-        for (int i = warp; i < chunks; i += 8) sum += sums[i * int64_t(columns) + column];
+        for (int i = warp; i < chunks; i += 32) sum += sums[i * int64_t(columns) + column];
     }
     shared[warp][lane] = sum;
     __syncthreads();
-    if (warp || column >= columns) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) sum += shared[i][lane];
-    out[column] = from_float<O>(sum);
+    // Warp w adds the 32 sums of column w.
+    sum = shared[lane][warp];
+    for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0 && blockIdx.x * 32 + warp < columns) out[blockIdx.x * 32 + warp] = from_float<O>(sum);
 }
 
 }  // namespace cpde::ops

@@ -69,23 +69,101 @@ Operand staged(const T* x, int64_t stride, const T* z, int64_t z_stride, int32_t
     return {out, c.pitch, rows, columns, Parts<T>::count, rows * c.pitch, Parts<T>::count};
 }
 
-template <class T, bool A_ROWS, bool B_ROWS>
-void product(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k, const GemmPlan& plan,
-             LinearEpilogue<T> epilogue, float* partial, int* error, cudaStream_t stream) {
+template <class T>
+Source<T> source(const T* p, int64_t stride, int64_t rows, int64_t columns) {
+    int width = 8;
+    while (width > 1 && !(aligned(p, std::min<int64_t>(width * sizeof(T), 16)) && (rows == 1 || stride % width == 0))) width /= 2;
+    return {p, stride, rows, int32_t(columns), width};
+}
+
+// How a product is computed: on operands that TMA reads, `a_made` and `b_made` being made
+// for it, or gathered from the arrays in one launch.
+struct Route {
+    GemmPlan plan;
+    bool gather;
+};
+// An operand: whether TMA reads it, or parts of it exist already, and what it takes to make them.
+struct Side {
+    bool there;
+    int64_t elements;
+    int width;
+};
+template <class T>
+Route route(int64_t m, int64_t n, int64_t k, const Side& a, const Side& b) {
     constexpr int P = Parts<T>::count;
-    constexpr bool bf16 = !std::is_same_v<T, __half>;
-    // Partial sums have whole rows, whatever the result's are.
-    if (plan.splits > 1) epilogue.partial = partial, epilogue.whole = true;
-    with_tile<P, A_ROWS, B_ROWS>(plan, [&](auto tile) {
-        launch_gemm<decltype(tile)>(a, b, m, n, k, 1, bf16, false, plan, epilogue, error, stream);
-    });
+    Route r = {gemm_plan<P>(m, n, k, 1, false, true), false};
+    if (a.there && b.there) return r;
+    // Parts: read and written at about 2000 bytes a clock, and a launch.
+    double made = r.plan.clocks;
+    for (const Side* s : {&a, &b})
+        if (!s->there) made += LAUNCH_CLOCKS + double(s->elements) * (sizeof(T) + 2 * P) / 2000;
+    // Gathered, where B's parts stay in shared memory or there is one part.
+    const bool resident = n <= 128 && P * ((k + GEMM_SLAB - 1) / GEMM_SLAB) <= GemmTile<1, 128, P, false, false, true>::HELD;
+    if (P > 1 && !resident) return r;
+    const int width = std::min(a.width, b.width);
+    const double slab = P > 1 ? 1500 : width == 8 ? 500 : width == 4 ? 1000 : width == 2 ? 1200 : 2000;
+    GemmPlan gathered = {};
+    consider(gathered, 1, 128, slab, m, n, k, 1, false, P == 1);
+    if (gathered.clocks < made) r = {gathered, true};
+    return r;
+}
+
+size_t partial_count(const GemmPlan& plan, int64_t m, int64_t n) {
+    return plan.splits > 1 ? size_t(plan.splits) * m * ((n + 15) / 16 * 16) : 0;
+}
+
+template <class T>
+void join(const GemmPlan& plan, int64_t m, int64_t n, const LinearEpilogue<T>& epilogue, cudaStream_t stream) {
     if (plan.splits == 1) return;
     GemmShape s = {};
     s.m = int(m), s.n = int(n), s.splits = plan.splits;
     const int64_t threads = m * (epilogue.fours ? n / 4 : n);
-    const dim3 grid(unsigned(std::min<int64_t>((threads + 255) / 256, GEMM_SMS * 8)));
-    if (epilogue.fours) launch_early(k_join<T, 4>, grid, 256, 0, 1, stream, epilogue, s);
-    else launch_early(k_join<T, 1>, grid, 256, 0, 1, stream, epilogue, s);
+    // Few results of many splits: a warp's threads share the splits of one.
+    const int share = plan.splits >= 16 && threads <= GEMM_SMS * 256 ? 8 : 1;
+    const dim3 grid(unsigned(std::min<int64_t>((threads * share + 255) / 256, GEMM_SMS * 8)));
+    if (epilogue.fours) launch_early(k_join<T, 4>, grid, 256, 0, 1, stream, epilogue, s, share);
+    else launch_early(k_join<T, 1>, grid, 256, 0, 1, stream, epilogue, s, share);
+}
+
+// Partial sums have whole rows, whatever the result's are.
+template <class T>
+LinearEpilogue<T> split_epilogue(const GemmPlan& plan, LinearEpilogue<T> epilogue, float* partial) {
+    if (plan.splits > 1) epilogue.partial = partial, epilogue.whole = true;
+    return epilogue;
+}
+
+template <class T, bool A_ROWS, bool B_ROWS>
+void product(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k, const GemmPlan& plan,
+             const LinearEpilogue<T>& epilogue, float* partial, int* error, cudaStream_t stream) {
+    constexpr int P = Parts<T>::count;
+    constexpr bool bf16 = !std::is_same_v<T, __half>;
+    const LinearEpilogue<T> e = split_epilogue(plan, epilogue, partial);
+    with_tile<P, A_ROWS, B_ROWS>(plan, [&](auto tile) {
+        launch_gemm<decltype(tile)>(a, b, m, n, k, 1, bf16, false, plan, e, error, stream);
+    });
+    join(plan, m, n, e, stream);
+}
+
+template <class C, class T>
+void launch_gather(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n, int64_t k, const GemmPlan& plan,
+                   const LinearEpilogue<T>& epilogue, int* error, cudaStream_t stream) {
+    constexpr bool bf16 = !std::is_same_v<T, __half>;
+    GemmShape s = gemm_shape(m, n, k, 1, C::BM, C::BN, false, plan);
+    s.instruction = mma_instruction(C::BM, C::BN, C::A_ROWS, C::B_ROWS, bf16);
+    static std::atomic<uint64_t> ready{0};
+    allow_shared(k_gather<C, T, LinearEpilogue<T>>, C::SHARED, ready);
+    const int64_t items = int64_t(s.tiles) * s.splits;
+    launch_early(k_gather<C, T, LinearEpilogue<T>>, dim3(unsigned(std::min<int64_t>(items, GEMM_SMS))), GATHER_THREADS<C>, C::SHARED, 1,
+                 stream, a, b, s, epilogue, error);
+}
+template <class T, bool A_ROWS, bool B_ROWS>
+void gathered_product(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n, int64_t k, const Route& r,
+                      const LinearEpilogue<T>& epilogue, float* partial, int* error, cudaStream_t stream) {
+    constexpr int P = Parts<T>::count;
+    const LinearEpilogue<T> e = split_epilogue(r.plan, epilogue, partial);
+    if constexpr (P > 1) launch_gather<GemmTile<1, 128, P, A_ROWS, B_ROWS, true>>(a, b, m, n, k, r.plan, e, error, stream);
+    else launch_gather<GemmTile<1, 128, P, A_ROWS, B_ROWS>>(a, b, m, n, k, r.plan, e, error, stream);
+    join(r.plan, m, n, e, stream);
 }
 
 // Whether rows of `n` elements at these addresses take the wide accesses of the epilogue, and those of fours.
@@ -100,87 +178,103 @@ void set_widths(LinearEpilogue<T>& e, int64_t n) {
     e.whole = all(16), e.fours = all(4);
 }
 
-size_t partial_count(const GemmPlan& plan, int64_t m, int64_t n) {
-    return plan.splits > 1 ? size_t(plan.splits) * m * ((n + 15) / 16 * 16) : 0;
-}
-
 template <class T>
 size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool launch) {
-    constexpr int P = Parts<T>::count;
     using O = typename Parts<T>::type;
     Room room = {launch ? static_cast<char*>(c.workspace) : nullptr};
-    const bool x_direct = direct(c.type, c.x, c.x_stride, c.points), w_direct = direct(c.type, c.weight, c.weight_stride, c.outputs);
-    const GemmPlan plan = gemm_plan<P>(c.points, c.outputs, c.inputs, 1, false, true);
-    O* x_parts = x_direct ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
-    O* w_parts = w_direct ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
-    float* partial = room.take<float>(partial_count(plan, c.points, c.outputs));
-    if (!launch) return room.bytes;
     const T *x = static_cast<const T*>(c.x), *w = static_cast<const T*>(c.weight);
-    const Operand a = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
-                               : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
-    const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
-                               : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
+    const Source<T> xs = source(x, c.x_stride, c.points, c.inputs), ws = source(w, c.weight_stride, c.outputs, c.inputs);
+    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
+    const Route r = route<T>(c.points, c.outputs, c.inputs, {x_direct, c.points * c.inputs, xs.width},
+                             {w_direct, c.outputs * c.inputs, ws.width});
+    O* x_parts = x_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
+    O* w_parts = w_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
+    float* partial = room.take<float>(partial_count(r.plan, c.points, c.outputs));
+    if (!launch) return room.bytes;
     LinearEpilogue<T> e = {};
     e.bias = c.bias, e.bias_wide = c.bias_type == F32;
     e.residual = static_cast<const T*>(c.residual), e.residual_stride = c.residual_stride;
     e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
     e.activation = c.activation;
     set_widths(e, c.outputs);
-    product<T, false, false>(a, b, c.points, c.outputs, c.inputs, plan, e, partial, error, stream);
+    if (r.gather) {
+        gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, partial, error, stream);
+        return room.bytes;
+    }
+    const Operand a = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
+                               : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
+    const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
+                               : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
+    product<T, false, false>(a, b, c.points, c.outputs, c.inputs, r.plan, e, partial, error, stream);
     return room.bytes;
 }
 
 template <class T>
 size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream, bool launch) {
-    constexpr int P = Parts<T>::count;
     using O = typename Parts<T>::type;
     Room room = {launch ? static_cast<char*>(c.workspace) : nullptr};
     const bool sloped = c.activation != 1;
-    const bool dz_direct = !sloped && direct(c.type, c.grad, c.grad_stride, c.points);
-    const bool x_direct = !c.dweight || direct(c.type, c.x, c.x_stride, c.points);
-    const bool w_direct = !c.dx || direct(c.type, c.weight, c.weight_stride, c.outputs);
-    const bool products = c.dx || c.dweight;
-    const GemmPlan dx_plan = gemm_plan<P>(c.points, c.inputs, c.outputs, 1, false, true);
-    const GemmPlan dw_plan = gemm_plan<P>(c.outputs, c.inputs, c.points, 1, false, true);
-    O* dz_parts = dz_direct || !products ? nullptr : room.take<O>(parts_count<T>(c.points, c.outputs));
-    O* x_parts = x_direct ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
-    O* w_parts = w_direct ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
-    const int64_t chunks = row_chunks(c.points, c.outputs, row_lanes(c.outputs));
-    float* sums = c.dbias ? room.take<float>(chunks * c.outputs) : nullptr;
-    float* partial = room.take<float>(std::max(c.dx ? partial_count(dx_plan, c.points, c.inputs) : 0,
-                                               c.dweight ? partial_count(dw_plan, c.outputs, c.inputs) : 0));
-    if (!launch) return room.bytes;
     const T *grad = static_cast<const T*>(c.grad), *z = sloped ? static_cast<const T*>(c.z) : nullptr;
     const T *x = static_cast<const T*>(c.x), *w = static_cast<const T*>(c.weight);
+    const bool dz_direct = !sloped && direct(c.type, grad, c.grad_stride, c.points);
+    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
+    // dz is made in the type's parts where the activation has a slope; otherwise it is
+    // grad, which is made into parts only if a product is not gathered.
+    const Source<T> gs = source(grad, c.grad_stride, c.points, c.outputs), xs = source(x, c.x_stride, c.points, c.inputs),
+                    ws = source(w, c.weight_stride, c.outputs, c.inputs);
+    const Side dz_side = {dz_direct, c.points * c.outputs, gs.width};
+    Route dx = {}, dw = {};
+    if (c.dx) dx = route<T>(c.points, c.inputs, c.outputs, dz_side, {w_direct, c.outputs * c.inputs, ws.width});
+    if (c.dweight) dw = route<T>(c.outputs, c.inputs, c.points, dz_side, {x_direct, c.points * c.inputs, xs.width});
+    if (sloped) dx.gather = dw.gather = false;
+    if (c.dx && !dx.gather) dx.plan = gemm_plan<Parts<T>::count>(c.points, c.inputs, c.outputs, 1, false, true);
+    if (c.dweight && !dw.gather) dw.plan = gemm_plan<Parts<T>::count>(c.outputs, c.inputs, c.points, 1, false, true);
+    const bool made = (c.dx && !dx.gather) || (c.dweight && !dw.gather);
+    O* dz_parts = dz_direct || !made ? nullptr : room.take<O>(parts_count<T>(c.points, c.outputs));
+    O* x_parts = x_direct || !c.dweight || dw.gather ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
+    O* w_parts = w_direct || !c.dx || dx.gather ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
+    const int64_t chunks = row_chunks(c.points, c.outputs, row_lanes(c.outputs));
+    float* sums = c.dbias ? room.take<float>(chunks * c.outputs) : nullptr;
+    float* partial = room.take<float>(std::max(c.dx ? partial_count(dx.plan, c.points, c.inputs) : 0,
+                                               c.dweight ? partial_count(dw.plan, c.outputs, c.inputs) : 0));
+    if (!launch) return room.bytes;
     Operand dz = {grad, c.grad_stride, c.points, c.outputs, 1, 0, 1};
     if (dz_parts || c.dbias) {
-        const Operand made = staged<T>(grad, c.grad_stride, z, c.z_stride, c.activation, c.points, c.outputs, dz_parts, sums, stream);
-        if (dz_parts) dz = made;
+        const Operand parts = staged<T>(grad, c.grad_stride, z, c.z_stride, c.activation, c.points, c.outputs, dz_parts, sums, stream);
+        if (dz_parts) dz = parts;
     }
     if (c.dbias) {
         const dim3 grid(unsigned((c.outputs + 31) / 32));
         if (c.bias_type == F32)
-            launch_early(k_column_sums<float>, grid, 256, 0, 1, stream, sums, int32_t(chunks), int32_t(c.outputs),
+            launch_early(k_column_sums<float>, grid, 1024, 0, 1, stream, sums, int32_t(chunks), int32_t(c.outputs),
                          static_cast<float*>(c.dbias));
         else
-            launch_early(k_column_sums<T>, grid, 256, 0, 1, stream, sums, int32_t(chunks), int32_t(c.outputs),
+            launch_early(k_column_sums<T>, grid, 1024, 0, 1, stream, sums, int32_t(chunks), int32_t(c.outputs),
                          static_cast<T*>(c.dbias));
     }
     LinearEpilogue<T> e = {};
     e.activation = 1;
     if (c.dx) {
-        const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
-                                   : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
         e.y = c.dx, e.y_wide = c.type == F32;
         set_widths(e, c.inputs);
-        product<T, false, true>(dz, b, c.points, c.inputs, c.outputs, dx_plan, e, partial, error, stream);
+        if (dx.gather) {
+            gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, partial, error, stream);
+        } else {
+            const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
+                                       : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
+            product<T, false, true>(dz, b, c.points, c.inputs, c.outputs, dx.plan, e, partial, error, stream);
+        }
     }
     if (c.dweight) {
-        const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
-                                   : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
         e.y = c.dweight, e.y_wide = c.weight_type == F32;
         set_widths(e, c.inputs);
-        product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw_plan, e, partial, error, stream);
+        if (dw.gather) {
+            gathered_product<T, true, true>(gs, xs, c.outputs, c.inputs, c.points, dw, e, partial, error, stream);
+        } else {
+            const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
+                                       : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
+            product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw.plan, e, partial, error, stream);
+        }
     }
     return room.bytes;
 }

@@ -403,8 +403,8 @@ def test_streams(engine):
 def test_workspace_is_not_read(engine):
     """The C entry with a workspace full of NaNs, and results between guards that stay."""
     lib = engine.lib
-    for kind, code in ((F32, 0), (BF16, 1)):
-        p, c, o = 150, 72, 136
+    for kind, code, p, c, o in ((F32, 0, 150, 72, 136), (BF16, 1, 150, 72, 136), (F32, 0, 700, 1500, 900), (BF16, 1, 33, 4096, 136),
+                                (BF16, 1, 40, 75, 30)):
         x, weight = made(130, p, c, dtype=kind), made(131, o, c, dtype=kind)
         size = ctypes.c_size_t()
         args = (code, x.data_ptr(), c, p, c, o, weight.data_ptr(), c)
@@ -477,18 +477,21 @@ def test_refusals(engine):
     refused(lambda: operators.muon(engine, x, x, x, float('inf')), 'finite')
     refused(lambda: operators.muon(engine, x.t(), x.t(), x.t(), 0.1, inplace=True), 'contiguous')
     refused(lambda: operators.muon(engine, x.clone().requires_grad_(), x, x, 0.1), 'requires gradients')
+    # At the C entry; a layer so wide that its operands are made into parts needs a workspace.
+    wide = made(145, 2048, 2048)
     size = ctypes.c_size_t()
-    assert engine.lib.cpde_linear_workspace(0, x.data_ptr(), 8, 6, 8, 4, weight.data_ptr(), 8, ctypes.byref(size)) == native.OK
+    assert engine.lib.cpde_linear_workspace(0, wide.data_ptr(), 2048, 2048, 2048, 2048, wide.data_ptr(), 2048,
+                                            ctypes.byref(size)) == native.OK and size.value > 0
     work = torch.empty(size.value + 256, dtype=torch.uint8, device='cuda')
-    y = torch.empty((6, 4), device='cuda')
+    y = torch.empty_like(wide)
     for bad in (dict(workspace=0), dict(workspace=work.data_ptr() + 16), dict(bytes=size.value - 1), dict(y=0), dict(x=0),
-                dict(y=y.data_ptr() + 1), dict(stride=7), dict(kind=3), dict(activation=4), dict(bias_type=2)):
-        got = dict(kind=0, x=x.data_ptr(), stride=8, bias_type=0, activation=1, y=y.data_ptr(), workspace=work.data_ptr(),
+                dict(y=y.data_ptr() + 1), dict(stride=2047), dict(kind=3), dict(activation=4), dict(bias_type=2)):
+        got = dict(kind=0, x=wide.data_ptr(), stride=2048, bias_type=0, activation=1, y=y.data_ptr(), workspace=work.data_ptr(),
                    bytes=size.value)
         got.update(bad)
-        status = engine.lib.cpde_linear(engine.handle, got['kind'], got['x'], got['stride'], 6, 8, 4, weight.data_ptr(), 8,
-                                        got['bias_type'], None, got['activation'], None, 0, got['y'], None, got['workspace'],
-                                        got['bytes'], None)
+        status = engine.lib.cpde_linear(engine.handle, got['kind'], got['x'], got['stride'], 2048, 2048, 2048, wide.data_ptr(),
+                                        2048, got['bias_type'], None, got['activation'], None, 0, got['y'], None,
+                                        got['workspace'], got['bytes'], None)
         assert status == native.REJECTED, bad
 
 

@@ -16,13 +16,16 @@ def test_workspace_sizes():
     for kind in (0, 1, 2):
         assert lib.cpde_linear_workspace(kind, x, 64, 1000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
         assert lib.cpde_linear_workspace(kind, x, 64, 0, 64, 32, w, 64, ctypes.byref(size)) == native.OK and size.value == 0
-    # Three BF16 parts of FP32; 16-bit rows in whole 16 bytes need nothing, others a copy.
-    assert lib.cpde_linear_workspace(0, x, 64, 100000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
-    assert size.value >= 100000 * 64 * 6
-    assert lib.cpde_linear_workspace(1, x, 64, 100000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
+    # Wide layers: three BF16 parts of FP32; 16-bit rows in whole 16 bytes need nothing, others a copy. Narrow ones are
+    # gathered from the arrays.
+    assert lib.cpde_linear_workspace(0, x, 2048, 30000, 2048, 2048, w, 2048, ctypes.byref(size)) == native.OK
+    assert size.value >= 30000 * 2048 * 6
+    assert lib.cpde_linear_workspace(1, x, 2048, 30000, 2048, 2048, w, 2048, ctypes.byref(size)) == native.OK
     assert size.value == 0
-    assert lib.cpde_linear_workspace(1, x + 2, 64, 100000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
-    assert size.value >= 100000 * 64 * 2
+    assert lib.cpde_linear_workspace(1, x + 2, 2048, 30000, 2048, 2048, w, 2048, ctypes.byref(size)) == native.OK
+    assert size.value >= 30000 * 2048 * 2
+    assert lib.cpde_linear_workspace(0, x, 64, 100000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
+    assert size.value == 0
     for bad in ((3, 10, 8, 8), (0, -1, 8, 8), (0, 1 << 31, 8, 8), (0, 10, 0, 8), (0, 10, 8, 0), (0, 10, (1 << 20) + 1, 8),
                 (0, 10, 8, (1 << 20) + 1)):
         kind, points, inputs, outputs = bad
