@@ -80,7 +80,15 @@ __device__ __forceinline__ Vector<T, 8> gather(const Source<T>& s, int64_t row, 
     const T* p = s.p + row * s.stride + column;
     if (column + 8 <= s.columns) {
         Vector<T, 8> v;
-        if (s.width == 8) return load_written<T, 8>(p);
+        if (s.width == 8) {
+            if constexpr (sizeof(T) == 4) {
+                const Wide w = load_wide(p);
+                memcpy(&v, &w, sizeof(v));
+                return v;
+            } else {
+                return load_written<T, 8>(p);
+            }
+        }
         if (s.width == 4) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -207,6 +215,7 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
             if constexpr (!C::RESIDENT) rb.load(b, int64_t(walk.w.tile_n) * C::BN, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
             walk.next();
         };
+        load(0);
         if constexpr (C::RESIDENT) {
             for (int slab = 0; slab < s.slabs; ++slab) {
                 uint8_t* to[C::P];
@@ -218,7 +227,7 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
             arrive(sh.held);
         }
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) load(i);
+        for (int i = 1; i < AHEAD; ++i) load(i);
         int st = 0;
         uint32_t parity = 1;
         bool ok = true;

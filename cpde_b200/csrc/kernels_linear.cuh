@@ -15,17 +15,32 @@ __device__ __forceinline__ float layer_sigmoid(float z) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return r;
 }
+// tanh z = 1 - 2 / (1 + e^2z), and its Taylor series below 0.35, where the difference would
+// lose the digits that are left (the next term is 1e-8 of the value). Both without a
+// branch: of a warp's values some are always on either side.
+__device__ __forceinline__ float layer_tanh(float z) {
+    const float a = fabsf(z), q = z * z;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(2.885390081777927f * a));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    float s = fmaf(q, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    s = fmaf(q, s, -17.0f / 315.0f);
+    s = fmaf(q, s, 2.0f / 15.0f);
+    s = fmaf(q, s, -1.0f / 3.0f);
+    const float near = fmaf(z * q, s, z), far = copysignf(fmaf(-2.0f, r, 1.0f), z);
+    return a < 0.35f ? near : far;
+}
 // The activations by their codes: 0 sigmoid, 1 linear, 2 tanh, 3 SiLU.
 __device__ __forceinline__ float layer_activation(float z, int32_t activation) {
     if (activation == 1) return z;
-    if (activation == 2) return tanhf(z);
+    if (activation == 2) return layer_tanh(z);
     const float f = layer_sigmoid(z);
     return activation == 3 ? z * f : f;
 }
 __device__ __forceinline__ float layer_slope(float z, int32_t activation) {
     if (activation == 1) return 1.0f;
     if (activation == 2) {
-        const float t = tanhf(z);
+        const float t = layer_tanh(z);
         return fmaf(-t, t, 1.0f);
     }
     const float f = layer_sigmoid(z);

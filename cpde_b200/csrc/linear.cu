@@ -72,7 +72,7 @@ Operand staged(const T* x, int64_t stride, const T* z, int64_t z_stride, int32_t
 template <class T>
 Source<T> source(const T* p, int64_t stride, int64_t rows, int64_t columns) {
     int width = 8;
-    while (width > 1 && !(aligned(p, std::min<int64_t>(width * sizeof(T), 16)) && (rows == 1 || stride % width == 0))) width /= 2;
+    while (width > 1 && !(aligned(p, width * sizeof(T)) && (rows == 1 || stride % width == 0))) width /= 2;
     return {p, stride, rows, int32_t(columns), width};
 }
 
