@@ -1,6 +1,6 @@
 // Launches of linear layers and their gradients (layers.hpp).
 #include "gemm_launch.hpp"
-#include "kernels_linear.cuh"
+#include "kernels_few.cuh"
 #include "layers.hpp"
 
 namespace cpde::ops {
@@ -26,6 +26,10 @@ struct Room {
         return p;
     }
 };
+
+// Layers of at most so many points take the kernel that reads the weights once, and
+// products of at most so many slabs of 32 x 32 x 64 the one on the FP32 units.
+constexpr int64_t FEW_POINTS = 8, SMALL_WORK = 2048;
 
 int64_t eights(int64_t n) { return (n + 7) / 8 * 8; }
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -178,12 +182,59 @@ void set_widths(LinearEpilogue<T>& e, int64_t n) {
     e.whole = all(16), e.fours = all(4);
 }
 
+// Whether a layer's product is computed on the FP32 units, in blocks of 32 x 32.
+bool small_product(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = ((m + SMALL_TILE - 1) / SMALL_TILE) * ((n + SMALL_TILE - 1) / SMALL_TILE);
+    return k <= 1024 && tiles * ((k + SMALL_SLAB - 1) / SMALL_SLAB) <= SMALL_WORK;
+}
+template <class T>
+SmallProduct<T> small_call(const SmallOperand<T>& a, const SmallOperand<T>& b, int64_t m, int64_t n, int64_t k,
+                           const LinearEpilogue<T>& e) {
+    const int64_t tiles_n = (n + SMALL_TILE - 1) / SMALL_TILE;
+    return {a, b, e, nullptr, false, int32_t(m), int32_t(n), int32_t(tiles_n), k, int32_t((m + SMALL_TILE - 1) / SMALL_TILE * tiles_n)};
+}
+template <class T>
+void launch_small(const SmallProduct<T>& first, const SmallProduct<T>& second, cudaStream_t stream) {
+    launch_early(k_small_products<T>, dim3(unsigned(first.tiles + second.tiles)), 32 * SMALL_WARPS, 0, 1, stream, first, second);
+}
+
+template <class T>
+void launch_few(const Source<T>& x, const Source<T>& w, const LinearEpilogue<T>& e, cudaStream_t stream) {
+    GemmShape s = {};
+    s.m = int(x.rows), s.n = int(w.rows);
+    auto go = [&](auto points) {
+        constexpr int POINTS = decltype(points)::value;
+        const int64_t each = FEW_THREADS / 32 * FEW_OUTPUTS<POINTS>;
+        launch_early(k_few_points<T, POINTS>, dim3(unsigned((s.n + each - 1) / each)), FEW_THREADS, 0, 1, stream, x, w, e, s);
+    };
+    if (s.m == 1) go(std::integral_constant<int, 1>{});
+    else if (s.m == 2) go(std::integral_constant<int, 2>{});
+    else if (s.m <= 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
+}
+
 template <class T>
 size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool launch) {
     using O = typename Parts<T>::type;
     Room room = {launch ? static_cast<char*>(c.workspace) : nullptr};
     const T *x = static_cast<const T*>(c.x), *w = static_cast<const T*>(c.weight);
     const Source<T> xs = source(x, c.x_stride, c.points, c.inputs), ws = source(w, c.weight_stride, c.outputs, c.inputs);
+    LinearEpilogue<T> e = {};
+    e.bias = c.bias, e.bias_wide = c.bias_type == F32;
+    e.residual = static_cast<const T*>(c.residual), e.residual_stride = c.residual_stride;
+    e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
+    e.activation = c.activation;
+    set_widths(e, c.outputs);
+    const bool few = c.points <= FEW_POINTS;
+    if (few || small_product(c.points, c.outputs, c.inputs)) {
+        if (!launch) return 0;
+        if (few)
+            launch_few(xs, ws, e, stream);
+        else
+            launch_small(small_call<T>({x, nullptr, c.x_stride, 1}, {w, nullptr, c.weight_stride, 1}, c.points, c.outputs, c.inputs, e),
+                         {}, stream);
+        return 0;
+    }
     const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
     const Route r = route<T>(c.points, c.outputs, c.inputs, {x_direct, c.points * c.inputs, xs.width},
                              {w_direct, c.outputs * c.inputs, ws.width});
@@ -191,12 +242,6 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     O* w_parts = w_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
     float* partial = room.take<float>(partial_count(r.plan, c.points, c.outputs));
     if (!launch) return room.bytes;
-    LinearEpilogue<T> e = {};
-    e.bias = c.bias, e.bias_wide = c.bias_type == F32;
-    e.residual = static_cast<const T*>(c.residual), e.residual_stride = c.residual_stride;
-    e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
-    e.activation = c.activation;
-    set_widths(e, c.outputs);
     if (r.gather) {
         gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, partial, error, stream);
         return room.bytes;
@@ -211,11 +256,36 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
 
 template <class T>
 size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream, bool launch) {
+    if (!c.dx && !c.dweight && !c.dbias) return 0;
     using O = typename Parts<T>::type;
     Room room = {launch ? static_cast<char*>(c.workspace) : nullptr};
     const bool sloped = c.activation != 1;
     const T *grad = static_cast<const T*>(c.grad), *z = sloped ? static_cast<const T*>(c.z) : nullptr;
     const T *x = static_cast<const T*>(c.x), *w = static_cast<const T*>(c.weight);
+    if ((!c.dx || small_product(c.points, c.inputs, c.outputs)) && ((!c.dweight && !c.dbias) || small_product(c.outputs, c.inputs, c.points))) {
+        if (!launch) return 0;
+        LinearEpilogue<T> e = {};
+        e.activation = 1;
+        const int64_t zs = c.z_stride;
+        SmallProduct<T> dx = {}, dw = {};
+        if (c.dx) {
+            e.y = c.dx, e.y_wide = c.type == F32;
+            set_widths(e, c.inputs);
+            dx = small_call<T>({grad, z, c.grad_stride, 1, zs, 1, c.activation}, {w, nullptr, 1, c.weight_stride}, c.points, c.inputs,
+                               c.outputs, e);
+        }
+        if (c.dweight || c.dbias) {
+            // dbias alone is the rows' sums of a product without columns.
+            e.y = c.dweight, e.y_wide = c.weight_type == F32;
+            set_widths(e, c.inputs);
+            dw = small_call<T>({grad, z, 1, c.grad_stride, 1, zs, c.activation}, {x, nullptr, 1, c.x_stride}, c.outputs,
+                               c.dweight ? c.inputs : 1, c.points, e);
+            if (!c.dweight) dw.n = 0;
+            dw.sums = c.dbias, dw.sums_wide = c.bias_type == F32;
+        }
+        launch_small(dx, dw, stream);
+        return 0;
+    }
     const bool dz_direct = !sloped && direct(c.type, grad, c.grad_stride, c.points);
     const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
     // dz is made in the type's parts where the activation has a slope; otherwise it is
