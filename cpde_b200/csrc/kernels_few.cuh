@@ -24,20 +24,40 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
     const int64_t output = (blockIdx.x * int64_t(FEW_THREADS / 32) + threadIdx.x / 32) * R;
     if (output >= s.n) return;
     float sum[R][POINTS] = {};
-#pragma unroll(POINTS == 1 ? 8 : POINTS == 2 ? 4 : 2)
-    for (int k = lane * 8; k < x.columns; k += 256) {
-        float a[R][8];
+    auto add = [&](const Vector<T, 8> (&a)[R], const Vector<T, 8>& b, int p) {
+        float y[8];
+        unpack<T, 8>(b, y);
 #pragma unroll
-        for (int r = 0; r < R; ++r) unpack<T, 8>(gemm::gather(w, output + r, k), a[r]);
+        for (int r = 0; r < R; ++r) {
+            float v[8];
+            unpack<T, 8>(a[r], v);
 #pragma unroll
-        for (int p = 0; p < POINTS; ++p) {
-            float b[8];
-            unpack<T, 8>(gemm::gather(x, p, k), b);
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum[r][p] = fmaf(a[r][j], b[j], sum[r][p]);
+            for (int j = 0; j < 8; ++j) sum[r][p] = fmaf(v[j], y[j], sum[r][p]);
         }
+    };
+    int k = lane * 8;
+    if (x.width == 8 && w.width == 8 && s.n % R == 0) {
+        // DEEP rounds' weights are under way at a time.
+        constexpr int DEEP = POINTS == 1 ? 8 : 4;
+        for (; k + 256 * (DEEP - 1) + 8 <= x.columns; k += 256 * DEEP) {
+            Vector<T, 8> a[DEEP][R];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+                for (int r = 0; r < R; ++r) a[i][r] = load_written<T, 8>(w.p + (output + r) * w.stride + k + 256 * i);
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+                for (int p = 0; p < POINTS; ++p)
+                    add(a[i], load_written<T, 8>(x.p + min(p, s.m - 1) * x.stride + k + 256 * i), p);
+        }
+    }
+    for (; k < x.columns; k += 256) {
+        Vector<T, 8> a[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) a[r] = gemm::gather(w, output + r, k);
+#pragma unroll
+        for (int p = 0; p < POINTS; ++p) add(a, gemm::gather(x, p, k), p);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -83,7 +103,7 @@ constexpr int SMALL_TILE = 32, SMALL_SLAB = 64, SMALL_PITCH = SMALL_TILE + 4, SM
 
 template <class T>
 struct SmallChunk {
-    float v[SMALL_TILE * SMALL_SLAB / (32 * SMALL_WARPS)];
+    T v[8], z[8];
     // The lanes run along whichever way is contiguous.
     __device__ __forceinline__ static int row_of(int i, bool along_k) {
         const int q = threadIdx.x + 256 * i;
@@ -97,16 +117,22 @@ struct SmallChunk {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = row0 + row_of(i, along_k), c = k0 + k_of(i, along_k);
-            v[i] = 0.0f;
-            if (r < rows && c < k) {
-                v[i] = to_float(o.p[r * o.row + c * o.k]);
-                if (o.z) v[i] *= layer_slope(to_float(o.z[r * o.z_row + c * o.z_k]), o.activation);
-            }
+            const bool there = r < rows && c < k;
+            v[i] = there ? o.p[r * o.row + c * o.k] : from_float<T>(0.0f);
+            z[i] = there && o.z ? o.z[r * o.z_row + c * o.z_k] : from_float<T>(0.0f);
         }
     }
-    __device__ __forceinline__ void store(float* to, bool along_k) const {
+    // The slopes here, behind the loads: a branch between those would make them wait for each other.
+    __device__ __forceinline__ void store(float* to, const SmallOperand<T>& o, bool along_k) const {
+        float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[k_of(i, along_k) * SMALL_PITCH + row_of(i, along_k)] = v[i];
+        for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]);
+        if (o.z) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] *= layer_slope(to_float(z[i]), o.activation);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[k_of(i, along_k) * SMALL_PITCH + row_of(i, along_k)] = f[i];
     }
 };
 
@@ -131,8 +157,8 @@ __global__ void __launch_bounds__(32 * SMALL_WARPS) k_small_products(const Small
     b.load(c.b, column0, c.n, 0, c.k, b_along);
     for (int64_t k0 = 0; k0 < c.k; k0 += SMALL_SLAB) {
         __syncthreads();
-        a.store(as, a_along);
-        b.store(bs, b_along);
+        a.store(as, c.a, a_along);
+        b.store(bs, c.b, b_along);
         __syncthreads();
         if (k0 + SMALL_SLAB < c.k) {
             a.load(c.a, row0, c.m, k0 + SMALL_SLAB, c.k, a_along);

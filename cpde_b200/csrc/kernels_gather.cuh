@@ -70,7 +70,7 @@ __device__ __forceinline__ void split_eight(float (&v)[8], uint4 (&part)[Parts<T
     }
 }
 
-constexpr int GATHER_WARPS = 8;
+constexpr int GATHER_WARPS = 8, GATHER_CHUNKS = 1024 / (32 * GATHER_WARPS);
 
 namespace gemm {
 
@@ -114,15 +114,15 @@ __device__ __forceinline__ Vector<T, 8> gather(const Source<T>& s, int64_t row, 
     return v;
 }
 
-// An operand's 128 x 64 of a slab as 1024 chunks of eight: four a thread. Neighbouring
+// An operand's 128 x 64 of a slab as 1024 chunks of eight, shared by the threads. Neighbouring
 // threads read neighbouring chunks of a row and write different banks.
 template <class T, bool ROWS>
 struct Chunks {
-    Vector<T, 8> raw[4];
+    Vector<T, 8> raw[GATHER_CHUNKS];
     __device__ __forceinline__ void load(const Source<T>& s, int64_t at, int64_t k, int thread) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = thread + 256 * i;
+        for (int i = 0; i < GATHER_CHUNKS; ++i) {
+            const int q = thread + 32 * GATHER_WARPS * i;
             if constexpr (ROWS) raw[i] = gather(s, k + q % 512 / 8, int(at) + q / 512 * 64 + q % 8 * 8);
             else raw[i] = gather(s, at + q / 8, int(k) + q % 8 * 8);
         }
@@ -130,8 +130,8 @@ struct Chunks {
     // To part p's place at to[p].
     __device__ __forceinline__ void store(uint8_t* const (&to)[Parts<T>::count], int thread) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = thread + 256 * i, row = ROWS ? q % 512 / 8 : q / 8;
+        for (int i = 0; i < GATHER_CHUNKS; ++i) {
+            const int q = thread + 32 * GATHER_WARPS * i, row = ROWS ? q % 512 / 8 : q / 8;
             const int at = (ROWS ? q / 512 * 8192 : 0) + row * 128 + ((q ^ row) & 7) * 16;
             if constexpr (Parts<T>::count == 1) {
                 *reinterpret_cast<uint4*>(to[0] + at) = raw[i].word[0];
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
             if (lane == 0) tc::mbar_arrive(bar);
         };
         // Slabs that are read ahead into registers.
-        constexpr int AHEAD = C::RESIDENT ? 2 : 1;
+        constexpr int AHEAD = 1;
         Chunks<T, C::A_ROWS> ra[AHEAD];
         Chunks<T, C::B_ROWS> rb;
         bool there[AHEAD];

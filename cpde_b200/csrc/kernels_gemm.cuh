@@ -57,7 +57,7 @@ struct GemmTile {
     static constexpr int STAGE = A_BYTES + (RESIDENT ? 0 : B_BYTES);  // one part of a slab of both operands
     // Of the epilogue. Its loads, conversions and stores are long chains, of which a
     // scheduler needs two warps' at least: four warps took twice the time.
-    static constexpr int WARPS = RESIDENT ? 4 : 8;
+    static constexpr int WARPS = 8;
     // Slabs that are summed in the accumulator before it is taken out. The way from the
     // last MMA to the epilogue and back takes 1.4 us a slab with two CTAs of 256 columns:
     // less than the six products of three parts (1.7), more than the three of two (0.83).
