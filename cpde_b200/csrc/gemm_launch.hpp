@@ -69,7 +69,7 @@ struct GemmPlan {
 struct GemmChoice {
     int ctas, bn, clocks;
 };
-constexpr GemmChoice GEMM_CHOICES[3] = {{2, 256, 130}, {2, 128, 100}, {1, 64, 70}};
+constexpr GemmChoice GEMM_CHOICES[4] = {{2, 256, 130}, {2, 128, 100}, {1, 128, 75}, {1, 64, 70}};
 
 inline int64_t lower_tiles(int64_t tiles_m, int64_t tiles_n, int64_t ratio) {
     int64_t sum = 0;
@@ -77,11 +77,12 @@ inline int64_t lower_tiles(int64_t tiles_m, int64_t tiles_n, int64_t ratio) {
     return sum;
 }
 
-// Clocks around a tile; those of a launch, and of joining a split contraction besides its
-// partial sums' way through memory.
-constexpr double TILE_CLOCKS = 1500, LAUNCH_CLOCKS = 3000, JOIN_CLOCKS = 5000;
+// Clocks around a tile, those of 32 columns in the epilogue, those of a launch, and of
+// joining a split contraction besides its partial sums' way through memory.
+constexpr double TILE_CLOCKS = 700, PIECE_CLOCKS = 900, LAUNCH_CLOCKS = 3000, JOIN_CLOCKS = 5000;
 
-// Takes the tile into `best` if it is estimated to be faster, with its best split.
+// Takes the tile into `best` if it is estimated to be faster, with its best split. A
+// tile's epilogue runs beside the next one's products.
 inline void consider(GemmPlan& best, int ctas, int bn, double slab, int64_t m, int64_t n, int64_t k, int64_t batches, bool lower,
                      bool may_split) {
     const int64_t slabs = (k + GEMM_SLAB - 1) / GEMM_SLAB;
@@ -89,23 +90,25 @@ inline void consider(GemmPlan& best, int ctas, int bn, double slab, int64_t m, i
     const int64_t tiles = (lower ? lower_tiles(tm, tn, bm / bn) : tm * tn) * batches, slots = GEMM_SMS / ctas;
     const int64_t fill = std::max<int64_t>(1, slots / std::max<int64_t>(tiles, 1));
     const int64_t most = may_split ? std::min(slabs / 2, 4 * fill) : 1;
+    const double epilogue = PIECE_CLOCKS * bn / 64;
     for (int64_t want : {int64_t(1), int64_t(2), int64_t(3), int64_t(4), int64_t(6), int64_t(8), fill, 2 * fill}) {
         if (want > 1 && want > most) continue;
         const int64_t each = (slabs + want - 1) / want, splits = (slabs + each - 1) / each;
-        double time = double((tiles * splits + slots - 1) / slots) * (each * slab + TILE_CLOCKS);
+        double time = double((tiles * splits + slots - 1) / slots) * (std::max(each * slab, epilogue) + TILE_CLOCKS) + epilogue;
         if (splits > 1) time += JOIN_CLOCKS + double(splits) * m * n * 8 / 4000;
         if (!best.ctas || time < best.clocks) best = {ctas, bn, int(splits), int(each), time};
     }
 }
 
-// The choice of the shortest estimate: waves of tiles, a slab at the rate of the MMAs or
-// of what L2 brings (64 bytes a clock an SM).
+// The choice of the shortest estimate: waves of tiles, a slab at the rate of the MMAs, of
+// what L2 brings (64 bytes a clock an SM), or of the accumulators' way out and back, which
+// is long between two CTAs (GemmTile::UNIT).
 template <int P>
 GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, int64_t batches, bool lower, bool may_split) {
     GemmPlan best = {};
     for (const GemmChoice& c : GEMM_CHOICES) {
-        const double bytes = P * (128 + c.bn / c.ctas) * 128.0;
-        consider(best, c.ctas, c.bn, std::max(PRODUCTS<P> * 4.0 * c.clocks, bytes / 64), m, n, k, batches, lower, may_split);
+        const double bytes = P * (128 + c.bn / c.ctas) * 128.0, way = P == 1 || c.ctas == 1 ? 0 : P == 2 ? 1300 : 2600;
+        consider(best, c.ctas, c.bn, std::max({PRODUCTS<P> * 4.0 * c.clocks, bytes / 64, way}), m, n, k, batches, lower, may_split);
     }
     return best;
 }
@@ -151,6 +154,7 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
     static std::atomic<uint64_t> ready{0};
     allow_shared(k_gemm<C, E>, C::SHARED, ready);
     const int64_t items = int64_t(s.tiles) * s.splits * s.batches;
+    require(items < (int64_t(1) << 31), "too many tiles for one product");
     const int clusters = int(std::min<int64_t>(items, GEMM_SMS / C::CTAS));
     launch_early(k_gemm<C, E>, dim3(clusters * C::CTAS), C::THREADS, C::SHARED, C::CTAS, stream, operand_map(a, a_box, bf16),
                  operand_map(b, b_box, bf16), s, epilogue, error);
@@ -160,7 +164,8 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
 template <int P, bool A_ROWS, bool B_ROWS, class F>
 void with_tile(const GemmPlan& plan, F&& f) {
     if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS>{});
-    if (plan.bn == 128) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS>{});
+    if (plan.bn == 128 && plan.ctas == 2) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS>{});
+    if (plan.bn == 128) return f(GemmTile<1, 128, P, A_ROWS, B_ROWS>{});
     f(GemmTile<1, 64, P, A_ROWS, B_ROWS>{});
 }
 

@@ -70,7 +70,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int p = 0; p < POINTS; ++p)
-            if (lane == r * POINTS + p && p < s.m && output + r < s.n) epilogue.one(sum[r][p], p, int(output + r), 0, 0, s);
+            if (lane == r * POINTS + p && p < s.m && output + r < s.n) {
+                float v[1] = {sum[r][p]};
+                epilogue.template some<1>(v, p, int(output + r), s);
+            }
 }
 
 // --- small products ----------------------------------------------------------
@@ -211,7 +214,10 @@ __global__ void __launch_bounds__(32 * SMALL_WARPS) k_small_products(const Small
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (column0 + column + j < c.n) c.epilogue.one(v[j], row0 + row, int(column0) + column + j, 0, 0, s);
+            if (column0 + column + j < c.n) {
+                float one[1] = {v[j]};
+                c.epilogue.template some<1>(one, row0 + row, int(column0) + column + j, s);
+            }
     }
 }
 

@@ -151,10 +151,9 @@ struct Chunks {
 template <class C>
 struct Walk {
     const GemmShape& s;
-    int64_t at, items;
-    int stride, slab;
+    int at, items, stride, slab;
     Work w;
-    __device__ Walk(const GemmShape& shape, int first, int step, int64_t count) : s(shape), at(first), items(count), stride(step) {
+    __device__ Walk(const GemmShape& shape, int first, int step, int count) : s(shape), at(first), items(count), stride(step) {
         if (there()) w = work_at<C>(s, at), slab = w.from;
     }
     __device__ bool there() const { return at < items; }
@@ -179,7 +178,7 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
     const Shared<C> sh(raw_shared);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int first = blockIdx.x, stride = gridDim.x;
-    const int64_t items = int64_t(s.tiles) * s.splits;
+    const int items = s.tiles * s.splits;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) tc::mbar_init(sh.full + i, GATHER_WARPS), tc::mbar_init(sh.empty + i, 1);
         for (int i = 0; i < 2; ++i) tc::mbar_init(sh.ready + i, 1), tc::mbar_init(sh.taken + i, C::WARPS);
@@ -208,9 +207,18 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
         Chunks<T, C::B_ROWS> rb;
         bool there[AHEAD];
         Walk<C> walk(s, first, stride, items);
+        // The rows of the tile after the next are brought into L2: what is under way into the
+        // registers covers the latency of L2, not that of memory. (Tiles follow each other down A.)
+        auto ahead = [&](int64_t row) {
+            row += threadIdx.x;
+            const uint32_t bytes = uint32_t(a.columns * sizeof(T)) / 16 * 16;
+            if (C::A_ROWS || a.width < 8 || threadIdx.x >= GEMM_ROWS || row >= a.rows || !bytes) return;
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.p + row * a.stride), "r"(bytes) : "memory");
+        };
         auto load = [&](int i) {
             there[i] = walk.there();
             if (!there[i]) return;
+            if (walk.slab == walk.w.from) ahead(int64_t(walk.w.tile_m + 2 * stride) * C::BM);
             ra[i].load(a, int64_t(walk.w.tile_m) * C::BM, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
             if constexpr (!C::RESIDENT) rb.load(b, int64_t(walk.w.tile_n) * C::BN, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
             walk.next();

@@ -30,8 +30,8 @@ namespace cpde::ops {
 
 constexpr int GEMM_ROWS = 128;   // rows of a CTA's tile: the lanes of tensor memory
 constexpr int GEMM_SLAB = 64;    // elements of a slab: 128 bytes, one swizzled row
-constexpr int GEMM_PIECE = 32;   // columns that an epilogue warp handles at a time
-constexpr int GEMM_STRIDE = 9;  // floats between rows of 8 columns in shared memory: no bank conflicts
+constexpr int GEMM_PIECE = 16;   // columns that an epilogue warp handles at a time
+constexpr int GEMM_STRIDE = 17;  // floats between rows of 16 columns in shared memory: no bank conflicts
 constexpr long long GEMM_WAIT = 2000000000LL;  // clocks, about a second
 
 struct GemmShape {
@@ -166,23 +166,6 @@ __device__ __forceinline__ void tmem_release(uint32_t base, uint32_t columns) {
         tc::tmem_dealloc(base, columns);
 }
 
-// 32 columns of a warp's lanes: thread i gets lane i's.
-__device__ __forceinline__ void tmem_piece(uint32_t at, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(at));
-    tc::tmem_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-    tc::tmem_landed(v);
-}
-
 // Descriptors of a tile in shared memory, 128-byte swizzle, 8-row groups 1024 bytes
 // apart. K-major: the groups follow each other along M or N. MN-major: they follow
 // each other along K, and blocks of 64 along M or N are 64 rows apart.
@@ -200,11 +183,11 @@ struct Work {
 // Work items in an order that keeps the operands of neighbours in L2: bands of 8
 // tiles high, batch after batch and split after split.
 template <class C>
-__device__ __forceinline__ Work work_at(const GemmShape& s, int64_t at) {
+__device__ __forceinline__ Work work_at(const GemmShape& s, int at) {
     Work w;
     const int each = s.tiles * s.splits;
-    w.batch = int(at / each);
-    const int rest = int(at % each), tile = rest % s.tiles;
+    w.batch = at / each;
+    const int rest = at % each, tile = rest % s.tiles;
     w.split = rest / s.tiles;
     if (s.lower) {
         constexpr int RATIO = C::BM / C::BN;  // tiles of a band up to the diagonal, a band
@@ -310,14 +293,14 @@ namespace gemm {
 
 // The MMAs of this cluster's work, by the one thread that calls this.
 template <class C>
-__device__ __forceinline__ void issue(const Shared<C>& sh, const GemmShape& s, uint32_t tmem, int first, int stride, int64_t items) {
+__device__ __forceinline__ void issue(const Shared<C>& sh, const GemmShape& s, uint32_t tmem, int first, int stride, int items) {
     const uint32_t stages = tc::smem_u32(sh.stages), held = stages + C::STAGES * C::STAGE;
     if (C::RESIDENT && !wait_for(sh.held, 0, sh.abort)) return;
     int st = 0;
     uint32_t parity = 0, unit = 0;
     int waiting = 0;  // the first part's stage of a resident unit's slab before
     bool ok = true;
-    for (int64_t at = first; ok && at < items; at += stride) {
+    for (int at = first; ok && at < items; at += stride) {
         const Work w = work_at<C>(s, at);
         for (int slab = w.from; ok && slab < w.to; ++slab) {
             const int in = (slab - w.from) % C::UNIT;
@@ -383,10 +366,12 @@ __device__ __forceinline__ void issue(const Shared<C>& sh, const GemmShape& s, u
     }
 }
 
-// The accumulators' way out, by epilogue warp e whose lanes are those of `quarter`.
+// The accumulators' way out, by epilogue warp e whose lanes are those of `quarter`. The
+// loop over a tile's pieces is not unrolled: its code would run out of the instruction
+// cache. (Unrolled, a piece of 32 columns without an activation took 1200 clocks.)
 template <class C, class E>
 __device__ __forceinline__ void finish(const Shared<C>& sh, const GemmShape& s, const E& epilogue, uint32_t tmem, int e, int quarter,
-                                       uint32_t rank, int first, int stride, int64_t items) {
+                                       uint32_t rank, int first, int stride, int items) {
     const int lane = threadIdx.x % 32, c0 = e / 4 * C::COLUMNS;
     float* piece = sh.pieces + e * 32 * GEMM_STRIDE;
     uint32_t unit = 0;
@@ -406,101 +391,82 @@ __device__ __forceinline__ void finish(const Shared<C>& sh, const GemmShape& s, 
         }
         ++unit;
     };
-    // What a piece needs beside D, read ahead.
-    struct Ahead {
-        typename E::Fetched half[2];
-    };
-    auto fetch = [&](Ahead& got, int row, int column, const Work& w) {
-        if (!epilogue.whole || row + lane >= s.m) return;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (column + 16 * h < s.n) epilogue.fetch(got.half[h], row + lane, column + 16 * h, w.batch, s);
-    };
-    auto put = [&](float (&v)[32], const Ahead& got, int row, int column, const Work& w) {
-        if (row >= s.m || column >= s.n) return;
-        if (epilogue.whole) {
-            if (row + lane >= s.m) return;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (column + 16 * h < s.n)
-                    epilogue.half(*reinterpret_cast<float(*)[16]>(v + 16 * h), got.half[h], row + lane, column + 16 * h, w.batch,
-                                  w.split, C::BM, C::BN, s);
-            return;
-        }
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) piece[lane * GEMM_STRIDE + i] = v[8 * h + i];
-            __syncwarp();
-            const int c = column + 8 * h + lane % 8;
-            if (c >= s.n) continue;
-#pragma unroll 4
-            for (int r = lane / 8; r < 32; r += 4)
-                if (row + r < s.m) epilogue.one(piece[r * GEMM_STRIDE + lane % 8], row + r, c, w.batch, w.split, s);
-        }
-    };
     bool ok = true;
-    for (int64_t at = first; ok && at < items; at += stride) {
+    for (int at = first; ok && at < items; at += stride) {
         const Work w = work_at<C>(s, at);
-        const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column = w.tile_n * C::BN + c0;
+        const int row = w.tile_m * C::BM + rank * GEMM_ROWS + quarter * 32, column0 = w.tile_n * C::BN + c0;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + c0;
+        const bool mine = row + lane < s.m;
+        // What a piece needs beside D is read ahead of it.
+        typename E::Fetched ahead;
+        auto fetch = [&](int column) {
+            if (epilogue.whole && mine && column < s.n) epilogue.fetch(ahead, row + lane, column, w.batch, s);
+        };
+        fetch(column0);
         if constexpr (C::WHOLE) {
-            Ahead got;
-            fetch(got, row, column, w);
             if (!(ok = wait())) break;
-            const uint32_t from = lanes + (unit & 1) * C::BN;
-#pragma unroll 1
-            for (int c = 0; c < C::COLUMNS; c += 32) {
-                float v[32];
-                tmem_piece(from + c, v);
-                const Ahead now = got;
-                if (c + 32 == C::COLUMNS) taken();
-                else fetch(got, row, column + c + 32, w);
-                put(v, now, row, column + c, w);
-            }
         } else {
-            float sum[C::COLUMNS / 32][32] = {};
+            // The units are added in registers, and their sum goes back to where the last was.
+            float sum[C::COLUMNS / 16][16] = {};
             for (int slab = w.from; ok && slab < w.to; slab += C::UNIT) {
                 if (!(ok = wait())) break;
 #pragma unroll
-                for (int c = 0; c < C::COLUMNS / 16; ++c) {  // few registers at a time: the sums take most of them
+                for (int c = 0; c < C::COLUMNS / 16; ++c) {
                     float v[16];
                     tc::tmem_read<16>(lanes + (unit & 1) * C::BN + 16 * c, v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[c / 2][c % 2 * 16 + i] += v[i];
+                    for (int i = 0; i < 16; ++i) sum[c][i] += v[i];
                 }
-                taken();
+                if (slab + C::UNIT < w.to) taken();
             }
             if (!ok) break;
 #pragma unroll
-            for (int c = 0; c < C::COLUMNS / 32; ++c) {
-                if (!epilogue.whole) {
-                    put(sum[c], {}, row, column + 32 * c, w);
-                    continue;
-                }
-                if (row + lane >= s.m) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // as in put, without reading ahead, for which there are no registers
-                    const int at_column = column + 32 * c + 16 * h;
-                    if (at_column >= s.n) continue;
-                    typename E::Fetched got;
-                    epilogue.fetch(got, row + lane, at_column, w.batch, s);
-                    epilogue.half(*reinterpret_cast<float(*)[16]>(sum[c] + 16 * h), got, row + lane, at_column, w.batch, w.split,
-                                  C::BM, C::BN, s);
-                }
+            for (int c = 0; c < C::COLUMNS / 16; ++c) {
+                tc::tmem_st8(lanes + (unit & 1) * C::BN + 16 * c, *reinterpret_cast<const float(*)[8]>(sum[c]));
+                tc::tmem_st8(lanes + (unit & 1) * C::BN + 16 * c + 8, *reinterpret_cast<const float(*)[8]>(sum[c] + 8));
             }
+            tc::tmem_wait_st();
+        }
+        const uint32_t from = lanes + (unit & 1) * C::BN;
+#pragma unroll 1
+        for (int c = 0; c < C::COLUMNS; c += GEMM_PIECE) {
+            const int column = column0 + c, left = s.n - column;
+            float v[16];
+            tc::tmem_read<16>(from + c, v);
+            const typename E::Fetched now = ahead;
+            if (c + GEMM_PIECE == C::COLUMNS) taken();
+            else fetch(column + GEMM_PIECE);
+            if (row >= s.m || left <= 0) continue;
+            if (epilogue.whole) {
+                if (mine) epilogue.whole_row(v, now, row + lane, column, w.batch, w.split, C::BM, C::BN, s);
+                continue;
+            }
+            // A thread ends its row's elements, then neighbouring threads write neighbouring ones.
+            float z[16];
+            if (mine) epilogue.odd(v, z, row + lane, column, left, w.batch, s);
+            auto out = [&](const float (&f)[16], auto which) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) piece[lane * GEMM_STRIDE + i] = f[i];
+                __syncwarp();
+                if (lane % 16 >= left) return;
+#pragma unroll 4
+                for (int r = lane / 16; r < 32; r += 2)
+                    if (row + r < s.m)
+                        epilogue.template write<which>(piece[r * GEMM_STRIDE + lane % 16], row + r, column + lane % 16, w.batch, s);
+            };
+            if (epilogue.writes_z()) out(z, std::integral_constant<int, 0>{});
+            out(v, std::integral_constant<int, 1>{});
         }
     }
 }
 
 }  // namespace gemm
 
-// The epilogue E gets a tile in pieces of 32 rows and 32 columns. Where its arrays have
-// rows of whole 32 bytes (`whole`), a thread keeps the row of its lane: `fetch` reads what
-// belongs to half a piece, 16 columns, ahead of `half`, which ends them. Otherwise the
-// piece goes through shared memory, so that neighbouring threads have neighbouring
-// columns, and `one` ends each element.
+// The epilogue E gets a tile in pieces of 32 rows and 16 columns, a thread the row of its
+// lane. Where its arrays have rows of whole 32 bytes (`whole`), `fetch` reads what belongs
+// to a thread's 16 elements ahead of `whole_row`, which ends them. Otherwise the results (`odd`)
+// go through shared memory, so that neighbouring threads write neighbouring elements.
 template <class C, class E>
 __global__ void __launch_bounds__(C::THREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const GemmShape s, const E epilogue,
@@ -511,7 +477,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = C::CTAS == 2 ? cluster_rank() : 0;
     const int first = blockIdx.x / C::CTAS, stride = gridDim.x / C::CTAS;
-    const int64_t items = int64_t(s.tiles) * s.splits * s.batches;
+    const int items = s.tiles * s.splits * s.batches;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) tc::mbar_init(sh.full + i, 1), tc::mbar_init(sh.empty + i, 1);
         for (int i = 0; i < 2; ++i) tc::mbar_init(sh.ready + i, 1), tc::mbar_init(sh.taken + i, C::CTAS * C::WARPS);
@@ -538,7 +504,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             // The barriers that the bytes count at, and the boxes' places.
             const uint32_t bars = C::CTAS == 2 ? at_rank(sh.full, 0) : tc::smem_u32(sh.full);
             const uint32_t stages = tc::smem_u32(sh.stages);
-            for (int64_t at = first; at < items && !*sh.abort; at += stride) {
+            for (int at = first; at < items && !*sh.abort; at += stride) {
                 const Work w = work_at<C>(s, at);
                 const int m0 = w.tile_m * C::BM + rank * GEMM_ROWS, n0 = w.tile_n * C::BN + rank * C::B_PART;
                 const int za = w.batch * s.a_planes, zb = w.batch * s.b_planes;

@@ -83,7 +83,7 @@ struct LinearEpilogue {
     __device__ __forceinline__ void fetch(Fetched& f, int64_t row, int column, int, const GemmShape&) const {
         if (residual && !partial) f.load(residual + row * residual_stride + column);
     }
-    __device__ __forceinline__ void half(float (&v)[16], const Fetched& f, int64_t row, int column, int, int split, int, int,
+    __device__ __forceinline__ void whole_row(float (&v)[16], const Fetched& f, int64_t row, int column, int, int split, int, int,
                                          const GemmShape& s) const {
         if (partial) {
             Sixteen<float>::store(partial + (split * int64_t(s.m) + row) * partial_pitch(s) + column, v);
@@ -108,6 +108,33 @@ struct LinearEpilogue {
         if (y_wide) Sixteen<float>::store(static_cast<float*>(y) + at, v);
         else Sixteen<T>::store(static_cast<T*>(y) + at, v);
     }
+    // The same of `left` columns in arrays of any layout; what goes to z and to y.
+    __device__ __forceinline__ void odd(float (&v)[16], float (&before)[16], int64_t row, int column, int left, int,
+                                        const GemmShape&) const {
+        float b[16];
+        if (bias) {
+            if (bias_wide) load_some<float, 16>(static_cast<const float*>(bias) + column, b, left, false);
+            else load_some<T, 16>(static_cast<const T*>(bias) + column, b, left, false);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += b[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) before[i] = v[i];
+        activate_all<16>(v, activation);
+        if (residual) {
+            load_some<T, 16>(residual + row * residual_stride + column, b, left, false);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += b[i];
+        }
+    }
+    __device__ __forceinline__ bool writes_z() const { return z; }
+    template <int WHICH>
+    __device__ __forceinline__ void write(float f, int64_t row, int column, int, const GemmShape& s) const {
+        const int64_t at = row * s.n + column;
+        if (WHICH == 0) z[at] = from_float<T>(f);
+        else if (y_wide) static_cast<float*>(y)[at] = f;
+        else static_cast<T*>(y)[at] = from_float<T>(f);
+    }
     // V elements, whatever the arrays' alignment if V is 1.
     template <int V>
     __device__ __forceinline__ void some(float (&v)[V], int64_t row, int column, const GemmShape& s) const {
@@ -129,14 +156,6 @@ struct LinearEpilogue {
         }
         if (y_wide) store<float, V>(static_cast<float*>(y) + at, pack<float, V>(v));
         else store<T, V>(static_cast<T*>(y) + at, pack<T, V>(v));
-    }
-    __device__ __forceinline__ void one(float d, int64_t row, int column, int, int split, const GemmShape& s) const {
-        if (partial) {
-            partial[(split * int64_t(s.m) + row) * partial_pitch(s) + column] = d;
-            return;
-        }
-        float v[1] = {d};
-        some<1>(v, row, column, s);
     }
 };
 

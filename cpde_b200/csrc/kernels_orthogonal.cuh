@@ -45,7 +45,7 @@ struct OrthogonalEpilogue {
         if constexpr (OUT == 0)
             if (weight) f.weight.load(weight + (int64_t(batch) * s.m + row) * s.n + column);
     }
-    __device__ __forceinline__ void half(float (&v)[16], const Fetched& f, int64_t row, int column, int batch, int, int bm, int bn,
+    __device__ __forceinline__ void whole_row(float (&v)[16], const Fetched& f, int64_t row, int column, int batch, int, int bm, int bn,
                                          const GemmShape& s) const {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] *= scale_d;
@@ -90,17 +90,31 @@ struct OrthogonalEpilogue {
             Sixteen<T>::store(final + (int64_t(batch) * s.m + row) * s.n + column, v);
         }
     }
-    __device__ __forceinline__ void one(float d, int64_t row, int column, int batch, int, const GemmShape& s) const {
+    __device__ __forceinline__ void odd(float (&v)[16], float (&)[16], int64_t row, int column, int left, int batch,
+                                        const GemmShape& s) const {
         if constexpr (OUT == 0) {
-            float v = scale_d * d;
             const __half* from = in + int64_t(batch) * in_planes * plane + row * pitch + column;
-            float x = __half2float(from[0]);
-            if constexpr (IN > 1) x += __half2float(from[plane]);
-            v = fmaf(scale_in, x, v);
-            const int64_t at = (int64_t(batch) * s.m + row) * s.n + column;
-            if (weight) v = fmaf(-rate, v, keep * to_float(weight[at]));
-            final[at] = from_float<T>(v);
+            float x[16], rest[16];
+            Sixteen<__half> part;
+            part.load(from);
+            part.get(x);
+            part.load(from + plane);
+            part.get(rest);
+            if (weight) {
+                float w[16];
+                load_some<T, 16>(weight + (int64_t(batch) * s.m + row) * s.n + column, w, left, false);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = fmaf(-rate, fmaf(scale_in, x[i] + rest[i], scale_d * v[i]), keep * w[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = fmaf(scale_in, x[i] + rest[i], scale_d * v[i]);
+            }
         }
+    }
+    __device__ __forceinline__ bool writes_z() const { return false; }
+    template <int WHICH>
+    __device__ __forceinline__ void write(float f, int64_t row, int column, int batch, const GemmShape& s) const {
+        if constexpr (OUT == 0 && WHICH == 1) final[(int64_t(batch) * s.m + row) * s.n + column] = from_float<T>(f);
     }
 };
 

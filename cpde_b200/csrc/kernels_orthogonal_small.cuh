@@ -55,6 +55,23 @@ __device__ __forceinline__ void small_product(uint32_t d, uint32_t a, uint32_t a
     }
 }
 
+// 32 columns of a warp's lanes: thread i gets lane i's.
+__device__ __forceinline__ void tmem_piece(uint32_t at, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    tc::tmem_landed(v);
+}
+
 // Eight neighbouring columns of a row, in the swizzle.
 __device__ __forceinline__ uint32_t small_at(int row, int column) {
     return column / 64 * SMALL_BLOCK + row * 128 + ((column % 64 / 8) ^ (row & 7)) * 16;
@@ -205,7 +222,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
     auto pieces = [&](int n, auto f) {
         for (int column = group * 32; column < n; column += SMALL_THREADS / 4) {
             float v[32];
-            gemm::tmem_piece(lanes + column, v);
+            tmem_piece(lanes + column, v);
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
                 if (column + i < n) f(column + i, *reinterpret_cast<float(*)[8]>(v + i));

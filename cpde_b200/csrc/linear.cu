@@ -86,11 +86,10 @@ struct Route {
     GemmPlan plan;
     bool gather;
 };
-// An operand: whether TMA reads it, or parts of it exist already, and what it takes to make them.
+// An operand: whether TMA reads it, and what there is to make into parts otherwise.
 struct Side {
     bool there;
     int64_t elements;
-    int width;
 };
 template <class T>
 Route route(int64_t m, int64_t n, int64_t k, const Side& a, const Side& b) {
@@ -101,14 +100,16 @@ Route route(int64_t m, int64_t n, int64_t k, const Side& a, const Side& b) {
     double made = r.plan.clocks;
     for (const Side* s : {&a, &b})
         if (!s->there) made += LAUNCH_CLOCKS + double(s->elements) * (sizeof(T) + 2 * P) / 2000;
-    // Gathered, where B's parts stay in shared memory or there is one part.
-    const bool resident = n <= 128 && P * ((k + GEMM_SLAB - 1) / GEMM_SLAB) <= GemmTile<1, 128, P, false, false, true>::HELD;
-    if (P > 1 && !resident) return r;
-    const int width = std::min(a.width, b.width);
-    const double slab = P > 1 ? 1500 : width == 8 ? 500 : width == 4 ? 1000 : width == 2 ? 1200 : 2000;
-    GemmPlan gathered = {};
-    consider(gathered, 1, 128, slab, m, n, k, 1, false, P == 1);
-    if (gathered.clocks < made) r = {gathered, true};
+    // Gathered, where B's parts stay in shared memory: 65,536 points of 128 inputs and outputs
+    // in FP32 take 37 us instead of 51 with parts. At 64 outputs half of its tile is empty:
+    // 25 instead of 20.
+    if constexpr (P > 1) {
+        const bool resident = n <= 128 && P * ((k + GEMM_SLAB - 1) / GEMM_SLAB) <= GemmTile<1, 128, P, false, false, true>::HELD;
+        if (!resident || n <= 64) return r;
+        GemmPlan gathered = {};
+        consider(gathered, 1, 128, 4500, m, n, k, 1, false, false);
+        if (gathered.clocks < made) r = {gathered, true};
+    }
     return r;
 }
 
@@ -162,12 +163,9 @@ void launch_gather(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n,
 }
 template <class T, bool A_ROWS, bool B_ROWS>
 void gathered_product(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n, int64_t k, const Route& r,
-                      const LinearEpilogue<T>& epilogue, float* partial, int* error, cudaStream_t stream) {
-    constexpr int P = Parts<T>::count;
-    const LinearEpilogue<T> e = split_epilogue(r.plan, epilogue, partial);
-    if constexpr (P > 1) launch_gather<GemmTile<1, 128, P, A_ROWS, B_ROWS, true>>(a, b, m, n, k, r.plan, e, error, stream);
-    else launch_gather<GemmTile<1, 128, P, A_ROWS, B_ROWS>>(a, b, m, n, k, r.plan, e, error, stream);
-    join(r.plan, m, n, e, stream);
+                      const LinearEpilogue<T>& epilogue, int* error, cudaStream_t stream) {
+    if constexpr (Parts<T>::count > 1)
+        launch_gather<GemmTile<1, 128, Parts<T>::count, A_ROWS, B_ROWS, true>>(a, b, m, n, k, r.plan, epilogue, error, stream);
 }
 
 // Whether rows of `n` elements at these addresses take the wide accesses of the epilogue, and those of fours.
@@ -236,14 +234,14 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
         return 0;
     }
     const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
-    const Route r = route<T>(c.points, c.outputs, c.inputs, {x_direct, c.points * c.inputs, xs.width},
-                             {w_direct, c.outputs * c.inputs, ws.width});
+    const Route r = route<T>(c.points, c.outputs, c.inputs, {x_direct, c.points * c.inputs},
+                             {w_direct, c.outputs * c.inputs});
     O* x_parts = x_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
     O* w_parts = w_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
     float* partial = room.take<float>(partial_count(r.plan, c.points, c.outputs));
     if (!launch) return room.bytes;
     if (r.gather) {
-        gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, partial, error, stream);
+        gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, error, stream);
         return room.bytes;
     }
     const Operand a = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
@@ -290,23 +288,19 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
     // dz is made in the type's parts where the activation has a slope; otherwise it is
     // grad, which is made into parts only if a product is not gathered.
-    const Source<T> gs = source(grad, c.grad_stride, c.points, c.outputs), xs = source(x, c.x_stride, c.points, c.inputs),
-                    ws = source(w, c.weight_stride, c.outputs, c.inputs);
-    const Side dz_side = {dz_direct, c.points * c.outputs, gs.width};
-    Route dx = {}, dw = {};
-    if (c.dx) dx = route<T>(c.points, c.inputs, c.outputs, dz_side, {w_direct, c.outputs * c.inputs, ws.width});
-    if (c.dweight) dw = route<T>(c.outputs, c.inputs, c.points, dz_side, {x_direct, c.points * c.inputs, xs.width});
-    if (sloped) dx.gather = dw.gather = false;
-    if (c.dx && !dx.gather) dx.plan = gemm_plan<Parts<T>::count>(c.points, c.inputs, c.outputs, 1, false, true);
-    if (c.dweight && !dw.gather) dw.plan = gemm_plan<Parts<T>::count>(c.outputs, c.inputs, c.points, 1, false, true);
-    const bool made = (c.dx && !dx.gather) || (c.dweight && !dw.gather);
+    const Source<T> gs = source(grad, c.grad_stride, c.points, c.outputs), ws = source(w, c.weight_stride, c.outputs, c.inputs);
+    Route dx = {};
+    if (c.dx && !sloped) dx = route<T>(c.points, c.inputs, c.outputs, {dz_direct, c.points * c.outputs}, {w_direct, c.outputs * c.inputs});
+    else dx.plan = gemm_plan<Parts<T>::count>(c.points, c.inputs, c.outputs, 1, false, true);
+    const GemmPlan dw_plan = gemm_plan<Parts<T>::count>(c.outputs, c.inputs, c.points, 1, false, true);
+    const bool made = (c.dx && !dx.gather) || c.dweight;
     O* dz_parts = dz_direct || !made ? nullptr : room.take<O>(parts_count<T>(c.points, c.outputs));
-    O* x_parts = x_direct || !c.dweight || dw.gather ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
+    O* x_parts = x_direct || !c.dweight ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
     O* w_parts = w_direct || !c.dx || dx.gather ? nullptr : room.take<O>(parts_count<T>(c.outputs, c.inputs));
     const int64_t chunks = row_chunks(c.points, c.outputs, row_lanes(c.outputs));
     float* sums = c.dbias ? room.take<float>(chunks * c.outputs) : nullptr;
     float* partial = room.take<float>(std::max(c.dx ? partial_count(dx.plan, c.points, c.inputs) : 0,
-                                               c.dweight ? partial_count(dw.plan, c.outputs, c.inputs) : 0));
+                                               c.dweight ? partial_count(dw_plan, c.outputs, c.inputs) : 0));
     if (!launch) return room.bytes;
     Operand dz = {grad, c.grad_stride, c.points, c.outputs, 1, 0, 1};
     if (dz_parts || c.dbias) {
@@ -328,7 +322,7 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
         e.y = c.dx, e.y_wide = c.type == F32;
         set_widths(e, c.inputs);
         if (dx.gather) {
-            gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, partial, error, stream);
+            gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, error, stream);
         } else {
             const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
                                        : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
@@ -338,13 +332,9 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     if (c.dweight) {
         e.y = c.dweight, e.y_wide = c.weight_type == F32;
         set_widths(e, c.inputs);
-        if (dw.gather) {
-            gathered_product<T, true, true>(gs, xs, c.outputs, c.inputs, c.points, dw, e, partial, error, stream);
-        } else {
-            const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
-                                       : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
-            product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw.plan, e, partial, error, stream);
-        }
+        const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
+                                   : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
+        product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw_plan, e, partial, error, stream);
     }
     return room.bytes;
 }

@@ -24,7 +24,7 @@ def test_workspace_sizes():
     assert size.value == 0
     assert lib.cpde_linear_workspace(1, x + 2, 2048, 30000, 2048, 2048, w, 2048, ctypes.byref(size)) == native.OK
     assert size.value >= 30000 * 2048 * 2
-    assert lib.cpde_linear_workspace(0, x, 64, 100000, 64, 32, w, 64, ctypes.byref(size)) == native.OK
+    assert lib.cpde_linear_workspace(0, x, 128, 100000, 128, 128, w, 128, ctypes.byref(size)) == native.OK
     assert size.value == 0
     for bad in ((3, 10, 8, 8), (0, -1, 8, 8), (0, 1 << 31, 8, 8), (0, 10, 0, 8), (0, 10, 8, 0), (0, 10, (1 << 20) + 1, 8),
                 (0, 10, 8, (1 << 20) + 1)):
