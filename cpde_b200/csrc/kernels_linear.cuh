@@ -202,18 +202,30 @@ struct PartsCall {
     int64_t x_stride, z_stride, rows, chunk;
     int32_t columns, pitch, activation;
     int32_t lanes;     // threads of a row, eight columns each: a power of two up to 32
+    int32_t strips, blocks;  // strips of columns; blocks, all strips of a chunk of rows in turn
     bool whole;        // x and z can be read in eights
 };
 
+// Up to three operands in one launch, block after block.
+constexpr int MOST_PARTS = 3;
 template <class T>
-__global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
-    using O = typename Parts<T>::type;
+struct PartsCalls {
+    PartsCall<T> call[MOST_PARTS];
+    int32_t count;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) k_parts(const __grid_constant__ PartsCalls<T> calls) {
     __shared__ float shared[256 * 8];
     next_launch_may_begin();
     after_previous_launch();
+    int which = 0, block = blockIdx.x;
+    while (which + 1 < calls.count && block >= calls.call[which].blocks) block -= calls.call[which++].blocks;
+    const PartsCall<T>& c = calls.call[which];
+    const int strip = block % c.strips, chunk = block / c.strips;
     const int lane = threadIdx.x % c.lanes, high = 256 / c.lanes;
-    const int column = (blockIdx.x * c.lanes + lane) * 8;
-    const int64_t from = blockIdx.y * c.chunk, to = min(c.rows, from + c.chunk);
+    const int column = (strip * c.lanes + lane) * 8;
+    const int64_t from = chunk * c.chunk, to = min(c.rows, from + c.chunk);
     float sum[8] = {};
     if (column < c.columns) {
         const int left = c.columns - column;
@@ -232,7 +244,7 @@ __global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += v[i];
             if (c.out) {
-                O* out = static_cast<O*>(c.out) + row * c.pitch + column;
+                auto* out = static_cast<typename Parts<T>::type*>(c.out) + row * c.pitch + column;
                 uint4 part[Parts<T>::count];
                 split_eight<T>(v, part);
 #pragma unroll
@@ -249,8 +261,8 @@ __global__ void __launch_bounds__(256) k_parts(const PartsCall<T> c) {
     for (int i = threadIdx.x; i < wide; i += 256) {
         float total = 0.0f;
         for (int r = 0; r < high; ++r) total += shared[r * wide + i];
-        const int at = blockIdx.x * wide + i;
-        if (at < c.columns) c.sums[blockIdx.y * int64_t(c.columns) + at] = total;
+        const int at = strip * wide + i;
+        if (at < c.columns) c.sums[chunk * int64_t(c.columns) + at] = total;
     }
 }
 

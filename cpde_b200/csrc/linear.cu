@@ -55,22 +55,28 @@ size_t parts_count(int64_t rows, int64_t columns) {
     return size_t(rows) * eights(columns) * Parts<T>::count;
 }
 
-// An array as an operand: as it is, or in parts of its own.
+// Adds an array to those that are made into parts, and gives the operand that it becomes;
+// `out` may be null where the column sums alone are wanted.
 template <class T>
-Operand staged(const T* x, int64_t stride, const T* z, int64_t z_stride, int32_t activation, int64_t rows, int64_t columns,
-               typename Parts<T>::type* out, float* sums, cudaStream_t stream) {
-    PartsCall<T> c = {};
+Operand staged(PartsCalls<T>& calls, const T* x, int64_t stride, const T* z, int64_t z_stride, int32_t activation, int64_t rows,
+               int64_t columns, typename Parts<T>::type* out, float* sums) {
+    PartsCall<T>& c = calls.call[calls.count++];
     c.x = x, c.z = z, c.out = out, c.sums = sums;
     c.x_stride = stride, c.z_stride = z_stride, c.rows = rows;
     c.columns = int(columns), c.pitch = int(eights(columns)), c.activation = activation;
     c.lanes = row_lanes(columns);
     const int64_t chunks = row_chunks(rows, columns, c.lanes);
     c.chunk = (rows + chunks - 1) / chunks;
+    c.strips = int((columns + 8 * c.lanes - 1) / (8 * c.lanes)), c.blocks = int(c.strips * chunks);
     constexpr int per = 16 / sizeof(T);
     c.whole = aligned(x, 16) && stride % per == 0 && (!z || (aligned(z, 16) && z_stride % per == 0));
-    const dim3 grid(unsigned((columns + 8 * c.lanes - 1) / (8 * c.lanes)), unsigned(chunks));
-    launch_early(k_parts<T>, grid, 256, 0, 1, stream, c);
     return {out, c.pitch, rows, columns, Parts<T>::count, rows * c.pitch, Parts<T>::count};
+}
+template <class T>
+void launch_parts(const PartsCalls<T>& calls, cudaStream_t stream) {
+    int64_t blocks = 0;
+    for (int i = 0; i < calls.count; ++i) blocks += calls.call[i].blocks;
+    if (blocks) launch_early(k_parts<T>, dim3(unsigned(blocks)), 256, 0, 1, stream, calls);
 }
 
 template <class T>
@@ -244,10 +250,12 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
         gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, error, stream);
         return room.bytes;
     }
+    PartsCalls<T> parts = {};
     const Operand a = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
-                               : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
+                               : staged<T>(parts, x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr);
     const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
-                               : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
+                               : staged<T>(parts, w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr);
+    launch_parts(parts, stream);
     product<T, false, false>(a, b, c.points, c.outputs, c.inputs, r.plan, e, partial, error, stream);
     return room.bytes;
 }
@@ -302,11 +310,16 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     float* partial = room.take<float>(std::max(c.dx ? partial_count(dx.plan, c.points, c.inputs) : 0,
                                                c.dweight ? partial_count(dw_plan, c.outputs, c.inputs) : 0));
     if (!launch) return room.bytes;
-    Operand dz = {grad, c.grad_stride, c.points, c.outputs, 1, 0, 1};
+    Operand dz = {grad, c.grad_stride, c.points, c.outputs, 1, 0, 1}, xo = {x, c.x_stride, c.points, c.inputs, 1, 0, 1},
+            wo = {w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1};
+    PartsCalls<T> parts = {};
     if (dz_parts || c.dbias) {
-        const Operand parts = staged<T>(grad, c.grad_stride, z, c.z_stride, c.activation, c.points, c.outputs, dz_parts, sums, stream);
-        if (dz_parts) dz = parts;
+        const Operand o = staged<T>(parts, grad, c.grad_stride, z, c.z_stride, c.activation, c.points, c.outputs, dz_parts, sums);
+        if (dz_parts) dz = o;
     }
+    if (w_parts) wo = staged<T>(parts, w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr);
+    if (x_parts) xo = staged<T>(parts, x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr);
+    launch_parts(parts, stream);
     if (c.dbias) {
         const dim3 grid(unsigned((c.outputs + 31) / 32));
         if (c.bias_type == F32)
@@ -321,20 +334,13 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     if (c.dx) {
         e.y = c.dx, e.y_wide = c.type == F32;
         set_widths(e, c.inputs);
-        if (dx.gather) {
-            gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, error, stream);
-        } else {
-            const Operand b = w_direct ? Operand{w, c.weight_stride, c.outputs, c.inputs, 1, 0, 1}
-                                       : staged<T>(w, c.weight_stride, nullptr, 0, 1, c.outputs, c.inputs, w_parts, nullptr, stream);
-            product<T, false, true>(dz, b, c.points, c.inputs, c.outputs, dx.plan, e, partial, error, stream);
-        }
+        if (dx.gather) gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, error, stream);
+        else product<T, false, true>(dz, wo, c.points, c.inputs, c.outputs, dx.plan, e, partial, error, stream);
     }
     if (c.dweight) {
         e.y = c.dweight, e.y_wide = c.weight_type == F32;
         set_widths(e, c.inputs);
-        const Operand b = x_direct ? Operand{x, c.x_stride, c.points, c.inputs, 1, 0, 1}
-                                   : staged<T>(x, c.x_stride, nullptr, 0, 1, c.points, c.inputs, x_parts, nullptr, stream);
-        product<T, true, true>(dz, b, c.outputs, c.inputs, c.points, dw_plan, e, partial, error, stream);
+        product<T, true, true>(dz, xo, c.outputs, c.inputs, c.points, dw_plan, e, partial, error, stream);
     }
     return room.bytes;
 }
