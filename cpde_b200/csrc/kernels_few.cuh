@@ -15,14 +15,17 @@ namespace cpde::ops {
 template <int POINTS> constexpr int FEW_OUTPUTS = POINTS >= 4 ? 2 : 1;
 constexpr int FEW_THREADS = 256;
 
-template <class T, int POINTS>
+// TURNED: x and W change places, for layers of at most 8 outputs (a field's head): then x is
+// what passes through once.
+template <class T, int POINTS, bool TURNED>
 __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, const Source<T> w, LinearEpilogue<T> epilogue, GemmShape s) {
     constexpr int R = FEW_OUTPUTS<POINTS>;
     next_launch_may_begin();
     after_previous_launch();
     const int lane = threadIdx.x % 32;
     const int64_t output = (blockIdx.x * int64_t(FEW_THREADS / 32) + threadIdx.x / 32) * R;
-    if (output >= s.n) return;
+    const int64_t points = x.rows, outputs = w.rows;
+    if (output >= outputs) return;
     float sum[R][POINTS] = {};
     auto add = [&](const Vector<T, 8> (&a)[R], const Vector<T, 8>& b, int p) {
         float y[8];
@@ -31,12 +34,14 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
         for (int r = 0; r < R; ++r) {
             float v[8];
             unpack<T, 8>(a[r], v);
+            float eight = v[0] * y[0];  // by itself: the long sum has an eighth of the roundings then
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[r][p] = fmaf(v[j], y[j], sum[r][p]);
+            for (int j = 1; j < 8; ++j) eight = fmaf(v[j], y[j], eight);
+            sum[r][p] += eight;
         }
     };
     int k = lane * 8;
-    if (x.width == 8 && w.width == 8 && s.n % R == 0) {
+    if (x.width == 8 && w.width == 8 && outputs % R == 0) {
         // DEEP rounds' weights are under way at a time.
         constexpr int DEEP = POINTS == 1 ? 8 : 4;
         for (; k + 256 * (DEEP - 1) + 8 <= x.columns; k += 256 * DEEP) {
@@ -49,7 +54,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
             for (int i = 0; i < DEEP; ++i)
 #pragma unroll
                 for (int p = 0; p < POINTS; ++p)
-                    add(a[i], load_written<T, 8>(x.p + min(p, s.m - 1) * x.stride + k + 256 * i), p);
+                    add(a[i], load_written<T, 8>(x.p + min(int64_t(p), points - 1) * x.stride + k + 256 * i), p);
         }
     }
     for (; k < x.columns; k += 256) {
@@ -70,9 +75,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int p = 0; p < POINTS; ++p)
-            if (lane == r * POINTS + p && p < s.m && output + r < s.n) {
+            if (lane == r * POINTS + p && p < points && output + r < outputs) {
                 float v[1] = {sum[r][p]};
-                epilogue.template some<1>(v, p, int(output + r), s);
+                if constexpr (TURNED) epilogue.template some<1>(v, output + r, p, s);
+                else epilogue.template some<1>(v, p, int(output + r), s);
             }
 }
 
@@ -132,7 +138,7 @@ struct SmallChunk {
         for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]);
         if (o.z) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= layer_slope(to_float(z[i]), o.activation);
+            for (int i = 0; i < 8; ++i) f[i] *= layer_slope<sizeof(T) == 4>(to_float(z[i]), o.activation);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) to[k_of(i, along_k) * SMALL_PITCH + row_of(i, along_k)] = f[i];

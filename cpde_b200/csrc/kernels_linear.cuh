@@ -30,35 +30,38 @@ __device__ __forceinline__ float layer_tanh(float z) {
     const float near = fmaf(z * q, s, z), far = copysignf(fmaf(-2.0f, r, 1.0f), z);
     return a < 0.35f ? near : far;
 }
-// The activations by their codes: 0 sigmoid, 1 linear, 2 tanh, 3 SiLU.
+// The activations by their codes: 0 sigmoid, 1 linear, 2 tanh, 3 SiLU. FP32 arrays
+// (EXACT) take the library's functions, good to an ulp or two, 16-bit ones those above.
+template <bool EXACT>
 __device__ __forceinline__ float layer_activation(float z, int32_t activation) {
     if (activation == 1) return z;
-    if (activation == 2) return layer_tanh(z);
-    const float f = layer_sigmoid(z);
+    if (activation == 2) return EXACT ? tanhf(z) : layer_tanh(z);
+    const float f = EXACT ? 1.0f / (1.0f + expf(-z)) : layer_sigmoid(z);
     return activation == 3 ? z * f : f;
 }
+template <bool EXACT>
 __device__ __forceinline__ float layer_slope(float z, int32_t activation) {
     if (activation == 1) return 1.0f;
     if (activation == 2) {
-        const float t = layer_tanh(z);
+        const float t = EXACT ? tanhf(z) : layer_tanh(z);
         return fmaf(-t, t, 1.0f);
     }
-    const float f = layer_sigmoid(z);
+    const float f = EXACT ? 1.0f / (1.0f + expf(-z)) : layer_sigmoid(z);
     return activation == 3 ? fmaf(f, z * (1.0f - f), f) : f * (1.0f - f);
 }
 
-template <int V>
+template <bool EXACT, int V>
 __device__ __forceinline__ void activate_all(float (&v)[V], int32_t activation) {
     if (activation == 1) return;
     if (activation == 2) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 2);
+        for (int i = 0; i < V; ++i) v[i] = layer_activation<EXACT>(v[i], 2);
     } else if (activation == 3) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 3);
+        for (int i = 0; i < V; ++i) v[i] = layer_activation<EXACT>(v[i], 3);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = layer_activation(v[i], 0);
+        for (int i = 0; i < V; ++i) v[i] = layer_activation<EXACT>(v[i], 0);
     }
 }
 
@@ -98,7 +101,7 @@ struct LinearEpilogue {
         }
         const int64_t at = row * s.n + column;
         if (z) Sixteen<T>::store(z + at, v);
-        activate_all<16>(v, activation);
+        activate_all<sizeof(T) == 4, 16>(v, activation);
         if (residual) {
             float r[16];
             f.get(r);
@@ -120,7 +123,7 @@ struct LinearEpilogue {
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) before[i] = v[i];
-        activate_all<16>(v, activation);
+        activate_all<sizeof(T) == 4, 16>(v, activation);
         if (residual) {
             load_some<T, 16>(residual + row * residual_stride + column, b, left, false);
 #pragma unroll
@@ -147,7 +150,7 @@ struct LinearEpilogue {
             for (int i = 0; i < V; ++i) v[i] += b[i];
         }
         if (z) store<T, V>(z + at, pack<T, V>(v));
-        activate_all<V>(v, activation);
+        activate_all<sizeof(T) == 4, V>(v, activation);
         if (residual) {
             float r[V];
             load_some<T, V>(residual + row * residual_stride + column, r, V, true);
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ PartsCall
                 load_some<T, 8>(c.z + row * c.z_stride + column, z, left, whole);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (i < left) v[i] *= layer_slope(z[i], c.activation);
+                    if (i < left) v[i] *= layer_slope<sizeof(T) == 4>(z[i], c.activation);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += v[i];

@@ -7,9 +7,9 @@
 //
 // X, A and Q are held as FP16 parts of value * 2^s, s from the bound that the
 // polynomials put on the singular values (no entry of a matrix is above its
-// largest one). X always has two parts, 22 bits. For FP32 matrices the products
-// take both parts of everything. For the 16-bit types they take the first: what
-// the steps amplify is an error of X itself in the directions of small singular
+// largest one). X always has two parts, 22 bits. For FP32 and FP16 matrices, and small
+// ones, the products take both parts of everything. For larger BF16 ones, and optimiser
+// steps of 16-bit weights, they take the first: what the steps amplify is an error of X itself in the directions of small singular
 // values, and those come through a X, which the epilogue adds from both parts. In
 // steps on bf16-like random matrices with a decaying spectrum the result is then
 // within 2e-4 to 7e-4 of the exact one in norm (X in one part: 6e-3, all in bf16:

@@ -1,6 +1,6 @@
 // Orthogonalised matrices whose smaller side is at most 128 and larger at most 256, an
 // optimiser step's with its momentum and weights: the whole of it in one launch, a CTA a
-// matrix. The formulas and parts are those of kernels_orthogonal.cuh; X (transposed
+// matrix. The formulas and parts are those of kernels_orthogonal.cuh, two of everything; X (transposed
 // where it is tall) and A stay in shared memory, in the layout that the MMAs read, and
 // each product's epilogue writes over what the product has read: Q over A, the next X
 // over X. Bound by the chain of 15 products of 128 x 128 and their epilogues, each of
@@ -33,24 +33,27 @@ struct SmallCall {
     SmallStep step[SMALL_STEPS];
 };
 
-// One product into tensor memory: the small products of parts first, over the whole contraction.
-template <int P, bool B_ROWS>
+// One product into tensor memory, in two sums that the epilogue adds: the first and the
+// second half of the contraction, SMALL_LENGTH columns apart. In each the small products
+// of parts come first: sums are cut toward zero at their size, and what that does to the
+// steps is seen in the result (1.2e-6 of its norm with one sum where two leave 0.8e-6).
+template <bool B_ROWS>
 __device__ __forceinline__ void small_product(uint32_t d, uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int n, int k) {
     const uint32_t instruction = 1u << 4 | uint32_t(B_ROWS) << 16 | uint32_t(n >> 3) << 17 | uint32_t(SMALL_SIDE >> 4) << 24;
     // MN-major blocks of 64 columns are SMALL_BLOCK apart.
     const uint64_t b_base = B_ROWS ? (gemm::descriptor<true>(0) & ~(uint64_t(0x3FFFu) << 16)) | uint64_t(SMALL_BLOCK >> 4) << 16
                                    : gemm::descriptor<false>(0);
-    bool accumulate = false;
+    const int middle = (k / 16 + 1) / 2 * 16;
 #pragma unroll
-    for (int i = 0; i < PRODUCTS<P>; ++i) {
-        const uint32_t from_a = a + (P == 2 && i == 0 ? a_part : 0), from_b = b + (P == 2 && i == 1 ? b_part : 0);
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t from_a = a + (i == 0 ? a_part : 0), from_b = b + (i == 1 ? b_part : 0);
         const uint64_t da = gemm::descriptor<false>(from_a), db = b_base | uint64_t((from_b >> 4) & 0x3FFFu);
 #pragma unroll
         for (int at = 0; at < SMALL_LENGTH; at += 16) {
             if (at >= k) break;
             const uint32_t to_a = at / 64 * SMALL_BLOCK + at % 64 * 2, to_b = B_ROWS ? at * 128 : to_a;
-            gemm::mma<1>(d, da + (to_a >> 4), db + (to_b >> 4), instruction, accumulate);
-            accumulate = true;
+            gemm::mma<1>(at < middle ? d : d + SMALL_LENGTH, da + (to_a >> 4), db + (to_b >> 4), instruction,
+                         i > 0 || (at != 0 && at != middle));
         }
     }
 }
@@ -76,12 +79,11 @@ __device__ __forceinline__ void tmem_piece(uint32_t at, float (&v)[32]) {
 __device__ __forceinline__ uint32_t small_at(int row, int column) {
     return column / 64 * SMALL_BLOCK + row * 128 + ((column % 64 / 8) ^ (row & 7)) * 16;
 }
-template <int PARTS>
 __device__ __forceinline__ void small_get(const uint8_t* base, uint32_t part, uint32_t at, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
+    for (int p = 0; p < 2; ++p) {
         Vector<__half, 8> h;
         h.word[0] = *reinterpret_cast<const uint4*>(base + p * part + at);
         float f[8];
@@ -90,10 +92,9 @@ __device__ __forceinline__ void small_get(const uint8_t* base, uint32_t part, ui
         for (int i = 0; i < 8; ++i) v[i] += f[i];
     }
 }
-template <int PARTS>
 __device__ __forceinline__ void small_put(uint8_t* base, uint32_t part, uint32_t at, float (&v)[8]) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
+    for (int p = 0; p < 2; ++p) {
         const auto h = pack<__half, 8>(v);
         *reinterpret_cast<uint4*>(base + p * part + at) = h.word[0];
         float f[8];
@@ -103,7 +104,7 @@ __device__ __forceinline__ void small_put(uint8_t* base, uint32_t part, uint32_t
     }
 }
 
-template <int P, class T, class M>
+template <class T, class M>
 __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __grid_constant__ SmallCall<T, M> c, int* error) {
     extern __shared__ uint8_t raw_shared[];
     __shared__ double sums[SMALL_THREADS / 32];
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= by;
-        small_put<2>(x_shared, x_part, small_at(row, column), v);
+        small_put(x_shared, x_part, small_at(row, column), v);
     }
 
     uint32_t parity = 0;
@@ -219,10 +220,16 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
     const uint32_t lanes = tmem + (uint32_t(warp % 4 * 32) << 16);
     const uint32_t x0 = tc::smem_u32(x_shared), a0 = tc::smem_u32(a_shared);
     // The product's pieces of 32 columns, in turn to the four warps of a row: f(column, eight of them).
-    auto pieces = [&](int n, auto f) {
+    auto pieces = [&](int n, int k, auto f) {
         for (int column = group * 32; column < n; column += SMALL_THREADS / 4) {
             float v[32];
             tmem_piece(lanes + column, v);
+            if (k > 16) {  // the second half's sums
+                float u[32];
+                tmem_piece(lanes + SMALL_LENGTH + column, u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += u[i];
+            }
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
                 if (column + i < n) f(column + i, *reinterpret_cast<float(*)[8]>(v + i));
@@ -231,31 +238,31 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
     bool ok = true;
     for (int k = 0; ok && k < c.steps; ++k) {
         const SmallStep s = c.step[k];
-        if (!(ok = run([&] { small_product<P, false>(tmem, x0, x_part, x0, x_part, side16, length16); }))) break;
-        pieces(side16, [&](int column, float(&d)[8]) {
+        if (!(ok = run([&] { small_product<false>(tmem, x0, x_part, x0, x_part, side16, length16); }))) break;
+        pieces(side16, length16, [&](int column, float(&d)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) d[i] *= s.gram;
-            small_put<P>(a_shared, a_part, small_at(row, column), d);
+            small_put(a_shared, a_part, small_at(row, column), d);
         });
-        if (!(ok = run([&] { small_product<P, false>(tmem, a0, a_part, a0, a_part, side16, side16); }))) break;
-        pieces(side16, [&](int column, float(&d)[8]) {
+        if (!(ok = run([&] { small_product<false>(tmem, a0, a_part, a0, a_part, side16, side16); }))) break;
+        pieces(side16, side16, [&](int column, float(&d)[8]) {
             const uint32_t at = small_at(row, column);
             float v[8];
-            small_get<P>(a_shared, a_part, at, v);
+            small_get(a_shared, a_part, at, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fmaf(s.poly_in, v[i], s.poly_d * d[i]);
-            small_put<P>(a_shared, a_part, at, v);
+            small_put(a_shared, a_part, at, v);
         });
-        if (!(ok = run([&] { small_product<P, true>(tmem, a0, a_part, x0, x_part, length16, side16); }))) break;
+        if (!(ok = run([&] { small_product<true>(tmem, a0, a_part, x0, x_part, length16, side16); }))) break;
         const bool last = k + 1 == c.steps;
-        pieces(length16, [&](int column, float(&d)[8]) {
+        pieces(length16, side16, [&](int column, float(&d)[8]) {
             const uint32_t at = small_at(row, column);
             float v[8];
-            small_get<2>(x_shared, x_part, at, v);
+            small_get(x_shared, x_part, at, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fmaf(s.x_in, v[i], s.x_d * d[i]);
             if (!last) {
-                small_put<2>(x_shared, x_part, at, v);
+                small_put(x_shared, x_part, at, v);
             } else if (row < side && column < length) {
                 float w[8];
                 auto ended = [&](int i) { return c.weight ? fmaf(-c.rate, v[i], c.keep * w[i]) : v[i]; };

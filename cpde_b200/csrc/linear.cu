@@ -27,7 +27,7 @@ struct Room {
     }
 };
 
-// Layers of at most so many points take the kernel that reads the weights once, and
+// Layers of at most so many points or outputs take the kernel that reads the other side once, and
 // products of at most so many slabs of 32 x 32 x 64 the one on the FP32 units.
 constexpr int64_t FEW_POINTS = 8, SMALL_WORK = 2048;
 
@@ -202,18 +202,18 @@ void launch_small(const SmallProduct<T>& first, const SmallProduct<T>& second, c
     launch_early(k_small_products<T>, dim3(unsigned(first.tiles + second.tiles)), 32 * SMALL_WARPS, 0, 1, stream, first, second);
 }
 
-template <class T>
+template <class T, bool TURNED>
 void launch_few(const Source<T>& x, const Source<T>& w, const LinearEpilogue<T>& e, cudaStream_t stream) {
     GemmShape s = {};
-    s.m = int(x.rows), s.n = int(w.rows);
+    s.m = int(TURNED ? w.rows : x.rows), s.n = int(TURNED ? x.rows : w.rows);
     auto go = [&](auto points) {
         constexpr int POINTS = decltype(points)::value;
         const int64_t each = FEW_THREADS / 32 * FEW_OUTPUTS<POINTS>;
-        launch_early(k_few_points<T, POINTS>, dim3(unsigned((s.n + each - 1) / each)), FEW_THREADS, 0, 1, stream, x, w, e, s);
+        launch_early(k_few_points<T, POINTS, TURNED>, dim3(unsigned((w.rows + each - 1) / each)), FEW_THREADS, 0, 1, stream, x, w, e, s);
     };
-    if (s.m == 1) go(std::integral_constant<int, 1>{});
-    else if (s.m == 2) go(std::integral_constant<int, 2>{});
-    else if (s.m <= 4) go(std::integral_constant<int, 4>{});
+    if (x.rows == 1) go(std::integral_constant<int, 1>{});
+    else if (x.rows == 2) go(std::integral_constant<int, 2>{});
+    else if (x.rows <= 4) go(std::integral_constant<int, 4>{});
     else go(std::integral_constant<int, 8>{});
 }
 
@@ -229,11 +229,13 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
     e.activation = c.activation;
     set_widths(e, c.outputs);
-    const bool few = c.points <= FEW_POINTS;
-    if (few || small_product(c.points, c.outputs, c.inputs)) {
+    const bool few = c.points <= FEW_POINTS, turned = c.outputs <= FEW_POINTS;
+    if (few || turned || small_product(c.points, c.outputs, c.inputs)) {
         if (!launch) return 0;
         if (few)
-            launch_few(xs, ws, e, stream);
+            launch_few<T, false>(xs, ws, e, stream);
+        else if (turned)
+            launch_few<T, true>(ws, xs, e, stream);
         else
             launch_small(small_call<T>({x, nullptr, c.x_stride, 1}, {w, nullptr, c.weight_stride, 1}, c.points, c.outputs, c.inputs, e),
                          {}, stream);

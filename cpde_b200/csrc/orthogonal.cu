@@ -11,6 +11,8 @@ namespace {
 
 enum Type : int32_t { F32 = 0, BF16 = 1, F16 = 2 };
 
+template <class T> struct Tag { using type = T; };
+
 struct Room {
     char* base;
     size_t bytes = 0;
@@ -78,7 +80,6 @@ bool small(const OrthogonalCall& c) {
 
 template <class T, class M>
 void run_small(const OrthogonalCall& c, int* error, cudaStream_t stream) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1;
     std::vector<Step> steps;
     plan_steps(c, steps);
     SmallCall<T, M> s = {};
@@ -104,25 +105,19 @@ void run_small(const OrthogonalCall& c, int* error, cudaStream_t stream) {
                      float(std::ldexp(1.0, next - v.x - v.poly))};
     }
     const int64_t side = std::min(c.rows, c.columns), length = std::max(c.rows, c.columns);
-    const size_t shared = 1024 + ((length + 63) / 64 * 2 + (side + 63) / 64 * P) * SMALL_BLOCK;
-    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's limit is raised
-    int device = 0;
-    CPDE_CUDA(cudaGetDevice(&device));
-    if (!(ready.load() >> (device & 63) & 1)) {
-        CPDE_CUDA(cudaFuncSetAttribute(k_orthogonal_small<P, T, M>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       1024 + (8 + 2 * P) * SMALL_BLOCK));
-        ready.fetch_or(uint64_t(1) << (device & 63));
-    }
-    launch_early(k_orthogonal_small<P, T, M>, dim3(unsigned(c.matrices)), SMALL_THREADS, shared, 1, stream, s, error);
+    const size_t shared = 1024 + ((length + 63) / 64 + (side + 63) / 64) * 2 * SMALL_BLOCK;
+    static std::atomic<uint64_t> ready{0};
+    allow_shared(k_orthogonal_small<T, M>, 1024 + 12 * SMALL_BLOCK, ready);
+    launch_early(k_orthogonal_small<T, M>, dim3(unsigned(c.matrices)), SMALL_THREADS, shared, 1, stream, s, error);
 }
 
-template <class T, class M>
+template <int P, class T, class M>
 size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch) {
     if (small(c)) {
-        if (launch) run_small<T, M>(c, error, stream);
+        if constexpr (P == 2)
+            if (launch) run_small<T, M>(c, error, stream);
         return 0;
     }
-    constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const int64_t m = c.rows, n = c.columns, side = std::min(m, n), batch = c.matrices;
     const bool tall = m > n;
     const int64_t pitch = (n + 15) / 16 * 16, gram_pitch = (side + 15) / 16 * 16;
@@ -214,12 +209,23 @@ size_t run(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch
     return room.bytes;
 }
 
+// Products of both parts for FP32; for FP16 matrices, whose own rounding is as small as the
+// steps' error with one part (not for FP16 weights, of which a step is a small fraction);
+// and where the smaller side is up to 256: there the errors do not average out, and the
+// products take no time.
 size_t run_types(const OrthogonalCall& c, int* error, cudaStream_t stream, bool launch) {
+    auto with = [&](auto element, auto momentum, bool both) {
+        using T = typename decltype(element)::type;
+        using M = typename decltype(momentum)::type;
+        if constexpr (sizeof(T) == 2)
+            if (!both) return run<1, T, M>(c, error, stream, launch);
+        return run<2, T, M>(c, error, stream, launch);
+    };
     const bool wide = c.step && c.momentum_type == F32;
-    if (c.type == F32) return run<float, float>(c, error, stream, launch);
-    if (c.type == BF16)
-        return wide ? run<__nv_bfloat16, float>(c, error, stream, launch) : run<__nv_bfloat16, __nv_bfloat16>(c, error, stream, launch);
-    return wide ? run<__half, float>(c, error, stream, launch) : run<__half, __half>(c, error, stream, launch);
+    const bool both = std::min(c.rows, c.columns) <= 256 || (c.type == F16 && !c.step);
+    if (c.type == F32) return with(Tag<float>{}, Tag<float>{}, true);
+    if (c.type == BF16) return wide ? with(Tag<__nv_bfloat16>{}, Tag<float>{}, both) : with(Tag<__nv_bfloat16>{}, Tag<__nv_bfloat16>{}, both);
+    return wide ? with(Tag<__half>{}, Tag<float>{}, both) : with(Tag<__half>{}, Tag<__half>{}, both);
 }
 
 }  // namespace

@@ -127,8 +127,9 @@ def orthogonalize(engine, x, steps=5, coefficients=QUINTIC, eps=1e-7):
     ``X = x / (|x| + eps)`` with the Frobenius norm, then ``steps`` times ``X = a X + b (X X') X + c (X X')^2 X``.
     ``coefficients`` is a triple (a, b, c), or one for each step (the last counts for the steps behind it).
 
-    Values are held in 22 bits. Products take all of them for float32, whose result is good to about 1e-6 of its norm, and
-    11 for the 16-bit types, which leaves less than their rounding to bfloat16 adds."""
+    Values are held in 22 bits. Products take all of them for float32, whose result is good to about 1e-6 of its norm, for
+    float16 and where a side is up to 256, and 11 for larger bfloat16 matrices, which leaves less than rounding to bfloat16
+    adds."""
     return _operators.orthogonalize(_handle(engine, x), engine.device, x, steps, _coefficients(coefficients), eps)
 
 

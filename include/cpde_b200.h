@@ -295,8 +295,8 @@ int cpde_linear_gradient(cpde_engine* engine, int32_t type, const void* grad, in
  * Frobenius norm, then X <- a X + b (X X') X + c (X X')^2 X, `steps` times. Step k
  * takes the k-th of `triples` (a, b, c) at `coefficients` (host memory), or the
  * last. Coefficients with which a singular value may pass 1024 are refused. Values
- * are held in 22 bits; products take all of them for FP32 matrices and 11 bits for
- * the 16-bit types. Entries of X below 2^-40 of the bound on the singular values
+ * are held in 22 bits; products take all of them for FP32 and FP16 matrices, and
+ * where a side is up to 256, and 11 bits for larger BF16 ones. Entries of X below 2^-40 of the bound on the singular values
  * are lost. */
 int cpde_orthogonalize_workspace(int32_t type, int64_t matrices, int64_t rows, int64_t columns, size_t* bytes);
 int cpde_orthogonalize(cpde_engine* engine, int32_t type, const void* x, int64_t matrices, int64_t rows, int64_t columns,
@@ -305,7 +305,8 @@ int cpde_orthogonalize(cpde_engine* engine, int32_t type, const void* x, int64_t
 /* Optimiser step of one weight matrix: m' = beta m + (1 - beta) g, u = m', or
  * beta m' + (1 - beta) g with `nesterov`, O = u orthogonalised as above,
  * weight' = (1 - rate decay) weight - rate scale O. grad and weight are of `type`,
- * momentum FP32 or of it. The new arrays may be the old ones. */
+ * momentum FP32 or of it. The products of larger 16-bit weights take 11 bits, of both types.
+ * The new arrays may be the old ones. */
 int cpde_muon_workspace(int32_t type, int64_t rows, int64_t columns, size_t* bytes);
 int cpde_muon(cpde_engine* engine, int32_t type, const void* weight, const void* grad, int32_t momentum_type,
               const void* momentum, int64_t rows, int64_t columns, double rate, double beta, int32_t nesterov,

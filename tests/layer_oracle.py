@@ -104,11 +104,11 @@ def _parts(v, count, shift):
     return out / 2.0 ** shift
 
 
-def orthogonalize_modelled(x, kind, steps=5, coefficients=QUINTIC, eps=1e-7):
-    """The same with the roundings of the kernels: X in two FP16 parts, products of two parts or of the first ones, sums in
-    FP32. How far it is from the exact result is the scale of a tolerance."""
-    f32, d = kind == torch.float32, torch.float64
-    count = 2 if f32 else 1
+def orthogonalize_modelled(x, kind, steps=5, coefficients=QUINTIC, eps=1e-7, step=False):
+    """The same with the roundings of the kernels: X in two FP16 parts, products of two parts (FP32, FP16 but for an optimiser's
+    step, and small sides) or of the first ones, sums in FP32. How far it is from the exact result is the scale of a tolerance."""
+    d = torch.float64
+    count = 2 if kind == torch.float32 or (kind == torch.float16 and not step) or min(x.shape) <= 256 else 1
 
     def summed(v):
         return v.to(torch.float32).to(d)

@@ -66,7 +66,7 @@ def check_gradient(engine, grad, x, weight, bias, activation, z, dtype=None):
 # --- linear layers -----------------------------------------------------------
 
 SIZES = [(1, 1, 1), (2, 3, 5), (1, 64, 64), (7, 1, 130), (130, 7, 1), (64, 128, 64), (129, 65, 257), (257, 48, 128),
-         (300, 100, 77), (1, 4096, 520), (16, 1000, 1024), (5, 640, 33), (1000, 512, 256), (2050, 192, 384)]
+         (300, 100, 77), (1, 4096, 520), (16, 1000, 1024), (5, 640, 33), (700, 129, 1), (900, 130, 8), (3000, 64, 3), (1000, 512, 256), (2050, 192, 384)]
 
 
 @pytest.mark.parametrize('kind', KINDS)
@@ -284,7 +284,7 @@ def test_muon(engine, kind, momentum_kind, rows, columns):
         size = 0.9 * momentum.double().abs() + 0.1 * grad.double().abs()
         within(new_momentum, m, (oracle.ROUNDING[momentum_kind] * (1 + 4 * oracle.E) + 4 * oracle.E) * size + oracle.TINY[momentum_kind])
         step = oracle.orthogonalize(u)
-        off = (oracle.orthogonalize_modelled(u, kind) - step).norm()
+        off = (oracle.orthogonalize_modelled(u, kind, step=True) - step).norm()
         s = max(1.0, rows / columns) ** 0.5 if scale is None else scale
         want = (1 - 0.02 * decay) * weight.double() - 0.02 * s * step
         bound = 0.02 * s * (8 * off + 2.0 ** -20 * step.norm()) + (oracle.ROUNDING[kind] + 4 * oracle.E) * want.norm()
