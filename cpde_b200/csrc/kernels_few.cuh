@@ -10,7 +10,8 @@ namespace cpde::ops {
 //
 // z = x W' for POINTS rows of x: the weights pass through the GPU once, which is all that
 // bounds it. A warp takes OUTPUTS rows of W, each lane eight neighbouring inputs at a time,
-// and holds a sum for each pair of a point and an output; x comes from L1.
+// and holds a sum for each pair of a point and an output; x comes from L1. One point of
+// 4096 x 4096 bf16: 9.5 us a call (3.5 TB/s), launch and host's way included.
 
 template <int POINTS> constexpr int FEW_OUTPUTS = POINTS >= 4 ? 2 : 1;
 constexpr int FEW_THREADS = 256;
@@ -88,6 +89,8 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_points(const Source<T> x, c
 // contraction each, so that also a small result keeps a block's warps busy: a lane holds
 // 4 x 8 of the warp's sums. The warps' sums are added in order. Two products go in one
 // launch: a layer's two gradients, whose dz is computed from dy and z as it is read.
+// 257 points of 48 x 128 FP32 take 5.8 us a call, the host's way; with parts and tensor
+// cores 12.6. Gradients of 300 points of 100 x 77: 12.7, before 29.6.
 
 template <class T>
 struct SmallOperand {

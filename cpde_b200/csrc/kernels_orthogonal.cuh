@@ -14,6 +14,9 @@
 // steps on bf16-like random matrices with a decaying spectrum the result is then
 // within 2e-4 to 7e-4 of the exact one in norm (X in one part: 6e-3, all in bf16:
 // 5e-2), below the 1.7e-3 of rounding it to bf16.
+//
+// A 2048 x 8192 bf16 matrix takes 0.72 ms, a step 16 us for A^2 (half of a wave of tiles), 38
+// for A and 72 for X, whose tiles fill 3.5 waves; 2048 x 2048 FP32 0.62 ms.
 #pragma once
 #include "kernels_gemm.cuh"
 

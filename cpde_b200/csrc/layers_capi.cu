@@ -6,8 +6,11 @@
 
 namespace {
 
+// Rows of the last tile count as 31-bit numbers too.
+constexpr int64_t kMostPoints = (int64_t(1) << 31) - 512;
+
 void check_linear(int64_t points, int64_t inputs, int64_t outputs) {
-    require(points >= 0 && points <= kMostIndexed, "points must not be negative, and below 2^31 - 1");
+    require(points >= 0 && points <= kMostPoints, "points must not be negative, and at most 2^31 - 512");
     require(inputs > 0 && inputs <= kMostChannels && outputs > 0 && outputs <= kMostChannels,
             "inputs and outputs must be between 1 and 2^20");
 }
@@ -36,7 +39,7 @@ cpde::ops::LinearCall linear_call(int32_t type, const void* x, int64_t x_stride,
     return c;
 }
 
-// Which gradients are wanted: any non-null address.
+// Bits of the gradients that are wanted.
 constexpr int32_t kWantInput = 1, kWantWeight = 2, kWantBias = 4;
 
 cpde::ops::LinearGradientCall gradient_call(int32_t type, const void* grad, int64_t grad_stride, int32_t activation, const void* x,

@@ -180,10 +180,10 @@ int cpde_layer_gradient_static(cpde_engine* engine, const float* dz, const float
 
 /* --- Operators on caller-owned device arrays (no reference counterpart) ---
  *
- * Embedding lookup, dropout and group norm with their gradients, for networks
- * that a caller trains beside the point networks above, such as one that learns a
- * family of their solutions (a latent code per instance, features per cell,
- * normalised and regularised trunk layers).
+ * Embedding lookup, dropout, group norm and linear layers with their gradients, and
+ * orthogonalised optimiser steps, for networks that a caller trains beside the point
+ * networks above, such as one that learns a family of their solutions (a latent code
+ * per instance, features per cell, normalised and regularised trunk layers).
  *  - All arrays are device memory of the engine's device, aligned to their
  *    element type. Addresses and strides of whole 16 bytes take the fast kernels;
  *    FP32 dropout and FP32-to-16-bit lookups want 32 bytes on their FP32 side.
@@ -267,9 +267,13 @@ int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad
  * (or NULL) takes the sums before the activation, for the gradient. Products of
  * the 16-bit types are exact and summed in FP32; those of FP32 arrays are of
  * three BF16 parts each (24 bits), so that they have the error of FP32 products; a
- * row with an infinity gives infinities or NaNs. 16-bit arrays whose address and
- * stride are whole 16 bytes are read in place; others, and FP32, go through the
- * workspace, whose query therefore takes the addresses too. */
+ * row with an infinity gives infinities or NaNs. Small layers, and those of at most
+ * 8 points or outputs, are computed on the FP32 units. Of larger ones 16-bit arrays
+ * whose address and stride are whole 16 bytes are read in place; others, and wide
+ * FP32 ones, go through the workspace, whose query therefore takes the addresses too.
+ * points up to 2^31 - 512, inputs and outputs up to 2^20. A kernel of these products
+ * whose waits run out (about a second) ends without results, which the engine's next
+ * synchronising call reports. */
 int cpde_linear_workspace(int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs,
                           const void* weight, int64_t weight_stride, size_t* bytes);
 int cpde_linear(cpde_engine* engine, int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs,
