@@ -27,14 +27,16 @@ def test_workspace_sizes():
     assert lib.cpde_linear_workspace(0, x, 128, 100000, 128, 128, w, 128, ctypes.byref(size)) == native.OK
     assert size.value == 0
     for bad in ((3, 10, 8, 8), (0, -1, 8, 8), (0, 1 << 31, 8, 8), (0, 10, 0, 8), (0, 10, 8, 0), (0, 10, (1 << 20) + 1, 8),
-                (0, 10, 8, (1 << 20) + 1)):
+                (0, (1 << 31) - 511, 8, 8), (0, 10, 8, (1 << 20) + 1)):
         kind, points, inputs, outputs = bad
         assert lib.cpde_linear_workspace(kind, x, 8, points, inputs, outputs, w, 8, ctypes.byref(size)) == native.REJECTED
         assert lib.cpde_linear_gradient_workspace(kind, x, 8, 1, x, 8, points, inputs, outputs, w, 8, 7,
                                                   ctypes.byref(size)) == native.REJECTED
     assert lib.cpde_linear_gradient_workspace(1, x, 64, 4, x, 64, 10, 64, 64, w, 64, 7, ctypes.byref(size)) == native.REJECTED
-    assert lib.cpde_orthogonalize_workspace(0, 3, 100, 50, ctypes.byref(size)) == native.OK and size.value > 3 * 100 * 50 * 8
-    assert lib.cpde_muon_workspace(0, 100, 50, ctypes.byref(size)) == native.OK and size.value > 100 * 50 * 12
+    # X twice in two parts, and a step's update in FP32; a matrix that one CTA holds needs nothing.
+    assert lib.cpde_orthogonalize_workspace(0, 3, 300, 400, ctypes.byref(size)) == native.OK and size.value > 3 * 300 * 400 * 8
+    assert lib.cpde_muon_workspace(0, 300, 400, ctypes.byref(size)) == native.OK and size.value > 300 * 400 * 12
+    assert lib.cpde_orthogonalize_workspace(0, 3, 100, 50, ctypes.byref(size)) == native.OK and size.value == 0
     for bad in ((3, 1, 5, 5), (0, -1, 5, 5), (0, 65536, 5, 5), (0, 1, 0, 5), (0, 1, 5, 0), (0, 1, 5, (1 << 20) + 1)):
         assert lib.cpde_orthogonalize_workspace(*bad, ctypes.byref(size)) == native.REJECTED
     for bad in ((3, 5, 5), (0, 0, 5), (0, 5, -1)):
