@@ -27,7 +27,7 @@ struct Room {
     }
 };
 
-// Layers of at most so many points or outputs take the kernel that reads the other side once, and
+// Layers of at most so many points (or outputs) may take the kernel that reads the other side once, and
 // products of at most so many slabs of 32 x 32 x 64 the one on the FP32 units.
 constexpr int64_t FEW_POINTS = 8, SMALL_WORK = 2048;
 
@@ -229,16 +229,28 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     e.z = static_cast<T*>(c.z), e.y = c.y, e.y_wide = c.type == F32;
     e.activation = c.activation;
     set_widths(e, c.outputs);
-    const bool few = c.points <= FEW_POINTS, turned = c.outputs <= FEW_POINTS;
+    // A warp's way through a row takes the same time up to 64 inputs a sum that it holds, so
+    // rows shorter than that are for the tensor cores if there are many: a million points of
+    // 16 inputs and 8 outputs take 171 us there in FP32 and 924 here, 20,000 of 2048 and 4
+    // take 126 and 38, 65,536 of 512 and 8 take 99 both; 16-bit x (21 and 24 us) is never
+    // turned.
+    const auto long_rows = [&](int64_t sums) {
+        int64_t held = 2;
+        while (held < sums) held *= 2;
+        return c.inputs >= 64 * held;
+    };
+    const bool few = c.points <= FEW_POINTS && (c.outputs <= 16384 || long_rows(c.points));
+    const bool turned = c.type == F32 && c.outputs <= FEW_POINTS && long_rows(c.outputs);
     if (few || turned || small_product(c.points, c.outputs, c.inputs)) {
         if (!launch) return 0;
-        if (few)
+        if (few) {
             launch_few<T, false>(xs, ws, e, stream);
-        else if (turned)
-            launch_few<T, true>(ws, xs, e, stream);
-        else
+        } else if (turned) {
+            if constexpr (sizeof(T) == 4) launch_few<T, true>(ws, xs, e, stream);
+        } else {
             launch_small(small_call<T>({x, nullptr, c.x_stride, 1}, {w, nullptr, c.weight_stride, 1}, c.points, c.outputs, c.inputs, e),
                          {}, stream);
+        }
         return 0;
     }
     const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);

@@ -267,8 +267,8 @@ int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad
  * (or NULL) takes the sums before the activation, for the gradient. Products of
  * the 16-bit types are exact and summed in FP32; those of FP32 arrays are of
  * three BF16 parts each (24 bits), so that they have the error of FP32 products; a
- * row with an infinity gives infinities or NaNs. Small layers, and those of at most
- * 8 points or outputs, are computed on the FP32 units. Of larger ones 16-bit arrays
+ * row with an infinity gives infinities or NaNs. Small layers, and most of at most
+ * 8 points (in FP32 also of 8 outputs), are computed on the FP32 units. Of larger ones 16-bit arrays
  * whose address and stride are whole 16 bytes are read in place; others, and wide
  * FP32 ones, go through the workspace, whose query therefore takes the addresses too.
  * points up to 2^31 - 512, inputs and outputs up to 2^20. A kernel of these products

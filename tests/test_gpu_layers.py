@@ -66,7 +66,7 @@ def check_gradient(engine, grad, x, weight, bias, activation, z, dtype=None):
 # --- linear layers -----------------------------------------------------------
 
 SIZES = [(1, 1, 1), (2, 3, 5), (1, 64, 64), (7, 1, 130), (130, 7, 1), (64, 128, 64), (129, 65, 257), (257, 48, 128),
-         (300, 100, 77), (1, 4096, 520), (16, 1000, 1024), (5, 640, 33), (700, 129, 1), (900, 130, 8), (3000, 64, 3), (1000, 512, 256), (2050, 192, 384)]
+         (300, 100, 77), (1, 4096, 520), (16, 1000, 1024), (5, 640, 33), (700, 129, 1), (900, 130, 8), (3000, 64, 3), (3001, 600, 7), (70000, 16, 8), (3, 20, 17000), (1000, 512, 256), (2050, 192, 384)]
 
 
 @pytest.mark.parametrize('kind', KINDS)
