@@ -218,7 +218,8 @@ class Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, weight, bias, z = ctx.saved_tensors
-        _, need_x, need_weight, need_bias, _, need_residual = ctx.needs_input_grad
+        # A flag for each argument that was passed: bias, activation and residual may be left out.
+        _, need_x, need_weight, need_bias, _, need_residual = (*ctx.needs_input_grad, False, False, False)[:6]
         dx = dweight = dbias = None
         if need_x or need_weight or need_bias:
             dx, dweight, dbias = linear_gradient(ctx.engine, grad, x, weight, bias if need_bias else None, ctx.activation, z,
