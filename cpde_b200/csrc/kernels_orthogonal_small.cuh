@@ -126,7 +126,15 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
         tc::fence_barrier_init();
         *abort = 0;
     }
+    __syncwarp();
     if (warp == 0) gemm::tmem_take<1>(&slot, 512);
+    tc::tc_fence_before();
+    // A block of the launch behind that took its tensor memory first would wait for this
+    // one's end, and this one for the columns: nothing says that it may begin before they
+    // are here.
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = slot;
     next_launch_may_begin();
     after_previous_launch();
 
@@ -164,10 +172,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
         *reinterpret_cast<uint4*>(x_shared + i) = make_uint4(0, 0, 0, 0);
     for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
     if (lane == 0) sums[warp] = sum;
-    tc::tc_fence_before();
     __syncthreads();
-    tc::tc_fence_after();
-    const uint32_t tmem = slot;
     sum = 0.0;
     for (int i = 0; i < SMALL_THREADS / 32; ++i) sum += sums[i];
     const float by = float(c.scale / (sqrt(sum) + c.eps));
