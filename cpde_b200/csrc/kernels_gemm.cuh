@@ -426,6 +426,7 @@ __device__ __forceinline__ void finish(const Shared<C>& sh, const GemmShape& s, 
         for (int c = 0; c < C::COLUMNS; c += GEMM_PIECE) {
             const int column = column0 + c, left = s.n - column;
             float v[16];
+            __syncwarp();  // behind the branches of the piece before: the warp loads as one
             tc::tmem_read<16>(from + c, v);
             const typename E::Fetched now = ahead;
             if (c + GEMM_PIECE == C::COLUMNS) taken();
@@ -484,6 +485,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
     if (warp == 1) tmem_take<C::CTAS>(sh.slot, C::TMEM);
     tc::tc_fence_before();
+    __syncwarp();  // the cluster's barrier is for whole warps
     if constexpr (C::CTAS == 2) cluster_sync();
     else __syncthreads();
     tc::tc_fence_after();

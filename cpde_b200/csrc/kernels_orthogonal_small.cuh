@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
     auto pieces = [&](int n, int k, auto f) {
         for (int column = group * 32; column < n; column += SMALL_THREADS / 4) {
             float v[32];
+            __syncwarp();  // behind the branches of the piece before: the warp loads as one
             tmem_piece(lanes + column, v);
             if (k > 16) {  // the second half's sums
                 float u[32];
