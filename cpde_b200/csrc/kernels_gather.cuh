@@ -268,6 +268,10 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
                 }
             }
         }
+        // No commit may be under way to the stages' barriers when the CTA ends.
+        if (threadIdx.x == 0)
+            for (int i = 0; i < C::STAGES && wait_for(sh.empty + st, parity, sh.abort); ++i)
+                if (++st == C::STAGES) st = 0, parity ^= 1;
     } else if (warp == GATHER_WARPS) {
         if (elected()) issue<C>(sh, s, tmem, first, stride, items);
     } else {
