@@ -103,4 +103,28 @@ struct PinnedBuffer {
     }
 };
 
+// A word of page-locked host memory that kernels write and the host reads without waiting.
+struct HostWord {
+    int* ptr = nullptr;
+    HostWord() = default;
+    HostWord(const HostWord&) = delete;
+    HostWord& operator=(const HostWord&) = delete;
+    ~HostWord() { if (ptr) cudaFreeHost(ptr); }
+    void create() {
+        CPDE_CUDA(cudaHostAlloc((void**)&ptr, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+        *ptr = 0;
+    }
+    int* device() const {
+        int* p = nullptr;
+        CPDE_CUDA(cudaHostGetDevicePointer((void**)&p, ptr, 0));
+        return p;
+    }
+    // What kernels have written since the last time.
+    int take() {
+        const int v = *const_cast<volatile int*>(ptr);
+        if (v) *const_cast<volatile int*>(ptr) = 0;
+        return v;
+    }
+};
+
 }  // namespace cpde

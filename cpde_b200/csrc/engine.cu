@@ -43,6 +43,8 @@ Engine::Engine(int dev) : device(dev) {
     tc_error.resize(1);
     CPDE_CUDA(cudaMemsetAsync(tc_error.ptr, 0, sizeof(int), stream));
     CPDE_CUDA(cudaStreamSynchronize(stream));
+    operator_error.create();
+    operator_error_device = operator_error.device();
 }
 
 // Cost totals <-> the buffers of the group reduction (sample indices made global).
@@ -72,6 +74,12 @@ void Engine::check_device_errors() {
         throw DeviceError(std::string("tensor-core kernel gave up waiting for ") +
                           (code == tcg::kErrTma ? "a TMA tile" : "an MMA") + "; results of this pass are invalid");
     }
+    check_operator_errors();
+}
+
+void Engine::check_operator_errors() {
+    if (operator_error.take())
+        throw DeviceError("a kernel of an earlier operator call gave up waiting; the results of the calls since the last check are invalid");
 }
 
 // Joins a sharded group: one NCCL communicator per engine, on its device.
@@ -102,6 +110,7 @@ Engine::~Engine() {
     contexts.clear();
     timer.reset();
     if (stream) cudaStreamDestroy(stream);
+    cudaDeviceSynchronize();  // operators on other streams may still write to operator_error
 }
 
 template <class M>

@@ -150,6 +150,8 @@ class Engine {
     long point_epoch_columns = 16384;  // automatic tier: point-tile epochs up to this many columns per chunk
     std::string last_error;
     DeviceBuffer<int> tc_error;  // nonzero after a tensor-core kernel gave up waiting
+    HostWord operator_error;     // the same of the operators' kernels, on any stream
+    int* operator_error_device = nullptr;
 
     // Point sharding: rank `rank` of `world` engines, one per device, each
     // holding a contiguous shard of every Data object; gradients and cost
@@ -177,6 +179,7 @@ class Engine {
     std::vector<int> shard_offsets_host;  // what shard_offsets holds
     DeviceBuffer<float> gather_send, gather_recv;
     void check_device_errors();
+    void check_operator_errors();  // what has reached the host: does not wait
 
     uint64_t next_id = 1;
     std::unordered_map<uint64_t, std::unique_ptr<DataRecord>> data;

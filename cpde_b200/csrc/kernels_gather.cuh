@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
         tc::tc_fence_after();
         tmem_release<1>(tmem, C::TMEM);
     }
-    if (threadIdx.x == 0 && *sh.abort) atomicExch(error, 3);
+    if (threadIdx.x == 0 && *sh.abort) gemm::report(error);
 }
 
 }  // namespace cpde::ops

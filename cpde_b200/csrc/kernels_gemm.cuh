@@ -87,6 +87,12 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatil
     return tc::mbar_try_wait(bar, parity) || tc::mbar_wait_or_abort(bar, parity, GEMM_WAIT, abort);
 }
 
+// Says on the host's word that a wait ran out.
+__device__ __forceinline__ void report(int* error) {
+    *const_cast<volatile int*>(error) = 3;
+    __threadfence_system();
+}
+
 // One thread of the warp. The loads and MMAs take their operands from registers of the
 // whole warp: a thread that the compiler knows to be the only one issues them directly.
 __device__ __forceinline__ bool elected() {
@@ -551,7 +557,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         tc::tc_fence_after();
         tmem_release<C::CTAS>(tmem, C::TMEM);
     }
-    if (threadIdx.x == 0 && *sh.abort) atomicExch(error, 3);
+    if (threadIdx.x == 0 && *sh.abort) gemm::report(error);
 }
 
 }  // namespace cpde::ops

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) k_orthogonal_small(const __g
         tc::tc_fence_after();
         gemm::tmem_release<1>(tmem, 512);
     }
-    if (threadIdx.x == 0 && *abort) atomicExch(error, 3);
+    if (threadIdx.x == 0 && *abort) gemm::report(error);
 }
 
 }  // namespace cpde::ops

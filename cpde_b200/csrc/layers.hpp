@@ -2,7 +2,7 @@
 // orthogonalised matrices and the optimiser step that takes them. Host interface
 // of linear.cu and orthogonal.cu; arguments have been checked by the C entry
 // points. Every call is asynchronous on `stream` and allocates nothing. `error` is
-// a device word that a kernel sets when it gives up a wait.
+// a word of the host that a kernel sets when it gives up a wait.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -62,5 +62,8 @@ struct OrthogonalCall {
 bool orthogonal_bounded(const OrthogonalCall& call);
 size_t orthogonal_workspace(const OrthogonalCall& call);
 void orthogonal(const OrthogonalCall& call, int* error, cudaStream_t stream);
+
+// A wait that nothing ends and that gives up after some microseconds.
+void give_up(int* error, cudaStream_t stream);
 
 }  // namespace cpde::ops

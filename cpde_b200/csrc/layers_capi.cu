@@ -75,6 +75,12 @@ void check_steps(cpde::ops::OrthogonalCall& c, int32_t steps, const double* coef
 
 extern "C" {
 
+int cpde_operator_check(cpde_engine* h) { return guard_operator(h, [] {}); }
+
+int cpde_operator_give_up(cpde_engine* h, void* stream) {
+    return guard_operator(h, [&] { cpde::ops::give_up(h->engine->operator_error_device, stream_of(h, stream)); });
+}
+
 int cpde_linear_workspace(int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs,
                           const void* weight, int64_t weight_stride, size_t* bytes) {
     return query(bytes, [&] {
@@ -103,7 +109,7 @@ int cpde_linear(cpde_engine* h, int32_t type, const void* x, int64_t x_stride, i
         c.residual = residual, c.residual_stride = residual_stride;
         c.y = y, c.z = z, c.workspace = workspace;
         check_workspace(workspace, workspace_bytes, cpde::ops::linear_workspace(c));
-        cpde::ops::linear(c, h->engine->tc_error.ptr, stream_of(h, stream));
+        cpde::ops::linear(c, h->engine->operator_error_device, stream_of(h, stream));
     });
 }
 
@@ -144,7 +150,7 @@ int cpde_linear_gradient(cpde_engine* h, int32_t type, const void* grad, int64_t
         c.z = z, c.z_stride = z_stride, c.weight_type = weight_type, c.bias_type = bias_type;
         c.dx = dx, c.dweight = dweight, c.dbias = dbias, c.workspace = workspace;
         check_workspace(workspace, workspace_bytes, cpde::ops::linear_gradient_workspace(c));
-        cpde::ops::linear_gradient(c, h->engine->tc_error.ptr, s);
+        cpde::ops::linear_gradient(c, h->engine->operator_error_device, s);
     });
 }
 
@@ -172,7 +178,7 @@ int cpde_orthogonalize(cpde_engine* h, int32_t type, const void* x, int64_t matr
         c.type = type, c.matrices = matrices, c.rows = rows, c.columns = columns;
         c.x = x, c.out = out, c.workspace = workspace;
         check_workspace(workspace, workspace_bytes, cpde::ops::orthogonal_workspace(c));
-        cpde::ops::orthogonal(c, h->engine->tc_error.ptr, stream_of(h, stream));
+        cpde::ops::orthogonal(c, h->engine->operator_error_device, stream_of(h, stream));
     });
 }
 
@@ -206,7 +212,7 @@ int cpde_muon(cpde_engine* h, int32_t type, const void* weight, const void* grad
         c.beta = beta, c.nesterov = nesterov != 0, c.keep = 1 - rate * decay, c.rate = rate * scale, c.step = true;
         c.workspace = workspace;
         check_workspace(workspace, workspace_bytes, cpde::ops::orthogonal_workspace(c));
-        cpde::ops::orthogonal(c, h->engine->tc_error.ptr, stream_of(h, stream));
+        cpde::ops::orthogonal(c, h->engine->operator_error_device, stream_of(h, stream));
     });
 }
 

@@ -359,8 +359,19 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     return room.bytes;
 }
 
+__global__ void k_give_up(int* error) {
+    __shared__ uint64_t never;
+    tc::mbar_init(&never, 1);
+    tc::fence_barrier_init();
+    if (!tc::mbar_wait(&never, 0, 10000)) gemm::report(error);
+}
+
 }  // namespace
 
+void give_up(int* error, cudaStream_t stream) {
+    k_give_up<<<1, 1, 0, stream>>>(error);
+    CPDE_LAUNCHED();
+}
 size_t linear_workspace(const LinearCall& call) {
     size_t bytes = 0;
     with_type(call.type, [&](auto t) { bytes = run_linear<typename decltype(t)::type>(call, nullptr, nullptr, false); });

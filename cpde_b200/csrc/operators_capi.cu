@@ -70,12 +70,16 @@ void check_workspace(const void* workspace, size_t bytes, size_t needed) {
 }
 
 // As guard(), and the caller's current device stays what it was: these calls mix
-// with those of a program that has a device of its own.
+// with those of a program that has a device of its own. A kernel that gave up a wait
+// in an earlier call is reported here: such a program may make no other call.
 template <class F>
 int guard_operator(cpde_engine* h, F&& f) {
     int before = 0;
     const bool known = h && h->engine && cudaGetDevice(&before) == cudaSuccess;
-    const int status = guard(h, f);
+    const int status = guard(h, [&] {
+        h->engine->check_operator_errors();
+        f();
+    });
     if (known && before != h->engine->device) cudaSetDevice(before);
     return status;
 }

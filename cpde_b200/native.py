@@ -69,6 +69,8 @@ SIGNATURES = {
                               P, SZ, P]),
     'cpde_group_norm_gradient': (I32, [P, I32, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I32, P, P, I32, P,
                                        F64, U64, U64, P, P, P, P, SZ, P]),
+    'cpde_operator_check': (I32, [P]),
+    'cpde_operator_give_up': (I32, [P, P]),
     'cpde_linear_workspace': (I32, [I32, P, I64, I64, I64, I64, P, I64, ctypes.POINTER(SZ)]),
     'cpde_linear': (I32, [P, I32, P, I64, I64, I64, I64, P, I64, I32, P, I32, P, I64, P, P, P, SZ, P]),
     'cpde_linear_gradient_workspace': (I32, [I32, P, I64, I32, P, I64, I64, I64, I64, P, I64, I32, ctypes.POINTER(SZ)]),

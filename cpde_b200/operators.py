@@ -51,6 +51,15 @@ def _activation(name):
         raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}') from None
 
 
+def check(engine):
+    """Raises :class:`cpde_b200.native.EngineError` if a kernel of an earlier call gave up waiting, so that its results are
+    invalid. Every other function does so too, before it launches anything; nothing waits, so that a program which wants to
+    know about its last calls synchronises first."""
+    if engine.handle is None:
+        raise native.EngineError(native.REJECTED, 'the engine is closed')
+    engine._check(engine.lib.cpde_operator_check(engine.handle))
+
+
 def embedding(engine, table, ids, scale=1.0, dtype=None):
     """``scale * table[ids]``; rows of ids outside the table are zeros. ``dtype`` (default: the table's) may be a 16-bit
     type for a float32 table."""

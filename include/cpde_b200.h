@@ -272,8 +272,7 @@ int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad
  * whose address and stride are whole 16 bytes are read in place; others, and wide
  * FP32 ones, go through the workspace, whose query therefore takes the addresses too.
  * points up to 2^31 - 512, inputs and outputs up to 2^20. A kernel of these products
- * whose waits run out (about a second) ends without results, which the engine's next
- * synchronising call reports. */
+ * whose waits run out (about a second) ends without results: see cpde_operator_check. */
 int cpde_linear_workspace(int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs,
                           const void* weight, int64_t weight_stride, size_t* bytes);
 int cpde_linear(cpde_engine* engine, int32_t type, const void* x, int64_t x_stride, int64_t points, int64_t inputs,
@@ -294,6 +293,14 @@ int cpde_linear_gradient(cpde_engine* engine, int32_t type, const void* grad, in
                          int64_t inputs, int64_t outputs, const void* weight, int64_t weight_stride, void* dx,
                          int32_t weight_type, void* dweight, int32_t bias_type, void* dbias, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/* CPDE_DEVICE_ERROR if a kernel of an operator gave up waiting and no call has said so yet.
+ * Every operator call and every synchronising call of the engine reports the same, once,
+ * and an operator call that does launches nothing. The query does not wait: after the
+ * last calls of a program synchronise their streams first. cpde_operator_give_up makes it
+ * happen: its kernel waits some microseconds for what never comes. */
+int cpde_operator_check(cpde_engine* engine);
+int cpde_operator_give_up(cpde_engine* engine, void* stream);
 
 /* Newton-Schulz steps on contiguous matrices: X = x / (|x| + eps) with the
  * Frobenius norm, then X <- a X + b (X X') X + c (X X')^2 X, `steps` times. Step k
