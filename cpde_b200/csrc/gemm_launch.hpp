@@ -160,13 +160,19 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
                  operand_map(b, b_box, bf16), s, epilogue, error);
 }
 
-// The tile of the plan as a type.
+// The tile of the plan as a type, that of a contraction of one part by its length.
 template <int P, bool A_ROWS, bool B_ROWS, class F>
 void with_tile(const GemmPlan& plan, F&& f) {
-    if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS>{});
-    if (plan.bn == 128 && plan.ctas == 2) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS>{});
-    if (plan.bn == 128) return f(GemmTile<1, 128, P, A_ROWS, B_ROWS>{});
-    f(GemmTile<1, 64, P, A_ROWS, B_ROWS>{});
+    auto with = [&](auto is_long) {
+        constexpr bool LONG = decltype(is_long)::value;
+        if (plan.bn == 256) return f(GemmTile<2, 256, P, A_ROWS, B_ROWS, false, LONG>{});
+        if (plan.bn == 128 && plan.ctas == 2) return f(GemmTile<2, 128, P, A_ROWS, B_ROWS, false, LONG>{});
+        if (plan.bn == 128) return f(GemmTile<1, 128, P, A_ROWS, B_ROWS, false, LONG>{});
+        f(GemmTile<1, 64, P, A_ROWS, B_ROWS, false, LONG>{});
+    };
+    if constexpr (P == 1)
+        if (plan.split_slabs > GEMM_LONG) return with(std::true_type{});
+    with(std::false_type{});
 }
 
 }  // namespace cpde::ops

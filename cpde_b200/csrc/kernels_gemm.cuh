@@ -11,10 +11,13 @@
 // parts the 24 of FP32 with its exponents. Of the products of parts those are
 // taken that are not below the last part's own rounding: 3 for two parts, 6 for
 // three, the small ones first. The tensor core rounds its sums toward zero, which
-// adds up over a long contraction (a sum of K terms of one sign falls short by up
-// to K/16 2^-24): with P > 1 the accumulator is therefore taken out after each
-// slab and the slabs are added in registers, rounded to nearest. Over 65,536
-// terms that leaves the error of an FP32 sum.
+// adds up over a long contraction: 262,144 terms of one sign fall short by 1.5e-3, 6e-9 a
+// term. The accumulator is therefore taken out after a unit of slabs, and units are added
+// in registers, rounded to nearest. With P > 1 a unit is a slab or two, which over 65,536
+// terms leaves the error of an FP32 sum. With one part it is 2048 terms: that sum is then
+// within 1.2e-5 however long it is, for 1% to 2% of the time. (1024 terms: 5e-6 and 4%;
+// 4096: 2.4e-5 and the time of 2048. Short contractions keep the kernel without units: the
+// other one takes 6% more there, for the registers.)
 //
 // A tile of 128 x BN of one CTA, or 256 x BN of a cluster of two whose CTAs hold
 // half of each operand (cta_group::2), by three roles that are up to two accumulators
@@ -35,6 +38,7 @@ namespace cpde::ops {
 
 constexpr int GEMM_ROWS = 128;   // rows of a CTA's tile: the lanes of tensor memory
 constexpr int GEMM_SLAB = 64;    // elements of a slab: 128 bytes, one swizzled row
+constexpr int GEMM_LONG = 32;    // slabs of one part that an accumulator sums at most
 constexpr int GEMM_PIECE = 16;   // columns that an epilogue warp handles at a time
 constexpr int GEMM_STRIDE = 17;  // floats between rows of 16 columns in shared memory: no bank conflicts
 constexpr long long GEMM_WAIT = 2000000000LL;  // clocks, about a second
@@ -51,10 +55,10 @@ struct GemmShape {
 
 // What a CTA holds. A_ROWS and B_ROWS: the contraction runs over the rows of the operand's array.
 // RESIDENT: the whole of B stays in shared memory, HELD parts of slabs at most.
-template <int CTAS_, int BN_, int P_, bool A_ROWS_, bool B_ROWS_, bool RESIDENT_ = false>
+template <int CTAS_, int BN_, int P_, bool A_ROWS_, bool B_ROWS_, bool RESIDENT_ = false, bool LONG_ = false>
 struct GemmTile {
     static constexpr int CTAS = CTAS_, BN = BN_, P = P_;
-    static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, RESIDENT = RESIDENT_;
+    static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, RESIDENT = RESIDENT_, LONG = LONG_;
     static constexpr int BM = GEMM_ROWS * CTAS;
     static constexpr int B_PART = BN / CTAS;  // columns of the tile whose operand this CTA loads
     static constexpr int A_BYTES = GEMM_ROWS * 128, B_BYTES = B_PART * 128;
@@ -66,9 +70,10 @@ struct GemmTile {
     // Slabs that are summed in the accumulator before it is taken out. The way from the
     // last MMA to the epilogue and back takes 1.4 us a slab with two CTAs of 256 columns:
     // less than the six products of three parts (1.7), more than the three of two (0.83).
-    // A resident B's few slabs are one unit, whose large products come last.
-    static constexpr bool WHOLE = P == 1 || RESIDENT;
-    static constexpr int UNIT = WHOLE ? 1 << 30 : P == 2 ? 2 : 1;
+    // A resident B's few slabs are one unit, whose large products come last, and so is a
+    // contraction of one part, unless it is LONG.
+    static constexpr bool WHOLE = (P == 1 && !LONG) || RESIDENT;
+    static constexpr int UNIT = WHOLE ? 1 << 30 : P == 1 ? GEMM_LONG : P == 2 ? 2 : 1;
     static constexpr int COLUMNS = BN / (WARPS / 4);  // of an epilogue warp
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int PIECES = WARPS * 32 * GEMM_STRIDE * 4;

@@ -105,6 +105,32 @@ def test_the_gathered_gradient_takes_no_parts(engine):
         within(alone[0], *oracle.linear_gradient(grad, x, weight, 'linear', None)[0])
 
 
+# Sums of one sign of 16-bit products. The tensor core cuts 2048 terms toward zero, which oracle.chain bounds (3.5e-5); what is
+# added of them, and the joined splits, is rounded to nearest, at most 2^-24 each time.
+def one_sign(terms):
+    return oracle.chain(2048, BF16) + (terms / 2048 + 8) * oracle.E
+
+
+@pytest.mark.parametrize('kind', [BF16, F16])
+@pytest.mark.parametrize('points,inputs,outputs', [(1 << 18, 1024, 1024), (100001, 520, 1032), (1 << 17, 2048, 256)])
+def test_long_sums_of_one_sign(engine, kind, points, inputs, outputs):
+    """The gradient of the weights over many points whose terms have one sign, as behind a sigmoid, in FP32."""
+    x, grad = (torch.sigmoid(made(120 + i, points, n)).to(kind) for i, n in enumerate((inputs, outputs)))
+    _, dweight, _ = operators.linear_gradient(engine, grad, x, torch.zeros((outputs, inputs), dtype=kind, device='cuda'),
+                                              need=(False, True), dtype=F32)
+    want = sum(grad[a:a + 32768].double().t() @ x[a:a + 32768].double() for a in range(0, points, 32768))
+    assert ((dweight.double() - want).abs() <= (one_sign(points) + 2 * oracle.E) * want).all()
+
+
+@pytest.mark.parametrize('kind', [BF16, F16])
+@pytest.mark.parametrize('points,inputs,outputs', [(2048, 65536, 512), (600, 9000, 1024), (40, 1 << 20, 16)])
+def test_long_rows_of_one_sign(engine, kind, points, inputs, outputs):
+    x, weight = (torch.sigmoid(made(122 + i, n, inputs)).to(kind) for i, n in enumerate((points, outputs)))
+    y, _ = operators.linear(engine, x / 64, weight)
+    want = sum((x / 64)[:, a:a + 65536].double() @ weight[:, a:a + 65536].double().t() for a in range(0, inputs, 65536))
+    within(y, want, (one_sign(inputs) + oracle.ROUNDING[kind] * (1 + 2 * one_sign(inputs))) * want)
+
+
 # FP32 against 64 bits in norm, on the routes of three parts. Parts are exact (3 x 8 bits); left out are products below 2^-25 of
 # |x||w|, at random signs. Inside a slab at most 24 times a sum is cut toward zero, by half of 2^-23 of it on average; a slab's sum is
 # some sqrt(64) of the result's sqrt(K) terms, and the cuts of the slabs add up at random: 24 * 2^-24 = 1.4e-6 of the result where
