@@ -393,7 +393,7 @@ PyObject* linear_gradient(Arguments& a) {
     size_t bytes = 0;
     check(entries.linear_gradient_workspace(kind, pointer(grad.t), grad.stride, activation, pointer(x.t), x.stride, x.rows,
                                             x.columns, weight.rows, pointer(weight.t), weight.stride,
-                                            want_x + 2 * want_weight + 4 * bias.defined(), &bytes) == CPDE_OK,
+                                            want_x + 2 * want_weight + 4 * bias.defined() + 8 * (weight_kind == kind), &bytes) == CPDE_OK,
           "invalid points, inputs or outputs");
     const at::Tensor workspace = made({int64_t(bytes)}, x.t, at::kByte);
     e.done(entries.linear_gradient(e.handle, kind, pointer(grad.t), grad.stride, pointer(z), z_stride, activation, pointer(x.t),

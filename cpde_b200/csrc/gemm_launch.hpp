@@ -144,6 +144,7 @@ void launch_gemm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64
                  const GemmPlan& plan, const E& epilogue, int* error, cudaStream_t stream) {
     GemmShape s = gemm_shape(m, n, k, batches, C::BM, C::BN, lower, plan);
     s.a_planes = a.each, s.b_planes = b.each;
+    s.array_slabs = int(((C::A_ROWS ? a.rows : a.columns) + GEMM_SLAB - 1) / GEMM_SLAB);
     // A single tile of few rows loads no more of them than there are; what the other
     // lanes compute from old bytes is never read.
     const bool few = !C::A_ROWS && C::CTAS == 1 && m < GEMM_ROWS;

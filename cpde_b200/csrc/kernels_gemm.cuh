@@ -46,6 +46,7 @@ constexpr long long GEMM_WAIT = 2000000000LL;  // clocks, about a second
 struct GemmShape {
     int m, n;                        // rows and columns of the result
     int slabs, splits, split_slabs;  // slabs of the contraction, and how they are split
+    int array_slabs;                 // of which an array of A has so many: a contraction of one part goes on in the next
     int tiles_m, tiles_n, tiles, batches;
     int a_planes, b_planes;          // arrays of an operand a batch (of which P are read)
     uint32_t stage_bytes;            // what a stage's loads bring, of all CTAs of the cluster
@@ -517,7 +518,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 const int za = w.batch * s.a_planes, zb = w.batch * s.b_planes;
                 bool ok = true;
                 for (int slab = w.from; ok && slab < w.to; ++slab) {
-                    const int k0 = slab * GEMM_SLAB;
+                    const bool next = C::P == 1 && slab >= s.array_slabs;
+                    const int k0 = (next ? slab - s.array_slabs : slab) * GEMM_SLAB, at_a = za + next;
 #pragma unroll
                     for (int i = 0; i < C::P; ++i, ++loaded) {  // the last part first: it is the first to be done with
                         const int p = C::P - 1 - i;
@@ -526,10 +528,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                         const uint32_t bar = bars + 8 * st;
                         const uint32_t a = stages + st * C::STAGE, b = a + C::A_BYTES;
                         if constexpr (C::A_ROWS) {
-                            load_box<C::CTAS>(a, &a_map, bar, m0, k0, za + p);
-                            load_box<C::CTAS>(a + 8192, &a_map, bar, m0 + 64, k0, za + p);
+                            load_box<C::CTAS>(a, &a_map, bar, m0, k0, at_a + p);
+                            load_box<C::CTAS>(a + 8192, &a_map, bar, m0 + 64, k0, at_a + p);
                         } else {
-                            load_box<C::CTAS>(a, &a_map, bar, k0, m0, za + p);
+                            load_box<C::CTAS>(a, &a_map, bar, k0, m0, at_a + p);
                         }
                         if constexpr (C::B_ROWS) {
 #pragma unroll

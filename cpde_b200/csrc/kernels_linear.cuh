@@ -207,6 +207,7 @@ struct PartsCall {
     int32_t lanes;     // threads of a row, eight columns each: a power of two up to 32
     int32_t strips, blocks;  // strips of columns; blocks, all strips of a chunk of rows in turn
     bool whole;        // x and z can be read in eights
+    bool rest;         // what rounding to a 16-bit type leaves follows as a second array
 };
 
 // Up to three operands in one launch, block after block. Bound by memory: dz of 32,768 x
@@ -251,6 +252,14 @@ __global__ void __launch_bounds__(256) k_parts(const __grid_constant__ PartsCall
             if (c.out) {
                 auto* out = static_cast<typename Parts<T>::type*>(c.out) + row * c.pitch + column;
                 uint4 part[Parts<T>::count];
+                if constexpr (sizeof(T) == 2)
+                    if (c.rest) {
+                        float h[8], left_over[8];
+                        unpack<T, 8>(pack<T, 8>(v), h);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) left_over[i] = finite(h[i]) ? v[i] - h[i] : 0.0f;
+                        store<T, 8>(out + c.rows * c.pitch, pack<T, 8>(left_over));
+                    }
                 split_eight<T>(v, part);
 #pragma unroll
                 for (int p = 0; p < Parts<T>::count; ++p, out += c.rows * c.pitch) *reinterpret_cast<uint4*>(out) = part[p];

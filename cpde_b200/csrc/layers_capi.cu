@@ -40,7 +40,7 @@ cpde::ops::LinearCall linear_call(int32_t type, const void* x, int64_t x_stride,
 }
 
 // Bits of the gradients that are wanted.
-constexpr int32_t kWantInput = 1, kWantWeight = 2, kWantBias = 4;
+constexpr int32_t kWantInput = 1, kWantWeight = 2, kWantBias = 4, kWeightOfType = 8;
 
 cpde::ops::LinearGradientCall gradient_call(int32_t type, const void* grad, int64_t grad_stride, int32_t activation, const void* x,
                                             int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs,
@@ -122,6 +122,7 @@ int cpde_linear_gradient_workspace(int32_t type, const void* grad, int64_t grad_
         c.dx = want & kWantInput ? &wanted : nullptr;
         c.dweight = want & kWantWeight ? &wanted : nullptr;
         c.dbias = want & kWantBias ? &wanted : nullptr;
+        c.weight_type = want & kWeightOfType ? type : CPDE_F32;
         return points ? cpde::ops::linear_gradient_workspace(c) : 0;
     });
 }

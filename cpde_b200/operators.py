@@ -114,7 +114,10 @@ def linear_gradient(engine, grad, x, weight, bias=None, activation='linear', z=N
     """``(dx, dweight, dbias)`` of :func:`linear` from the gradient of y, its inputs and z (not needed for a linear
     activation); the residual's gradient is ``grad`` itself. ``need`` says which of dx and dweight are computed, the others
     are None, and so is dbias without a bias. ``dtype`` of dweight and dbias (default: the parameters') may be float32 for
-    a 16-bit weight."""
+    a 16-bit weight.
+
+    16-bit layers hold grad times the activation's slope in their type where they are large. With ``dtype=torch.float32``
+    dweight sums what that rounding leaves too, in twice the time."""
     need_x, need_weight = need
     return _operators.linear_gradient(_handle(engine, x), engine.device, grad, x, weight, bias, _activation(activation), z,
                                       need_x, need_weight, dtype)

@@ -284,8 +284,10 @@ int cpde_linear(cpde_engine* engine, int32_t type, const void* x, int64_t x_stri
  * dbias = sum of dz; the residual's gradient is grad. z is the forward's (any
  * pointer where the activation is linear). Gradients that are NULL are not
  * computed, and what only they need (x, weight) is not read. dweight is FP32 or of
- * `type`, and so is dbias. For the 16-bit types dz is rounded to the type where the
- * activation is not linear. `want` of the query: 1 dx, 2 dweight, 4 dbias, added. */
+ * `type`, and so is dbias. For the 16-bit types dz of larger layers is rounded to the type
+ * where the activation is not linear; an FP32 dweight sums over what that leaves too.
+ * `want` of the query: 1 dx, 2 dweight, 4 dbias, added, and 8 if dweight is of `type`:
+ * without it the bytes are enough for both. */
 int cpde_linear_gradient_workspace(int32_t type, const void* grad, int64_t grad_stride, int32_t activation, const void* x,
                                    int64_t x_stride, int64_t points, int64_t inputs, int64_t outputs, const void* weight,
                                    int64_t weight_stride, int32_t want, size_t* bytes);

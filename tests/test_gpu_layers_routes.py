@@ -206,6 +206,38 @@ def test_parameters_of_float32_on_tiles(engine, kind, points, inputs, outputs):
         assert dweight.dtype == kind and dbias.dtype == F32
 
 
+@pytest.mark.parametrize('kind', [BF16, F16])
+@pytest.mark.parametrize('points,inputs,outputs', [(1500, 264, 600), (1501, 257, 603), (20000, 64, 72), (70, 40, 24), (4096, 1024, 1024)])
+def test_float32_gradients_of_16_bit_layers(engine, kind, points, inputs, outputs):
+    """Two numbers of the type hold a term to 2^-16. Cuts of sums of random signs, 2 * 2048 / 16 at most before they are taken out,
+    each below 2^-24 of what has been reached on average, leave 1.5e-5; the slope's roundings are some 2^-20. Together below 2^-15:
+    terms rounded once to bfloat16 leave 1e-3, to float16 1e-4."""
+    x, weight, bias, grad = (made(54 + i, *s, dtype=kind) for i, s in enumerate(((points, inputs), (outputs, inputs), (outputs,), (points, outputs))))
+    for activation in ACTIVATIONS[1:]:
+        z = operators.linear(engine, x, weight / inputs ** 0.5, bias, activation, keep=True)[1]
+        _, dweight, dbias = check_gradient(engine, grad, x, weight, bias, activation, z, dtype=F32)
+        dz = grad.double() * oracle.slope(z.double(), activation)
+        for got, want in ((dweight, dz.t() @ x.double()), (dbias, dz.sum(0))):
+            assert (got.double() - want).norm() <= 2.0 ** -15 * want.norm(), float((got.double() - want).norm() / want.norm())
+        alone = operators.linear_gradient(engine, grad, x, weight, None, activation, z, need=(False, True), dtype=F32)[1]
+        assert same_bits(alone, dweight)
+
+
+@pytest.mark.parametrize('kind', [BF16, F16])
+def test_float32_gradients_of_bad_values(engine, kind):
+    """Infinite terms and those that overflow the type stay infinite."""
+    x, weight, grad = (made(58 + i, *s, dtype=kind).abs() for i, s in enumerate(((1500, 264), (600, 264), (1500, 600))))
+    z = torch.ones_like(grad)
+    grad[7, 3] = float('inf')
+    grad[9, 5] = torch.finfo(kind).max  # times a slope of silu above 1, if the type holds no more
+    z[9, 5] = 2.0
+    _, dweight, _ = operators.linear_gradient(engine, grad, x, weight, None, 'silu', z, need=(False, True), dtype=F32)
+    assert (dweight[3] == float('inf')).all()
+    assert (dweight[5] == float('inf')).all()
+    keep = [i for i in range(600) if i not in (3, 5)]
+    assert dweight[keep].isfinite().all()
+
+
 @pytest.mark.parametrize('kind', KINDS)
 def test_needs_on_tiles(engine, kind):
     x, weight, bias, grad = (made(60 + i, *s, dtype=kind) for i, s in enumerate(((1500, 264), (600, 264), (600,), (1500, 600))))

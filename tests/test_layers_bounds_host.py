@@ -7,6 +7,20 @@ torch = pytest.importorskip('torch')
 from test_gpu_layers_routes import NORM  # noqa: E402
 
 
+def test_gradient_workspace_is_enough_for_both_types():
+    """Without a word about the type of dweight the query covers both."""
+    import ctypes
+
+    from cpde_b200 import native
+    lib, size = native.load(), ctypes.c_size_t()
+    sizes = {}
+    for want in (2, 2 + 8, 7, 7 + 8):
+        assert lib.cpde_linear_gradient_workspace(1, 1 << 20, 2048, 3, 1 << 30, 2048, 30000, 2048, 2048, 1 << 35, 2048, want,
+                                                  ctypes.byref(size)) == native.OK
+        sizes[want] = size.value
+    assert sizes[2] >= sizes[2 + 8] + 30000 * 2048 * 2 and sizes[7] >= sizes[7 + 8] + 30000 * 2048 * 2
+
+
 def parts(v, count):
     out = []
     for _ in range(count):
