@@ -243,7 +243,8 @@ class Linear(torch.autograd.Function):
 
 class Muon(torch.optim.Optimizer):
     """Steps of :func:`muon`, in place, for the weight matrices of hidden layers; other parameters (biases, embeddings,
-    heads) are for another optimiser."""
+    heads) are for another optimiser. Momentum is float32 whatever the weights' type: a part 1 - beta of a gradient would be
+    lost beside a 16-bit one. A state that was saved in another type is taken over in float32."""
 
     def __init__(self, engine, params, lr=0.02, beta=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=QUINTIC,
                  eps=1e-7):
@@ -257,6 +258,13 @@ class Muon(torch.optim.Optimizer):
             self.param_groups.pop()
             raise ValueError('Muon takes matrices alone')
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)  # which gives the state the parameters' type
+        ours = (p for group in self.param_groups for p in group['params'])
+        for key, p in zip((key for group in state_dict['param_groups'] for key in group['params']), ours):
+            if 'momentum' in state_dict['state'].get(key, {}):
+                self.state[p]['momentum'] = state_dict['state'][key]['momentum'].to(p.device, torch.float32, copy=True).contiguous()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -269,7 +277,7 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if 'momentum' not in state:
-                    state['momentum'] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                    state['momentum'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 muon(self.engine, p, p.grad, state['momentum'], group['lr'], group['beta'], group['nesterov'],
                      group['weight_decay'], None, group['steps'], group['coefficients'], group['eps'], inplace=True)
         return loss
