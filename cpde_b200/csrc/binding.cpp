@@ -409,7 +409,9 @@ struct Steps {
     std::vector<double> coefficients;
     double eps;
     explicit Steps(Arguments& a) {
-        count = int32_t(a.integer());
+        const int64_t n = a.integer();
+        check(n == int32_t(n), "steps must be between 1 and 64");
+        count = int32_t(n);
         PyObject* items = a.take();
         check(PyTuple_Check(items), "coefficients must be triples");
         for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(items); ++i) {
@@ -443,7 +445,7 @@ PyObject* muon(Arguments& a) {
     const Engine e = a.engine();
     at::Tensor weight = a.tensor(e, "weight"), grad = a.tensor(e, "grad"), momentum = a.tensor(e, "momentum");
     const double rate = a.number(), beta = a.number();
-    const int32_t nesterov = int32_t(a.integer());
+    const int32_t nesterov = a.integer() != 0;
     const double decay = a.number(), scale = a.number();
     const Steps steps(a);
     const bool inplace = a.integer() != 0;

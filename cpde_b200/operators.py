@@ -14,6 +14,7 @@ higher derivatives are not supported.
 Equal calls on equally laid out inputs give equal bits: no result depends on the order in which blocks run.
 """
 import ctypes
+import numbers
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -128,10 +129,17 @@ QUINTIC = (3.4445, -4.775, 2.0315)
 
 def _coefficients(coefficients):
     """A triple, or a sequence of triples, as one tuple."""
-    flat = coefficients if isinstance(coefficients[0], (int, float)) else [v for triple in coefficients for v in triple]
-    if len(flat) % 3:
-        raise ValueError('coefficients must be triples')
-    return tuple(flat)
+    message = 'coefficients must be triples of numbers, one at least'
+    try:
+        items = list(coefficients)
+        if items and not isinstance(items[0], numbers.Real):
+            items = [v for a, b, c in items for v in (a, b, c)]
+        flat = tuple(float(v) for v in items)
+    except (TypeError, ValueError):
+        raise ValueError(message) from None
+    if not flat or len(flat) % 3:
+        raise ValueError(message)
+    return flat
 
 
 def orthogonalize(engine, x, steps=5, coefficients=QUINTIC, eps=1e-7):
@@ -152,6 +160,8 @@ def muon(engine, weight, grad, momentum, rate, beta=0.95, nesterov=True, decay=0
     ``(1 - rate decay) weight - rate scale O``, O being u as :func:`orthogonalize` gives it and the scale by default
     ``max(1, rows / columns) ** 0.5``. momentum is float32 or of the weight's type. With ``inplace`` the given tensors
     are written and returned."""
+    if weight.dim() != 2 or not weight.numel():
+        raise ValueError('weight must have shape (rows, columns), both positive')
     if scale is None:
         scale = max(1.0, weight.shape[0] / weight.shape[-1]) ** 0.5
     return _operators.muon(_handle(engine, weight), engine.device, weight, grad, momentum, rate, beta, nesterov, decay, scale,

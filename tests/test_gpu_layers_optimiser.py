@@ -65,3 +65,11 @@ def test_a_loaded_state_goes_on_as_the_saved_one(engine, kind):
         p.grad = q.grad = update(70 + step, 30, 20, dtype=kind)
         a.step(), b.step()
         assert same_bits(p.detach(), q.detach()) and same_bits(a.state[p]['momentum'], b.state[q]['momentum'])
+
+
+def test_steps_are_not_cut_to_32_bits(engine):
+    x = made(80, 8, 8)
+    for steps in ((1 << 32) + 5, -(1 << 32) + 5, 65, 0):
+        for call in (lambda: operators.orthogonalize(engine, x, steps=steps), lambda: operators.muon(engine, x, x, x, 0.1, steps=steps)):
+            with pytest.raises((ValueError, native.EngineError), match='steps'):
+                call()
