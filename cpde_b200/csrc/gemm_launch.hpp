@@ -1,4 +1,5 @@
-// Launches of kernels_gemm.cuh: tensor maps, tiles and splits.
+// Launches of kernels_gemm.cuh: tensor maps, tiles and splits; what the launches of layers
+// and of orthogonalised matrices have in common.
 #pragma once
 #include <algorithm>
 #include <atomic>
@@ -10,6 +11,29 @@
 namespace cpde::ops {
 
 constexpr int GEMM_SMS = 148;
+
+enum Type : int32_t { F32 = 0, BF16 = 1, F16 = 2 };
+template <class T> struct Tag { using type = T; };
+
+// Parts of a workspace, 256-byte aligned.
+struct Room {
+    char* base;
+    size_t bytes = 0;
+    template <class T> T* take(size_t count) {
+        T* p = base ? reinterpret_cast<T*>(base + bytes) : nullptr;
+        bytes += (count * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+inline bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Threads of a row, eight columns each: a power of two.
+inline int row_lanes(int64_t columns) {
+    int lanes = 1;
+    while (lanes < 32 && lanes * 8 < columns) lanes *= 2;
+    return lanes;
+}
 
 // A launch that may begin before the one ahead in the stream has ended: every kernel
 // behind it says after_previous_launch() before it touches memory. CLUSTER CTAs each.

@@ -133,16 +133,12 @@ struct Chunks {
         for (int i = 0; i < GATHER_CHUNKS; ++i) {
             const int q = thread + 32 * GATHER_WARPS * i, row = ROWS ? q % 512 / 8 : q / 8;
             const int at = (ROWS ? q / 512 * 8192 : 0) + row * 128 + ((q ^ row) & 7) * 16;
-            if constexpr (Parts<T>::count == 1) {
-                *reinterpret_cast<uint4*>(to[0] + at) = raw[i].word[0];
-            } else {
-                float v[8];
-                uint4 part[Parts<T>::count];
-                unpack<T, 8>(raw[i], v);
-                split_eight<T>(v, part);
+            float v[8];
+            uint4 part[Parts<T>::count];
+            unpack<T, 8>(raw[i], v);
+            split_eight<T>(v, part);
 #pragma unroll
-                for (int p = 0; p < Parts<T>::count; ++p) *reinterpret_cast<uint4*>(to[p] + at) = part[p];
-            }
+            for (int p = 0; p < Parts<T>::count; ++p) *reinterpret_cast<uint4*>(to[p] + at) = part[p];
         }
     }
 };
@@ -173,7 +169,7 @@ template <class C, class T, class E>
 __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
     k_gather(const Source<T> a, const Source<T> b, const GemmShape s, const E epilogue, int* error) {
     using namespace gemm;
-    static_assert(C::CTAS == 1 && C::BN == 128 && C::P == Parts<T>::count);
+    static_assert(C::CTAS == 1 && C::BN == 128 && C::P == Parts<T>::count && C::P > 1 && C::RESIDENT && !C::A_ROWS);
     extern __shared__ uint8_t raw_shared[];
     const Shared<C> sh(raw_shared);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -195,77 +191,58 @@ __global__ void __launch_bounds__(GATHER_THREADS<C>, 1)
     after_previous_launch();
 
     if (warp < GATHER_WARPS) {
-        // What this thread has written is there for the MMAs.
-        auto arrive = [&](uint64_t* bar) {
-            tc::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(bar);
-        };
-        // Slabs that are read ahead into registers.
-        constexpr int AHEAD = 1;
-        Chunks<T, C::A_ROWS> ra[AHEAD];
+        Chunks<T, false> ra;
         Chunks<T, C::B_ROWS> rb;
-        bool there[AHEAD];
         Walk<C> walk(s, first, stride, items);
         // The rows of the tile after the next are brought into L2: what is under way into the
         // registers covers the latency of L2, not that of memory. (Tiles follow each other down A.)
         auto ahead = [&](int64_t row) {
             row += threadIdx.x;
             const uint32_t bytes = uint32_t(a.columns * sizeof(T)) / 16 * 16;
-            if (C::A_ROWS || a.width < 8 || threadIdx.x >= GEMM_ROWS || row >= a.rows || !bytes) return;
+            if (a.width < 8 || threadIdx.x >= GEMM_ROWS || row >= a.rows || !bytes) return;
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.p + row * a.stride), "r"(bytes) : "memory");
         };
-        auto load = [&](int i) {
-            there[i] = walk.there();
-            if (!there[i]) return;
+        // A slab into registers, one ahead; false behind the last.
+        auto load = [&] {
+            if (!walk.there()) return false;
             if (walk.slab == walk.w.from) ahead(int64_t(walk.w.tile_m + 2 * stride) * C::BM);
-            ra[i].load(a, int64_t(walk.w.tile_m) * C::BM, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
-            if constexpr (!C::RESIDENT) rb.load(b, int64_t(walk.w.tile_n) * C::BN, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
+            ra.load(a, int64_t(walk.w.tile_m) * C::BM, int64_t(walk.slab) * GEMM_SLAB, threadIdx.x);
             walk.next();
+            return true;
         };
-        load(0);
-        if constexpr (C::RESIDENT) {
-            for (int slab = 0; slab < s.slabs; ++slab) {
-                uint8_t* to[C::P];
+        bool there = load();
+        for (int slab = 0; slab < s.slabs; ++slab) {
+            uint8_t* to[C::P];
 #pragma unroll
-                for (int p = 0; p < C::P; ++p) to[p] = sh.stages + C::STAGES * C::STAGE + (slab * C::P + p) * C::B_BYTES;
-                rb.load(b, 0, int64_t(slab) * GEMM_SLAB, threadIdx.x);
-                rb.store(to, threadIdx.x);
-            }
-            arrive(sh.held);
+            for (int p = 0; p < C::P; ++p) to[p] = sh.stages + C::STAGES * C::STAGE + (slab * C::P + p) * C::B_BYTES;
+            rb.load(b, 0, int64_t(slab) * GEMM_SLAB, threadIdx.x);
+            rb.store(to, threadIdx.x);
         }
-#pragma unroll
-        for (int i = 1; i < AHEAD; ++i) load(i);
+        // What this thread has written is there for the MMAs.
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(sh.held);
         int st = 0;
         uint32_t parity = 1;
-        bool ok = true;
-        while (ok) {
+        while (there) {
+            // The slab's stages, the last part's first.
+            uint8_t* to[C::P];
+            uint64_t* bar[C::P];
+            bool ok = true;
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (!(ok = ok && there[i])) break;
-                // The slab's stages, the last part's first.
-                uint8_t* to[C::P];
-                uint64_t* bar[C::P];
+            for (int p = C::P - 1; p >= 0; --p) {
+                ok = ok && (lane || wait_for(sh.empty + st, parity, sh.abort));
+                to[p] = sh.stages + st * C::STAGE, bar[p] = sh.full + st;
+                if (++st == C::STAGES) st = 0, parity ^= 1;
+            }
+            if (!__all_sync(~0u, ok)) break;
+            ra.store(to, threadIdx.x);
+            there = load();
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
 #pragma unroll
-                for (int p = C::P - 1; p >= 0; --p) {
-                    ok = ok && (lane || wait_for(sh.empty + st, parity, sh.abort));
-                    to[p] = sh.stages + st * C::STAGE, bar[p] = sh.full + st;
-                    if (++st == C::STAGES) st = 0, parity ^= 1;
-                }
-                if (!(ok = __all_sync(~0u, ok))) break;
-                ra[i].store(to, threadIdx.x);
-                if constexpr (!C::RESIDENT) {
-#pragma unroll
-                    for (int p = 0; p < C::P; ++p) to[p] += C::A_BYTES;
-                    rb.store(to, threadIdx.x);
-                }
-                load(i);
-                tc::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) {
-#pragma unroll
-                    for (int p = 0; p < C::P; ++p) tc::mbar_arrive(bar[p]);
-                }
+                for (int p = 0; p < C::P; ++p) tc::mbar_arrive(bar[p]);
             }
         }
         // No commit may be under way to the stages' barriers when the CTA ends.

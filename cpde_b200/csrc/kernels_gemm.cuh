@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     using namespace gemm;
     extern __shared__ uint8_t raw_shared[];
     const Shared<C> sh(raw_shared);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32;
     const uint32_t rank = C::CTAS == 2 ? cluster_rank() : 0;
     const int first = blockIdx.x / C::CTAS, stride = gridDim.x / C::CTAS;
     const int items = s.tiles * s.splits * s.batches;

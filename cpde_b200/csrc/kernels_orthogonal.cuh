@@ -130,8 +130,7 @@ struct UpdateCall {
     M* new_momentum;
     float* update;         // u in FP32, for the second pass
     double* sums;          // (matrix, block) sums of squares
-    __half* out;           // two parts of pitch
-    int64_t rows, pitch, plane;
+    int64_t rows;
     int32_t columns, lanes, blocks;
     float beta, rest;      // 1 - beta, rounded by itself: the difference of rounded numbers would be off by more
     bool nesterov, whole;

@@ -6,9 +6,6 @@
 namespace cpde::ops {
 namespace {
 
-enum Type : int32_t { F32 = 0, BF16 = 1, F16 = 2 };
-
-template <class T> struct Tag { using type = T; };
 template <class F>
 void with_type(int32_t type, F&& f) {
     if (type == F32) f(Tag<float>{});
@@ -16,23 +13,11 @@ void with_type(int32_t type, F&& f) {
     else f(Tag<__half>{});
 }
 
-// Parts of a workspace, 256-byte aligned.
-struct Room {
-    char* base;
-    size_t bytes = 0;
-    template <class T> T* take(size_t count) {
-        T* p = base ? reinterpret_cast<T*>(base + bytes) : nullptr;
-        bytes += (count * sizeof(T) + 255) / 256 * 256;
-        return p;
-    }
-};
-
 // Layers of at most so many points (or outputs) may take the kernel that reads the other side once, and
 // products of at most so many slabs of 32 x 32 x 64 the one on the FP32 units.
 constexpr int64_t FEW_POINTS = 8, SMALL_WORK = 2048;
 
 int64_t eights(int64_t n) { return (n + 7) / 8 * 8; }
-bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // Whether TMA reads the array as it is: whole 16-byte units from row to row.
 bool direct(int32_t type, const void* p, int64_t stride, int64_t rows) {
@@ -43,11 +28,6 @@ int64_t row_chunks(int64_t rows, int64_t columns, int lanes) {
     const int64_t strips = (columns + 8 * lanes - 1) / (8 * lanes), high = 256 / lanes;
     // About eight blocks an SM, and four passes of a block's threads at least.
     return std::max<int64_t>(1, std::min<int64_t>({GEMM_SMS * 8 / strips, (rows + 4 * high - 1) / (4 * high), 1024}));
-}
-int row_lanes(int64_t columns) {
-    int lanes = 1;
-    while (lanes < 32 && lanes * 8 < columns) lanes *= 2;
-    return lanes;
 }
 
 template <class T>
@@ -167,11 +147,11 @@ void launch_gather(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n,
     launch_early(k_gather<C, T, LinearEpilogue<T>>, dim3(unsigned(std::min<int64_t>(items, GEMM_SMS))), GATHER_THREADS<C>, C::SHARED, 1,
                  stream, a, b, s, epilogue, error);
 }
-template <class T, bool A_ROWS, bool B_ROWS>
+template <class T, bool B_ROWS>
 void gathered_product(const Source<T>& a, const Source<T>& b, int64_t m, int64_t n, int64_t k, const Route& r,
                       const LinearEpilogue<T>& epilogue, int* error, cudaStream_t stream) {
     if constexpr (Parts<T>::count > 1)
-        launch_gather<GemmTile<1, 128, Parts<T>::count, A_ROWS, B_ROWS, true>>(a, b, m, n, k, r.plan, epilogue, error, stream);
+        launch_gather<GemmTile<1, 128, Parts<T>::count, false, B_ROWS, true>>(a, b, m, n, k, r.plan, epilogue, error, stream);
 }
 
 // Whether rows of `n` elements at these addresses take the wide accesses of the epilogue, and those of fours.
@@ -261,7 +241,7 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     float* partial = room.take<float>(partial_count(r.plan, c.points, c.outputs));
     if (!launch) return room.bytes;
     if (r.gather) {
-        gathered_product<T, false, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, error, stream);
+        gathered_product<T, false>(xs, ws, c.points, c.outputs, c.inputs, r, e, error, stream);
         return room.bytes;
     }
     PartsCalls<T> parts = {};
@@ -355,7 +335,7 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     if (c.dx) {
         e.y = c.dx, e.y_wide = c.type == F32;
         set_widths(e, c.inputs);
-        if (dx.gather) gathered_product<T, false, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, error, stream);
+        if (dx.gather) gathered_product<T, true>(gs, ws, c.points, c.inputs, c.outputs, dx, e, error, stream);
         else product<T, false, true>(dz, wo, c.points, c.inputs, c.outputs, dx.plan, e, partial, error, stream);
     }
     if (c.dweight) {

@@ -9,22 +9,6 @@
 namespace cpde::ops {
 namespace {
 
-enum Type : int32_t { F32 = 0, BF16 = 1, F16 = 2 };
-
-template <class T> struct Tag { using type = T; };
-
-struct Room {
-    char* base;
-    size_t bytes = 0;
-    template <class T> T* take(size_t count) {
-        T* p = base ? reinterpret_cast<T*>(base + bytes) : nullptr;
-        bytes += (count * sizeof(T) + 255) / 256 * 256;
-        return p;
-    }
-};
-
-bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
 struct Step {
     double a, b, c;
     int x, gram, poly;  // exponents of what the step holds: X, A and Q
@@ -65,12 +49,6 @@ bool plan_steps(const OrthogonalCall& c, std::vector<Step>& steps) {
         steps.push_back(s);
     }
     return true;
-}
-
-int row_lanes(int64_t columns) {
-    int lanes = 1;
-    while (lanes < 32 && lanes * 8 < columns) lanes *= 2;
-    return lanes;
 }
 
 // Whether one CTA holds a matrix.
