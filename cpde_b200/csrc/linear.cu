@@ -13,9 +13,8 @@ void with_type(int32_t type, F&& f) {
     else f(Tag<__half>{});
 }
 
-// Layers of at most so many points (or outputs) may take the kernel that reads the other side once, and
-// products of at most so many slabs of 32 x 32 x 64 the one on the FP32 units.
-constexpr int64_t FEW_POINTS = 8, SMALL_WORK = 2048;
+// Layers of at most so many points (or outputs) may take the kernel that reads the other side once.
+constexpr int64_t FEW_POINTS = 8;
 
 int64_t eights(int64_t n) { return (n + 7) / 8 * 8; }
 
@@ -87,7 +86,7 @@ Route route(int64_t m, int64_t n, int64_t k, const Side& a, const Side& b) {
     for (const Side* s : {&a, &b})
         if (!s->there) made += LAUNCH_CLOCKS + double(s->elements) * (sizeof(T) + 2 * P) / 2000;
     // Gathered, where B's parts stay in shared memory: 65,536 points of 128 inputs and outputs
-    // in FP32 take 37 us instead of 51 with parts. At 64 outputs half of its tile is empty:
+    // in FP32 take 40 us instead of 51 with parts. At 64 outputs half of its tile is empty:
     // 25 instead of 20.
     if constexpr (P > 1) {
         const bool resident = n <= 128 && P * ((k + GEMM_SLAB - 1) / GEMM_SLAB) <= GemmTile<1, 128, P, false, false, true>::HELD;
@@ -166,11 +165,22 @@ void set_widths(LinearEpilogue<T>& e, int64_t n) {
     e.whole = all(16), e.fours = all(4);
 }
 
-// Whether a layer's product is computed on the FP32 units, in blocks of 32 x 32.
-bool small_product(int64_t m, int64_t n, int64_t k) {
-    const int64_t tiles = ((m + SMALL_TILE - 1) / SMALL_TILE) * ((n + SMALL_TILE - 1) / SMALL_TILE);
-    return k <= 1024 && tiles * ((k + SMALL_SLAB - 1) / SMALL_SLAB) <= SMALL_WORK;
-}
+// Products on the FP32 units in blocks of 32 x 32, and the microseconds that they take: an SM has
+// one block at a time, which goes through its slabs one after the other. Against them stand the
+// launches of the tensor cores' tiles, which for layers of this size take about as long each
+// whatever it is. Measured, blocks against tiles: 1000 x 64 -> 64 FP32 5.0 and 10.2, 600 x 128 ->
+// 128 6.3 and 10.9, 100 x 512 -> 64 13.4 and 12.8; bf16 5.3 and 5.5, 6.7 and 5.9, 14.3 and 6.7 in
+// whole 16 bytes, 5.2 and 8.9, 6.7 and 9.1, 14.3 and 10.0 where x and W are copied; 1440 x 64 ->
+// 1440 bf16 58 and 8.3. Gradients of 300 x 104 -> 80 with SiLU and bias FP32 13.4 and 29.4, bf16
+// 13.0 and 20.4, of 1000 x 64 -> 64 34.6 and 26.1, 30.2 and 20.6.
+struct SmallWork {
+    int64_t blocks = 0, slabs = 0;
+    void add(int64_t m, int64_t n, int64_t k) {
+        blocks += ((m + SMALL_TILE - 1) / SMALL_TILE) * ((n + SMALL_TILE - 1) / SMALL_TILE);
+        slabs = std::max(slabs, (k + SMALL_SLAB - 1) / SMALL_SLAB);
+    }
+    double time(double slab) const { return 1.1 + double((blocks + GEMM_SMS - 1) / GEMM_SMS) * (2.8 + slab * slabs); }
+};
 template <class T>
 SmallProduct<T> small_call(const SmallOperand<T>& a, const SmallOperand<T>& b, int64_t m, int64_t n, int64_t k,
                            const LinearEpilogue<T>& e) {
@@ -221,7 +231,11 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
     };
     const bool few = c.points <= FEW_POINTS && (c.outputs <= 16384 || long_rows(c.points));
     const bool turned = c.type == F32 && c.outputs <= FEW_POINTS && long_rows(c.outputs);
-    if (few || turned || small_product(c.points, c.outputs, c.inputs)) {
+    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
+    SmallWork work;
+    work.add(c.points, c.outputs, c.inputs);
+    const bool small = work.time(1.3) <= (sizeof(T) == 4 ? 11.0 : x_direct && w_direct ? 5.6 : 8.8);
+    if (few || turned || small) {
         if (!launch) return 0;
         if (few) {
             launch_few<T, false>(xs, ws, e, stream);
@@ -233,7 +247,6 @@ size_t run_linear(const LinearCall& c, int* error, cudaStream_t stream, bool lau
         }
         return 0;
     }
-    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
     const Route r = route<T>(c.points, c.outputs, c.inputs, {x_direct, c.points * c.inputs},
                              {w_direct, c.outputs * c.inputs});
     O* x_parts = x_direct || r.gather ? nullptr : room.take<O>(parts_count<T>(c.points, c.inputs));
@@ -262,7 +275,16 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
     const bool sloped = c.activation != 1;
     const T *grad = static_cast<const T*>(c.grad), *z = sloped ? static_cast<const T*>(c.z) : nullptr;
     const T *x = static_cast<const T*>(c.x), *w = static_cast<const T*>(c.weight);
-    if ((!c.dx || small_product(c.points, c.inputs, c.outputs)) && ((!c.dweight && !c.dbias) || small_product(c.outputs, c.inputs, c.points))) {
+    const bool dz_direct = !sloped && direct(c.type, grad, c.grad_stride, c.points);
+    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
+    SmallWork work;
+    if (c.dx) work.add(c.points, c.inputs, c.outputs);
+    if (c.dweight || c.dbias) work.add(c.outputs, c.dweight ? c.inputs : 1, c.points);
+    // Parts, the bias' sums (a pass of their own if nothing becomes parts) and the products.
+    const bool parts_made = !dz_direct || (c.dweight && !x_direct) || (c.dx && !w_direct);
+    const double tiles = (parts_made ? sloped ? 8.0 : 4.0 : 0.0) + (c.dbias ? parts_made ? 2.0 : 4.5 : 0.0) +
+                         ((c.dx != nullptr) + (c.dweight != nullptr)) * (sizeof(T) == 4 ? 7.5 : 5.6);
+    if (work.time(sloped ? 1.9 : 1.2) <= tiles) {
         if (!launch) return 0;
         LinearEpilogue<T> e = {};
         e.activation = 1;
@@ -286,8 +308,6 @@ size_t run_gradient(const LinearGradientCall& c, int* error, cudaStream_t stream
         launch_small(dx, dw, stream);
         return 0;
     }
-    const bool dz_direct = !sloped && direct(c.type, grad, c.grad_stride, c.points);
-    const bool x_direct = direct(c.type, x, c.x_stride, c.points), w_direct = direct(c.type, w, c.weight_stride, c.outputs);
     // dz is made in the type's parts where the activation has a slope; otherwise it is
     // grad, which is made into parts only if a product is not gathered.
     const Source<T> gs = source(grad, c.grad_stride, c.points, c.outputs), ws = source(w, c.weight_stride, c.outputs, c.inputs);

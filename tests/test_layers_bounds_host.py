@@ -21,6 +21,30 @@ def test_gradient_workspace_is_enough_for_both_types():
     assert sizes[2] >= sizes[2 + 8] + 30000 * 2048 * 2 and sizes[7] >= sizes[7 + 8] + 30000 * 2048 * 2
 
 
+def test_blocks_of_small_layers_go_through_few_slabs():
+    """Layers whose blocks would go through many slabs in turn, or come in many waves, take the tensor cores' tiles, which need a
+    workspace for FP32 arrays; small ones take blocks, which need none."""
+    import ctypes
+
+    from cpde_b200 import native
+    lib, size = native.load(), ctypes.c_size_t()
+
+    def forward(points, inputs, outputs):
+        assert lib.cpde_linear_workspace(0, 1 << 20, inputs, points, inputs, outputs, 1 << 35, inputs, ctypes.byref(size)) == native.OK
+        return size.value
+
+    def gradient(points, inputs, outputs, kind=0):
+        assert lib.cpde_linear_gradient_workspace(kind, 1 << 20, outputs, 3, 1 << 30, inputs, points, inputs, outputs, 1 << 35, inputs, 7,
+                                                  ctypes.byref(size)) == native.OK
+        return size.value
+
+    assert not any(forward(*s) for s in ((257, 48, 128), (1000, 64, 64), (256, 256, 256), (40, 10, 10)))
+    assert all(forward(*s) for s in ((1440, 64, 1440), (1000, 128, 1024), (352, 1024, 352), (700, 256, 256)))
+    for kind in (0, 1, 2):
+        assert not any(gradient(*s, kind) for s in ((300, 100, 77), (60, 64, 64), (256, 256, 256)))
+        assert all(gradient(*s, kind) for s in ((1000, 100, 77), (1024, 40, 16), (1025, 40, 16), (512, 256, 256)))
+
+
 def parts(v, count):
     out = []
     for _ in range(count):
