@@ -37,7 +37,8 @@ struct SmallCall {
 // One product into tensor memory, in two sums that the epilogue adds: the first and the
 // second half of the contraction, SMALL_LENGTH columns apart. In each the small products
 // of parts come first: sums are cut toward zero at their size, and what that does to the
-// steps is seen in the result (1.2e-6 of its norm with one sum where two leave 0.8e-6).
+// steps is seen in the result (of one matrix 1.2e-6 of its norm with one sum, 0.8e-6 with two;
+// with two the updates of four layers of 128 x 128 come out at 1.7e-6, FP32 products at 2.9e-6).
 template <bool B_ROWS>
 __device__ __forceinline__ void small_product(uint32_t d, uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int n, int k) {
     const uint32_t instruction = 1u << 4 | uint32_t(B_ROWS) << 16 | uint32_t(n >> 3) << 17 | uint32_t(SMALL_SIDE >> 4) << 24;

@@ -107,7 +107,8 @@ def linear(engine, x, weight, bias=None, activation='linear', residual=None, kee
     """``(y, z)`` of ``y = residual + act(x @ weight.T + bias)`` over x of shape (..., inputs) and weight of shape
     (outputs, inputs). z, the sums before the activation that :func:`linear_gradient` takes, is None unless ``keep``.
 
-    The products of 16-bit types are summed in FP32, to 1.2e-5 of the terms' absolute values; those of float32 have the error of FP32 products."""
+    The products of 16-bit types are summed in FP32, to 1.2e-5 of the terms' absolute values; those of float32 have the
+    error of FP32 products. A row of float32 x with an infinity gives infinities or NaNs."""
     return _operators.linear(_handle(engine, x), engine.device, x, weight, bias, _activation(activation), residual, keep)
 
 
@@ -147,7 +148,7 @@ def orthogonalize(engine, x, steps=5, coefficients=QUINTIC, eps=1e-7):
     ``X = x / (|x| + eps)`` with the Frobenius norm, then ``steps`` times ``X = a X + b (X X') X + c (X X')^2 X``.
     ``coefficients`` is a triple (a, b, c), or one for each step (the last counts for the steps behind it).
 
-    Values are held in 22 bits. Products take all of them for float32, whose result is good to about 1e-6 of its norm, for
+    Values are held in 22 bits. Products take all of them for float32, whose result is good to about 2e-6 of its norm, for
     float16 and where a side is up to 256, and 11 for larger bfloat16 matrices, which leaves less than rounding to bfloat16
     adds."""
     return _operators.orthogonalize(_handle(engine, x), engine.device, x, steps, _coefficients(coefficients), eps)

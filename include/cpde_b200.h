@@ -267,8 +267,9 @@ int cpde_group_norm_gradient(cpde_engine* engine, int32_t type, const void* grad
  * (or NULL) takes the sums before the activation, for the gradient. Products of
  * the 16-bit types are exact and summed in FP32, in which up to 2048 terms may be cut
  * toward zero (1.2e-5 of a sum of one sign) and such sums are rounded; those of FP32 arrays are of
- * three BF16 parts each (24 bits), so that they have the error of FP32 products; a
- * row with an infinity gives infinities or NaNs. Small layers, and most of at most
+ * three BF16 parts each (24 bits), so that they have the error of FP32 products (less
+ * of values below 2^-110); a row with an infinity gives infinities or NaNs, with any
+ * activation. Small layers, and most of at most
  * 8 points (in FP32 also of 8 outputs), are computed on the FP32 units. Of larger ones 16-bit arrays
  * whose address and stride are whole 16 bytes are read in place; others, and wide
  * FP32 ones, go through the workspace, whose query therefore takes the addresses too.
