@@ -26,7 +26,7 @@
 // 256 x 256 has the tensor core's rate: a slab takes 518 clocks where its MMAs take 512.
 // 32,768 points of 2048 x 2048 bf16: 185 us (1.49 PFLOP/s; the library's product takes
 // 183), with bias and SiLU 188, with a residual and the sums kept 223. 8192 x 8192 x 8192:
-// 717 us (678), bound by what L2 brings (47 bytes a clock an SM). Six products of FP32's
+// 710 us (678), bound by what L2 brings (47 bytes a clock an SM). Six products of FP32's
 // parts: 2048 x 2048 x 2048 in 88 us (195 TFLOP/s, 1.2 PFLOP/s of BF16).
 // Every wait is bounded: a role that gives up raises the CTA's abort flag, the
 // loads in flight are waited for, tensor memory is released and `error` is set.

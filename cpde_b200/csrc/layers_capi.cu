@@ -122,8 +122,12 @@ int cpde_linear_gradient_workspace(int32_t type, const void* grad, int64_t grad_
         c.dx = want & kWantInput ? &wanted : nullptr;
         c.dweight = want & kWantWeight ? &wanted : nullptr;
         c.dbias = want & kWantBias ? &wanted : nullptr;
-        c.weight_type = want & kWeightOfType ? type : CPDE_F32;
-        return points ? cpde::ops::linear_gradient_workspace(c) : 0;
+        if (!points) return size_t(0);
+        c.weight_type = type;
+        size_t bytes = cpde::ops::linear_gradient_workspace(c);
+        if (want & kWeightOfType) return bytes;
+        c.weight_type = CPDE_F32;
+        return std::max(bytes, cpde::ops::linear_gradient_workspace(c));
     });
 }
 

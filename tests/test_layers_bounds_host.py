@@ -21,6 +21,25 @@ def test_gradient_workspace_is_enough_for_both_types():
     assert sizes[2] >= sizes[2 + 8] + 30000 * 2048 * 2 and sizes[7] >= sizes[7 + 8] + 30000 * 2048 * 2
 
 
+def test_gradient_workspace_of_any_size_is_enough_for_both_types():
+    """Contractions of different lengths are split differently, so that either type may need more for its partial sums."""
+    import ctypes
+    import random
+
+    from cpde_b200 import native
+    lib, size, rng = native.load(), ctypes.c_size_t(), random.Random(0)
+
+    def query(points, inputs, outputs, kind, activation, want):
+        assert lib.cpde_linear_gradient_workspace(kind, 1 << 20, outputs, activation, 1 << 30, inputs, points, inputs, outputs, 1 << 35,
+                                                  inputs, want, ctypes.byref(size)) == native.OK
+        return size.value
+
+    for _ in range(20000):
+        shape = [int(2 ** rng.uniform(0, top)) for top in (20, 13, 13)]
+        kind, activation, want = rng.choice((0, 1, 2)), rng.choice((1, 3)), rng.choice((2, 3, 6, 7))
+        assert query(*shape, kind, activation, want) >= query(*shape, kind, activation, want + 8), (shape, kind, activation, want)
+
+
 def test_blocks_of_small_layers_go_through_few_slabs():
     """Layers whose blocks would go through many slabs in turn, or come in many waves, take the tensor cores' tiles, which need a
     workspace for FP32 arrays; small ones take blocks, which need none."""
